@@ -241,6 +241,46 @@ int stgcn_mul_many(const float* a, const float* const* inputs, int n, float* out
  * Replaces: nn.CrossEntropyLoss() of the training step (processor/recognition.py:44, 91) and its autograd. */
 int stgcn_cross_entropy(const float* logits, const int64_t* labels, float* loss, float* dlogits, int N, int ncls, void* stream);
 
+/* ---- learning from and answering with class scores --------------------------------------------------------------
+ * No counterpart in the reference, whose training step knows hard labels only (processor/recognition.py:44, 91) and
+ * whose test step keeps the scores as they are (recognition.py:110-143).
+ * `logits` here: rows of ncls scores, float32 or bf16, `row_stride` ELEMENTS apart (>= ncls), any alignment of an element;
+ * 1 <= ncls <= 2^20, 1 <= rows.  Classes are ordered by (score descending, class ascending), NaN first. */
+
+/* The k (1..256, <= ncls) first classes of every row in that order: values [rows][k], indices [rows][k], and rest [rows] =
+ * log sum over the other classes of exp(logits / temperature) (-inf: nothing is left). */
+int stgcn_top_logits(int dtype, const void* logits, size_t row_stride, int rows, int ncls, int k, double temperature,
+                     float* values, int64_t* indices, float* rest, void* stream);
+
+/* Distillation from a teacher's top logits: values / indices [rows][k] (k <= 256; an index < 0 is no entry), rest [rows] the
+ * log of the teacher's other mass at the same temperature T (null: the teacher's entries are renormalised), labels [rows]
+ * (< 0: none; null when label_weight w is 0).  With p the teacher's and q the student's distribution at T over the listed
+ * classes and, where the teacher has a rest, all others together:
+ *     loss[row] = (1 - w) T^2 sum p log(p / q) + w (-log softmax(logits)[label])
+ * A row without an entry has no first term, without a label no second; with neither, or with every logit -inf, it is 0
+ * and so is its gradient.  Classes >= ncls and teacher scores that are NaN or +inf make the row's loss and gradient NaN.
+ * reduction 0: loss [rows]; 1: loss [1] = mean over all rows; 2: loss [1] = sum (1 and 2 add up loss_rows, double [rows],
+ * in a fixed order).  stats [rows][4] and probs [rows][k] are what the gradient needs. */
+int stgcn_distill_fwd(int dtype, const void* logits, size_t row_stride, const float* values, const int64_t* indices,
+                      const float* rest, const int64_t* labels, int rows, int ncls, int k, double temperature, double label_weight,
+                      int reduction, float* loss, double* loss_rows, float* stats, float* probs, void* stream);
+/* dlogits [rows][ncls] (contiguous, the type of logits) = grad * scale * d loss[row] / d logits; grad: null (1), one float,
+ * or one a row. */
+int stgcn_distill_bwd(int dtype, const void* logits, size_t row_stride, const int64_t* indices, const int64_t* labels,
+                      const float* stats, const float* probs, const float* grad, int grad_per_row, double scale, int rows,
+                      int ncls, int k, double temperature, double label_weight, void* dlogits, void* stream);
+
+/* A label per row drawn from softmax(logits / temperature) with the given random number u in [0, 1): of the classes in
+ * order the first top_k (0: all); of these the shortest prefix that reaches top_p of their mass; of these those at least
+ * min_p times as likely as the first; the label is the first of them, by class number, at which their running mass exceeds
+ * u times their mass; logp is the log of its share of that mass.  temperature 0: the first class, logp 0.  Each parameter
+ * is one number or, where its array is given, one a row.  Weights and sums are held in 64 bits.
+ * A row of -inf only answers label -1 and logp -inf; a row with a NaN, or with a parameter out of range (temperature >= 0,
+ * top_k >= 0, 0 < top_p <= 1, 0 <= min_p <= 1, 0 <= u < 1), answers label -1 and logp NaN. */
+int stgcn_sample_labels(int dtype, const void* logits, size_t row_stride, const float* u, const float* temperatures, float temperature,
+                        const int* top_ks, int top_k, const float* top_ps, float top_p, const float* min_ps, float min_p,
+                        int64_t* labels, float* logp, int rows, int ncls, void* stream);
+
 /* Re-packs every convolution weight of a model in one launch.  table: ndesc descriptors in device memory, each
  * 10 x 8 bytes { const float* src; void* w; void* wt; int64 G, Cout, Cin, Cinp, sg, sco, sci }: element (g, co, ci) =
  * src[g*sg + co*sco + ci*sci] is written in the compute dtype to w[g][co][cip] and wt[g][cip][co] (cip < Cinp,

@@ -1,0 +1,87 @@
+// Device helpers shared by the kernels over class scores (top_logits, distill, sample).
+//
+// A row of scores is [ncls] float32 or bf16, contiguous, at any element alignment: a row of an odd class count starts
+// anywhere.  RowSpan splits it into the elements in front of the first 16-byte boundary, whole 16-byte vectors, and the
+// elements behind the last one, so that no load or store touches a byte outside the row.
+#pragma once
+#include "stgcn_common.h"
+
+template <typename T> struct RowSpan {
+    static constexpr int VEC = ET<T>::VEC;
+    int head, nvec, edge;                  // elements in front, vectors, elements in front and behind together
+    __device__ __forceinline__ RowSpan(const void* row, int n) {
+        const int off = (int)((uintptr_t)row & 15) / ET<T>::ES;
+        head = off ? VEC - off : 0;
+        if (head > n) head = n;
+        nvec = (n - head) / VEC;
+        edge = n - nvec * VEC;
+    }
+    __device__ __forceinline__ int vec_at(int v) const { return head + v * VEC; }           // first class of vector v
+    __device__ __forceinline__ int edge_at(int e) const { return e < head ? e : e + nvec * VEC; }   // class of edge element e
+};
+
+template <typename T> __device__ __forceinline__ i32x4 load_vec(const T* row, int at) {
+    return *reinterpret_cast<const i32x4*>((const char*)row + (size_t)at * ET<T>::ES);
+}
+template <typename T> __device__ __forceinline__ void store_vec(T* row, int at, const i32x4& raw) {
+    *reinterpret_cast<i32x4*>((char*)row + (size_t)at * ET<T>::ES) = raw;
+}
+
+// Order of the scores as unsigned integers: a > b as floats <=> key(a) > key(b); -0 and 0 are one key; NaN is above
+// everything.
+constexpr uint32_t KEY_NAN = 0xFFFFFFFFu, KEY_NEG_INF = 0x007FFFFFu;
+__device__ __forceinline__ uint32_t score_key(float x) {
+    if (x != x) return KEY_NAN;
+    const uint32_t b = __float_as_uint(x + 0.f);           // -0 + 0 = 0
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+    if (k == KEY_NAN) return __uint_as_float(0x7FC00000u);
+    return __uint_as_float(k ^ ((k & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+// v_exp_f32: 2^y to one unit in the last place, 0 below 2^-126.
+__device__ __forceinline__ float exp2_32(float y) { return __builtin_amdgcn_exp2f(y); }
+
+// 2^y in 64 bits for y <= 1000: y = n + f, |f| <= 1/2, the Taylor series of e^(f ln 2) to the 11th power (remainder
+// (ln2/2)^12 / 12! = 6e-15), times 2^n.  Exactly 1 at y = 0.  The fp64 vector rate of this chip is its fp32 rate, so
+// this costs about 18 issue slots against 5 for v_exp_f32.
+__device__ __forceinline__ double exp2_64(double y) {
+    y = fmax(y, -1100.0);
+    const double n = rint(y), f = y - n;
+    double p = 4.4455382718708114976e-10;                  // ln2^k / k!, k = 11 .. 1
+    p = fma(p, f, 7.0549116208011233299e-09);
+    p = fma(p, f, 1.0178086009239699728e-07);
+    p = fma(p, f, 1.3215486790144309488e-06);
+    p = fma(p, f, 1.5252733804059840280e-05);
+    p = fma(p, f, 1.5403530393381609954e-04);
+    p = fma(p, f, 1.3333558146428443423e-03);
+    p = fma(p, f, 9.6181291076284771619e-03);
+    p = fma(p, f, 5.5504108664821579953e-02);
+    p = fma(p, f, 2.4022650695910071233e-01);
+    p = fma(p, f, 6.9314718055994530942e-01);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n);
+}
+
+// ---- reductions of a workgroup of W waves: every thread gets the result; `red` is W entries of LDS -------------------
+struct OpMax { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
+struct OpFMax { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct OpSum { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; } };
+
+template <typename V, typename Op> __device__ __forceinline__ V wave_reduce(V v, Op op) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v = op(v, __shfl_xor(v, d));
+    return v;
+}
+template <int W, typename V, typename Op> __device__ __forceinline__ V block_reduce(V v, Op op, V* red) {
+    v = wave_reduce(v, op);
+    if constexpr (W == 1) return v;
+    __syncthreads();                                       // the previous use of `red` has been read
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    V r = red[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) r = op(r, red[w]);
+    return r;
+}

@@ -4,8 +4,13 @@
   StGcnBlockFn  st_gcn.forward                       (net/st_gcn.py:191-197)
   DataBnFn      Model.forward input normalisation    (net/st_gcn.py:72-78)
   HeadFn        pooling + fcn                        (net/st_gcn.py:85-90)
+
+and, beside the reference, the operators that learn from and answer with class scores: top_logits, distillation,
+sample_labels.
 """
+import collections
 import contextlib
+import copy
 import os
 
 import torch
@@ -380,6 +385,56 @@ def cross_entropy(logits, labels):
             and logits.shape[0] <= 8192:
         return CrossEntropyFn.apply(logits, labels)
     return torch.nn.functional.cross_entropy(logits, labels)
+
+
+TopLogits = collections.namedtuple("TopLogits", "values indices rest")
+
+
+def top_logits(logits, k, temperature=1.0):
+    """What of a teacher's scores [rows, classes] is kept for distillation: TopLogits(values, indices, rest), see
+    ops.top_logits.  Carries no gradient."""
+    return TopLogits(*P.top_logits(logits, k, temperature))
+
+
+class DistillationFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, indices, rest, labels, temperature, label_weight, reduction):
+        call = P.DistillCall(logits, values, indices, rest, labels, temperature, label_weight, reduction)
+        loss = call.forward()
+        ctx.save_for_backward(logits, call.indices, call.labels, call.stats, call.probs)
+        call.x = call.values = call.rest = call.indices = call.labels = call.stats = call.probs = None
+        ctx.call = call
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        call = copy.copy(ctx.call)
+        logits, call.indices, call.labels, call.stats, call.probs = ctx.saved_tensors
+        call.x = P._check_scores(logits)
+        return (call.backward(g.float().contiguous()),) + (None,) * 7
+
+
+def distillation(logits, values, indices, rest=None, labels=None, temperature=1.0, label_weight=0.0, reduction="mean"):
+    """Distillation loss of student scores [rows, classes] (float32 or bfloat16) against a teacher's top logits.
+
+    values, indices [rows, k] (k <= 256; float32, int64) are the teacher's listed classes, an index < 0 being no entry;
+    rest [rows] is the log of its other classes' mass at the same temperature T, as top_logits returns it.  With rest, p
+    and q are the teacher's and the student's distributions at T over the listed classes and all others together;
+    without it the teacher's listed classes are renormalised.  With w = label_weight:
+
+        loss[row] = (1 - w) T^2 sum p log(p / q) + w cross_entropy(logits[row], labels[row])
+
+    A row without entries has no first term, one whose label is < 0 no second; a row with neither (padding) or with
+    every score -inf gives 0 and a zero gradient, whatever it holds.  A class listed twice counts with both entries.  A
+    class or label >= classes, or a teacher score that is NaN or +inf, makes the row's loss and gradient NaN.  The mean is
+    over all rows.  Differentiable in logits, once."""
+    return DistillationFn.apply(logits, values, indices, rest, labels, temperature, label_weight, reduction)
+
+
+def sample_labels(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(labels, logp) drawn from class scores with the given random numbers, see ops.sample_labels.  Carries no gradient."""
+    return P.sample_labels(logits, u, temperature, top_k, top_p, min_p)
 
 
 class DataBnFn(torch.autograd.Function):

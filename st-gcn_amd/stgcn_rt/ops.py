@@ -490,6 +490,159 @@ def cross_entropy(logits, labels):
     return loss, dlogits
 
 
+MAX_CLASSES, MAX_TOP = 1 << 20, 256
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _check_scores(x, name="logits"):
+    """[rows, classes] float32 / bfloat16, classes contiguous (else a contiguous copy); check_device comes last, after the
+    other arguments."""
+    if x.dim() != 2:
+        raise ValueError("%s wants [rows, classes], got %s" % (name, tuple(x.shape)))
+    L.dtype_code(x.dtype)
+    if not 1 <= x.shape[1] <= MAX_CLASSES:
+        raise ValueError("%s: 1 to %d classes, got %d" % (name, MAX_CLASSES, x.shape[1]))
+    if x.shape[0] >= 1 << 31:
+        raise ValueError("%s: fewer than 2^31 rows, got %d" % (name, x.shape[0]))
+    x = x.detach()
+    if (x.stride(1) == 1 or x.shape[1] == 1) and (x.shape[0] < 2 or x.stride(0) >= x.shape[1]):
+        return x
+    return x.contiguous()
+
+
+def _row_stride(x):
+    return max(x.stride(0), x.shape[1])
+
+
+def _check_like(t, name, shape, dtype, like):
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError("%s wants %s %s, got %s %s" % (name, tuple(shape), dtype, tuple(t.shape), t.dtype))
+    if t.device != like.device:
+        raise RuntimeError("%s lives on %s, the logits on %s" % (name, t.device, like.device))
+    return t.detach().contiguous()
+
+
+def _check_temperature(t):
+    t = float(t)
+    if not 0.0 < t < 1e30:
+        raise ValueError("temperature wants a positive number, got %r" % t)
+    return t
+
+
+def top_logits(logits, k, temperature=1.0):
+    """The k largest scores of every row: (values [rows, k] float32, indices [rows, k] int64, rest [rows] float32).
+
+    Descending, ties by class, NaN first; rest = log sum of exp(logits / temperature) over the classes that are not
+    listed (-inf when there are none)."""
+    x = _check_scores(logits)
+    rows, ncls = x.shape
+    k, temperature = int(k), _check_temperature(temperature)
+    if not 1 <= k <= min(ncls, MAX_TOP):
+        raise ValueError("top_logits: 1 to %d of %d classes, got k = %d" % (min(ncls, MAX_TOP), ncls, k))
+    check_device(x, "logits")
+    values = torch.empty((rows, k), dtype=torch.float32, device=x.device)
+    indices = torch.empty((rows, k), dtype=torch.int64, device=x.device)
+    rest = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    if rows:
+        _launch((str(x.dtype), rows, ncls, k), "stgcn_top_logits", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), rows, ncls, k, temperature,
+                L.ptr(values), L.ptr(indices), L.ptr(rest), L.stream_ptr())
+    return values, indices, rest
+
+
+class DistillCall:
+    """The checked arguments of one distillation call and what its forward leaves for the gradient."""
+
+    def __init__(self, logits, values, indices, rest, labels, temperature, label_weight, reduction):
+        self.x = x = _check_scores(logits)
+        self.rows, self.ncls = rows, ncls = x.shape
+        if values.dim() != 2 or not 1 <= values.shape[1] <= MAX_TOP:
+            raise ValueError("distillation: values wants [rows, 1 to %d], got %s" % (MAX_TOP, tuple(values.shape)))
+        self.k = values.shape[1]
+        self.values = _check_like(values, "values", (rows, self.k), torch.float32, x)
+        self.indices = _check_like(indices, "indices", (rows, self.k), torch.int64, x)
+        self.rest = None if rest is None else _check_like(rest, "rest", (rows,), torch.float32, x)
+        self.temperature, self.label_weight = _check_temperature(temperature), float(label_weight)
+        if not 0.0 <= self.label_weight <= 1.0:
+            raise ValueError("label_weight wants a number from 0 to 1, got %r" % label_weight)
+        if self.label_weight > 0 and labels is None:
+            raise ValueError("label_weight %g wants labels" % self.label_weight)
+        self.labels = None if labels is None else _check_like(labels, "labels", (rows,), torch.int64, x)
+        if reduction not in _REDUCTIONS:
+            raise ValueError("reduction wants one of %s, got %r" % (", ".join(_REDUCTIONS), reduction))
+        if reduction == "mean" and rows == 0:
+            raise ValueError("distillation: the mean over no rows")
+        check_device(x, "logits")
+        self.reduction = reduction
+
+    def forward(self):
+        x, rows, dev = self.x, self.rows, self.x.device
+        none = self.reduction == "none"
+        loss = torch.empty((rows,) if none else (), dtype=torch.float32, device=dev)
+        self.stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+        self.probs = torch.empty((rows, self.k), dtype=torch.float32, device=dev)
+        if rows == 0:
+            return loss if none else loss.zero_()
+        loss_rows = None if none else torch.empty((rows,), dtype=torch.float64, device=dev)
+        _launch((str(x.dtype), rows, self.ncls, self.k), "stgcn_distill_fwd", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(self.values),
+                L.ptr(self.indices), L.ptr(self.rest), L.ptr(self.labels), rows, self.ncls, self.k, self.temperature, self.label_weight,
+                _REDUCTIONS[self.reduction], L.ptr(loss), L.ptr(loss_rows), L.ptr(self.stats), L.ptr(self.probs), L.stream_ptr())
+        return loss
+
+    def backward(self, grad):
+        """d loss / d logits times grad (a float32 tensor on the device: one number, or one a row for "none"; None: 1)."""
+        x, rows = self.x, self.rows
+        dx = torch.empty((rows, self.ncls), dtype=x.dtype, device=x.device)
+        if rows:
+            _launch((str(x.dtype), rows, self.ncls, self.k), "stgcn_distill_bwd", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(self.indices),
+                    L.ptr(self.labels), L.ptr(self.stats), L.ptr(self.probs), L.ptr(grad), 1 if self.reduction == "none" else 0,
+                    1.0 / rows if self.reduction == "mean" else 1.0, rows, self.ncls, self.k, self.temperature, self.label_weight, L.ptr(dx),
+                    L.stream_ptr())
+        return dx
+
+
+def distillation(logits, values, indices, rest=None, labels=None, temperature=1.0, label_weight=0.0, reduction="mean"):
+    """Distillation from a teacher's top logits -> (loss, d loss / d logits), as cross_entropy returns its pair
+    (functional.distillation is the same loss as an autograd operator, with the formula)."""
+    if reduction == "none":
+        raise ValueError("ops.distillation returns the gradient of one number: reduction 'mean' or 'sum'")
+    call = DistillCall(logits, values, indices, rest, labels, temperature, label_weight, reduction)
+    return call.forward(), call.backward(None)
+
+
+def _row_parameter(v, name, dtype, rows, like, ok, want):
+    """(array or None, scalar) of a parameter that is one number or one a row."""
+    if torch.is_tensor(v):
+        return _check_like(v, name, (rows,), dtype, like), 0
+    if not ok(v):
+        raise ValueError("sample_labels: %s wants %s, got %r" % (name, want, v))
+    return None, v
+
+
+def sample_labels(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One label per row drawn from softmax(logits / temperature) with the random numbers u: (labels int64, logp float32).
+
+    Of the classes by descending score (ties by class): the first top_k (0: all); of these the shortest prefix that reaches
+    top_p of their mass; of these those at least min_p times as likely as the first.  The label is the first of what is
+    kept, by class number, at which the running mass exceeds u times the kept mass; logp is the log of its share.
+    temperature 0 answers the first class.  Each of the four is a number, or a tensor with one a row (float32; top_k
+    int32).  u: float32 [rows] in [0, 1).  A row whose scores are all -inf answers -1 (logp -inf); one with a NaN, or whose
+    own parameters are out of range, -1 (logp NaN)."""
+    x = _check_scores(logits)
+    rows, ncls = x.shape
+    u = _check_like(u, "u", (rows,), torch.float32, x)
+    tt, ts = _row_parameter(temperature, "temperature", torch.float32, rows, x, lambda v: 0.0 <= float(v) < 1e30, "a number >= 0")
+    kt, ks = _row_parameter(top_k, "top_k", torch.int32, rows, x, lambda v: int(v) == v and 0 <= v < 1 << 31, "a whole number >= 0")
+    pt, ps = _row_parameter(top_p, "top_p", torch.float32, rows, x, lambda v: 1e-37 < float(v) <= 1.0, "a number above 0, up to 1")
+    qt, qs = _row_parameter(min_p, "min_p", torch.float32, rows, x, lambda v: 0.0 <= float(v) <= 1.0, "a number from 0 to 1")
+    check_device(x, "logits")
+    labels = torch.empty((rows,), dtype=torch.int64, device=x.device)
+    logp = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    if rows:
+        _launch((str(x.dtype), rows, ncls), "stgcn_sample_labels", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(u), L.ptr(tt), float(ts),
+                L.ptr(kt), int(ks), L.ptr(pt), float(ps), L.ptr(qt), float(qs), L.ptr(labels), L.ptr(logp), rows, ncls, L.stream_ptr())
+    return labels, logp
+
+
 def sgd_step(params, grads, mom, lr, momentum, weight_decay, nesterov, first_step, grad_scale=1.0):
     L.call("stgcn_sgd_step", L.ptr(params), L.ptr(grads), L.ptr(mom), params.numel(), float(lr), float(momentum), float(weight_decay),
            1 if nesterov else 0, 1 if first_step else 0, float(grad_scale), L.stream_ptr())
