@@ -14,194 +14,534 @@
 
 namespace {
 
-constexpr int MAX_K = 256;
-constexpr int SEG = 65536;                    // classes per bit map (8 KB of LDS)
+constexpr int MAX_K = 256, EPL = MAX_K / 64;  // a row's entries: one wave's, EPL a lane
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.6931471805599453094;
 
-// What a row's forward leaves for its gradient: e^{z_j} = 2^{(x_j - xmax) c}, and the factors of the three sums.
+// What a row's forward leaves for its gradient: e^{z_j} = 2^{(x_j - xmax) c}, and the factors of the three sums.  xmax is
+// NaN for a row whose gradient is zero whatever it holds.
 struct RowStats { float xmax, gl, gr, g1; };   // gl = (1-w) T / S, gr = (1-w) T (1/S - p_r/S_r), g1 = w / sum e^x
 
 struct DistillArgs {
     const void* x; size_t stride;
     const float* val; const long long* idx; const float* rest; const long long* labels;
     double* loss_rows; float* loss; RowStats* stats; float* probs;
-    int n, k;
-    float c, c1;                               // log2(e) / T, log2(e)
+    void* dx; float scale;                     // of the gradient, where it is written
+    int rows, n, k;
+    float c, c1, fp, w1;                       // log2(e) / T, log2(e), (1 - w) T, w
     double T, w;
 };
 
-// Running (maximum, sum of 2^{(x - maximum) c}, the same at temperature 1) of one thread's scores.
-template <bool TWO> struct Online {
-    float m = -INFINITY, s = 0.f, s1 = 0.f;
-    __device__ __forceinline__ void raise(float to, float c, float c1) {
-        if (to > m) {
-            s *= m == -INFINITY ? 0.f : exp2_32((m - to) * c);
-            if constexpr (TWO) s1 *= m == -INFINITY ? 0.f : exp2_32((m - to) * c1);
-            m = to;
-        }
-    }
-    __device__ __forceinline__ void add(float x, float c, float c1) {      // x <= m, or m = -inf and x = -inf
-        if (x == -INFINITY) return;
-        s += exp2_32((x - m) * c);
-        if constexpr (TWO) s1 += exp2_32((x - m) * c1);
-    }
+// Waves that work on one row: W of them, and for W = 1 four rows share a workgroup and no barrier is needed.
+template <int W> __device__ __forceinline__ void group_sync() {
+    if constexpr (W == 1) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
+    else __syncthreads();
+}
+
+// ---- the teacher's side of a row, held by one wave -------------------------------------------------------------------
+struct Teacher {
+    int my[EPL]; float tv[EPL], xl[EPL];       // class (-1: none, or a class that an earlier entry has), score, student's score
+    double p[EPL];                             // the class's share; with duplicates their sum
+    double A, pr, own;                         // own: sum of p log p
+    bool any, bad;
 };
 
-template <typename T, bool TWO>
-__global__ __launch_bounds__(256) void distill_fwd_kernel(DistillArgs a) {
-    constexpr int VEC = ET<T>::VEC;
-    __shared__ uint32_t bits[SEG / 32 + 1];
-    __shared__ int li[MAX_K];
-    __shared__ double redd[4];
-    __shared__ float redf[4];
-    const size_t r = blockIdx.x;
-    const int tid = threadIdx.x, n = a.n, k = a.k;
-    const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
-
-    // the teacher: thread q holds entry q
-    int my = -1; bool bad = false; double tz = -INFINITY;
-    if (tid < k) {
-        const long long i = a.idx[r * k + tid];
-        bad = i >= n;
-        my = i < 0 || i >= n ? -1 : (int)i;
-        if (my >= 0) {
-            const float t = a.val[r * k + tid];
-            bad = !(t < INFINITY);
-            tz = bad ? -INFINITY : (double)t / a.T;
-        }
-        li[tid] = my;
+// Entries into registers (nothing waits for them yet).
+__device__ __forceinline__ void teacher_load(const DistillArgs& a, size_t r, int lane, long long* i, float* t) {
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        i[e] = -1; t[e] = 0.f;
+        if (lane + 64 * e < a.k) { i[e] = a.idx[r * a.k + lane + 64 * e]; t[e] = a.val[r * a.k + lane + 64 * e]; }
     }
-    const double rho = a.rest ? (double)a.rest[r] : -INFINITY;
-    const bool soft = a.w < 1.0;
-    const bool any = __syncthreads_or(my >= 0 && tz > -INFINITY) && soft;      // this row has a teacher
-    const bool any_bad = __syncthreads_or(bad) || (any && !(rho < INFINITY));
-    bool first = my >= 0;
-    for (int q = 0; q < tid && q < k; ++q) if (li[q] == my) first = false;
-    const double tmax = fmax(block_reduce<4>(tz, OpMax(), redd), any ? rho : -INFINITY);
-    double A = 0, p = 0, pr = 0;
+}
+
+// p, p_r and the sum of p log p, by one wave.  `rho` is only looked at where there is an entry.
+__device__ __forceinline__ void teacher_shares(const DistillArgs& a, const long long* i, const float* t, float rho32, Teacher& q) {
+    double z[EPL], m = -INFINITY;
+    bool bad = false, has = false;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        q.my[e] = i[e] >= 0 && i[e] < a.n ? (int)i[e] : -1;
+        q.p[e] = 0; z[e] = -INFINITY;
+        if (i[e] >= a.n) bad = true;
+        if (q.my[e] >= 0) {
+            if (!(t[e] < INFINITY)) bad = true;
+            else if (t[e] > -INFINITY) { z[e] = (double)t[e] / a.T; has = true; }
+        }
+        m = fmax(m, z[e]);
+    }
+    q.any = __ballot(has) != 0 && a.w < 1.0;
+    q.bad = __ballot(bad) != 0;
+    q.A = 0; q.pr = 0; q.own = 0;
+    if (!q.any) return;
+    const double rho = (double)rho32;
+    if (!(rho < INFINITY)) { q.bad = true; return; }
+    m = fmax(wave_reduce(m, OpMax()), rho);
+    double s = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) if (64 * e < a.k) { z[e] = z[e] > -INFINITY ? z[e] - m : -INFINITY; q.p[e] = exp(z[e]); s += q.p[e]; }
+    const double er = exp(rho - m);
+    s = wave_reduce(s, OpSum()) + er;
+    const double ls = log(s), inv = 1.0 / s;
+    q.A = m + ls; q.pr = er * inv;
+    double own = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) if (q.p[e] > 0) { q.p[e] *= inv; own += q.p[e] * (z[e] - ls); }
+    q.own = own;                               // this lane's
+    if (q.pr > 0) q.own += (threadIdx.x & 63) == 0 ? q.pr * (rho - m - ls) : 0.0;
+}
+
+// Entries of one class: the first keeps the sum of their p, the others leave the list.  Rare; `li` is MAX_K ints and `pk`
+// MAX_K doubles of LDS that only this wave uses.
+__device__ void teacher_merge(const DistillArgs& a, int lane, Teacher& q, int* li, double* pk) {
+    for (int e = 0; e < EPL; ++e) { li[lane + 64 * e] = q.my[e]; pk[lane + 64 * e] = q.p[e]; }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    for (int e = 0; e < EPL; ++e) {
+        if (q.my[e] < 0) continue;
+        const int at = lane + 64 * e;
+        double s = 0;
+        bool first = true;
+        for (int o = 0; o < a.k; ++o)
+            if (li[o] == q.my[e]) { if (o < at) first = false; s += pk[o]; }
+        if (first) q.p[e] = s; else { q.my[e] = -1; q.p[e] = 0; }
+    }
+}
+
+// ---- bit map of the listed classes -----------------------------------------------------------------------------------
+// Bit BIT0 + (class - base): a vector's bits lie within one byte (base = the first whole vector's class, or a vector's).
+constexpr int BIT0 = 16;
+template <typename T> __device__ __forceinline__ uint32_t vec_bits(const uint32_t* bits, int v) {
+    const int b = BIT0 + v * ET<T>::VEC;
+    const uint32_t byte = ((const uint8_t*)bits)[b >> 3];
+    return ET<T>::IS_BF16 ? byte : (byte >> (b & 7)) & 15u;
+}
+// listed classes of a vector become -inf
+template <typename T> __device__ __forceinline__ void drop_listed(i32x4& v, uint32_t b) {
+    if constexpr (ET<T>::IS_BF16) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w = (uint32_t)v[q];
+            if (b >> (2 * q) & 1) w = (w & 0xFFFF0000u) | 0xFF80u;
+            if (b >> (2 * q + 1) & 1) w = (w & 0xFFFFu) | 0xFF800000u;
+            v[q] = (int)w;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (b >> q & 1) v[q] = (int)0xFF800000u;
+    }
+}
+template <typename T> __device__ __forceinline__ i32x4 neg_inf_vec() {
+    const int w = ET<T>::IS_BF16 ? (int)0xFF80FF80u : (int)0xFF800000u;
+    i32x4 v = {w, w, w, w};
+    return v;
+}
+template <typename T> __device__ __forceinline__ float vec_max(const i32x4& v) {
+    float f[ET<T>::VEC];
+    unpack16<T>(v, f);
+    float m = f[0];
+#pragma unroll
+    for (int j = 1; j < ET<T>::VEC; ++j) m = fmaxf(m, f[j]);
+    return m;
+}
+
+// ---- loss and factors of a row from its sums -------------------------------------------------------------------------
+// In every thread; the loss (a few logarithms in 64 bits) in one.
+struct RowSums { double sr, sl, s1; };
+__device__ __forceinline__ RowStats row_factors(const DistillArgs& a, const RowSums& s, float xmax, bool any, bool hard, bool bad, double pr) {
+    const double S = s.sl + s.sr;
+    RowStats st = {xmax, 0.f, 0.f, 0.f};
     if (any) {
-        const double sum = block_reduce<4>(tid < k ? exp(tz - tmax) : 0.0, OpSum(), redd) + exp(rho - tmax);
-        A = tmax + log(sum);
-        p = exp(tz - A);
-        pr = exp(rho - A);
+        const double f = (1.0 - a.w) * a.T;
+        st.gl = (float)(f / S);
+        st.gr = (float)(f * (1.0 / S - (pr > 0 && s.sr > 0 ? pr / s.sr : 0.0)));
     }
-    long long y = -1;
-    if constexpr (TWO) y = a.labels[r];
-    else if (a.labels) y = a.labels[r];
-    const bool hard = a.w > 0.0 && y >= 0;
-    const bool bad_row = any_bad || (a.w > 0.0 && y >= n);
+    if (hard) st.g1 = (float)(a.w / s.s1);
+    if (bad || S != S || s.s1 != s.s1) st.gl = st.gr = st.g1 = NAN;
+    if (!bad && ((!any && !hard) || S == 0)) st.xmax = NAN;   // nothing to learn from, or no class to learn: zeros
+    return st;
+}
+// `terms` = sum of p (log p - z_k) over the entries, z relative to xmax, plus p_r log p_r
+__device__ __forceinline__ double row_loss(const DistillArgs& a, const RowSums& s, const RowStats& st, bool any, bool hard, double pr, double terms, float xy, float xmax) {
+    if (st.xmax != st.xmax) return 0.0;
+    if (st.gl != st.gl) return NAN;
+    double loss = 0;
+    if (any) {
+        // sum of p is 1 - p_r for the listed classes, so log S enters with weight 1 in all
+        double kl = terms + log(s.sl + s.sr);
+        if (pr > 0) kl -= pr * log(s.sr);
+        loss = (1.0 - a.w) * a.T * a.T * kl;
+    }
+    if (hard) loss += a.w * (log(s.s1) - ((double)xy - (double)xmax) * (double)a.c1 * LN2);
+    return loss;
+}
 
-    // the student: a running maximum and sums over the classes that are not listed
-    const float xl = first ? load_elem(x, my) : -INFINITY;
-    Online<TWO> o;
-    bool nan = xl != xl;
+template <typename T, bool TWO> struct Grad {
+    float m, c, c1, g1;
+    __device__ __forceinline__ float operator()(float x, float gz) const {
+        const float t = x - m, e = exp2_32(t * c);
+        if constexpr (TWO) return fmaf(gz, e, g1 * exp2_32(t * c1)); else return gz * e;   // one temperature: g1 is in gz
+    }
+};
+template <typename T, bool TWO> __device__ __forceinline__ i32x4 grad_vec(const i32x4& v, const Grad<T, TWO>& g, float gz) {
+    float f[ET<T>::VEC];
+    unpack16<T>(v, f);
+#pragma unroll
+    for (int j = 0; j < ET<T>::VEC; ++j) f[j] = g(f[j], gz);
+    return pack16<T>(f);
+}
+
+// One row by W waves, its scores held in registers (NV vectors a thread): read once, and with GRAD the gradient is
+// written from there, so loss and gradient cost one read and one write of the scores.
+// What the listed classes need (their student scores, p, the gradient at their places) is wave 0's.  The gradient is first
+// written as if no class were listed; behind a barrier the listed ones and the label are written over.
+template <typename T, int W, int NV, bool TWO, bool GRAD>
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(DistillArgs a) {
+    constexpr int VEC = ET<T>::VEC, G = W * 64, ROWS = W == 1 ? 4 : 1, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
+    __shared__ uint32_t bits_[ROWS][WORDS];
+    __shared__ int li_[ROWS][MAX_K];
+    __shared__ double pk_[ROWS][MAX_K];
+    __shared__ double rsum[4][W];
+    __shared__ float rmax[W];
+    __shared__ double t_pr; __shared__ int t_flags;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x, sub = W == 1 ? wave : 0;
+    const size_t r = (size_t)blockIdx.x * ROWS + sub;
+    if (W == 1 && r >= (size_t)a.rows) return;
+    const bool lead = W == 1 || wave == 0;
+    uint32_t* bits = bits_[sub];
+    const int n = a.n;
+    const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
     const RowSpan<T> sp(x, n);
-    for (int seg = 0; seg < n; seg += SEG) {
-        __syncthreads();
-        for (int i = tid; i < SEG / 32 + 1; i += 256) bits[i] = 0;
-        __syncthreads();
-        if (first && my >= seg && my < seg + SEG) atomicOr(&bits[(my - seg) >> 5], 1u << ((my - seg) & 31));
-        __syncthreads();
-        const int end = min(seg + SEG, n);
-        for (int j = seg + tid; j < end; j += 256) {
-            if (bits[(j - seg) >> 5] >> ((j - seg) & 31) & 1) continue;
-            const float v = load_elem(x, j);
-            nan |= v != v;
-            o.raise(v, a.c, a.c1);
-            o.add(v, a.c, a.c1);
+
+    long long ei[EPL]; float et[EPL]; float rho = -INFINITY;
+    if (lead) { teacher_load(a, r, lane, ei, et); if (a.rest) rho = a.rest[r]; }
+    const long long y = a.labels ? a.labels[r] : -1;
+    i32x4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>();
+    float xe = tid < sp.edge ? load_elem(x, sp.edge_at(tid)) : -INFINITY;
+    for (int i = tid; i < WORDS; i += G) bits[i] = 0;
+    group_sync<W>();
+
+    Teacher q;
+    const bool hard = a.w > 0.0 && y >= 0 && y < n;
+    float xy = 0.f;
+    if (lead) {
+        teacher_shares(a, ei, et, rho, q);
+        bool dup = false;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            if (q.my[e] >= 0) {
+                const int b = BIT0 + q.my[e] - sp.head;
+                dup |= (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1;
+            }
+        if (__ballot(dup)) teacher_merge(a, lane, q, li_[sub], pk_[sub]);
+        if (a.w > 0.0 && y >= n) q.bad = true;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_elem(x, q.my[e]) : -INFINITY;
+        if (hard) xy = load_elem(x, (size_t)y);
+        if (W > 1 && lane == 0) { t_pr = q.pr; t_flags = (q.any ? 1 : 0) | (q.bad ? 2 : 0); }
+    }
+    group_sync<W>();
+
+    // the maximum; listed classes leave the registers
+    float m = -INFINITY;
+    if (xe > -INFINITY || xe != xe) {
+        const int b = BIT0 + sp.edge_at(tid) - sp.head;
+        if (bits[b >> 5] >> (b & 31) & 1) xe = -INFINITY;
+        m = fmaxf(m, xe);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (i * G < sp.nvec) {
+            const uint32_t b = vec_bits<T>(bits, i * G + tid);
+            if (b) drop_listed<T>(v[i], b);
+            m = fmaxf(m, vec_max<T>(v[i]));
         }
     }
-    nan = __syncthreads_or(nan);
-    const float xmax = block_reduce<4>(fmaxf(o.m, xl), OpFMax(), redf);
-    double sr = 0, sl = 0, s1 = 0;
-    if (o.m > -INFINITY) {
-        sr = (double)o.s * (double)exp2_32((o.m - xmax) * a.c);
-        if constexpr (TWO) s1 = (double)o.s1 * (double)exp2_32((o.m - xmax) * a.c1);
+    if (lead) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) m = fmaxf(m, q.xl[e]);
     }
-    if (xl > -INFINITY) {
-        sl = (double)exp2_32((xl - xmax) * a.c);
-        if constexpr (TWO) s1 += (double)exp2_32((xl - xmax) * a.c1);
+    m = wave_reduce(m, OpFMax());
+    if constexpr (W > 1) {
+        if (lane == 0) rmax[wave] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = fmaxf(m, rmax[w]);
     }
-    sr = block_reduce<4>(sr, OpSum(), redd);
-    sl = block_reduce<4>(sl, OpSum(), redd);
-    if constexpr (TWO) s1 = block_reduce<4>(s1, OpSum(), redd);
-    const double S = sl + sr;
-    if constexpr (!TWO) s1 = S;                            // temperature 1: one sum serves both terms
-    double term = 0;
-    if (any && p > 0) {
-        const double lq = ((double)load_elem(x, my < 0 ? 0 : my) - (double)xmax) * (double)a.c * LN2 - log(S);
-        if (my >= 0) term = p * (log(p) - lq);
+    const float xmax = m == -INFINITY ? 0.f : m;
+
+    // the sums
+    float s = exp2_32((xe - xmax) * a.c), s1 = TWO ? exp2_32((xe - xmax) * a.c1) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (i * G < sp.nvec) {
+            float f[VEC];
+            unpack16<T>(v[i], f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float t = f[j] - xmax;
+                s += exp2_32(t * a.c);
+                if constexpr (TWO) s1 += exp2_32(t * a.c1);
+            }
+        }
     }
-    double kl = block_reduce<4>(term, OpSum(), redd);
-    // duplicates: the first occurrence carries the sum
+    RowSums sum = {wave_reduce((double)s, OpSum()), 0, TWO ? wave_reduce((double)s1, OpSum()) : 0.0};
+    double terms = 0;
+    if (lead) {
+        double sl = 0, sl1 = 0, t = q.any ? q.own : 0.0;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e)
+            if (64 * e < a.k && q.my[e] >= 0) {
+                const float d = q.xl[e] - xmax;
+                sl += (double)exp2_32(d * a.c);
+                if constexpr (TWO) sl1 += (double)exp2_32(d * a.c1);
+                if (q.p[e] > 0) t -= q.p[e] * ((double)q.xl[e] - (double)xmax) * (double)a.c * LN2;
+            }
+        sum.sl = wave_reduce(sl, OpSum());
+        if constexpr (TWO) sum.s1 += wave_reduce(sl1, OpSum());
+        terms = wave_reduce(t, OpSum());
+    }
+    bool any = q.any, bad = q.bad;
+    double pr = q.pr;
+    if constexpr (W > 1) {
+        if (lane == 0) { rsum[0][wave] = sum.sr; rsum[1][wave] = sum.s1; if (wave == 0) rsum[2][0] = sum.sl; }
+        __syncthreads();
+        sum = {0, rsum[2][0], 0};
+#pragma unroll
+        for (int w = 0; w < W; ++w) { sum.sr += rsum[0][w]; if constexpr (TWO) sum.s1 += rsum[1][w]; }
+        any = t_flags & 1; bad = t_flags & 2; pr = t_pr;
+    }
+    if constexpr (!TWO) sum.s1 = sum.sl + sum.sr;
+    const RowStats st = row_factors(a, sum, xmax, any, hard, bad, pr);
+    const bool empty = st.xmax != st.xmax;
+    if (lead && lane == 0) {
+        const double loss = row_loss(a, sum, st, any, hard, pr, terms, xy, xmax);
+        if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
+        if constexpr (!GRAD) a.stats[r] = st;
+    }
+    if constexpr (!GRAD) {
+        if (lead) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) if (lane + 64 * e < a.k) a.probs[r * a.k + lane + 64 * e] = q.my[e] >= 0 ? (float)q.p[e] : -1.f;
+        }
+    } else {
+        T* dx = (T*)a.dx + r * (size_t)n;
+        const Grad<T, TWO> g = {empty ? 0.f : st.xmax, a.c, a.c1, st.g1 * a.scale};
+        const float gr = (TWO ? st.gr : st.gr + st.g1) * a.scale, gl = (TWO ? st.gl : st.gl + st.g1) * a.scale;
+        const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i * G + tid < sp.nvec) {
+                i32x4 o = grad_vec<T, TWO>(v[i], g, gr);
+                if (empty) o = zero16();
+                const int at = sp.vec_at(i * G + tid);
+                if (same) store_vec(dx, at, o);
+                else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if constexpr (ET<T>::IS_BF16) ((uint16_t*)dx)[at + j] = (uint16_t)((uint32_t)o[j >> 1] >> (16 * (j & 1)));
+                        else ((int*)dx)[at + j] = o[j];
+                }
+            }
+        }
+        if (tid < sp.edge) store_elem(dx, sp.edge_at(tid), empty ? 0.f : g(xe, gr));
+        group_sync<W>();
+        if (lead && !empty) {
+            const float fp = a.fp * a.scale, w = a.w1 * a.scale;
+            bool mine = false;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e)
+                if (q.my[e] >= 0) {
+                    float d = g(q.xl[e], gl) - fp * (float)q.p[e];
+                    if (hard && q.my[e] == (int)y) { d -= w; mine = true; }
+                    store_elem(dx, q.my[e], d);
+                }
+            if (hard && !__ballot(mine) && lane == 0) store_elem(dx, (size_t)y, g(xy, gr) - w);
+        }
+    }
+}
+
+// A row that does not fit in registers: segment after segment, every thread with a running maximum and sums relative to
+// it.  Forward only; the gradient then reads the scores a second time (distill_bwd_kernel).
+template <typename T, bool TWO>
+__global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
+    constexpr int VEC = ET<T>::VEC, W = 16, G = 1024, NV = 64 / VEC, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
+    __shared__ uint32_t bits[WORDS];
+    __shared__ int li[MAX_K];
     __shared__ double pk[MAX_K];
-    if (tid < k) pk[tid] = my >= 0 ? p : 0.0;
-    __syncthreads();
-    if (tid < k && a.probs) {
-        double t = 0;
-        if (first) for (int q = tid; q < k; ++q) if (li[q] == my) t += pk[q];
-        a.probs[r * k + tid] = first ? (float)t : -1.f;
+    __shared__ double rsum[3][W];
+    __shared__ float rmax[W];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = threadIdx.x, n = a.n;
+    const size_t r = blockIdx.x;
+    const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
+    const RowSpan<T> sp(x, n);
+    const bool lead = wave == 0;
+    const long long y = a.labels ? a.labels[r] : -1;
+    const bool hard = a.w > 0.0 && y >= 0 && y < n;
+    Teacher q;
+    float m = -INFINITY, s = 0.f, s1 = 0.f, xy = 0.f;
+    auto raise = [&](float to) {
+        if (to > m) {
+            const float up = m == -INFINITY ? 0.f : exp2_32((m - to) * a.c);
+            s *= up;
+            if constexpr (TWO) s1 *= m == -INFINITY ? 0.f : exp2_32((m - to) * a.c1);
+            m = to;
+        }
+    };
+    auto add = [&](float f) {
+        const float t = f - (m == -INFINITY ? 0.f : m);
+        s += exp2_32(t * a.c);
+        if constexpr (TWO) s1 += exp2_32(t * a.c1);
+    };
+    if (lead) {
+        long long ei[EPL]; float et[EPL];
+        teacher_load(a, r, lane, ei, et);
+        teacher_shares(a, ei, et, a.rest ? a.rest[r] : -INFINITY, q);
+        if (a.w > 0.0 && y >= n) q.bad = true;
+        teacher_merge(a, lane, q, li, pk);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_elem(x, q.my[e]) : -INFINITY;
+        if (hard) xy = load_elem(x, (size_t)y);
     }
-    if (tid == 0) {
-        double loss = 0;
-        RowStats st = {xmax, 0.f, 0.f, 0.f};
-        if (any) {
-            if (pr > 0) kl += pr * (log(pr) - log(sr) + log(S));
-            loss += (1.0 - a.w) * a.T * a.T * kl;
-            st.gl = (float)((1.0 - a.w) * a.T / S);
-            st.gr = (float)((1.0 - a.w) * a.T * (1.0 / S - (pr > 0 && sr > 0 ? pr / sr : 0.0)));
+    for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NV) {
+        // classes of this segment: [c0, c1), the row's edges with the first one
+        const int base = sp.vec_at(v0);
+        __syncthreads();
+        for (int i = tid; i < WORDS; i += G) bits[i] = 0;
+        __syncthreads();
+        if (lead) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                const int b = BIT0 + q.my[e] - base;
+                if (q.my[e] >= base && q.my[e] < base + G * NV * VEC) atomicOr(&bits[b >> 5], 1u << (b & 31));
+            }
         }
-        if (hard && y < n) {
-            loss += a.w * (log(s1) - ((double)load_elem(x, (size_t)y) - (double)xmax) * (double)a.c1 * LN2);
-            st.g1 = (float)(a.w / s1);
+        __syncthreads();
+        if (v0 == 0 && tid < sp.edge) {
+            const int j = sp.edge_at(tid);
+            bool is_listed = false;
+            for (int o = 0; o < a.k; ++o) is_listed |= li[o] == j;
+            if (!is_listed) { const float f = load_elem(x, j); raise(f); add(f); }
         }
-        const bool empty = (!any && !hard && !bad_row) || (xmax == -INFINITY && !nan && !bad_row);
-        if (bad_row || nan) { loss = NAN; st.gl = st.gr = st.g1 = NAN; }
-        if (empty) { loss = 0; st.xmax = NAN; }            // nothing to learn from, or no class to learn: zeros
+        i32x4 v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = v0 + i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(v0 + i * G + tid)) : neg_inf_vec<T>();
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t b = vec_bits<T>(bits, i * G + tid);
+            if (b) drop_listed<T>(v[i], b);
+            top = fmaxf(top, vec_max<T>(v[i]));
+        }
+        raise(top);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float f[VEC];
+            unpack16<T>(v[i], f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) add(f[j]);
+        }
+    }
+    float all = m;
+    if (lead) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) all = fmaxf(all, q.xl[e]);
+    }
+    all = block_reduce<W>(all, OpFMax(), rmax);
+    const float xmax = all == -INFINITY ? 0.f : all;
+    const bool none = m == -INFINITY;              // then s is 0, or NaN
+    RowSums sum;
+    sum.sr = block_reduce<W>((double)s * (none ? 1.0 : (double)exp2_32((m - xmax) * a.c)), OpSum(), rsum[0]);
+    sum.s1 = TWO ? block_reduce<W>((double)s1 * (none ? 1.0 : (double)exp2_32((m - xmax) * a.c1)), OpSum(), rsum[1]) : 0.0;
+    if (!lead) return;
+    double sl = 0, sl1 = 0, terms = q.any ? q.own : 0.0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e)
+        if (q.my[e] >= 0) {
+            const float d = q.xl[e] - xmax;
+            sl += (double)exp2_32(d * a.c);
+            if constexpr (TWO) sl1 += (double)exp2_32(d * a.c1);
+            if (q.p[e] > 0) terms -= q.p[e] * ((double)q.xl[e] - (double)xmax) * (double)a.c * LN2;
+        }
+    sum.sl = wave_reduce(sl, OpSum());
+    sum.s1 = TWO ? sum.s1 + wave_reduce(sl1, OpSum()) : sum.sl + sum.sr;
+    terms = wave_reduce(terms, OpSum());
+    const RowStats st = row_factors(a, sum, xmax, q.any, hard, q.bad, q.pr);
+    if (lane == 0) {
+        const double loss = row_loss(a, sum, st, q.any, hard, q.pr, terms, xy, xmax);
+        if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
         a.stats[r] = st;
-        if (a.loss_rows) a.loss_rows[r] = loss;
-        if (a.loss) a.loss[r] = (float)loss;
     }
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) if (lane + 64 * e < a.k) a.probs[r * a.k + lane + 64 * e] = q.my[e] >= 0 ? (float)q.p[e] : -1.f;
 }
 
 struct GradArgs {
     const void* x; size_t stride;
     const long long* idx; const long long* labels; const RowStats* stats; const float* probs;
     const float* g; int g_per_row; float scale; void* dx;
-    int n, k; float c, c1, fp, w;              // fp = (1 - w) T
+    int rows, n, k; float c, c1, fp, w;        // fp = (1 - w) T
 };
 
-template <typename T, bool TWO>
+// The gradient from a forward's factors.  W waves a piece of NV vectors a thread; blockIdx.x pieces of blockIdx.y-th rows
+// (W = 1: four rows a workgroup, one piece each).  Written as if nothing were listed, the listed classes of the piece and
+// the label over it.
+template <typename T, int W, int NV, bool TWO>
 __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
-    const size_t r = blockIdx.x;
-    const int tid = threadIdx.x, n = a.n, k = a.k;
+    constexpr int VEC = ET<T>::VEC, G = W * 64;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
+    const size_t r = W == 1 ? (size_t)blockIdx.x * 4 + wave : (size_t)blockIdx.y + (size_t)blockIdx.z * 65535;
+    if (r >= (size_t)a.rows) return;
+    const int n = a.n, v0 = W == 1 ? 0 : blockIdx.x * (G * NV);
     const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
-    T* dx = (T*)((char*)a.dx + r * (size_t)n * ET<T>::ES);
+    T* dx = (T*)a.dx + r * (size_t)n;
+    const RowSpan<T> sp(x, n);
+    i32x4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) if (v0 + i * G + tid < sp.nvec) v[i] = load_vec(x, sp.vec_at(v0 + i * G + tid));
     const RowStats st = a.stats[r];
     const bool empty = st.xmax != st.xmax;
-    const float g = (a.g ? a.g[a.g_per_row ? r : 0] : 1.f) * a.scale;
+    const float up = (a.g ? a.g[a.g_per_row ? r : 0] : 1.f) * a.scale;
     const long long y = a.labels ? a.labels[r] : -1;
-    auto grad = [&](float v, float gz) {
-        const float t = v - st.xmax;
-        const float e = exp2_32(t * a.c);
-        return (TWO ? gz * e + st.g1 * exp2_32(t * a.c1) : (gz + st.g1) * e) * g;
-    };
-    for (int j = tid; j < n; j += 256) store_elem(dx, j, empty ? 0.f : grad(load_elem(x, j), st.gr));
-    __syncthreads();
-    if (empty) return;
-    bool y_listed = false;
-    if (tid < k) {
-        const float p = a.probs[r * k + tid];
-        if (p >= 0.f) {
-            const long long j = a.idx[r * k + tid];
-            float v = grad(load_elem(x, (size_t)j), st.gl) - a.fp * p * g;
-            if (j == y && a.w > 0.f) { v -= a.w * g; y_listed = true; }
-            store_elem(dx, (size_t)j, v);
+    const bool hard = a.w > 0.f && y >= 0 && y < n;
+    const Grad<T, TWO> g = {empty ? 0.f : st.xmax, a.c, a.c1, st.g1 * up};
+    const float gr = (TWO ? st.gr : st.gr + st.g1) * up, gl = (TWO ? st.gl : st.gl + st.g1) * up;
+    const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (v0 + i * G + tid < sp.nvec) {
+            i32x4 o = grad_vec<T, TWO>(v[i], g, gr);
+            if (empty) o = zero16();
+            const int at = sp.vec_at(v0 + i * G + tid);
+            if (same) store_vec(dx, at, o);
+            else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if constexpr (ET<T>::IS_BF16) ((uint16_t*)dx)[at + j] = (uint16_t)((uint32_t)o[j >> 1] >> (16 * (j & 1)));
+                    else ((int*)dx)[at + j] = o[j];
+            }
         }
     }
-    y_listed = __syncthreads_or(y_listed);
-    if (tid == 0 && a.w > 0.f && y >= 0 && y < n && !y_listed)
-        store_elem(dx, (size_t)y, grad(load_elem(x, (size_t)y), st.gr) - a.w * g);
+    if (v0 == 0 && tid < sp.edge) { const int j = sp.edge_at(tid); store_elem(dx, j, empty ? 0.f : g(load_elem(x, j), gr)); }
+    if (empty) return;
+    group_sync<W>();
+    // the classes of this piece; the row's edges belong to piece 0
+    const int lo = sp.vec_at(v0), hi = min(lo + G * NV * VEC, sp.vec_at(sp.nvec));
+    auto here = [&](long long j) { return (j >= lo && j < hi) || (v0 == 0 && (j < sp.head || j >= sp.vec_at(sp.nvec))); };
+    bool mine = false;
+    for (int e = tid; e < a.k; e += G) {
+        const float p = a.probs[r * a.k + e];
+        if (p < 0.f) continue;
+        const long long j = a.idx[r * a.k + e];
+        if (j < 0 || j >= n || !here(j)) continue;
+        float d = g(load_elem(x, (size_t)j), gl) - a.fp * p * up;
+        if (hard && j == y) { d -= a.w * up; mine = true; }
+        store_elem(dx, (size_t)j, d);
+    }
+    if (!hard || !here(y)) return;
+    if constexpr (W == 1) mine = __ballot(mine) != 0; else mine = __syncthreads_or(mine);
+    if (tid == 0 && !mine) store_elem(dx, (size_t)y, g(load_elem(x, (size_t)y), gr) - a.w * up);
 }
 
 // Sum of the rows' losses, added in row order within a thread and by fixed butterflies: the same bits every run.
@@ -218,6 +558,49 @@ bool bad_common(int dtype, const void* x, size_t stride, const void* idx, int ro
         || k < 1 || k > MAX_K || !(T > 0.0) || !(T < 1e30) || !(w >= 0.0) || !(w <= 1.0);
 }
 
+// The widest row that fits in registers: 8 waves of 16 vectors a lane (64 registers of scores).
+template <typename T> constexpr int row_fits() { return 512 * 16 * ET<T>::VEC; }
+
+template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a, hipStream_t s) {
+    constexpr int VEC = ET<T>::VEC;
+    const int nv = a.n / VEC;                      // at most, whatever the alignment
+    const unsigned rows = (unsigned)a.rows, quads = (unsigned)((a.rows + 3) / 4);
+    if (nv <= 64) distill_row_kernel<T, 1, 1, TWO, GRAD><<<quads, 256, 0, s>>>(a);
+    else if (nv <= 128) distill_row_kernel<T, 1, 2, TWO, GRAD><<<quads, 256, 0, s>>>(a);
+    else if (nv <= 256) distill_row_kernel<T, 1, 4, TWO, GRAD><<<quads, 256, 0, s>>>(a);
+    else if (nv <= 1024) distill_row_kernel<T, 4, 4, TWO, GRAD><<<rows, 256, 0, s>>>(a);
+    else if (nv <= 2048) distill_row_kernel<T, 4, 8, TWO, GRAD><<<rows, 256, 0, s>>>(a);
+    else if (nv <= 4096) distill_row_kernel<T, 8, 8, TWO, GRAD><<<rows, 512, 0, s>>>(a);
+    else distill_row_kernel<T, 8, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
+}
+template <typename T> void launch_fwd(const DistillArgs& a, bool two, hipStream_t s) {
+    if (a.n <= row_fits<T>()) { if (two) launch_rows<T, true, false>(a, s); else launch_rows<T, false, false>(a, s); }
+    else if (two) distill_stream_kernel<T, true><<<a.rows, 1024, 0, s>>>(a);
+    else distill_stream_kernel<T, false><<<a.rows, 1024, 0, s>>>(a);
+}
+template <typename T, bool TWO> void launch_bwd(const GradArgs& a, hipStream_t s) {
+    constexpr int VEC = ET<T>::VEC;
+    const int nv = a.n / VEC > 0 ? a.n / VEC : 1;
+    const unsigned quads = (unsigned)((a.rows + 3) / 4);
+    if (nv <= 64) distill_bwd_kernel<T, 1, 1, TWO><<<quads, 256, 0, s>>>(a);
+    else if (nv <= 256) distill_bwd_kernel<T, 1, 4, TWO><<<quads, 256, 0, s>>>(a);
+    else {
+        const dim3 grid((nv + 1023) / 1024, a.rows < 65535 ? a.rows : 65535, (a.rows + 65534) / 65535);
+        distill_bwd_kernel<T, 4, 4, TWO><<<grid, 256, 0, s>>>(a);
+    }
+}
+
+DistillArgs fwd_args(const void* logits, size_t row_stride, const float* values, const int64_t* indices, const float* rest, const int64_t* labels,
+                     int rows, int ncls, int k, double temperature, double label_weight) {
+    return {logits, row_stride, values, (const long long*)indices, rest, label_weight > 0 ? (const long long*)labels : nullptr,
+            nullptr, nullptr, nullptr, nullptr, nullptr, 1.f, rows, ncls, k, (float)(LOG2E / temperature), (float)LOG2E,
+            (float)((1.0 - label_weight) * temperature), (float)label_weight, temperature, label_weight};
+}
+int loss_sum(const double* loss_rows, int rows, int reduction, float* loss, hipStream_t s) {
+    if (reduction) loss_sum_kernel<<<1, 1024, 0, s>>>(loss_rows, rows, reduction == 1 ? 1.0 / rows : 1.0, loss);
+    return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
+}
+
 }  // namespace
 
 extern "C" int stgcn_distill_fwd(int dtype, const void* logits, size_t row_stride, const float* values, const int64_t* indices,
@@ -225,18 +608,11 @@ extern "C" int stgcn_distill_fwd(int dtype, const void* logits, size_t row_strid
                                  double label_weight, int reduction, float* loss, double* loss_rows, float* stats, float* probs, void* stream) {
     if (bad_common(dtype, logits, row_stride, indices, rows, ncls, k, temperature, label_weight) || !values || !loss || !stats || !probs
         || (label_weight > 0 && !labels) || reduction < 0 || reduction > 2 || (reduction && !loss_rows)) return STGCN_ERR_ARG;
-    DistillArgs a = {logits, row_stride, values, (const long long*)indices, rest, label_weight > 0 ? (const long long*)labels : nullptr,
-                     reduction ? loss_rows : nullptr, reduction ? nullptr : loss, (RowStats*)stats, probs, ncls, k,
-                     (float)(LOG2E / temperature), (float)LOG2E, temperature, label_weight};
+    DistillArgs a = fwd_args(logits, row_stride, values, indices, rest, labels, rows, ncls, k, temperature, label_weight);
+    a.loss_rows = reduction ? loss_rows : nullptr; a.loss = loss; a.stats = (RowStats*)stats; a.probs = probs;
     const bool two = label_weight > 0 && temperature != 1.0;
-    const hipStream_t s = (hipStream_t)stream;
-    if (dtype == STGCN_BF16) {
-        if (two) distill_fwd_kernel<bf16, true><<<rows, 256, 0, s>>>(a); else distill_fwd_kernel<bf16, false><<<rows, 256, 0, s>>>(a);
-    } else {
-        if (two) distill_fwd_kernel<float, true><<<rows, 256, 0, s>>>(a); else distill_fwd_kernel<float, false><<<rows, 256, 0, s>>>(a);
-    }
-    if (reduction) loss_sum_kernel<<<1, 1024, 0, s>>>(loss_rows, rows, reduction == 1 ? 1.0 / rows : 1.0, loss);
-    return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
+    if (dtype == STGCN_BF16) launch_fwd<bf16>(a, two, (hipStream_t)stream); else launch_fwd<float>(a, two, (hipStream_t)stream);
+    return loss_sum(loss_rows, rows, reduction, loss, (hipStream_t)stream);
 }
 
 extern "C" int stgcn_distill_bwd(int dtype, const void* logits, size_t row_stride, const int64_t* indices, const int64_t* labels,
@@ -245,14 +621,31 @@ extern "C" int stgcn_distill_bwd(int dtype, const void* logits, size_t row_strid
     if (bad_common(dtype, logits, row_stride, indices, rows, ncls, k, temperature, label_weight) || !stats || !probs || !dlogits
         || (label_weight > 0 && !labels)) return STGCN_ERR_ARG;
     GradArgs a = {logits, row_stride, (const long long*)indices, label_weight > 0 ? (const long long*)labels : nullptr, (const RowStats*)stats,
-                  probs, grad, grad_per_row, (float)scale, dlogits, ncls, k, (float)(LOG2E / temperature), (float)LOG2E,
+                  probs, grad, grad_per_row, (float)scale, dlogits, rows, ncls, k, (float)(LOG2E / temperature), (float)LOG2E,
                   (float)((1.0 - label_weight) * temperature), (float)label_weight};
     const bool two = label_weight > 0 && temperature != 1.0;
     const hipStream_t s = (hipStream_t)stream;
-    if (dtype == STGCN_BF16) {
-        if (two) distill_bwd_kernel<bf16, true><<<rows, 256, 0, s>>>(a); else distill_bwd_kernel<bf16, false><<<rows, 256, 0, s>>>(a);
-    } else {
-        if (two) distill_bwd_kernel<float, true><<<rows, 256, 0, s>>>(a); else distill_bwd_kernel<float, false><<<rows, 256, 0, s>>>(a);
-    }
+    if (dtype == STGCN_BF16) { if (two) launch_bwd<bf16, true>(a, s); else launch_bwd<bf16, false>(a, s); }
+    else { if (two) launch_bwd<float, true>(a, s); else launch_bwd<float, false>(a, s); }
     return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
+}
+
+extern "C" int stgcn_distill_step(int dtype, const void* logits, size_t row_stride, const float* values, const int64_t* indices,
+                                  const float* rest, const int64_t* labels, int rows, int ncls, int k, double temperature,
+                                  double label_weight, int reduction, float* loss, double* loss_rows, float* stats, float* probs, void* dlogits, void* stream) {
+    if (bad_common(dtype, logits, row_stride, indices, rows, ncls, k, temperature, label_weight) || !values || !loss || !loss_rows || !stats
+        || !probs || !dlogits || (label_weight > 0 && !labels) || (reduction != 1 && reduction != 2)) return STGCN_ERR_ARG;
+    DistillArgs a = fwd_args(logits, row_stride, values, indices, rest, labels, rows, ncls, k, temperature, label_weight);
+    a.loss_rows = loss_rows; a.dx = dlogits; a.scale = reduction == 1 ? (float)(1.0 / rows) : 1.f;
+    a.stats = (RowStats*)stats; a.probs = probs;
+    const bool two = label_weight > 0 && temperature != 1.0;
+    const hipStream_t s = (hipStream_t)stream;
+    if (ncls > (dtype == STGCN_BF16 ? row_fits<bf16>() : row_fits<float>())) {
+        if (dtype == STGCN_BF16) launch_fwd<bf16>(a, two, s); else launch_fwd<float>(a, two, s);
+        const int rc = stgcn_distill_bwd(dtype, logits, row_stride, indices, labels, stats, probs, nullptr, 0, reduction == 1 ? 1.0 / rows : 1.0, rows, ncls, k,
+                                         temperature, label_weight, dlogits, stream);
+        if (rc != STGCN_OK) return rc;
+    } else if (dtype == STGCN_BF16) { if (two) launch_rows<bf16, true, true>(a, s); else launch_rows<bf16, false, true>(a, s); }
+    else { if (two) launch_rows<float, true, true>(a, s); else launch_rows<float, false, true>(a, s); }
+    return loss_sum(loss_rows, rows, reduction, loss, s);
 }

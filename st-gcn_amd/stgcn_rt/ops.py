@@ -574,19 +574,38 @@ class DistillCall:
         check_device(x, "logits")
         self.reduction = reduction
 
-    def forward(self):
-        x, rows, dev = self.x, self.rows, self.x.device
-        none = self.reduction == "none"
-        loss = torch.empty((rows,) if none else (), dtype=torch.float32, device=dev)
+    def _buffers(self):
+        rows, dev = self.rows, self.x.device
         self.stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
         self.probs = torch.empty((rows, self.k), dtype=torch.float32, device=dev)
+        return torch.empty((rows,), dtype=torch.float64, device=dev)
+
+    def _inputs(self):
+        x = self.x
+        return (L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(self.values), L.ptr(self.indices), L.ptr(self.rest), L.ptr(self.labels),
+                self.rows, self.ncls, self.k, self.temperature, self.label_weight, _REDUCTIONS[self.reduction])
+
+    def forward(self):
+        rows, dev = self.rows, self.x.device
+        loss_rows = self._buffers()
+        loss = torch.empty((rows,) if self.reduction == "none" else (), dtype=torch.float32, device=dev)
         if rows == 0:
-            return loss if none else loss.zero_()
-        loss_rows = None if none else torch.empty((rows,), dtype=torch.float64, device=dev)
-        _launch((str(x.dtype), rows, self.ncls, self.k), "stgcn_distill_fwd", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(self.values),
-                L.ptr(self.indices), L.ptr(self.rest), L.ptr(self.labels), rows, self.ncls, self.k, self.temperature, self.label_weight,
-                _REDUCTIONS[self.reduction], L.ptr(loss), L.ptr(loss_rows), L.ptr(self.stats), L.ptr(self.probs), L.stream_ptr())
+            return loss if self.reduction == "none" else loss.zero_()
+        _launch((str(self.x.dtype), rows, self.ncls, self.k), "stgcn_distill_fwd", *self._inputs(), L.ptr(loss), L.ptr(loss_rows),
+                L.ptr(self.stats), L.ptr(self.probs), L.stream_ptr())
         return loss
+
+    def step(self):
+        """(loss, d loss / d logits) of one call."""
+        rows, dev = self.rows, self.x.device
+        loss_rows = self._buffers()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        dx = torch.empty((rows, self.ncls), dtype=self.x.dtype, device=dev)
+        if rows == 0:
+            return loss.zero_(), dx
+        _launch((str(self.x.dtype), rows, self.ncls, self.k), "stgcn_distill_step", *self._inputs(), L.ptr(loss), L.ptr(loss_rows),
+                L.ptr(self.stats), L.ptr(self.probs), L.ptr(dx), L.stream_ptr())
+        return loss, dx
 
     def backward(self, grad):
         """d loss / d logits times grad (a float32 tensor on the device: one number, or one a row for "none"; None: 1)."""
@@ -605,8 +624,7 @@ def distillation(logits, values, indices, rest=None, labels=None, temperature=1.
     (functional.distillation is the same loss as an autograd operator, with the formula)."""
     if reduction == "none":
         raise ValueError("ops.distillation returns the gradient of one number: reduction 'mean' or 'sum'")
-    call = DistillCall(logits, values, indices, rest, labels, temperature, label_weight, reduction)
-    return call.forward(), call.backward(None)
+    return DistillCall(logits, values, indices, rest, labels, temperature, label_weight, reduction).step()
 
 
 def _row_parameter(v, name, dtype, rows, like, ok, want):
