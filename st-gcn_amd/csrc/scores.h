@@ -27,6 +27,35 @@ template <typename T> __device__ __forceinline__ void store_vec(T* row, int at, 
     *reinterpret_cast<i32x4*>((char*)row + (size_t)at * ET<T>::ES) = raw;
 }
 
+// the elements of a vector whose bit is set become -inf
+template <typename T> __device__ __forceinline__ void drop_listed(i32x4& v, uint32_t b) {
+    if constexpr (ET<T>::IS_BF16) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w = (uint32_t)v[q];
+            if (b >> (2 * q) & 1) w = (w & 0xFFFF0000u) | 0xFF80u;
+            if (b >> (2 * q + 1) & 1) w = (w & 0xFFFFu) | 0xFF800000u;
+            v[q] = (int)w;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) if (b >> q & 1) v[q] = (int)0xFF800000u;
+    }
+}
+template <typename T> __device__ __forceinline__ i32x4 neg_inf_vec() {
+    const int w = ET<T>::IS_BF16 ? (int)0xFF80FF80u : (int)0xFF800000u;
+    i32x4 v = {w, w, w, w};
+    return v;
+}
+template <typename T> __device__ __forceinline__ float vec_max(const i32x4& v) {
+    float f[ET<T>::VEC];
+    unpack16<T>(v, f);
+    float m = f[0];
+#pragma unroll
+    for (int j = 1; j < ET<T>::VEC; ++j) m = fmaxf(m, f[j]);
+    return m;
+}
+
 // Order of the scores as unsigned integers: a > b as floats <=> key(a) > key(b); -0 and 0 are one key; NaN is above
 // everything.
 constexpr uint32_t KEY_NAN = 0xFFFFFFFFu, KEY_NEG_INF = 0x007FFFFFu;
