@@ -248,9 +248,11 @@ int stgcn_cross_entropy(const float* logits, const int64_t* labels, float* loss,
  * 1 <= ncls <= 2^20, 1 <= rows.  Classes are ordered by (score descending, class ascending), NaN first. */
 
 /* The k (1..256, <= ncls) first classes of every row in that order: values [rows][k], indices [rows][k], and rest [rows] =
- * log sum over the other classes of exp(logits / temperature) (-inf: nothing is left). */
+ * log sum over the other classes of exp(logits / temperature) (-inf: nothing is left).  Few rows are split over workgroups
+ * that meet in `workspace` (16-byte aligned, at least the bytes that stgcn_top_logits_workspace tells; may be null if 0). */
 int stgcn_top_logits(int dtype, const void* logits, size_t row_stride, int rows, int ncls, int k, double temperature,
-                     float* values, int64_t* indices, float* rest, void* stream);
+                     float* values, int64_t* indices, float* rest, void* workspace, size_t workspace_bytes, void* stream);
+int stgcn_top_logits_workspace(int rows, int ncls, int k, size_t* bytes);      /* bytes: host memory */
 
 /* Distillation from a teacher's top logits: values / indices [rows][k] (k <= 256; an index < 0 is no entry), rest [rows] the
  * log of the teacher's other mass at the same temperature T (null: the teacher's entries are renormalised), labels [rows]

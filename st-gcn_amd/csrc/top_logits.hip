@@ -38,117 +38,138 @@ template <int W> __device__ __forceinline__ void group_sync() {
     else lds_barrier();                            // LDS only: loads of the next batch stay in flight
 }
 
-// Buffer of candidates of a group of W waves.
+// Buffer of candidates of a group of W waves.  Its order is the same every run (places are dealt by prefix counts, not by
+// atomics), and with it the order in which dropped scores are added to the rest.  `add` holds what each wave appends in a
+// batch; three sets take turns, so that one barrier a batch is enough: while all read a batch's counts, nobody writes them.
 template <int W> struct Shared {
     static constexpr int CAP = W == 1 ? 512 : 2048;
     u64 cand[CAP];
-    u64 kept[MAX_K];
     uint32_t maxima[W == 1 ? 64 : 1024];
-    u64 tau;
-    int count, missed, nkept;
+    u64 tau; float lim;                            // the bound; scores x with !(x <= lim) may be earlier in the order
+    int add[3][W], nkept;
     float rm[4]; double rs[4];
 };
+__device__ __forceinline__ int buffer_limit(int k) { return 2 * k + 64; }       // beyond it the bound is raised
 
-// The k-th largest of `c` (> k) distinct places, by one wave: bisection of the key, then of the class among equal keys.
-// With at most 512 of them their keys stay in registers.
-__device__ __forceinline__ u64 kth_place(const u64* cand, int c, int k) {
+// The largest score before key `k` (> -inf) in the order of the scores.
+__device__ __forceinline__ float score_before(uint32_t k) { return key_score(k == 0x80000000u ? 0x7FFFFFFEu : k - 1); }   // -0 is 0
+
+// Bits of a key that carry something: a bf16 score has 16.
+template <typename T> constexpr int KEY_SHIFT = ET<T>::IS_BF16 ? 16 : 0;
+template <typename T> __device__ __forceinline__ uint32_t short_key(u64 p) { return (uint32_t)(p >> (32 + KEY_SHIFT<T>)); }
+template <typename T> __device__ __forceinline__ uint32_t long_key(uint32_t s) {
+    return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s;
+}
+
+// The k-th largest of `c` (> k) distinct places, by one wave: the key bit by bit below those that all have in common,
+// then the class among equal keys.  With at most 512 of them their keys stay in registers.
+template <typename T> __device__ __forceinline__ u64 kth_place(const u64* cand, int c, int k) {
     const int lane = threadIdx.x & 63;
-    uint32_t v = 0;
-    if (c <= 512) {
-        uint32_t key[8];
+    uint32_t key[8], lo = ~0u, hi = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) key[i] = lane + 64 * i < c ? (uint32_t)(cand[lane + 64 * i] >> 32) : 0;
-        for (int b = 31; b >= 0; --b) {
+    for (int i = 0; i < 8; ++i) {
+        key[i] = lane + 64 * i < c ? short_key<T>(cand[lane + 64 * i]) : 0;
+        if (lane + 64 * i < c) { lo = min(lo, key[i]); hi = max(hi, key[i]); }
+    }
+    for (int i = lane + 512; i < c; i += 64) { const uint32_t s = short_key<T>(cand[i]); lo = min(lo, s); hi = max(hi, s); }
+    lo = wave_reduce(lo, [](uint32_t a, uint32_t b) { return min(a, b); });
+    hi = wave_reduce(hi, OpMax());
+    uint32_t v = lo;
+    if (lo != hi) {
+        const int first = 31 - __clz(lo ^ hi);
+        v = first == 31 ? 0 : hi >> (first + 1) << (first + 1);
+        for (int b = first; b >= 0; --b) {
+            const uint32_t to = v | 1u << b;
             int n = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) if (64 * i < c) n += __popcll(__ballot(key[i] >= (v | 1u << b)));
-            if (n >= k) v |= 1u << b;
-        }
-    } else {
-        for (int b = 31; b >= 0; --b) {
-            int n = 0;
-            for (int i = lane; i - lane < c; i += 64) n += __popcll(__ballot(i < c && (uint32_t)(cand[i < c ? i : 0] >> 32) >= (v | 1u << b)));
-            if (n >= k) v |= 1u << b;
+            for (int i = 0; i < 8; ++i) if (64 * i < c) n += __popcll(__ballot(key[i] >= to));
+            for (int i = lane + 512; i - lane < c; i += 64) n += __popcll(__ballot(i < c && short_key<T>(cand[i < c ? i : 0]) >= to));
+            if (n >= k) v = to;
         }
     }
     int above = 0, equal = 0;
     for (int i = lane; i - lane < c; i += 64) {
-        const uint32_t key = i < c ? (uint32_t)(cand[i] >> 32) : 0;
-        above += __popcll(__ballot(i < c && key > v));
-        equal += __popcll(__ballot(i < c && key == v));
+        const uint32_t s = i < c ? short_key<T>(cand[i]) : 0;
+        above += __popcll(__ballot(i < c && s > v));
+        equal += __popcll(__ballot(i < c && s == v));
     }
-    if (above + equal == k) return (u64)v << 32;
+    const u64 t = (u64)long_key<T>(v) << 32;
+    if (above + equal == k) return t;
     uint32_t l = 0;
     for (int b = 31; b >= 0; --b) {
         int n = above;
         for (int i = lane; i - lane < c; i += 64) {
             const u64 p = i < c ? cand[i] : 0;
-            n += __popcll(__ballot(i < c && (uint32_t)(p >> 32) == v && (uint32_t)p >= (l | 1u << b)));
+            n += __popcll(__ballot(i < c && short_key<T>(p) == v && (uint32_t)p >= (l | 1u << b)));
         }
         if (n >= k) l |= 1u << b;
     }
-    return (u64)v << 32 | l;
+    return t | l;
 }
 
-// Keeps the k first of the buffer's entries; the others go to the rest.  tau = the k-th.
-template <int W> __device__ __forceinline__ void compact(Shared<W>& sh, int tid, int k, RestSum& rest, float c) {
-    constexpr int G = W * 64, CAP = Shared<W>::CAP;
+__device__ __forceinline__ int lanes_below(u64 mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
+
+// Keeps the k first of the buffer's n entries, in the order in which they stand; the others go to the rest.  The k-th becomes
+// the bound.  One wave's work.
+template <typename T, int W> __device__ __forceinline__ void compact(Shared<W>& sh, int tid, int& n, int k, RestSum& rest, float c) {
     group_sync<W>();
-    const int n = min(sh.count, CAP);
     if (n <= k) return;                            // the same in every thread
     if (tid < 64) {
-        const u64 t = kth_place(sh.cand, n, k);
-        if (tid == 0) { sh.tau = t; sh.nkept = 0; }
+        const u64 t = kth_place<T>(sh.cand, n, k);
+        int at = 0;
+        for (int i = 0; i < n; i += 64) {          // entries only move towards the front
+            const u64 p = i + tid < n ? sh.cand[i + tid] : 0;
+            const u64 keep = __ballot(p >= t && p);
+            if (p >= t && p) sh.cand[at + lanes_below(keep)] = p;
+            else if (p) rest.take(key_score((uint32_t)(p >> 32)), c);
+            at += __popcll(keep);
+        }
+        if (tid == 0) { sh.tau = t; sh.lim = key_score((uint32_t)(t >> 32)); }
     }
-    group_sync<W>();
-    const u64 t = sh.tau;
-    for (int i = tid; i < n; i += G) {
-        const u64 p = sh.cand[i];
-        if (p >= t) sh.kept[atomicAdd(&sh.nkept, 1)] = p;
-        else if (p) rest.take(key_score((uint32_t)(p >> 32)), c);
-    }
-    group_sync<W>();
-    for (int i = tid; i < k; i += G) sh.cand[i] = sh.kept[i];
-    if (tid == 0) sh.count = k;
+    n = k;
     group_sync<W>();
 }
 
-// Offers this thread's pending scores (bit e of `pending`: x(e), class(e)) to the buffer until all of the group's are kept
-// or beyond the bound.  Returns the bits of the scores that are kept.
-template <int W, typename X, typename J>
-__device__ __forceinline__ u64 offer(Shared<W>& sh, int tid, int k, u64 pending, X x, J cls, RestSum& rest, float c) {
+// Appends this thread's pending scores (bit e: emit(e, slot) writes it) to the buffer of n entries; raises the bound when
+// many have gathered.  Where the buffer is full, what is left is held against the raised bound (beyond(e)) and offered
+// again.  Returns the bits of the scores that are kept; the others belong to the rest.  `turn` counts the appends.
+template <typename T, int W, typename Emit, typename Beyond>
+__device__ __forceinline__ uint32_t offer(Shared<W>& sh, int tid, int& n, int& turn, int k, uint32_t pending, Emit emit, Beyond beyond, RestSum& rest, float c) {
     constexpr int CAP = Shared<W>::CAP;
-    u64 kept = 0;
+    const int wave = W == 1 ? 0 : tid >> 6;
+    uint32_t kept = 0;
     for (;;) {
-        int n = 0, base = 0;
-        if (pending) {
-            n = __popcll(pending);
-            base = atomicAdd(&sh.count, n);
-            if (base + n <= CAP) {
-                for (u64 q = pending; q; q &= q - 1) {
-                    const int e = __ffsll(q) - 1;
-                    sh.cand[base++] = place(score_key(x(e)), cls(e));
-                }
-                kept |= pending;
-                pending = 0;
-            } else {
-                for (; base < CAP; ++base) sh.cand[base] = 0;
-                sh.missed = 1;
+        const int m = __popc(pending);             // 17 at most
+        int below = 0, all = 0;
+        if (__ballot(pending != 0)) {
+#pragma unroll
+            for (int b = 0; b < 5; ++b) {
+                const u64 q = __ballot(m >> b & 1);
+                below += lanes_below(q) << b;
+                all += __popcll(q) << b;
             }
         }
-        group_sync<W>();
-        const int count = sh.count, missed = sh.missed;
-        group_sync<W>();
-        if (!missed && count <= (CAP / 4 > 3 * k ? CAP / 4 : 3 * k)) return kept;
-        if (tid == 0) sh.missed = 0;
-        compact<W>(sh, tid, k, rest, c);
-        if (!missed) return kept;
-        const u64 t = sh.tau;
-        u64 left = 0;
-        for (u64 q = pending; q; q &= q - 1) {
-            const int e = __ffsll(q) - 1;
-            if (place(score_key(x(e)), cls(e)) > t) left |= q & -q;    // else it stays where it is and is summed as rest
+        int slot = n;
+        if constexpr (W == 1) n += all;
+        else {
+            if ((tid & 63) == 0) sh.add[turn % 3][wave] = all;
+            group_sync<W>();
+#pragma unroll
+            for (int w = 0; w < W; ++w) { const int s = sh.add[turn % 3][w]; if (w < wave) slot += s; n += s; }
+            ++turn;
         }
+        slot += below;
+        const bool full = n > CAP;
+        if (pending) {
+            if (slot + m <= CAP) { emit(pending, slot); kept |= pending; pending = 0; }
+            else for (; slot < CAP; ++slot) sh.cand[slot] = 0;
+        }
+        if (full) n = CAP;
+        if (!full && n <= buffer_limit(k)) return kept;
+        compact<T, W>(sh, tid, n, k, rest, c);
+        if (!full) return kept;
+        uint32_t left = 0;
+        for (uint32_t q = pending; q; q &= q - 1) if (beyond(__ffs(q) - 1, sh.tau)) left |= q & -q;
         pending = left;
     }
 }
@@ -189,8 +210,6 @@ __device__ void slow_row(const T* x, int lo, int hi, int tid, int k, Shared<W>& 
         if (place(score_key(v), j) < last) { if (v != v) rest.s = NAN; else rest.take(v, c); }
     }
     group_sync<W>();
-    if (tid == 0) sh.count = k;
-    group_sync<W>();
 }
 
 // rest of the group: its threads' sums joined.  Every thread gets the pair.
@@ -226,7 +245,7 @@ template <int W> __device__ void write_row(const TopArgs& a, size_t r, Shared<W>
 
 template <typename T, int W>
 __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
-    constexpr int VEC = ET<T>::VEC, G = W * 64, NB = 16 / VEC, PER = NB * VEC, ROWS = W == 1 ? 4 : 1;
+    constexpr int VEC = ET<T>::VEC, G = W * 64, PER = 16, NB = PER / VEC, ROWS = W == 1 ? 4 : 1;
     __shared__ Shared<W> sh_[ROWS];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
     const size_t job = W == 1 ? (size_t)blockIdx.x * ROWS + wave : blockIdx.x;
@@ -244,104 +263,108 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
     const bool with_head = piece == 0, with_tail = piece == a.pieces - 1;
     const int v1 = min(b1 * G * NB, sp.nvec);
 
-    if (tid == 0) { sh.count = 0; sh.missed = 0; sh.tau = 0; }
+    if (tid == 0) sh.tau = 0;
     RestSum rest;
+    int have = 0, turn = 0;                        // entries in the buffer
     i32x4 v[NB], nx[NB];
     auto load = [&](int b, i32x4* to) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int at = b * G * NB + i * G + tid;
-            if (at < v1) to[i] = load_vec(x, sp.vec_at(at));
-            else { const int w = ET<T>::IS_BF16 ? (int)0xFF80FF80u : (int)0xFF800000u; to[i] = i32x4{w, w, w, w}; }
+            to[i] = at < v1 ? load_vec(x, sp.vec_at(at)) : neg_inf_vec<T>();
         }
     };
     load(b0, nx);
     const float xh = with_head && tid < sp.head ? load_elem(x, tid) : -INFINITY;
 
     for (int b = b0; b < b1 || b == b0; ++b) {
+        float f[PER];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) v[i] = nx[i];
+        for (int i = 0; i < NB; ++i) unpack16<T>(nx[i], f + i * VEC);
         if (b + 1 < b1) load(b + 1, nx);
-        float top = vec_max<T>(v[0]);
+        float top = f[0];
 #pragma unroll
-        for (int i = 1; i < NB; ++i) top = fmaxf(top, vec_max<T>(v[i]));
+        for (int e = 1; e < PER; ++e) top = fmaxf(top, f[e]);
         if (b == b0) {
             // a bound that k scores of this batch reach, to 16 bits of the key: from 64 W maxima of threads, or 64 W NB of vectors
             const bool fine = W > 1 && k > 64;
             if (fine) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) sh.maxima[(i * G + tid) & 1023] = score_key(vec_max<T>(v[i]));
+                for (int i = 0; i < NB; ++i) {
+                    float m = f[i * VEC];
+#pragma unroll
+                    for (int j = 1; j < VEC; ++j) m = fmaxf(m, f[i * VEC + j]);
+                    sh.maxima[(i * G + tid) & (W == 1 ? 63 : 1023)] = score_key(m);
+                }
             } else sh.maxima[tid] = score_key(top);
             group_sync<W>();
             if (tid < 64) {
-                const int have = fine ? W * NB : W;
-                uint32_t m[16], t = 0;
+                constexpr int MOST = W == 1 ? 1 : W * NB;
+                const int some = fine ? MOST : W;
+                uint32_t m[MOST], t = 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) m[i] = i < have ? sh.maxima[(lane + 64 * i) & (W == 1 ? 63 : 1023)] : 0;
+                for (int i = 0; i < MOST; ++i) m[i] = i < some ? sh.maxima[lane + 64 * i] : 0;
                 for (int bit = 31; bit >= 16; --bit) {
                     const uint32_t to = t | 1u << bit;
                     int cnt = 0;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) if (i < have) cnt += __popcll(__ballot(m[i] >= to));
+                    for (int i = 0; i < MOST; ++i) if (i < some) cnt += __popcll(__ballot(m[i] >= to));
                     if (cnt >= k) t = to;
                 }
                 // a bound at or below -inf: everything
-                if (lane == 0) sh.tau = t <= KEY_NEG_INF ? 0 : (u64)t << 32;
+                if (lane == 0) sh.lim = t <= KEY_NEG_INF ? NAN : score_before(t);
             }
             group_sync<W>();
         }
-        const u64 tau = sh.tau;
-        // The first batch's bound is a key that k scores reach; a later batch's classes come after the buffer's, and of
-        // those only larger keys than tau's are earlier in the order.
-        const uint32_t tk = (uint32_t)(tau >> 32), least = tau == 0 ? 0 : b == b0 ? tk : tk + 1;
-        u64 pending = 0;
-        if (least == 0 || score_key(top) >= least) {
+        // The first batch's bound is one that k scores reach.  A later batch's classes come after the buffer's: of those
+        // only scores beyond the bound's are earlier in the order.  lim is NaN while there is no bound.
+        const float lim = sh.lim;
+        uint32_t pending = 0;
+        if (!(top <= lim) || b == b0) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const int at = b * G * NB + i * G + tid;
-                float f[VEC];
-                unpack16<T>(v[i], f);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (at < v1 && score_key(f[j]) >= least) pending |= 1ull << (i * VEC + j);
+            for (int e = 0; e < PER; ++e) {
+                const int at = b * G * NB + (e / VEC) * G + tid;
+                if (!(f[e] <= lim) && at < v1) pending |= 1u << e;
             }
         }
-        if (b == b0 && with_head && tid < sp.head && score_key(xh) >= least) pending |= 1ull << PER;
+        if (b == b0 && with_head && tid < sp.head && !(xh <= lim)) pending |= 1u << PER;
         auto cls = [&](int e) { return e == PER ? tid : sp.vec_at(b * G * NB + (e / VEC) * G + tid) + e % VEC; };
-        const u64 kept = offer<W>(sh, tid, k, pending, [&](int e) { return load_elem(x, cls(e)); }, cls, rest, c);
+        const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, pending,
+            [&](uint32_t q, int slot) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) asm volatile("" : "+v"(v[i]));        // unpacked again below rather than held as floats
+                for (int e = 0; e < PER; ++e) {
+                    asm volatile("" : "+v"(q));    // one score's key at a time: all at once take fifty registers
+                    if (q >> e & 1) sh.cand[slot++] = place(score_key(f[e]), cls(e));
+                }
+                if (q >> PER & 1) sh.cand[slot] = place(score_key(xh), tid);
+            },
+            [&](int e, u64 tau) { return place(score_key(e == PER ? xh : load_elem(x, cls(e))), cls(e)) > tau; }, rest, c);
         if (kept) {
             top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                drop_listed<T>(v[i], (uint32_t)(kept >> (i * VEC)) & ((1u << VEC) - 1));
-                top = fmaxf(top, vec_max<T>(v[i]));
-            }
+            for (int e = 0; e < PER; ++e) { if (kept >> e & 1) f[e] = -INFINITY; top = fmaxf(top, f[e]); }
         }
         rest.raise(top, c);
+        const float ref = rest.m == -INFINITY ? 0.f : rest.m;
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            float f[VEC];
-            unpack16<T>(v[i], f);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) rest.add(f[j], c);
-        }
+        for (int e = 0; e < PER; ++e) rest.s += exp2_32((f[e] - ref) * c);
         if (b == b0 && with_head && tid < sp.head && !(kept >> PER & 1)) { if (xh != xh) rest.s = NAN; else rest.take(xh, c); }
     }
-    if (with_tail) {                               // the classes behind the last whole vector, last in the order of classes
+    if (with_tail && sp.edge > sp.head) {          // the classes behind the last whole vector, last in the order of classes
         const int tail = sp.edge - sp.head, j = n - tail + tid;
         const float xt = tid < tail ? load_elem(x, j) : 0.f;
-        const u64 kept = offer<W>(sh, tid, k, tid < tail && place(score_key(xt), j) > sh.tau ? 1ull : 0ull, [&](int) { return xt; },
-                                  [&](int) { return j; }, rest, c);
+        const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, tid < tail && !(xt <= sh.lim) ? 1u : 0u,
+            [&](uint32_t, int slot) { sh.cand[slot] = place(score_key(xt), j); },
+            [&](int, u64 tau) { return place(score_key(xt), j) > tau; }, rest, c);
         if (tid < tail && !kept) { if (xt != xt) rest.s = NAN; else rest.take(xt, c); }
     }
-    compact<W>(sh, tid, k, rest, c);
+    compact<T, W>(sh, tid, have, k, rest, c);
     bool nan = rest.s != rest.s;
     if constexpr (W == 1) nan = __ballot(nan) != 0; else nan = __syncthreads_or(nan);
     if (nan) {
         const int lo = with_head ? 0 : sp.vec_at(b0 * G * NB), hi = with_tail ? n : sp.vec_at(v1);
         slow_row<T, W>(x, lo, hi, tid, k, sh, rest, c);
+        have = min(k, hi - lo);
     }
     float m; double s;
     join_rest<W>(sh, tid, rest, c, m, s);
@@ -349,33 +372,111 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
         write_row<W>(a, r, sh, tid);
         if (tid == 0) a.rest[r] = s != s ? NAN : m == -INFINITY ? -INFINITY : (float)((double)m / a.T + log(s));
     } else {
-        const int have = min(sh.count, k);
         for (int i = tid; i < k; i += G) a.part[job * k + i] = i < have ? sh.cand[i] : 0;
         if (tid == 0) a.part_rest[job] = make_float2(m, (float)s);
     }
 }
 
+// A row's pieces joined: the k first of their places; the others go to the rest.  At most MAX_MERGE places.
+constexpr int MAX_MERGE = 8192;
+template <typename T>
+__global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a) {
+    constexpr int R = MAX_MERGE / 256;
+    __shared__ Shared<4> sh;
+    __shared__ int cnt[2][4];
+    const int tid = threadIdx.x, wave = tid >> 6, k = a.k, c = a.pieces * k;
+    const size_t r = blockIdx.x;
+    const u64* part = a.part + r * c;
+    uint32_t key[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = i * 256 < c && tid + 256 * i < c ? short_key<T>(part[tid + 256 * i]) : 0;
+    RestSum rest;
+    for (int i = tid; i < a.pieces; i += 256) {
+        const float2 p = a.part_rest[r * a.pieces + i];
+        if (p.x > rest.m) { rest.raise(p.x, a.c); }
+        rest.s += p.x == rest.m ? p.y : p.y * exp2_32((p.x - (rest.m == -INFINITY ? 0.f : rest.m)) * a.c);
+    }
+    // the k-th key, bit by bit; every thread counts its own, the waves' counts meet in LDS (two sets take turns)
+    uint32_t v = 0;
+    int turn = 0;
+    auto total = [&](int mine) {
+        if ((tid & 63) == 0) cnt[turn & 1][wave] = mine;
+        lds_barrier();
+        const int t = cnt[turn & 1][0] + cnt[turn & 1][1] + cnt[turn & 1][2] + cnt[turn & 1][3];
+        ++turn;
+        return t;
+    };
+    for (int b = 31 - KEY_SHIFT<T>; b >= 0; --b) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) if (256 * i < c) n += __popcll(__ballot(key[i] >= (v | 1u << b)));
+        if (total(n) >= k) v |= 1u << b;
+    }
+    int n = 0, e = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) if (256 * i < c) { n += __popcll(__ballot(key[i] > v)); e += __popcll(__ballot(key[i] == v)); }
+    const int above = total(n), equal = total(e);
+    uint32_t l = 0;
+    if (above + equal > k) {
+        for (int b = 31; b >= 0; --b) {
+            int m = 0;
+            for (int i = tid; i - tid < c; i += 256) m += __popcll(__ballot(i < c && short_key<T>(part[i < c ? i : 0]) == v && (uint32_t)part[i < c ? i : 0] >= (l | 1u << b)));
+            if (above + total(m) >= k) l |= 1u << b;
+        }
+    }
+    const u64 t = (u64)long_key<T>(v) << 32 | l;
+    if (tid == 0) sh.nkept = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (256 * i < c && tid + 256 * i < c) {
+            const u64 p = part[tid + 256 * i];
+            if (p >= t && p) { const int at = atomicAdd(&sh.nkept, 1); if (at < k) sh.cand[at] = p; }
+            else if (p) { const float x = key_score((uint32_t)(p >> 32)); if (x != x) rest.s = NAN; else rest.take(x, a.c); }
+        }
+    __syncthreads();
+    write_row<4>(a, r, sh, tid);
+    float m; double s;
+    join_rest<4>(sh, tid, rest, a.c, m, s);
+    if (tid == 0) a.rest[r] = s != s ? NAN : m == -INFINITY ? -INFINITY : (float)((double)m / a.T + log(s));
+}
+
 }  // namespace
 
-// Pieces a row is split into: rows fill the chip by themselves from two workgroups a compute unit on; below that a row
-// is cut into pieces of at least one batch.
-static int top_pieces(int dtype, int rows, int ncls, int k) {
-    (void)dtype; (void)rows; (void)ncls; (void)k;
-    return 1;
+// Pieces a row is split into.  512 rows fill the chip (two workgroups of four waves a compute unit) and are not split;
+// fewer rows are cut into pieces of at least one batch (4096 scores) until 1024 workgroups run.
+static int top_pieces(int rows, int ncls, int k) {
+    if (rows >= 512 || ncls <= 512) return 1;
+    const int batches = (ncls + 4095) / 4096;
+    int p = (1024 + rows - 1) / rows;
+    if (p > batches) p = batches;
+    if (p * k > MAX_MERGE) p = MAX_MERGE / k;
+    return p;
+}
+static size_t top_workspace(int rows, int pieces, int k) { return pieces == 1 ? 0 : (size_t)rows * pieces * ((size_t)k * 8 + 8); }
+
+extern "C" int stgcn_top_logits_workspace(int rows, int ncls, int k, size_t* bytes) {
+    if (!bytes || rows < 1 || ncls < 1 || ncls > (1 << 20) || k < 1 || k > MAX_K || k > ncls) return STGCN_ERR_ARG;
+    *bytes = top_workspace(rows, top_pieces(rows, ncls, k), k);
+    return STGCN_OK;
 }
 
 extern "C" int stgcn_top_logits(int dtype, const void* logits, size_t row_stride, int rows, int ncls, int k, double temperature,
-                                float* values, int64_t* indices, float* rest, void* stream) {
+                                float* values, int64_t* indices, float* rest, void* workspace, size_t workspace_bytes, void* stream) {
     if (!logits || !values || !indices || !rest || rows < 1 || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls || k < 1 || k > MAX_K
         || k > ncls || !(temperature > 0.0) || !(temperature < 1e30) || (dtype != STGCN_F32 && dtype != STGCN_BF16)) return STGCN_ERR_ARG;
-    TopArgs a = {logits, row_stride, rows, ncls, k, top_pieces(dtype, rows, ncls, k), (float)(LOG2E / temperature), temperature, values, (long long*)indices, rest,
-                 nullptr, nullptr};
+    const int pieces = top_pieces(rows, ncls, k);
+    if (pieces > 1 && (!workspace || workspace_bytes < top_workspace(rows, pieces, k))) return STGCN_ERR_WORKSPACE;
+    TopArgs a = {logits, row_stride, rows, ncls, k, pieces, (float)(LOG2E / temperature), temperature, values, (long long*)indices, rest,
+                 (u64*)workspace, (float2*)((char*)workspace + (pieces > 1 ? (size_t)rows * pieces * k * 8 : 0))};
     const hipStream_t s = (hipStream_t)stream;
-    if (ncls <= 512) {
-        const unsigned quads = (unsigned)((rows + 3) / 4);
-        if (dtype == STGCN_BF16) top_scan_kernel<bf16, 1><<<quads, 256, 0, s>>>(a); else top_scan_kernel<float, 1><<<quads, 256, 0, s>>>(a);
+    const unsigned grid = ncls <= 512 ? (unsigned)((rows + 3) / 4) : (unsigned)rows * pieces;
+    if (dtype == STGCN_BF16) {
+        if (ncls <= 512) top_scan_kernel<bf16, 1><<<grid, 256, 0, s>>>(a); else top_scan_kernel<bf16, 4><<<grid, 256, 0, s>>>(a);
+        if (pieces > 1) top_merge_kernel<bf16><<<rows, 256, 0, s>>>(a);
     } else {
-        if (dtype == STGCN_BF16) top_scan_kernel<bf16, 4><<<rows, 256, 0, s>>>(a); else top_scan_kernel<float, 4><<<rows, 256, 0, s>>>(a);
+        if (ncls <= 512) top_scan_kernel<float, 1><<<grid, 256, 0, s>>>(a); else top_scan_kernel<float, 4><<<grid, 256, 0, s>>>(a);
+        if (pieces > 1) top_merge_kernel<float><<<rows, 256, 0, s>>>(a);
     }
     return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
 }

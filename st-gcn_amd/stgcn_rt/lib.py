@@ -51,7 +51,8 @@ _SIGS = {
     "stgcn_pool_bwd": [_i, _vp, _vp, _i, _i, _i, _i, _vp],
     "stgcn_mul_many": [_vp, _vp, _i, _vp, _sz, _vp],
     "stgcn_cross_entropy": [_vp, _vp, _vp, _vp, _i, _i, _vp],
-    "stgcn_top_logits": [_i, _vp, _sz, _i, _i, _i, _d, _vp, _vp, _vp, _vp],
+    "stgcn_top_logits": [_i, _vp, _sz, _i, _i, _i, _d, _vp, _vp, _vp, _vp, _sz, _vp],
+    "stgcn_top_logits_workspace": [_i, _i, _i, _vp],
     "stgcn_distill_fwd": [_i, _vp, _sz, _vp, _vp, _vp, _vp, _i, _i, _i, _d, _d, _i, _vp, _vp, _vp, _vp, _vp],
     "stgcn_distill_bwd": [_i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _i, _d, _i, _i, _i, _d, _d, _vp, _vp],
     "stgcn_distill_step": [_i, _vp, _sz, _vp, _vp, _vp, _vp, _i, _i, _i, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _vp],

@@ -529,6 +529,13 @@ def _check_temperature(t):
     return t
 
 
+def _call_workspace(device, name, *sizes):
+    """A workspace of the call's own: calls on two streams, or in two graphs, share none.  (None, 0) when it wants none."""
+    need = ctypes.c_size_t(0)
+    L.call(name, *sizes, ctypes.addressof(need))
+    return (torch.empty(need.value, dtype=torch.uint8, device=device), need.value) if need.value else (None, 0)
+
+
 def top_logits(logits, k, temperature=1.0):
     """The k largest scores of every row: (values [rows, k] float32, indices [rows, k] int64, rest [rows] float32).
 
@@ -544,8 +551,9 @@ def top_logits(logits, k, temperature=1.0):
     indices = torch.empty((rows, k), dtype=torch.int64, device=x.device)
     rest = torch.empty((rows,), dtype=torch.float32, device=x.device)
     if rows:
+        ws, nbytes = _call_workspace(x.device, "stgcn_top_logits_workspace", rows, ncls, k)
         _launch((str(x.dtype), rows, ncls, k), "stgcn_top_logits", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), rows, ncls, k, temperature,
-                L.ptr(values), L.ptr(indices), L.ptr(rest), L.stream_ptr())
+                L.ptr(values), L.ptr(indices), L.ptr(rest), L.ptr(ws), nbytes, L.stream_ptr())
     return values, indices, rest
 
 

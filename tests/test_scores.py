@@ -6,6 +6,7 @@ value; |y| <= 127 where the value is not flushed to zero), added up in 32 bits b
 (chain * 2^-24) and joined in 64 bits.  EPS_S(case) = 2^-23 + (2.1 D + chain) 2^-24 bounds the relative error of S, D the
 largest |y|.  The gradients are products of e, of factors of 1/S and of the incoming gradient (each rounded once:
 8 * 2^-24 covers them) minus p, rounded once more to the type of the scores: eps / 2 of the value."""
+import ctypes
 import itertools
 import math
 
@@ -56,7 +57,7 @@ def eps_sum(x, T):
 # ---- top_logits --------------------------------------------------------------------------------------------------
 
 TOP = [(1, 1, 1), (3, 2, 2), (5, 7, 3), (64, 60, 5), (33, 61, 61), (9, 400, 16), (4, 401, 256), (3, 1027, 100), (2, 8191, 128),
-       (2, 8200, 1), (3, 20011, 256), (1, 70001, 64), (1, 131075, 200)]
+       (2, 8200, 1), (3, 20011, 256), (1, 70001, 64), (1, 131075, 200), (600, 5000, 20), (520, 9001, 256)]
 
 
 def check_top(F, x, k, T):
@@ -602,9 +603,14 @@ def test_c_entry_points_refuse():
     from stgcn_rt import lib as L
     l = L.load()
     p = 4096                                                   # never dereferenced by the host
-    top = lambda dt=0, x=p, st=10, r=4, n=10, k=3, T=1.0: l.stgcn_top_logits(dt, x, st, r, n, k, T, p, p, p, None)       # noqa: E731
+    top = lambda dt=0, x=p, st=10, r=4, n=10, k=3, T=1.0: l.stgcn_top_logits(dt, x, st, r, n, k, T, p, p, p, None, 0, None)   # noqa: E731
     for kw in (dict(dt=7), dict(x=None), dict(st=9), dict(r=0), dict(n=0), dict(n=1 << 21, st=1 << 21), dict(k=0), dict(k=11), dict(T=0.0), dict(T=math.nan)):
         assert top(**kw) == 1, kw
+    assert top(n=100000, st=100000) == 3                       # few rows want a workspace
+    need = ctypes.c_size_t(7)
+    assert l.stgcn_top_logits_workspace(4, 100000, 3, ctypes.addressof(need)) == 0 and need.value > 0
+    assert l.stgcn_top_logits_workspace(4000, 100000, 3, ctypes.addressof(need)) == 0 and need.value == 0
+    assert l.stgcn_top_logits_workspace(4, 100000, 300, ctypes.addressof(need)) == 1 and l.stgcn_top_logits_workspace(4, 10, 3, None) == 1
     fwd = lambda dt=0, x=p, st=10, v=p, i=p, lab=None, r=4, n=10, k=3, T=1.0, w=0.0, red=1, rows=p: l.stgcn_distill_fwd(      # noqa: E731
         dt, x, st, v, i, None, lab, r, n, k, T, w, red, p, rows, p, p, None)
     for kw in (dict(dt=2), dict(x=None), dict(st=9), dict(v=None), dict(i=None), dict(r=-1), dict(n=0), dict(k=257), dict(T=-1.0), dict(w=0.5), dict(w=1.5, lab=p),
