@@ -44,7 +44,8 @@ template <int W> __device__ __forceinline__ void group_sync() {
 template <int W> struct Shared {
     static constexpr int CAP = W == 1 ? 512 : 2048;
     u64 cand[CAP];
-    uint32_t maxima[W == 1 ? 64 : 1024];
+    static constexpr int EQ = W == 1 ? 128 : 1024;
+    uint32_t maxima[EQ];                           // of the first batch; later the classes of equal scores
     u64 tau; float lim;                            // the bound; scores x with !(x <= lim) may be earlier in the order
     int add[3][W], nkept;
     float rm[4]; double rs[4];
@@ -61,41 +62,57 @@ template <typename T> __device__ __forceinline__ uint32_t long_key(uint32_t s) {
     return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s;
 }
 
-// The k-th largest of `c` (> k) distinct places, by one wave: the key bit by bit below those that all have in common,
-// then the class among equal keys.  With at most 512 of them their keys stay in registers.
-template <typename T> __device__ __forceinline__ u64 kth_place(const u64* cand, int c, int k) {
+__device__ __forceinline__ int lanes_below(u64 mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
+
+// The k-th largest of `c` numbers v(i) (i < c, c >= k) that are not all distinct, by one wave, bit by bit below those that
+// all have in common; with at most 512 of them they stay in registers.
+template <typename V> __device__ __forceinline__ uint32_t kth_largest(V v, int c, int k) {
     const int lane = threadIdx.x & 63;
-    uint32_t key[8], lo = ~0u, hi = 0;
+    uint32_t r[8], lo = ~0u, hi = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        key[i] = lane + 64 * i < c ? short_key<T>(cand[lane + 64 * i]) : 0;
-        if (lane + 64 * i < c) { lo = min(lo, key[i]); hi = max(hi, key[i]); }
+        r[i] = 0;
+        if (64 * i < c && lane + 64 * i < c) { r[i] = v(lane + 64 * i); lo = min(lo, r[i]); hi = max(hi, r[i]); }
     }
-    for (int i = lane + 512; i < c; i += 64) { const uint32_t s = short_key<T>(cand[i]); lo = min(lo, s); hi = max(hi, s); }
+    for (int i = lane + 512; i < c; i += 64) { const uint32_t s = v(i); lo = min(lo, s); hi = max(hi, s); }
     lo = wave_reduce(lo, [](uint32_t a, uint32_t b) { return min(a, b); });
     hi = wave_reduce(hi, OpMax());
-    uint32_t v = lo;
-    if (lo != hi) {
-        const int first = 31 - __clz(lo ^ hi);
-        v = first == 31 ? 0 : hi >> (first + 1) << (first + 1);
-        for (int b = first; b >= 0; --b) {
-            const uint32_t to = v | 1u << b;
-            int n = 0;
+    if (lo == hi) return lo;
+    const int first = 31 - __clz(lo ^ hi);
+    uint32_t t = first == 31 ? 0 : hi >> (first + 1) << (first + 1);
+    for (int b = first; b >= 0; --b) {
+        const uint32_t to = t | 1u << b;
+        int n = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) if (64 * i < c) n += __popcll(__ballot(key[i] >= to));
-            for (int i = lane + 512; i - lane < c; i += 64) n += __popcll(__ballot(i < c && short_key<T>(cand[i < c ? i : 0]) >= to));
-            if (n >= k) v = to;
-        }
+        for (int i = 0; i < 8; ++i) if (64 * i < c) n += __popcll(__ballot(r[i] >= to));
+        for (int i = lane + 512; i - lane < c; i += 64) n += __popcll(__ballot(i < c && v(i < c ? i : 0) >= to));
+        if (n >= k) t = to;
     }
-    int above = 0, equal = 0;
+    return t;
+}
+
+// The k-th largest of `c` (> k) distinct places, by one wave: the key, then the class among equal keys, which are
+// gathered in `equal` (EQ numbers of LDS) first.
+template <typename T, int EQ> __device__ __forceinline__ u64 kth_place(const u64* cand, uint32_t* equal, int c, int k) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t v = kth_largest([&](int i) { return short_key<T>(cand[i]); }, c, k);
+    int above = 0, same = 0;
     for (int i = lane; i - lane < c; i += 64) {
-        const uint32_t s = i < c ? short_key<T>(cand[i]) : 0;
+        const u64 p = i < c ? cand[i] : 0;
+        const uint32_t s = short_key<T>(p);
+        const u64 q = __ballot(i < c && s == v);
         above += __popcll(__ballot(i < c && s > v));
-        equal += __popcll(__ballot(i < c && s == v));
+        if (i < c && s == v && same + lanes_below(q) < EQ) equal[same + lanes_below(q)] = (uint32_t)p;
+        same += __popcll(q);
     }
     const u64 t = (u64)long_key<T>(v) << 32;
-    if (above + equal == k) return t;
-    uint32_t l = 0;
+    if (above + same == k) return t;
+    if (same <= EQ) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        return t | kth_largest([&](int i) { return equal[i]; }, same, k - above);
+    }
+    uint32_t l = 0;                                // many equal scores
     for (int b = 31; b >= 0; --b) {
         int n = above;
         for (int i = lane; i - lane < c; i += 64) {
@@ -107,15 +124,13 @@ template <typename T> __device__ __forceinline__ u64 kth_place(const u64* cand, 
     return t | l;
 }
 
-__device__ __forceinline__ int lanes_below(u64 mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
-
 // Keeps the k first of the buffer's n entries, in the order in which they stand; the others go to the rest.  The k-th becomes
 // the bound.  One wave's work.
 template <typename T, int W> __device__ __forceinline__ void compact(Shared<W>& sh, int tid, int& n, int k, RestSum& rest, float c) {
     group_sync<W>();
     if (n <= k) return;                            // the same in every thread
     if (tid < 64) {
-        const u64 t = kth_place<T>(sh.cand, n, k);
+        const u64 t = kth_place<T, Shared<W>::EQ>(sh.cand, sh.maxima, n, k);
         int at = 0;
         for (int i = 0; i < n; i += 64) {          // entries only move towards the front
             const u64 p = i + tid < n ? sh.cand[i + tid] : 0;
@@ -130,46 +145,55 @@ template <typename T, int W> __device__ __forceinline__ void compact(Shared<W>& 
     group_sync<W>();
 }
 
-// Appends this thread's pending scores (bit e: emit(e, slot) writes it) to the buffer of n entries; raises the bound when
-// many have gathered.  Where the buffer is full, what is left is held against the raised bound (beyond(e)) and offered
-// again.  Returns the bits of the scores that are kept; the others belong to the rest.  `turn` counts the appends.
-template <typename T, int W, typename Emit, typename Beyond>
-__device__ __forceinline__ uint32_t offer(Shared<W>& sh, int tid, int& n, int& turn, int k, uint32_t pending, Emit emit, Beyond beyond, RestSum& rest, float c) {
+// What the waves append in a batch: `mine` entries of this wave; returns this wave's first slot, n becomes the new count
+// (which may be beyond CAP).
+template <int W> __device__ __forceinline__ int deal_slots(Shared<W>& sh, int tid, int& n, int& turn, int mine) {
+    int slot = n;
+    if constexpr (W == 1) { n += mine; return slot; }
+    const int wave = tid >> 6;
+    if ((tid & 63) == 0) sh.add[turn][wave] = mine;
+    group_sync<W>();
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const int s = __builtin_amdgcn_readfirstlane(sh.add[turn][w]);
+        if (w < wave) slot += s;
+        n += s;
+    }
+    turn = turn == 2 ? 0 : turn + 1;
+    return slot;
+}
+
+// Appends this thread's pending scores (bit e: the score x(e) of class cls(e)), however many there are: what finds no
+// room is held against the raised bound and offered again.  Returns the bits that are kept; the others belong to the rest.
+// The way of row ends and of full buffers.
+template <typename T, int W, typename X, typename J>
+__device__ __forceinline__ uint32_t offer(Shared<W>& sh, int tid, int& n, int& turn, int k, uint32_t pending, X x, J cls, RestSum& rest, float c) {
     constexpr int CAP = Shared<W>::CAP;
-    const int wave = W == 1 ? 0 : tid >> 6;
     uint32_t kept = 0;
     for (;;) {
         const int m = __popc(pending);             // 17 at most
         int below = 0, all = 0;
-        if (__ballot(pending != 0)) {
 #pragma unroll
-            for (int b = 0; b < 5; ++b) {
-                const u64 q = __ballot(m >> b & 1);
-                below += lanes_below(q) << b;
-                all += __popcll(q) << b;
-            }
+        for (int b = 0; b < 5; ++b) {
+            const u64 q = __ballot(m >> b & 1);
+            below += lanes_below(q) << b;
+            all += __popcll(q) << b;
         }
-        int slot = n;
-        if constexpr (W == 1) n += all;
-        else {
-            if ((tid & 63) == 0) sh.add[turn % 3][wave] = all;
-            group_sync<W>();
-#pragma unroll
-            for (int w = 0; w < W; ++w) { const int s = sh.add[turn % 3][w]; if (w < wave) slot += s; n += s; }
-            ++turn;
-        }
-        slot += below;
+        int slot = deal_slots<W>(sh, tid, n, turn, all) + below;
         const bool full = n > CAP;
         if (pending) {
-            if (slot + m <= CAP) { emit(pending, slot); kept |= pending; pending = 0; }
-            else for (; slot < CAP; ++slot) sh.cand[slot] = 0;
+            if (slot + m <= CAP) {
+                for (uint32_t q = pending; q; q &= q - 1) { const int e = __ffs(q) - 1; sh.cand[slot++] = place(score_key(x(e)), cls(e)); }
+                kept |= pending;
+                pending = 0;
+            } else for (; slot < CAP; ++slot) sh.cand[slot] = 0;
         }
         if (full) n = CAP;
         if (!full && n <= buffer_limit(k)) return kept;
         compact<T, W>(sh, tid, n, k, rest, c);
         if (!full) return kept;
         uint32_t left = 0;
-        for (uint32_t q = pending; q; q &= q - 1) if (beyond(__ffs(q) - 1, sh.tau)) left |= q & -q;
+        for (uint32_t q = pending; q; q &= q - 1) { const int e = __ffs(q) - 1; if (place(score_key(x(e)), cls(e)) > sh.tau) left |= q & -q; }
         pending = left;
     }
 }
@@ -230,16 +254,18 @@ template <int W> __device__ __forceinline__ void join_rest(Shared<W>& sh, int ti
     }
 }
 
-// The buffer's k first in order, into the answer.
-template <int W> __device__ void write_row(const TopArgs& a, size_t r, Shared<W>& sh, int tid) {
+// The k first of the buffer's n entries, in order, into the answer; the others into the rest.
+template <int W> __device__ __forceinline__ void write_row(const TopArgs& a, size_t r, Shared<W>& sh, int tid, int n, RestSum& rest) {
     constexpr int G = W * 64;
     const int k = a.k;
-    for (int i = tid; i < k; i += G) {
+    for (int i = tid; i < n; i += G) {
         const u64 p = sh.cand[i];
         int rank = 0;
-        for (int o = 0; o < k; ++o) rank += sh.cand[o] > p ? 1 : 0;
-        a.values[r * k + rank] = key_score((uint32_t)(p >> 32));
-        a.indices[r * k + rank] = place_class(p);
+#pragma unroll 8
+        for (int o = 0; o < n; ++o) rank += sh.cand[o] > p ? 1 : 0;
+        const float x = key_score((uint32_t)(p >> 32));
+        if (rank < k) { a.values[r * k + rank] = x; a.indices[r * k + rank] = place_class(p); }
+        else { if (x != x) rest.s = NAN; else rest.take(x, a.c); }
     }
 }
 
@@ -275,7 +301,6 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
         }
     };
     load(b0, nx);
-    const float xh = with_head && tid < sp.head ? load_elem(x, tid) : -INFINITY;
 
     for (int b = b0; b < b1 || b == b0; ++b) {
         float f[PER];
@@ -294,7 +319,7 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
                     float m = f[i * VEC];
 #pragma unroll
                     for (int j = 1; j < VEC; ++j) m = fmaxf(m, f[i * VEC + j]);
-                    sh.maxima[(i * G + tid) & (W == 1 ? 63 : 1023)] = score_key(m);
+                    sh.maxima[(i * G + tid) & (Shared<W>::EQ - 1)] = score_key(m);
                 }
             } else sh.maxima[tid] = score_key(top);
             group_sync<W>();
@@ -319,27 +344,38 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
         // The first batch's bound is one that k scores reach.  A later batch's classes come after the buffer's: of those
         // only scores beyond the bound's are earlier in the order.  lim is NaN while there is no bound.
         const float lim = sh.lim;
-        uint32_t pending = 0;
-        if (!(top <= lim) || b == b0) {
+        u64 mask[PER];                             // lanes whose score e may be among the first, in scalar registers
+        int found = 0;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                const int at = b * G * NB + (e / VEC) * G + tid;
-                if (!(f[e] <= lim) && at < v1) pending |= 1u << e;
-            }
+        for (int e = 0; e < PER; ++e) {
+            mask[e] = __ballot(!(f[e] <= lim) && b * G * NB + (e / VEC) * G + tid < v1);
+            found += __popcll(mask[e]);
         }
-        if (b == b0 && with_head && tid < sp.head && !(xh <= lim)) pending |= 1u << PER;
-        auto cls = [&](int e) { return e == PER ? tid : sp.vec_at(b * G * NB + (e / VEC) * G + tid) + e % VEC; };
-        const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, pending,
-            [&](uint32_t q, int slot) {
+        const int before = have;
+        int slot = deal_slots<W>(sh, tid, have, turn, found);
+        if (have <= Shared<W>::CAP) {
+            if (found) {
+                top = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    asm volatile("" : "+v"(q));    // one score's key at a time: all at once take fifty registers
-                    if (q >> e & 1) sh.cand[slot++] = place(score_key(f[e]), cls(e));
+                    if (mask[e]) {
+                        if (mask[e] >> lane & 1) {
+                            sh.cand[slot + lanes_below(mask[e])] = place(score_key(f[e]), sp.vec_at(b * G * NB + (e / VEC) * G + tid) + e % VEC);
+                            f[e] = -INFINITY;
+                        }
+                        slot += __popcll(mask[e]);
+                    }
+                    top = fmaxf(top, f[e]);
                 }
-                if (q >> PER & 1) sh.cand[slot] = place(score_key(xh), tid);
-            },
-            [&](int e, u64 tau) { return place(score_key(e == PER ? xh : load_elem(x, cls(e))), cls(e)) > tau; }, rest, c);
-        if (kept) {
+            }
+            if (have > buffer_limit(k)) compact<T, W>(sh, tid, have, k, rest, c);
+        } else {
+            uint32_t pending = 0;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) pending |= (uint32_t)(mask[e] >> lane & 1) << e;
+            auto cls = [&](int e) { return sp.vec_at(b * G * NB + (e / VEC) * G + tid) + e % VEC; };
+            have = before;
+            const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, pending, [&](int e) { return load_elem(x, cls(e)); }, cls, rest, c);
             top = -INFINITY;
 #pragma unroll
             for (int e = 0; e < PER; ++e) { if (kept >> e & 1) f[e] = -INFINITY; top = fmaxf(top, f[e]); }
@@ -348,17 +384,20 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
         const float ref = rest.m == -INFINITY ? 0.f : rest.m;
 #pragma unroll
         for (int e = 0; e < PER; ++e) rest.s += exp2_32((f[e] - ref) * c);
-        if (b == b0 && with_head && tid < sp.head && !(kept >> PER & 1)) { if (xh != xh) rest.s = NAN; else rest.take(xh, c); }
     }
-    if (with_tail && sp.edge > sp.head) {          // the classes behind the last whole vector, last in the order of classes
-        const int tail = sp.edge - sp.head, j = n - tail + tid;
-        const float xt = tid < tail ? load_elem(x, j) : 0.f;
-        const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, tid < tail && !(xt <= sh.lim) ? 1u : 0u,
-            [&](uint32_t, int slot) { sh.cand[slot] = place(score_key(xt), j); },
-            [&](int, u64 tau) { return place(score_key(xt), j) > tau; }, rest, c);
-        if (tid < tail && !kept) { if (xt != xt) rest.s = NAN; else rest.take(xt, c); }
+    // the row's ends, behind the last whole vector last in the order of classes; in front of the first they come first, so
+    // those are held against the bound with their class
+    for (int end = 0; end < 2; ++end) {
+        const int some = end ? sp.edge - sp.head : sp.head, j = end ? n - some + tid : tid;
+        if (!(end ? with_tail : with_head) || some == 0) continue;
+        const float xe = tid < some ? load_elem(x, j) : 0.f;
+        const u64 tau = sh.tau;
+        const bool maybe = tid < some && (tau ? place(score_key(xe), j) > tau : !(xe <= sh.lim));
+        const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, maybe ? 1u : 0u, [&](int) { return xe; }, [&](int) { return j; }, rest, c);
+        if (tid < some && !kept) { if (xe != xe) rest.s = NAN; else rest.take(xe, c); }
     }
-    compact<T, W>(sh, tid, have, k, rest, c);
+    if (have > G || a.pieces > 1) compact<T, W>(sh, tid, have, k, rest, c);
+    else group_sync<W>();
     bool nan = rest.s != rest.s;
     if constexpr (W == 1) nan = __ballot(nan) != 0; else nan = __syncthreads_or(nan);
     if (nan) {
@@ -366,10 +405,10 @@ __global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
         slow_row<T, W>(x, lo, hi, tid, k, sh, rest, c);
         have = min(k, hi - lo);
     }
+    if (a.pieces == 1) write_row<W>(a, r, sh, tid, have, rest);
     float m; double s;
     join_rest<W>(sh, tid, rest, c, m, s);
     if (a.pieces == 1) {
-        write_row<W>(a, r, sh, tid);
         if (tid == 0) a.rest[r] = s != s ? NAN : m == -INFINITY ? -INFINITY : (float)((double)m / a.T + log(s));
     } else {
         for (int i = tid; i < k; i += G) a.part[job * k + i] = i < have ? sh.cand[i] : 0;
@@ -435,7 +474,7 @@ __global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a) {
             else if (p) { const float x = key_score((uint32_t)(p >> 32)); if (x != x) rest.s = NAN; else rest.take(x, a.c); }
         }
     __syncthreads();
-    write_row<4>(a, r, sh, tid);
+    write_row<4>(a, r, sh, tid, k, rest);
     float m; double s;
     join_rest<4>(sh, tid, rest, a.c, m, s);
     if (tid == 0) a.rest[r] = s != s ? NAN : m == -INFINITY ? -INFINITY : (float)((double)m / a.T + log(s));
