@@ -4,14 +4,27 @@
 //   keep the first top_k (0: all); of these the shortest prefix whose sum reaches top_p times the sum of all of these;
 //   of these those with w_j >= min_p (the first class is always kept);
 //   answer the first kept class j, by class number, with  sum_{i <= j, kept} w_i > u * sum of the kept w.
-// All three cuts keep a prefix of that order, so the kept set is a pair (key, class): every class with a larger key, and
-// of the classes with that key those up to that class.  Weights and sums are held in 64 bits: the answer is a whole number,
-// and a sum in 32 bits would move it wherever u falls within 1e-7 of a border between two classes.
+// All three cuts keep a prefix of that order, so the kept set is a pair (score xt, class ti): every class with a larger
+// score, and of the classes with that score those up to ti.  Weights and sums are held in 64 bits: the answer is a whole
+// number, and a sum in 32 bits would move it wherever u falls within 1e-7 of a border between two classes.
+//
+// One workgroup a row.  Every look at the row is a pass over it; after the first one it comes from the caches (a row in
+// registers was tried: fully unrolled passes with 64-bit weights spill).  What the cuts need of it:
+//   top_k up to a few hundred: k of the threads' maxima reach a bound that about k to 2k scores reach; those go to a list
+//     in LDS, where everything else happens, and no weight of any other class is computed;
+//   larger top_k: bisection of the key, one comparison a score and step;
+//   top_p: the weights of all that is kept so far, summed up and at the same time by 128 bins of their score (64-bit
+//     integers, so that the order of the additions does not matter); the bin in which the sum crosses gives a short list
+//     in which the border is bisected; what lies above it is summed exactly;
+//   the answer: sums of the kept weights by cells (64 consecutive vectors: one wave's step), the cell in which u falls,
+//     then the lane, then the class.
 #include "scores.h"
 
 namespace {
 
 constexpr double LOG2E = 1.4426950408889634074;
+constexpr int BINS = 128;
+typedef unsigned long long u64;
 
 struct SampleArgs {
     const void* x; size_t stride; const float* u;
@@ -20,121 +33,601 @@ struct SampleArgs {
     long long* labels; float* logp; int n;
 };
 
-constexpr int W = 16, NT = W * 64;
+__device__ __forceinline__ u64 place(uint32_t key, int j) { return ((u64)key << 32) | (uint32_t)~j; }
+__device__ __forceinline__ int place_class(u64 p) { return (int)~(uint32_t)p; }
+__device__ __forceinline__ float place_score(u64 p) { return key_score((uint32_t)(p >> 32)); }
 
-template <typename T>
-__global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
-    __shared__ unsigned long long redu[W];
-    __shared__ int redi[W];
-    __shared__ double redd[W];
+// Weights relative to the row's maximum.  With a maximum of +inf its classes weigh 1, all others nothing.
+struct Weight {
+    double xmax, c; bool inf;
+    __device__ __forceinline__ double operator()(float x) const {
+        if (inf) return x == INFINITY ? 1.0 : 0.0;
+        return exp2_64(((double)x - xmax) * c);
+    }
+};
+
+// The kept set: x > xt, or x == xt and class <= ti.
+struct Cut {
+    float xt; int ti;
+    __device__ __forceinline__ bool operator()(float x, int j) const { return x > xt || (x == xt && j <= ti); }
+};
+
+template <int W, int CELLS> struct Shared {
+    static constexpr int CAP = W * 256;            // four places a thread
+    static constexpr int COPIES = W * 4;           // of the bins: one for every fourth lane of a wave
+    union {
+        u64 bins[COPIES][BINS];
+        struct { u64 list[CAP]; double mass[CAP]; } l;
+    };
+    union { double sum[CELLS]; int count[CELLS]; } cell;
+    u64 total[BINS];
+    double redd[W]; u64 redu[W]; int redi[W]; uint32_t red2[2][W];
+    int pick; double before; Cut cut;
+};
+
+// One row as its workgroup of W waves sees it: steps of one vector a thread.
+// Cells in the order of the classes: the row's front end, then vector cells (step i, wave w), then its back end.
+template <typename T, int W> struct Row {
+    static constexpr int VEC = ET<T>::VEC, G = W * 64;
+    const T* x;
+    RowSpan<T> sp;
+    int n, tid, lane, wave, steps;
+    float xe;                                      // of the threads below sp.edge
+
+    __device__ __forceinline__ Row(const T* x_, int n_) : x(x_), sp(x_, n_), n(n_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6) {
+        steps = (sp.nvec + G - 1) / G;
+        xe = tid < sp.edge ? load_elem(x, sp.edge_at(tid)) : -INFINITY;
+    }
+    __device__ __forceinline__ i32x4 load(int i) const { return i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>(); }
+    __device__ __forceinline__ bool valid(int i) const { return i * G + tid < sp.nvec; }
+    __device__ __forceinline__ int cls(int i, int e) const { return sp.vec_at(i * G + tid) + e; }
+    __device__ __forceinline__ int cells() const { return steps * W + 2; }
+    __device__ __forceinline__ int cell(int i) const { return 1 + i * W + wave; }
+    // f(i, scores of vector i); scores beyond the row are -inf.  Three steps' loads are under way at a time.
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        i32x4 v0 = load(0), v1 = load(1), v2 = load(2);
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+            float s[VEC];
+            unpack16<T>(v0, s);
+            v0 = v1; v1 = v2; v2 = load(i + 3);
+            f(i, s);
+        }
+    }
+    // f(scores of vector i), by the wave that has that cell
+    template <typename F> __device__ __forceinline__ void at_cell(int c, F f) const {
+        const int i = (c - 1) / W;
+        if (c < 1 || c > steps * W || (c - 1) % W != wave) return;
+        float s[VEC];
+        unpack16<T>(load(i), s);
+        f(i, s);
+    }
+};
+
+// Largest v in [lo, hi] with enough(v), which holds at lo.
+template <typename F> __device__ __forceinline__ uint32_t last_enough(uint32_t lo, uint32_t hi, F enough) {
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        if (enough(mid)) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// How many of `ties` equal weights `one` the sum needs to get from `over` to target: at least one, at most all.
+__device__ __forceinline__ int ties_needed(double over, double one, double target, int ties) {
+    int m = (int)fmin(fmax(ceil((target - over) / one), 1.0), (double)ties);
+    while (m > 1 && over + (m - 1) * one >= target) --m;
+    while (m < ties && over + m * one < target) ++m;
+    return m;
+}
+
+// Places in LDS, four a thread of a workgroup of W waves or, for lists of at most 256, of its first wave alone (V = 1: no
+// barriers).
+template <int V, typename S> struct List {
+    static constexpr int G = V * 64;
+    S& sh;
+    int tid, lane, wave, n;                        // n: classes of the row
+    u64 lp[4]; double lw[4];
+    __device__ __forceinline__ List(S& s, int c, int n_, const Weight& weight) : sh(s), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), n(n_) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { lp[i] = tid + G * i < c ? sh.l.list[tid + G * i] : 0; lw[i] = lp[i] ? weight(place_score(lp[i])) : 0.0; }
+    }
+    template <typename P> __device__ __forceinline__ int count(P pred) {
+        int m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m += __popcll(__ballot(lp[i] && pred(lp[i])));
+        if constexpr (V == 1) return m;
+        __syncthreads();
+        if (lane == 0) sh.redi[wave] = m;
+        __syncthreads();
+        m = 0;
+#pragma unroll
+        for (int w = 0; w < V; ++w) m += sh.redi[w];
+        return m;
+    }
+    template <typename P> __device__ __forceinline__ double mass(P pred) {
+        double m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (lp[i] && pred(lp[i])) m += lw[i];
+        m = wave_sum(m);
+        if constexpr (V == 1) return m;
+        __syncthreads();
+        if (lane == 0) sh.redd[wave] = m;
+        __syncthreads();
+        m = 0;
+#pragma unroll
+        for (int w = 0; w < V; ++w) m += sh.redd[w];
+        return m;
+    }
+    __device__ __forceinline__ void range(uint32_t& lo, uint32_t& hi) {
+        uint32_t l = 0, h = 0;                     // ~ of the smallest key, the largest
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (lp[i]) { l = max(l, ~(uint32_t)(lp[i] >> 32)); h = max(h, (uint32_t)(lp[i] >> 32)); }
+        lo = ~block_reduce<V>(l, OpMax(), sh.red2[0]);
+        hi = block_reduce<V>(h, OpMax(), sh.red2[1]);
+    }
+    static __device__ __forceinline__ uint32_t key(u64 e) { return (uint32_t)(e >> 32); }
+    // the m-th by class of the entries with key v
+    __device__ __forceinline__ int tie(uint32_t v, int m) {
+        return (int)~last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return count([&](u64 e) { return key(e) == v && (uint32_t)e >= mid; }) >= m; });
+    }
+    // the first k entries
+    __device__ __forceinline__ Cut cut_count(int k) {
+        uint32_t lo, hi;
+        range(lo, hi);
+        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return count([&](u64 e) { return key(e) >= mid; }) >= k; });
+        const int above = count([&](u64 e) { return key(e) > v; }), ties = count([&](u64 e) { return key(e) == v; });
+        return {key_score(v), above + ties > k ? tie(v, k - above) : n};
+    }
+    // the shortest prefix that, after `above`, reaches the target; `was`: what cut the entries so far
+    __device__ __forceinline__ Cut cut_mass(double above, double target, const Weight& weight, const Cut& was) {
+        uint32_t lo, hi;
+        range(lo, hi);
+        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass([&](u64 e) { return key(e) >= mid; }) >= target; });
+        const double over = above + mass([&](u64 e) { return key(e) > v; });
+        const int ties = count([&](u64 e) { return key(e) == v; });
+        const int m = ties_needed(over, weight(key_score(v)), target, ties);
+        const float x = key_score(v);
+        return {x, m < ties ? tie(v, m) : x == was.xt ? was.ti : n};
+    }
+    __device__ __forceinline__ void keep(const Cut& cut) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (lp[i] && !cut(place_score(lp[i]), place_class(lp[i]))) { lp[i] = 0; lw[i] = 0; }
+    }
+    // The answer, from entries that are all there is: (class, log of its share) by one thread.
+    template <typename A> __device__ __forceinline__ void draw(float u, double least, A answer) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (lw[i] == 0 || lw[i] < least) lp[i] = 0;
+        int c = 0;                                 // packed: places and weights
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u64 b = __ballot(lp[i] != 0);
+            int at = c;
+            if constexpr (V == 1) c += __popcll(b);
+            else {
+                __syncthreads();
+                if (lane == 0) sh.redi[wave] = __popcll(b);
+                __syncthreads();
+                for (int w = 0; w < V; ++w) { if (w < wave) at += sh.redi[w]; c += sh.redi[w]; }
+            }
+            if (lp[i]) { sh.l.list[at + lanes_below(b)] = lp[i]; sh.l.mass[at + lanes_below(b)] = lw[i]; }
+        }
+        if constexpr (V == 1) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); } else __syncthreads();
+        double all = 0, front[4] = {0, 0, 0, 0};   // the mass of lower classes
+        for (int o = 0; o < c; ++o) {
+            const u64 e = sh.l.list[o];
+            const double w = sh.l.mass[o];
+            all += w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if ((uint32_t)e > (uint32_t)lp[i]) front[i] += w;
+        }
+        const double target = (double)u * all;
+        // the first class whose sum exceeds the target; the last one if rounding leaves none.  Lower class = larger ~class.
+        u64 best = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lp[i]) best = max(best, front[i] + lw[i] > target ? (1ull << 32) | (uint32_t)lp[i] : (u64)(uint32_t)~(uint32_t)lp[i] + 1);
+        best = block_reduce<V>(best, OpMax(), sh.redu);
+        const uint32_t who = best >> 32 ? (uint32_t)best : ~(uint32_t)(best - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (lp[i] && (uint32_t)lp[i] == who) answer(place_class(lp[i]), (float)log(lw[i] / all));
+    }
+};
+
+template <typename T, int W, int CELLS>
+__global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
+    typedef Row<T, W> R;
+    typedef Shared<W, CELLS> S;
+    constexpr int VEC = R::VEC, G = R::G, CAP = S::CAP;
+    __shared__ S sh;
     const size_t r = blockIdx.x;
-    const int tid = threadIdx.x, n = a.n;
-    const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
+    const R row((const T*)((const char*)a.x + r * a.stride * ET<T>::ES), a.n);
+    const int tid = row.tid, lane = row.lane, wave = row.wave, n = a.n;
     const float u = a.u[r], t = a.tp ? a.tp[r] : a.t, p = a.pp ? a.pp[r] : a.p, q = a.qp ? a.qp[r] : a.q;
     int k = a.kp ? a.kp[r] : a.k;
-    auto answer = [&](int label, float lp) { if (tid == 0) { a.labels[r] = label; a.logp[r] = lp; } };
+    auto answer = [&](int label, float lp) { a.labels[r] = label; a.logp[r] = lp; };       // by one thread
 
-    unsigned long long best = 0;
-    for (int j = tid; j < n; j += NT) {
-        const unsigned long long v = ((unsigned long long)score_key(load_elem(x, j)) << 32) | (uint32_t)~j;
-        if (v > best) best = v;
+    // the row's maximum, its smallest finite score, and whether a NaN is there
+    float mine = row.xe, low = row.xe > -INFINITY ? row.xe : INFINITY;
+    bool nan = row.xe != row.xe;
+    row.each([&](int i, const float* s) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { mine = fmaxf(mine, s[e]); nan |= s[e] != s[e]; low = fminf(low, s[e] > -INFINITY ? s[e] : INFINITY); }
+    });
+    const uint32_t top = block_reduce<W>(nan ? KEY_NAN : score_key(mine), OpMax(), sh.red2[0]);
+    if (top == KEY_NAN || !(t >= 0.f) || !(t < INFINITY) || k < 0 || !(p > 0.f) || !(p <= 1.f) || !(q >= 0.f) || !(q <= 1.f) || !(u >= 0.f) || !(u < 1.f)) {
+        if (tid == 0) answer(-1, NAN);
+        return;
     }
-    best = block_reduce<W>(best, OpMax(), redu);
-    const uint32_t top = (uint32_t)(best >> 32);
-    if (top == KEY_NAN || !(t >= 0.f) || !(t < INFINITY) || k < 0 || !(p > 0.f) || !(p <= 1.f) || !(q >= 0.f) || !(q <= 1.f) || !(u >= 0.f) || !(u < 1.f))
-        return answer(-1, NAN);
-    if (top == KEY_NEG_INF) return answer(-1, -INFINITY);
-    if (t == 0.f || k == 1) return answer((int)~(uint32_t)best, 0.f);
-    if (k == 0 || k > n) k = n;
+    if (top == KEY_NEG_INF) { if (tid == 0) answer(-1, -INFINITY); return; }
     const float xmax = key_score(top);
-    const double c = LOG2E / (double)t;
-    auto weight = [&](float v) { return v == xmax ? 1.0 : exp2_64(((double)v - (double)xmax) * c); };
+    const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, xmax == INFINITY};
+    if (t == 0.f || k == 1) {
+        int at = n;
+        row.each([&](int i, const float* s) {
+#pragma unroll
+            for (int e = VEC - 1; e >= 0; --e) if (s[e] == xmax) at = min(at, row.cls(i, e));
+        });
+        if (tid < row.sp.edge && row.xe == xmax) at = min(at, row.sp.edge_at(tid));
+        at = (int)~block_reduce<W>(~(uint32_t)at, OpMax(), sh.red2[1]);
+        if (tid == 0) answer(at, 0.f);
+        return;
+    }
+    if (k == 0 || k > n) k = n;
 
-    uint32_t tk = 0; int ti = n;                           // kept: key > tk, or key == tk and class <= ti
-    auto kept = [&](uint32_t key, int j) { return key > tk || (key == tk && j <= ti); };
+    Cut cut = {-INFINITY, n};
+    auto count_waves = [&](int m) {                // sum over the waves of a number that is the same in a wave's lanes
+        __syncthreads();
+        if (lane == 0) sh.redi[wave] = m;
+        __syncthreads();
+        int s = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += sh.redi[w];
+        return s;
+    };
+    auto sum_double = [&](double m) {
+        m = wave_sum(m);
+        if constexpr (W == 1) return m;
+        __syncthreads();
+        if (lane == 0) sh.redd[wave] = m;
+        __syncthreads();
+        double s = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += sh.redd[w];
+        return s;
+    };
+    // scores that pass, counted
     auto count = [&](auto pred) {
         int m = 0;
-        for (int j = tid; j < n; j += NT) m += pred(score_key(load_elem(x, j)), j) ? 1 : 0;
-        return block_reduce<W>(m, OpSum(), redi);
+        row.each([&](int i, const float* s) {
+            const bool ok = row.valid(i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m += __popcll(__ballot(ok && pred(s[e], row.cls(i, e))));
+        });
+        if (wave == 0) m += __popcll(__ballot(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))));
+        return count_waves(m);
     };
+    // weights of the scores that pass, summed in a fixed order
     auto mass = [&](auto pred) {
         double m = 0;
-        for (int j = tid; j < n; j += NT) { const float v = load_elem(x, j); if (pred(score_key(v), j)) m += weight(v); }
-        return block_reduce<W>(m, OpSum(), redd);
+        row.each([&](int i, const float* s) {
+            const bool ok = row.valid(i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (ok && pred(s[e], row.cls(i, e))) m += weight(s[e]);
+        });
+        if (tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))) m += weight(row.xe);
+        return sum_double(m);
     };
-    // the largest key v with enough(v), which holds for 0 and not beyond `top`
-    auto bisect = [&](auto enough) {
-        uint32_t lo = tk, hi = top;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo + 1) / 2;
-            if (enough(mid)) lo = mid; else hi = mid - 1;
+    // counts by cells of the scores that pass, as prefix sums: cell.count[c] = how many lie in front of cell c.  Returns all.
+    auto count_cells = [&](auto pred) {
+        __syncthreads();
+        const int cells = row.cells();
+        row.each([&](int i, const float* s) {
+            const bool ok = row.valid(i);
+            int m = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m += __popcll(__ballot(ok && pred(s[e], row.cls(i, e))));
+            if (lane == 0) sh.cell.count[row.cell(i)] = m;
+        });
+        if (wave == 0) {
+            const u64 b = __ballot(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))), front = (1ull << row.sp.head) - 1;
+            if (lane == 0) { sh.cell.count[0] = __popcll(b & front); sh.cell.count[cells - 1] = __popcll(b & ~front); }
         }
-        return lo;
-    };
-    // the class of the m-th one with key v (among the kept)
-    auto nth = [&](uint32_t v, int m) {
-        int lo = 0, hi = n - 1;
-        while (lo < hi) {
-            const int mid = lo + (hi - lo) / 2;
-            if (count([&](uint32_t key, int j) { return key == v && j <= mid; }) >= m) hi = mid; else lo = mid + 1;
+        __syncthreads();
+        if (wave == 0) {
+            int run = 0;
+            for (int c = 0; c < cells; c += 64) {
+                const int m = c + lane < cells ? sh.cell.count[c + lane] : 0;
+                int s = m;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(s, d); if (lane >= d) s += o; }
+                if (c + lane < cells) sh.cell.count[c + lane] = run + s - m;
+                run += __shfl(s, 63);
+            }
+            if (lane == 0) sh.pick = run;
         }
-        return lo;
+        __syncthreads();
+        return sh.pick;
     };
+    // The scores that pass, as places in the list, in the order of the cells; count_cells(pred) was called before.
+    auto collect = [&](auto pred) {
+        row.each([&](int i, const float* s) {
+            const bool ok = row.valid(i);
+            int at = -1;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const bool in = ok && pred(s[e], row.cls(i, e));
+                const u64 b = __ballot(in);
+                if (b) {
+                    if (at < 0) at = sh.cell.count[row.cell(i)];
+                    if (in) sh.l.list[at + lanes_below(b)] = place(score_key(s[e]), row.cls(i, e));
+                    at += __popcll(b);
+                }
+            }
+        });
+        if (wave == 0) {
+            const bool in = tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid));
+            const u64 b = __ballot(in), front = (1ull << row.sp.head) - 1;
+            if (in) {
+                const bool f = tid < row.sp.head;
+                sh.l.list[sh.cell.count[f ? 0 : row.cells() - 1] + lanes_below(f ? b : b & ~front)] = place(score_key(row.xe), row.sp.edge_at(tid));
+            }
+        }
+        __syncthreads();
+    };
+    // The class of the m-th one, by class, of the scores equal to x.
+    auto nth = [&](float x, int m) {
+        auto is = [&](float s, int) { return s == x; };
+        count_cells(is);
+        if (wave == 0) {                           // the last cell with fewer than m in front of it
+            int c = 0;
+            for (int b = 0; b < row.cells(); b += 64) {
+                const bool in = b + lane < row.cells() && sh.cell.count[b + lane] < m;
+                c += __popcll(__ballot(in));
+            }
+            if (lane == 0) sh.pick = c - 1;
+        }
+        __syncthreads();
+        const int c = sh.pick, cells = row.cells();
+        const int left = m - sh.cell.count[c];     // the left-th one of that cell
+        row.at_cell(c, [&](int i, const float* s) {
+            int own = 0;
+            const bool ok = row.valid(i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) own += ok && s[e] == x ? 1 : 0;
+            int s0 = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(s0, d); if (lane >= d) s0 += o; }
+            if (s0 - own < left && left <= s0) {
+                int rank = s0 - own;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) if (s[e] == x && ++rank == left) sh.redi[0] = row.cls(i, e);
+            }
+        });
+        if (wave == 0 && (c == 0 || c == cells - 1)) {
+            const u64 b = __ballot(tid < row.sp.edge && row.xe == x), front = (1ull << row.sp.head) - 1, here = c == 0 ? b & front : b & ~front;
+            if ((here >> lane & 1) && lanes_below(here) == left - 1) sh.redi[0] = row.sp.edge_at(tid);
+        }
+        __syncthreads();
+        const int j = sh.redi[0];
+        __syncthreads();
+        return j;
+    };
+    constexpr int SHIFT = ET<T>::IS_BF16 ? 16 : 0; // bits of a key that carry nothing
+    auto wide_key = [](uint32_t s) { return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s; };
+
+    // min_p: a weight is only computed where a 32-bit estimate of the border, with room, says that it may pass
+    const double least = q > 0.f ? (double)q : 0.0;
+    const float xq = q > 0.f && !weight.inf ? (float)((double)xmax + (log2((double)q) - 1e-3) / weight.c) : -INFINITY;
+    const float xlow = xq - fabsf(xq) * 1e-6f;
+
+    // ---- top_k ------------------------------------------------------------------------------------------------------
     if (k < n) {
-        const uint32_t v = bisect([&](uint32_t mid) { return count([&](uint32_t key, int) { return key >= mid; }) >= k; });
-        const int above = count([&](uint32_t key, int) { return key > v; });
-        ti = nth(v, k - above);
-        tk = v;
+        int c = 0;
+        float bound = -INFINITY;
+        if (k <= G / 2) {                          // k of the threads' maxima
+            const uint32_t key = score_key(mine) >> SHIFT;
+            const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) { return count_waves(__popcll(__ballot(key >= mid))) >= k; });
+            bound = wide_key(v) > KEY_NEG_INF ? key_score(wide_key(v)) : -INFINITY;
+            if (bound > -INFINITY) c = count_cells([&](float s, int) { return s >= bound; });
+        }
+        if (c >= k && c <= CAP) {
+            // the list holds everything: top_k, top_p and the answer from it
+            collect([&](float s, int) { return s >= bound; });
+            auto rest = [&](auto list) {
+                cut = list.cut_count(k);
+                list.keep(cut);
+                if (p < 1.f) { cut = list.cut_mass(0.0, (double)p * list.mass([](u64) { return true; }), weight, cut); list.keep(cut); }
+                list.draw(u, least, answer);
+            };
+            if (c <= 256) { if (wave == 0) rest(List<1, S>(sh, c, n, weight)); }
+            else rest(List<W, S>(sh, c, n, weight));
+            return;
+        }
+        const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) {
+            const float s = key_score(wide_key(mid));
+            return wide_key(mid) <= KEY_NEG_INF || count([&](float x, int) { return x >= s; }) >= k; });
+        if (wide_key(v) > KEY_NEG_INF) {           // else only scores of -inf, which weigh nothing, are cut
+            const float x = key_score(wide_key(v));
+            const int above = count([&](float s, int) { return s > x; }), ties = count([&](float s, int) { return s == x; });
+            cut = {x, above + ties > k ? nth(x, k - above) : n};
+        }
     }
+    // ---- top_p ------------------------------------------------------------------------------------------------------
     if (p < 1.f) {
-        const double target = (double)p * mass(kept);
-        const uint32_t v = bisect([&](uint32_t mid) { return mass([&](uint32_t key, int j) { return kept(key, j) && key >= mid; }) >= target; });
-        const double above = mass([&](uint32_t key, int) { return key > v; }), one = weight(key_score(v));
-        const int ties = count([&](uint32_t key, int j) { return key == v && kept(key, j); });
-        int m = ties;
-        if (above + (ties - 1) * one >= target) {          // not all of them: the smallest m with above + m * one >= target
-            m = (int)ceil((target - above) / one);
-            if (m < 1) m = 1;
-            if (m > ties) m = ties;
-            while (m > 1 && above + (m - 1) * one >= target) --m;
-            while (m < ties && above + m * one < target) ++m;
+        auto from_list = [&](int c, double above, double target) {         // the border lies among c listed classes
+            if (c <= 256) {
+                if (wave == 0) {
+                    List<1, S> list(sh, c, n, weight);
+                    if (target < 0) target = (double)p * list.mass([](u64) { return true; });
+                    const Cut to = list.cut_mass(above, target, weight, cut);
+                    if (lane == 0) sh.cut = to;
+                }
+                __syncthreads();
+                cut = sh.cut;
+            } else {
+                List<W, S> list(sh, c, n, weight);
+                if (target < 0) target = (double)p * list.mass([](u64) { return true; });
+                cut = list.cut_mass(above, target, weight, cut);
+            }
+        };
+        if (n <= CAP) {                            // a row that fits in the list
+            const int c = count_cells(cut);
+            collect(cut);
+            from_list(c, 0.0, -1.0);
+        } else {
+            // all weights, and their sums by bins of the score
+            const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
+            float scale = (float)fmin(4.0 * weight.c, 1e30);               // quarter octaves of the weight, or finer where the row is narrower
+            if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
+            auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
+            __syncthreads();
+            for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
+            __syncthreads();
+            u64* mybins = sh.bins[wave * 4 + (lane & 3)];
+            double m = 0;
+            auto drop = [&](float x) {
+                const double w = weight(x);
+                m += w;
+                // w in units of 2^-44: the low bits of w + 2^8
+                const u64 fixed = (u64)__double_as_longlong(w + 256.0) & ((1ull << 52) - 1);
+                if (fixed) atomicAdd(&mybins[bin(x)], fixed);
+            };
+            row.each([&](int i, const float* s) {
+                const bool ok = row.valid(i);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) if (ok && cut(s[e], row.cls(i, e))) drop(s[e]);
+            });
+            if (tid < row.sp.edge && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe);
+            const double target = (double)p * sum_double(m);
+            __syncthreads();
+            for (int b = tid; b < BINS; b += G) {
+                u64 s = 0;
+                for (int i = 0; i < S::COPIES; ++i) s += sh.bins[i][b];
+                sh.total[b] = s;
+            }
+            __syncthreads();
+            // the bins in which the sum may cross the target: units of 2^-44, half a unit a weight of doubt
+            const double unit = 5.684341886080802e-14, doubt = unit * n + 1e-12 * target;
+            double run = 0;
+            int b1 = -1, b2 = -1;
+            for (int b = 0; b < BINS; ++b) {
+                run += (double)sh.total[b] * unit;
+                if (b1 < 0 && run >= target - doubt) b1 = b;
+                if (b2 < 0 && run >= target + doubt) b2 = b;
+            }
+            if (b1 < 0) b1 = BINS - 1;
+            if (b2 < 0) b2 = BINS - 1;
+            auto inside = [&](float x, int j) { const int b = bin(x); return b >= b1 && b <= b2 && cut(x, j); };
+            const double above = mass([&](float x, int j) { return bin(x) < b1 && cut(x, j); });
+            const int c = count_cells(inside);
+            if (c <= CAP) {
+                collect(inside);
+                from_list(c, above, target);
+            } else {
+                // many equal or nearly equal scores: bisection over the row
+                uint32_t l = 0, h = 0;
+                auto reach = [&](float x, int j) { if (inside(x, j)) { const uint32_t key = score_key(x); l = max(l, ~key); h = max(h, key); } };
+                row.each([&](int i, const float* s) {
+                    const bool ok = row.valid(i);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) if (ok) reach(s[e], row.cls(i, e));
+                });
+                if (tid < row.sp.edge) reach(row.xe, row.sp.edge_at(tid));
+                const uint32_t lo = ~block_reduce<W>(l, OpMax(), sh.red2[0]), hi = block_reduce<W>(h, OpMax(), sh.red2[1]);
+                const float x = key_score(wide_key(last_enough(lo >> SHIFT, hi >> SHIFT, [&](uint32_t mid) {
+                    const float s = key_score(wide_key(mid));
+                    return above + mass([&](float x, int j) { return x >= s && inside(x, j); }) >= target; })));
+                const double over = above + mass([&](float s, int j) { return s > x && inside(s, j); });
+                const int ties = count([&](float s, int j) { return s == x && cut(s, j); });
+                const int need = ties_needed(over, weight(x), target, ties);
+                cut = {x, need < ties ? nth(x, need) : x == cut.xt ? cut.ti : n};
+            }
         }
-        ti = nth(v, m);
-        tk = v;
     }
-    if (q > 0.f) {
-        uint32_t lo = tk, hi = top;                        // the smallest key that weighs enough
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (weight(key_score(mid)) >= (double)q) hi = mid; else lo = mid + 1;
-        }
-        if (lo > tk) { tk = lo; ti = n; }
-    }
-    const double total = mass(kept), target = (double)u * total;
-    double before = 0;
-    __shared__ int found; __shared__ double wave_sum[W];
-    int last = 0;
-    for (int base = 0; base < n; base += NT) {
-        const int j = base + tid;
+    // ---- the answer -------------------------------------------------------------------------------------------------
+    auto share = [&](float x, int j) {             // the weight of a class that is kept, else 0
         double w = 0;
-        if (j < n) { const float v = load_elem(x, j); if (kept(score_key(v), j)) w = weight(v); }
-        double s = w;                                      // inclusive prefix within the wave
-        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(s, d); if ((tid & 63) >= d) s += o; }
-        __syncthreads();
-        if (tid == 0) found = n;
-        if ((tid & 63) == 63) wave_sum[tid >> 6] = s;
-        __syncthreads();
-        double b = before;
-        for (int i = 0; i < (tid >> 6); ++i) b += wave_sum[i];
-        if (w > 0 && b + s > target) atomicMin(&found, j);
-        for (int i = 0; i < W; ++i) before += wave_sum[i];
-        __syncthreads();
-        if (found < n) break;
-        const unsigned long long any = w > 0 ? (unsigned long long)j + 1 : 0;
-        last = max(last, (int)block_reduce<W>(any, OpMax(), redu));
+        if (x >= xlow && cut(x, j)) { w = weight(x); if (w < least) w = 0; }
+        return w;
+    };
+    __syncthreads();
+    row.each([&](int i, const float* s) {
+        const bool ok = row.valid(i);
+        double m = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) if (ok) m += share(s[e], row.cls(i, e));
+        m = __ballot(m != 0) ? wave_sum(m) : 0.0;
+        if (lane == 0) sh.cell.sum[row.cell(i)] = m;
+    });
+    const int cells = row.cells();
+    if (wave == 0) {
+        const double w = tid < row.sp.edge ? share(row.xe, row.sp.edge_at(tid)) : 0.0;
+        const double f = wave_sum(tid < row.sp.head ? w : 0.0), b = wave_sum(tid < row.sp.head ? 0.0 : w);
+        if (lane == 0) { sh.cell.sum[0] = f; sh.cell.sum[cells - 1] = b; }
     }
-    const int j = found < n ? found : last - 1;            // u next to 1 and the last sum rounded down
-    answer(j, (float)log(weight(load_elem(x, j)) / total));
+    __syncthreads();
+    double all = 0;
+    if (wave == 0) {
+        for (int c = 0; c < cells; c += 64) all += wave_sum(c + lane < cells ? sh.cell.sum[c + lane] : 0.0);
+        const double target = (double)u * all;
+        // the first cell whose running sum exceeds the target, or the last one that holds anything
+        double run = 0, found_before = 0;
+        int found = -1, last = 0; double last_before = 0;
+        for (int c = 0; c < cells; c += 64) {
+            const double m = c + lane < cells ? sh.cell.sum[c + lane] : 0.0;
+            double s = m;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(s, d); if (lane >= d) s += o; }
+            const u64 hit = __ballot(m > 0 && run + s > target), some = __ballot(m > 0);
+            if (some) { const int l = 63 - __clzll(some); last = c + l; last_before = run + __shfl(s - m, l); }
+            if (hit) { const int l = __ffsll(hit) - 1; found = c + l; found_before = run + __shfl(s - m, l); break; }
+            run += __shfl(s, 63);
+        }
+        if (lane == 0) { sh.pick = found >= 0 ? found : last; sh.before = found >= 0 ? found_before : last_before; sh.redd[0] = all; }
+    }
+    __syncthreads();
+    const int c = sh.pick;
+    const double before = sh.before;
+    all = sh.redd[0];
+    const double target = (double)u * all;
+    auto finish = [&](const double* w, const int* cl, int m) {             // one wave: m weights a lane, classes ascending over lanes
+        double own = 0;
+        for (int e = 0; e < m; ++e) own += w[e];
+        double s = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(s, d); if (lane >= d) s += o; }
+        const double front = before + (s - own);
+        int hit = -1; double hw = 0, run = front;
+        int lastc = -1; double lastw = 0;
+        for (int e = 0; e < m; ++e) {
+            run += w[e];
+            if (w[e] > 0) { lastc = cl[e]; lastw = w[e]; if (hit < 0 && run > target) { hit = cl[e]; hw = w[e]; } }
+        }
+        const u64 b = __ballot(hit >= 0), l = __ballot(lastc >= 0);
+        const int who = b ? __ffsll(b) - 1 : 63 - __clzll(l);
+        if (lane == who) answer(b ? hit : lastc, (float)log((b ? hw : lastw) / all));
+    };
+    row.at_cell(c, [&](int i, const float* s) {
+        double w[VEC]; int cl[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { cl[e] = row.cls(i, e); w[e] = row.valid(i) ? share(s[e], cl[e]) : 0.0; }
+        finish(w, cl, VEC);
+    });
+    if (wave == 0 && (c == 0 || c == cells - 1)) {
+        const bool here = tid < row.sp.edge && (tid < row.sp.head) == (c == 0);
+        const int j = here ? row.sp.edge_at(tid) : 0;
+        const double w = here ? share(row.xe, j) : 0.0;
+        finish(&w, &j, 1);
+    }
+}
+
+template <typename T> void launch(const SampleArgs& a, int rows, hipStream_t s) {
+    constexpr int VEC = ET<T>::VEC;
+    const int nv = a.n / VEC;
+    if (nv <= 128) sample_kernel<T, 1, 4><<<rows, 64, 0, s>>>(a);
+    else if (nv <= 2048) sample_kernel<T, 4, 34><<<rows, 256, 0, s>>>(a);
+    else sample_kernel<T, 16, (1 << 20) / VEC / 64 + 18><<<rows, 1024, 0, s>>>(a);
 }
 
 }  // namespace
@@ -144,9 +637,8 @@ extern "C" int stgcn_sample_labels(int dtype, const void* logits, size_t row_str
                                    int64_t* labels, float* logp, int rows, int ncls, void* stream) {
     if (!logits || !u || !labels || !logp || rows < 1 || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls) return STGCN_ERR_ARG;
     SampleArgs a = {logits, row_stride, u, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p, (long long*)labels, logp, ncls};
-    const hipStream_t s = (hipStream_t)stream;
-    if (dtype == STGCN_BF16) sample_kernel<bf16><<<rows, NT, 0, s>>>(a);
-    else if (dtype == STGCN_F32) sample_kernel<float><<<rows, NT, 0, s>>>(a);
+    if (dtype == STGCN_BF16) launch<bf16>(a, rows, (hipStream_t)stream);
+    else if (dtype == STGCN_F32) launch<float>(a, rows, (hipStream_t)stream);
     else return STGCN_ERR_ARG;
     return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
 }

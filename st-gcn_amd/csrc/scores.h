@@ -27,6 +27,10 @@ template <typename T> __device__ __forceinline__ void store_vec(T* row, int at, 
     *reinterpret_cast<i32x4*>((char*)row + (size_t)at * ET<T>::ES) = raw;
 }
 
+__device__ __forceinline__ int lanes_below(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 // the elements of a vector whose bit is set become -inf
 template <typename T> __device__ __forceinline__ void drop_listed(i32x4& v, uint32_t b) {
     if constexpr (ET<T>::IS_BF16) {
@@ -103,6 +107,24 @@ template <typename V, typename Op> __device__ __forceinline__ V wave_reduce(V v,
     for (int d = 32; d >= 1; d >>= 1) v = op(v, __shfl_xor(v, d));
     return v;
 }
+// Sum over the wave by adds through the data-parallel crossbar (rows of 16 by shifts, then row to row), for every lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, true);
+    return v + __longlong_as_double((long long)hi << 32 | (uint32_t)lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = dpp_add<0x111, 0xF>(v);                            // row_shr 1, 2, 4, 8: lane 15 of a row holds the row's sum
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);                            // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+    v = dpp_add<0x143, 0xC>(v);
+    const long long b = __double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
+    return __longlong_as_double((long long)hi << 32 | lo);
+}
+
 template <int W, typename V, typename Op> __device__ __forceinline__ V block_reduce(V v, Op op, V* red) {
     v = wave_reduce(v, op);
     if constexpr (W == 1) return v;

@@ -62,7 +62,6 @@ template <typename T> __device__ __forceinline__ uint32_t long_key(uint32_t s) {
     return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s;
 }
 
-__device__ __forceinline__ int lanes_below(u64 mask) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)); }
 
 // The k-th largest of `c` numbers v(i) (i < c, c >= k) that are not all distinct, by one wave, bit by bit below those that
 // all have in common; with at most 512 of them they stay in registers.
@@ -269,8 +268,12 @@ template <int W> __device__ __forceinline__ void write_row(const TopArgs& a, siz
     }
 }
 
+// Waves a SIMD that the registers are cut for.  Measured at 4096 x 65536 bf16, k 64: 4 waves 223, 5 waves 207, 6 waves 233 us
+// (spills); 2048 x 65536 float32: 4 waves 102, 5 waves 119 us (k 1); 200000 x 512 bf16, one wave a row, k 16: 247 / 228 / 220 us.
+template <typename T, int W> constexpr int TOP_WAVES = W == 1 ? 6 : ET<T>::IS_BF16 ? 5 : 4;
+
 template <typename T, int W>
-__global__ __launch_bounds__(256) void top_scan_kernel(TopArgs a) {
+__global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArgs a) {
     constexpr int VEC = ET<T>::VEC, G = W * 64, PER = 16, NB = PER / VEC, ROWS = W == 1 ? 4 : 1;
     __shared__ Shared<W> sh_[ROWS];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x;
