@@ -529,8 +529,8 @@ bool bad_common(int dtype, const void* x, size_t stride, const void* idx, int ro
         || k < 1 || k > MAX_K || !(T > 0.0) || !(T < 1e30) || !(w >= 0.0) || !(w <= 1.0);
 }
 
-// The widest row that fits in registers: 8 waves of 16 vectors a lane (64 registers of scores).
-template <typename T> constexpr int row_fits() { return 512 * 16 * ET<T>::VEC; }
+// The widest row that fits in registers: 16 waves of 16 vectors a lane (64 registers of scores).
+template <typename T> constexpr int row_fits() { return 1024 * 16 * ET<T>::VEC; }
 
 template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a, hipStream_t s) {
     constexpr int VEC = ET<T>::VEC;
@@ -542,7 +542,8 @@ template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a
     else if (nv <= 1024) distill_row_kernel<T, 4, 4, TWO, GRAD><<<rows, 256, 0, s>>>(a);
     else if (nv <= 2048) distill_row_kernel<T, 4, 8, TWO, GRAD><<<rows, 256, 0, s>>>(a);
     else if (nv <= 4096) distill_row_kernel<T, 8, 8, TWO, GRAD><<<rows, 512, 0, s>>>(a);
-    else distill_row_kernel<T, 8, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
+    else if (nv <= 8192) distill_row_kernel<T, 8, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
+    else distill_row_kernel<T, 16, 16, TWO, GRAD><<<rows, 1024, 0, s>>>(a);
 }
 template <typename T> void launch_fwd(const DistillArgs& a, bool two, hipStream_t s) {
     if (a.n <= row_fits<T>()) { if (two) launch_rows<T, true, false>(a, s); else launch_rows<T, false, false>(a, s); }

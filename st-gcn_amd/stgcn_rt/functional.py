@@ -10,7 +10,6 @@ sample_labels.
 """
 import collections
 import contextlib
-import copy
 import os
 
 import torch
@@ -401,18 +400,17 @@ class DistillationFn(torch.autograd.Function):
     def forward(ctx, logits, values, indices, rest, labels, temperature, label_weight, reduction):
         call = P.DistillCall(logits, values, indices, rest, labels, temperature, label_weight, reduction)
         loss = call.forward()
-        ctx.save_for_backward(logits, call.indices, call.labels, call.stats, call.probs)
-        call.x = call.values = call.rest = call.indices = call.labels = call.stats = call.probs = None
+        ctx.save_for_backward(logits, call.indices, call.labels, call.kept)
+        call.x = call.values = call.indices = call.rest = call.labels = call.kept = None     # the sizes stay
         ctx.call = call
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        call = copy.copy(ctx.call)
-        logits, call.indices, call.labels, call.stats, call.probs = ctx.saved_tensors
-        call.x = P._check_scores(logits)
-        return (call.backward(g.float().contiguous()),) + (None,) * 7
+        logits, indices, labels, kept = ctx.saved_tensors
+        dx = ctx.call.backward(P._check_scores(logits), indices, labels, kept, g.contiguous())
+        return dx, None, None, None, None, None, None, None
 
 
 def distillation(logits, values, indices, rest=None, labels=None, temperature=1.0, label_weight=0.0, reduction="mean"):

@@ -504,10 +504,11 @@ def _check_scores(x, name="logits"):
         raise ValueError("%s: 1 to %d classes, got %d" % (name, MAX_CLASSES, x.shape[1]))
     if x.shape[0] >= 1 << 31:
         raise ValueError("%s: fewer than 2^31 rows, got %d" % (name, x.shape[0]))
-    x = x.detach()
+    if x.is_contiguous():
+        return x
     if (x.stride(1) == 1 or x.shape[1] == 1) and (x.shape[0] < 2 or x.stride(0) >= x.shape[1]):
         return x
-    return x.contiguous()
+    return x.detach().contiguous()
 
 
 def _row_stride(x):
@@ -515,11 +516,11 @@ def _row_stride(x):
 
 
 def _check_like(t, name, shape, dtype, like):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError("%s wants %s %s, got %s %s" % (name, tuple(shape), dtype, tuple(t.shape), t.dtype))
     if t.device != like.device:
         raise RuntimeError("%s lives on %s, the logits on %s" % (name, t.device, like.device))
-    return t.detach().contiguous()
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
 def _check_temperature(t):
@@ -552,13 +553,16 @@ def top_logits(logits, k, temperature=1.0):
     rest = torch.empty((rows,), dtype=torch.float32, device=x.device)
     if rows:
         ws, nbytes = _call_workspace(x.device, "stgcn_top_logits_workspace", rows, ncls, k)
-        _launch((str(x.dtype), rows, ncls, k), "stgcn_top_logits", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), rows, ncls, k, temperature,
+        _launch(() if TIMING is None else (str(x.dtype), rows, ncls, k), "stgcn_top_logits", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), rows, ncls, k, temperature,
                 L.ptr(values), L.ptr(indices), L.ptr(rest), L.ptr(ws), nbytes, L.stream_ptr())
     return values, indices, rest
 
 
 class DistillCall:
-    """The checked arguments of one distillation call and what its forward leaves for the gradient."""
+    """The checked arguments of one distillation call.  forward() and step() leave `kept` (one buffer: the rows' losses in 64
+    bits, four factors and k shares a row), which the gradient is made from."""
+
+    __slots__ = ("x", "rows", "ncls", "k", "values", "indices", "rest", "labels", "temperature", "label_weight", "reduction", "kept")
 
     def __init__(self, logits, values, indices, rest, labels, temperature, label_weight, reduction):
         self.x = x = _check_scores(logits)
@@ -582,47 +586,49 @@ class DistillCall:
         check_device(x, "logits")
         self.reduction = reduction
 
-    def _buffers(self):
-        rows, dev = self.rows, self.x.device
-        self.stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-        self.probs = torch.empty((rows, self.k), dtype=torch.float32, device=dev)
-        return torch.empty((rows,), dtype=torch.float64, device=dev)
+    def _key(self):
+        return () if TIMING is None else (str(self.x.dtype), self.rows, self.ncls, self.k)
 
-    def _inputs(self):
-        x = self.x
-        return (L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(self.values), L.ptr(self.indices), L.ptr(self.rest), L.ptr(self.labels),
-                self.rows, self.ncls, self.k, self.temperature, self.label_weight, _REDUCTIONS[self.reduction])
+    def _forward(self, name, loss, *more):
+        x, rows = self.x, self.rows
+        self.kept = torch.empty(rows * (6 + self.k), dtype=torch.float32, device=x.device)
+        at = self.kept.data_ptr()                       # losses [rows] float64, factors [rows][4], shares [rows][k]
+        _launch(self._key(), name, L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), self.values.data_ptr(), self.indices.data_ptr(),
+                L.ptr(self.rest), L.ptr(self.labels), rows, self.ncls, self.k, self.temperature, self.label_weight,
+                _REDUCTIONS[self.reduction], loss.data_ptr(), at, at + 8 * rows, at + 24 * rows, *more, L.stream_ptr())
 
     def forward(self):
-        rows, dev = self.rows, self.x.device
-        loss_rows = self._buffers()
-        loss = torch.empty((rows,) if self.reduction == "none" else (), dtype=torch.float32, device=dev)
-        if rows == 0:
-            return loss if self.reduction == "none" else loss.zero_()
-        _launch((str(self.x.dtype), rows, self.ncls, self.k), "stgcn_distill_fwd", *self._inputs(), L.ptr(loss), L.ptr(loss_rows),
-                L.ptr(self.stats), L.ptr(self.probs), L.stream_ptr())
+        none = self.reduction == "none"
+        loss = torch.empty((self.rows,) if none else (), dtype=torch.float32, device=self.x.device)
+        if self.rows:
+            self._forward("stgcn_distill_fwd", loss)
+        else:
+            self.kept = loss
+            if not none:
+                loss.zero_()
         return loss
 
     def step(self):
         """(loss, d loss / d logits) of one call."""
-        rows, dev = self.rows, self.x.device
-        loss_rows = self._buffers()
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        dx = torch.empty((rows, self.ncls), dtype=self.x.dtype, device=dev)
-        if rows == 0:
-            return loss.zero_(), dx
-        _launch((str(self.x.dtype), rows, self.ncls, self.k), "stgcn_distill_step", *self._inputs(), L.ptr(loss), L.ptr(loss_rows),
-                L.ptr(self.stats), L.ptr(self.probs), L.ptr(dx), L.stream_ptr())
+        x = self.x
+        loss = torch.empty((), dtype=torch.float32, device=x.device)
+        dx = torch.empty((self.rows, self.ncls), dtype=x.dtype, device=x.device)
+        if self.rows:
+            self._forward("stgcn_distill_step", loss, dx.data_ptr())
+        else:
+            loss.zero_()
         return loss, dx
 
-    def backward(self, grad):
-        """d loss / d logits times grad (a float32 tensor on the device: one number, or one a row for "none"; None: 1)."""
-        x, rows = self.x, self.rows
+    def backward(self, x, indices, labels, kept, grad):
+        """d loss / d logits times grad (a float32 tensor on the device: one number, or one a row for "none") from what a
+        forward kept."""
+        rows = self.rows
         dx = torch.empty((rows, self.ncls), dtype=x.dtype, device=x.device)
         if rows:
-            _launch((str(x.dtype), rows, self.ncls, self.k), "stgcn_distill_bwd", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(self.indices),
-                    L.ptr(self.labels), L.ptr(self.stats), L.ptr(self.probs), L.ptr(grad), 1 if self.reduction == "none" else 0,
-                    1.0 / rows if self.reduction == "mean" else 1.0, rows, self.ncls, self.k, self.temperature, self.label_weight, L.ptr(dx),
+            at = kept.data_ptr()
+            _launch(self._key(), "stgcn_distill_bwd", L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), indices.data_ptr(), L.ptr(labels),
+                    at + 8 * rows, at + 24 * rows, grad.data_ptr(), 1 if self.reduction == "none" else 0,
+                    1.0 / rows if self.reduction == "mean" else 1.0, rows, self.ncls, self.k, self.temperature, self.label_weight, dx.data_ptr(),
                     L.stream_ptr())
         return dx
 
@@ -664,7 +670,7 @@ def sample_labels(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     labels = torch.empty((rows,), dtype=torch.int64, device=x.device)
     logp = torch.empty((rows,), dtype=torch.float32, device=x.device)
     if rows:
-        _launch((str(x.dtype), rows, ncls), "stgcn_sample_labels", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(u), L.ptr(tt), float(ts),
+        _launch(() if TIMING is None else (str(x.dtype), rows, ncls), "stgcn_sample_labels", L.dtype_code(x.dtype), L.ptr(x), _row_stride(x), L.ptr(u), L.ptr(tt), float(ts),
                 L.ptr(kt), int(ks), L.ptr(pt), float(ps), L.ptr(qt), float(qs), L.ptr(labels), L.ptr(logp), rows, ncls, L.stream_ptr())
     return labels, logp
 
