@@ -12,10 +12,10 @@
 // registers was tried: fully unrolled passes with 64-bit weights spill).  What the cuts need of it:
 //   top_k up to a few hundred: k of the threads' maxima reach a bound that about k to 2k scores reach; those go to a list
 //     in LDS, where everything else happens, and no weight of any other class is computed;
-//   larger top_k: bisection of the key, one comparison a score and step;
-//   top_p: the weights of all that is kept so far, summed up and at the same time by 128 bins of their score (64-bit
-//     integers, so that the order of the additions does not matter); the bin in which the sum crosses gives a short list
-//     in which the border is bisected; what lies above it is summed exactly;
+//   larger top_k, and top_p: the scores (or their weights) counted by 128 bins of the score; the bin in which the count
+//     (the sum) crosses gives a short list, in which the border is bisected.  Bins and list hold weights as 64-bit integers
+//     in units of 2^-s (s = 42 to 50 by the class count): their sums are the same in any order.  A border that falls within
+//     such a unit of a class moves that class alone, by a share of 2^-s of the first class's weight;
 //   the answer: sums of the kept weights by cells (64 consecutive vectors: one wave's step), the cell in which u falls,
 //     then the lane, then the class.
 #include "scores.h"
@@ -39,7 +39,8 @@ __device__ __forceinline__ float place_score(u64 p) { return key_score((uint32_t
 
 // Weights relative to the row's maximum.  With a maximum of +inf its classes weigh 1, all others nothing.
 struct Weight {
-    double xmax, c; bool inf;
+    double xmax, c, unit; bool inf;                // unit: 2^(52 - s); the low 52 bits of w + unit are w in units of 2^-s
+    __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double_as_longlong(w + unit) & ((1ull << 52) - 1); }
     __device__ __forceinline__ double operator()(float x) const {
         if (inf) return x == INFINITY ? 1.0 : 0.0;
         return exp2_64(((double)x - xmax) * c);
@@ -61,7 +62,7 @@ template <int W, int CELLS> struct Shared {
     };
     union { double sum[CELLS]; int count[CELLS]; } cell;
     u64 total[BINS];
-    double redd[W]; u64 redu[W]; int redi[W]; uint32_t red2[2][W];
+    double all; u64 redu[W]; int redi[W]; uint32_t red2[2][W];
     int pick; double before; Cut cut;
 };
 
@@ -114,11 +115,10 @@ template <typename F> __device__ __forceinline__ uint32_t last_enough(uint32_t l
 }
 
 // How many of `ties` equal weights `one` the sum needs to get from `over` to target: at least one, at most all.
-__device__ __forceinline__ int ties_needed(double over, double one, double target, int ties) {
-    int m = (int)fmin(fmax(ceil((target - over) / one), 1.0), (double)ties);
-    while (m > 1 && over + (m - 1) * one >= target) --m;
-    while (m < ties && over + m * one < target) ++m;
-    return m;
+__device__ __forceinline__ int ties_needed(u64 over, u64 one, u64 target, int ties) {
+    if (one == 0 || over + one >= target) return one == 0 ? ties : 1;
+    const u64 m = (target - over + one - 1) / one;
+    return m < (u64)ties ? (int)m : ties;
 }
 
 // Places in LDS, four a thread of a workgroup of W waves or, for lists of at most 256, of its first wave alone (V = 1: no
@@ -145,18 +145,19 @@ template <int V, typename S> struct List {
         for (int w = 0; w < V; ++w) m += sh.redi[w];
         return m;
     }
-    template <typename P> __device__ __forceinline__ double mass(P pred) {
-        double m = 0;
+    // weights of the entries that pass, in integer units
+    template <typename P> __device__ __forceinline__ u64 mass(const Weight& weight, P pred) {
+        u64 m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lp[i] && pred(lp[i])) m += lw[i];
+        for (int i = 0; i < 4; ++i) if (lp[i] && pred(lp[i])) m += weight.fixed(lw[i]);
         m = wave_sum(m);
         if constexpr (V == 1) return m;
         __syncthreads();
-        if (lane == 0) sh.redd[wave] = m;
+        if (lane == 0) sh.redu[wave] = m;
         __syncthreads();
         m = 0;
 #pragma unroll
-        for (int w = 0; w < V; ++w) m += sh.redd[w];
+        for (int w = 0; w < V; ++w) m += sh.redu[w];
         return m;
     }
     __device__ __forceinline__ void range(uint32_t& lo, uint32_t& hi) {
@@ -180,16 +181,17 @@ template <int V, typename S> struct List {
         return {key_score(v), above + ties > k ? tie(v, k - above) : n};
     }
     // the shortest prefix that, after `above`, reaches the target; `was`: what cut the entries so far
-    __device__ __forceinline__ Cut cut_mass(double above, double target, const Weight& weight, const Cut& was) {
+    __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Weight& weight, const Cut& was) {
         uint32_t lo, hi;
         range(lo, hi);
-        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass([&](u64 e) { return key(e) >= mid; }) >= target; });
-        const double over = above + mass([&](u64 e) { return key(e) > v; });
+        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass(weight, [&](u64 e) { return key(e) >= mid; }) >= target; });
+        const u64 over = above + mass(weight, [&](u64 e) { return key(e) > v; });
         const int ties = count([&](u64 e) { return key(e) == v; });
-        const int m = ties_needed(over, weight(key_score(v)), target, ties);
         const float x = key_score(v);
+        const int m = ties_needed(over, weight.fixed(weight(x)), target, ties);
         return {x, m < ties ? tie(v, m) : x == was.xt ? was.ti : n};
     }
+    __device__ __forceinline__ u64 all(const Weight& weight) { return mass(weight, [](u64) { return true; }); }
     __device__ __forceinline__ void keep(const Cut& cut) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) if (lp[i] && !cut(place_score(lp[i]), place_class(lp[i]))) { lp[i] = 0; lw[i] = 0; }
@@ -261,7 +263,8 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     }
     if (top == KEY_NEG_INF) { if (tid == 0) answer(-1, -INFINITY); return; }
     const float xmax = key_score(top);
-    const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, xmax == INFINITY};
+    const int s = min(50, 30 + __clz(n));          // n sums of at most 2^s stay below 2^63
+    const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, (double)(1ull << (52 - s)), xmax == INFINITY};
     if (t == 0.f || k == 1) {
         int at = n;
         row.each([&](int i, const float* s) {
@@ -276,6 +279,7 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     if (k == 0 || k > n) k = n;
 
     Cut cut = {-INFINITY, n};
+    auto mass_target = [&](u64 all) { return (u64)ceil((double)p * (double)all); };
     auto count_waves = [&](int m) {                // sum over the waves of a number that is the same in a wave's lanes
         __syncthreads();
         if (lane == 0) sh.redi[wave] = m;
@@ -283,17 +287,6 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         int s = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) s += sh.redi[w];
-        return s;
-    };
-    auto sum_double = [&](double m) {
-        m = wave_sum(m);
-        if constexpr (W == 1) return m;
-        __syncthreads();
-        if (lane == 0) sh.redd[wave] = m;
-        __syncthreads();
-        double s = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) s += sh.redd[w];
         return s;
     };
     // scores that pass, counted
@@ -307,16 +300,16 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         if (wave == 0) m += __popcll(__ballot(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))));
         return count_waves(m);
     };
-    // weights of the scores that pass, summed in a fixed order
+    // weights of the scores that pass, in integer units
     auto mass = [&](auto pred) {
-        double m = 0;
+        u64 m = 0;
         row.each([&](int i, const float* s) {
             const bool ok = row.valid(i);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) if (ok && pred(s[e], row.cls(i, e))) m += weight(s[e]);
+            for (int e = 0; e < VEC; ++e) if (ok && pred(s[e], row.cls(i, e))) m += weight.fixed(weight(s[e]));
         });
-        if (tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))) m += weight(row.xe);
-        return sum_double(m);
+        if (tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))) m += weight.fixed(weight(row.xe));
+        return block_reduce<W>(m, OpSum(), sh.redu);
     };
     // counts by cells of the scores that pass, as prefix sums: cell.count[c] = how many lie in front of cell c.  Returns all.
     auto count_cells = [&](auto pred) {
@@ -349,31 +342,31 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         __syncthreads();
         return sh.pick;
     };
-    // The scores that pass, as places in the list, in the order of the cells; count_cells(pred) was called before.
+    // The scores that pass, as places in the list (in no particular order: everything that is made of it is a set, or a sum
+    // of integers).  Returns how many there are; more than CAP are not all in it.
     auto collect = [&](auto pred) {
+        __syncthreads();
+        if (tid == 0) sh.pick = 0;
+        __syncthreads();
+        auto append = [&](bool in, float x, int j) {
+            const u64 b = __ballot(in);
+            if (b) {
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&sh.pick, __popcll(b));
+                at = __builtin_amdgcn_readfirstlane(at) + lanes_below(b);
+                if (in && at < CAP) sh.l.list[at] = place(score_key(x), j);
+            }
+        };
         row.each([&](int i, const float* s) {
             const bool ok = row.valid(i);
-            int at = -1;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const bool in = ok && pred(s[e], row.cls(i, e));
-                const u64 b = __ballot(in);
-                if (b) {
-                    if (at < 0) at = sh.cell.count[row.cell(i)];
-                    if (in) sh.l.list[at + lanes_below(b)] = place(score_key(s[e]), row.cls(i, e));
-                    at += __popcll(b);
-                }
-            }
+            for (int e = 0; e < VEC; ++e) append(ok && pred(s[e], row.cls(i, e)), s[e], row.cls(i, e));
         });
-        if (wave == 0) {
-            const bool in = tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid));
-            const u64 b = __ballot(in), front = (1ull << row.sp.head) - 1;
-            if (in) {
-                const bool f = tid < row.sp.head;
-                sh.l.list[sh.cell.count[f ? 0 : row.cells() - 1] + lanes_below(f ? b : b & ~front)] = place(score_key(row.xe), row.sp.edge_at(tid));
-            }
-        }
+        if (wave == 0) append(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid)), row.xe, row.sp.edge_at(tid));
         __syncthreads();
+        const int c = sh.pick;
+        __syncthreads();
+        return c;
     };
     // The class of the m-th one, by class, of the scores equal to x.
     auto nth = [&](float x, int m) {
@@ -421,127 +414,118 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     const float xq = q > 0.f && !weight.inf ? (float)((double)xmax + (log2((double)q) - 1e-3) / weight.c) : -INFINITY;
     const float xlow = xq - fabsf(xq) * 1e-6f;
 
+    // ---- borders ----------------------------------------------------------------------------------------------------
+    // The kept scores (`cut`) by bins: one each, or their weights.
+    float scale = 0.f;                             // quarter octaves of the weight, or finer where the row is narrower
+    auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
+    auto fill_bins = [&](bool weigh) {
+        const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
+        scale = (float)fmin(4.0 * weight.c, 1e30);
+        if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
+        __syncthreads();
+        for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
+        __syncthreads();
+        u64* mybins = sh.bins[wave * 4 + (lane & 3)];
+        auto drop = [&](float x) {
+            const u64 v = weigh ? weight.fixed(weight(x)) : 1;
+            if (v) atomicAdd(&mybins[bin(x)], v);
+        };
+        row.each([&](int i, const float* s) {
+            const bool ok = row.valid(i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (ok && cut(s[e], row.cls(i, e))) drop(s[e]);
+        });
+        if (tid < row.sp.edge && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe);
+        __syncthreads();
+        for (int b = tid; b < BINS; b += G) {
+            u64 s = 0;
+            for (int i = 0; i < S::COPIES; ++i) s += sh.bins[i][b];
+            sh.total[b] = s;
+        }
+        __syncthreads();
+    };
+    // Sum of the bins; the first bin at which the running sum reaches target (by every wave: two bins a lane).
+    auto bin_sum = [&]() { return wave_sum(sh.total[2 * lane] + sh.total[2 * lane + 1]); };
+    auto bin_reach = [&](u64 target, u64& above) {
+        const u64 a0 = sh.total[2 * lane], a1 = sh.total[2 * lane + 1];
+        u64 s = a0 + a1;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const u64 o = __shfl_up(s, d); if (lane >= d) s += o; }
+        const u64 hit = __ballot(s >= target);
+        const int l = hit ? __ffsll(hit) - 1 : 63;
+        const u64 f = __shfl(s, l) - __shfl(a0 + a1, l), m0 = __shfl(a0, l);   // in front of the pair, its first
+        const bool second = f + m0 < target;
+        above = second ? f + m0 : f;
+        return 2 * l + (second ? 1 : 0);
+    };
+    // list(c): work on a list of c places by the first wave alone if they are few; its cut to all
+    auto with_list = [&](int c, auto work) {
+        if (c <= 256) {
+            if (wave == 0) { List<1, S> list(sh, c, n, weight); const Cut to = work(list); if (lane == 0) sh.cut = to; }
+            __syncthreads();
+            cut = sh.cut;
+        } else { List<W, S> list(sh, c, n, weight); cut = work(list); }
+    };
+    // What equal scores x leave of it: all, or the first `need` by class.
+    auto cut_ties = [&](float x, int need, int ties) { cut = {x, need < ties ? nth(x, need) : x == cut.xt ? cut.ti : n}; };
+
     // ---- top_k ------------------------------------------------------------------------------------------------------
     if (k < n) {
-        int c = 0;
-        float bound = -INFINITY;
-        if (k <= G / 2) {                          // k of the threads' maxima
+        if (k <= G / 2) {                          // k of the threads' maxima reach a bound
             const uint32_t key = score_key(mine) >> SHIFT;
             const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) { return count_waves(__popcll(__ballot(key >= mid))) >= k; });
-            bound = wide_key(v) > KEY_NEG_INF ? key_score(wide_key(v)) : -INFINITY;
-            if (bound > -INFINITY) c = count_cells([&](float s, int) { return s >= bound; });
+            const float bound = wide_key(v) > KEY_NEG_INF ? key_score(wide_key(v)) : NAN;
+            const int c = collect([&](float s, int) { return s >= bound; });
+            if (c >= k && c <= CAP) {
+                // the list holds everything: top_k, top_p and the answer from it
+                auto rest = [&](auto list) {
+                    cut = list.cut_count(k);
+                    list.keep(cut);
+                    if (p < 1.f) { cut = list.cut_mass(0, mass_target(list.all(weight)), weight, cut); list.keep(cut); }
+                    list.draw(u, least, answer);
+                };
+                if (c <= 256) { if (wave == 0) rest(List<1, S>(sh, c, n, weight)); }
+                else rest(List<W, S>(sh, c, n, weight));
+                return;
+            }
         }
-        if (c >= k && c <= CAP) {
-            // the list holds everything: top_k, top_p and the answer from it
-            collect([&](float s, int) { return s >= bound; });
-            auto rest = [&](auto list) {
-                cut = list.cut_count(k);
-                list.keep(cut);
-                if (p < 1.f) { cut = list.cut_mass(0.0, (double)p * list.mass([](u64) { return true; }), weight, cut); list.keep(cut); }
-                list.draw(u, least, answer);
-            };
-            if (c <= 256) { if (wave == 0) rest(List<1, S>(sh, c, n, weight)); }
-            else rest(List<W, S>(sh, c, n, weight));
-            return;
-        }
-        const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) {
-            const float s = key_score(wide_key(mid));
-            return wide_key(mid) <= KEY_NEG_INF || count([&](float x, int) { return x >= s; }) >= k; });
-        if (wide_key(v) > KEY_NEG_INF) {           // else only scores of -inf, which weigh nothing, are cut
-            const float x = key_score(wide_key(v));
-            const int above = count([&](float s, int) { return s > x; }), ties = count([&](float s, int) { return s == x; });
-            cut = {x, above + ties > k ? nth(x, k - above) : n};
+        fill_bins(false);
+        u64 above;
+        const int b = bin_reach((u64)k, above);
+        auto inside = [&](float x, int) { return bin(x) == b; };
+        const int c = collect(inside), need = k - (int)above;
+        if (c <= CAP) with_list(c, [&](auto& list) { return list.cut_count(need); });
+        else {                                     // many equal or nearly equal scores: bisection over the row
+            const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) {
+                const float s = key_score(wide_key(mid));
+                return wide_key(mid) <= KEY_NEG_INF || count([&](float x, int) { return x >= s; }) >= k; });
+            if (wide_key(v) > KEY_NEG_INF) {       // else only scores of -inf, which weigh nothing, are cut
+                const float x = key_score(wide_key(v));
+                const int over = count([&](float s, int) { return s > x; }), ties = count([&](float s, int) { return s == x; });
+                cut_ties(x, k - over, ties);
+            }
         }
     }
     // ---- top_p ------------------------------------------------------------------------------------------------------
     if (p < 1.f) {
-        auto from_list = [&](int c, double above, double target) {         // the border lies among c listed classes
-            if (c <= 256) {
-                if (wave == 0) {
-                    List<1, S> list(sh, c, n, weight);
-                    if (target < 0) target = (double)p * list.mass([](u64) { return true; });
-                    const Cut to = list.cut_mass(above, target, weight, cut);
-                    if (lane == 0) sh.cut = to;
-                }
-                __syncthreads();
-                cut = sh.cut;
-            } else {
-                List<W, S> list(sh, c, n, weight);
-                if (target < 0) target = (double)p * list.mass([](u64) { return true; });
-                cut = list.cut_mass(above, target, weight, cut);
-            }
-        };
         if (n <= CAP) {                            // a row that fits in the list
-            const int c = count_cells(cut);
-            collect(cut);
-            from_list(c, 0.0, -1.0);
+            const int c = collect(cut);
+            with_list(c, [&](auto& list) { return list.cut_mass(0, mass_target(list.all(weight)), weight, cut); });
         } else {
-            // all weights, and their sums by bins of the score
-            const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
-            float scale = (float)fmin(4.0 * weight.c, 1e30);               // quarter octaves of the weight, or finer where the row is narrower
-            if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
-            auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
-            __syncthreads();
-            for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
-            __syncthreads();
-            u64* mybins = sh.bins[wave * 4 + (lane & 3)];
-            double m = 0;
-            auto drop = [&](float x) {
-                const double w = weight(x);
-                m += w;
-                // w in units of 2^-44: the low bits of w + 2^8
-                const u64 fixed = (u64)__double_as_longlong(w + 256.0) & ((1ull << 52) - 1);
-                if (fixed) atomicAdd(&mybins[bin(x)], fixed);
-            };
-            row.each([&](int i, const float* s) {
-                const bool ok = row.valid(i);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) if (ok && cut(s[e], row.cls(i, e))) drop(s[e]);
-            });
-            if (tid < row.sp.edge && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe);
-            const double target = (double)p * sum_double(m);
-            __syncthreads();
-            for (int b = tid; b < BINS; b += G) {
-                u64 s = 0;
-                for (int i = 0; i < S::COPIES; ++i) s += sh.bins[i][b];
-                sh.total[b] = s;
-            }
-            __syncthreads();
-            // the bins in which the sum may cross the target: units of 2^-44, half a unit a weight of doubt
-            const double unit = 5.684341886080802e-14, doubt = unit * n + 1e-12 * target;
-            double run = 0;
-            int b1 = -1, b2 = -1;
-            for (int b = 0; b < BINS; ++b) {
-                run += (double)sh.total[b] * unit;
-                if (b1 < 0 && run >= target - doubt) b1 = b;
-                if (b2 < 0 && run >= target + doubt) b2 = b;
-            }
-            if (b1 < 0) b1 = BINS - 1;
-            if (b2 < 0) b2 = BINS - 1;
-            auto inside = [&](float x, int j) { const int b = bin(x); return b >= b1 && b <= b2 && cut(x, j); };
-            const double above = mass([&](float x, int j) { return bin(x) < b1 && cut(x, j); });
-            const int c = count_cells(inside);
-            if (c <= CAP) {
-                collect(inside);
-                from_list(c, above, target);
-            } else {
-                // many equal or nearly equal scores: bisection over the row
-                uint32_t l = 0, h = 0;
-                auto reach = [&](float x, int j) { if (inside(x, j)) { const uint32_t key = score_key(x); l = max(l, ~key); h = max(h, key); } };
-                row.each([&](int i, const float* s) {
-                    const bool ok = row.valid(i);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) if (ok) reach(s[e], row.cls(i, e));
-                });
-                if (tid < row.sp.edge) reach(row.xe, row.sp.edge_at(tid));
-                const uint32_t lo = ~block_reduce<W>(l, OpMax(), sh.red2[0]), hi = block_reduce<W>(h, OpMax(), sh.red2[1]);
-                const float x = key_score(wide_key(last_enough(lo >> SHIFT, hi >> SHIFT, [&](uint32_t mid) {
+            fill_bins(true);
+            const u64 target = mass_target(bin_sum());
+            u64 above;
+            const int b = bin_reach(target, above);
+            auto inside = [&](float x, int j) { return bin(x) == b && cut(x, j); };
+            const int c = collect(inside);
+            if (c <= CAP) with_list(c, [&](auto& list) { return list.cut_mass(above, target, weight, cut); });
+            else {
+                const float x = key_score(wide_key(last_enough(0, top >> SHIFT, [&](uint32_t mid) {
                     const float s = key_score(wide_key(mid));
-                    return above + mass([&](float x, int j) { return x >= s && inside(x, j); }) >= target; })));
-                const double over = above + mass([&](float s, int j) { return s > x && inside(s, j); });
+                    return wide_key(mid) <= KEY_NEG_INF || mass([&](float x, int j) { return x >= s && cut(x, j); }) >= target; })));
+                const u64 over = mass([&](float s, int j) { return s > x && cut(s, j); });
                 const int ties = count([&](float s, int j) { return s == x && cut(s, j); });
-                const int need = ties_needed(over, weight(x), target, ties);
-                cut = {x, need < ties ? nth(x, need) : x == cut.xt ? cut.ti : n};
+                cut_ties(x, ties_needed(over, weight.fixed(weight(x)), target, ties), ties);
             }
         }
     }
@@ -584,12 +568,12 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
             if (hit) { const int l = __ffsll(hit) - 1; found = c + l; found_before = run + __shfl(s - m, l); break; }
             run += __shfl(s, 63);
         }
-        if (lane == 0) { sh.pick = found >= 0 ? found : last; sh.before = found >= 0 ? found_before : last_before; sh.redd[0] = all; }
+        if (lane == 0) { sh.pick = found >= 0 ? found : last; sh.before = found >= 0 ? found_before : last_before; sh.all = all; }
     }
     __syncthreads();
     const int c = sh.pick;
     const double before = sh.before;
-    all = sh.redd[0];
+    all = sh.all;
     const double target = (double)u * all;
     auto finish = [&](const double* w, const int* cl, int m) {             // one wave: m weights a lane, classes ascending over lanes
         double own = 0;
@@ -625,7 +609,7 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
 template <typename T> void launch(const SampleArgs& a, int rows, hipStream_t s) {
     constexpr int VEC = ET<T>::VEC;
     const int nv = a.n / VEC;
-    if (nv <= 128) sample_kernel<T, 1, 4><<<rows, 64, 0, s>>>(a);
+    if (a.n <= 256) sample_kernel<T, 1, 4><<<rows, 64, 0, s>>>(a);
     else if (nv <= 2048) sample_kernel<T, 4, 34><<<rows, 256, 0, s>>>(a);
     else sample_kernel<T, 16, (1 << 20) / VEC / 64 + 18><<<rows, 1024, 0, s>>>(a);
 }

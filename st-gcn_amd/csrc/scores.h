@@ -76,25 +76,27 @@ __device__ __forceinline__ float key_score(uint32_t k) {
 // v_exp_f32: 2^y to one unit in the last place, 0 below 2^-126.
 __device__ __forceinline__ float exp2_32(float y) { return __builtin_amdgcn_exp2f(y); }
 
-// 2^y in 64 bits for y <= 1000: y = n + f, |f| <= 1/2, the Taylor series of e^(f ln 2) to the 11th power (remainder
-// (ln2/2)^12 / 12! = 6e-15), times 2^n.  Exactly 1 at y = 0.  The fp64 vector rate of this chip is its fp32 rate, so
-// this costs about 18 issue slots against 5 for v_exp_f32.
+// 2^y in 64 bits for y <= 1000: y = n + f, |f| <= 1/2, and 2^f = 1 + f q(f), q the polynomial of degree 8 that agrees with
+// (2^f - 1) / f at the nine Chebyshev points of [-1/2, 1/2] (3.7e-14 of the value at most, exactly 1 at y = 0).  n comes
+// from adding 1.5 * 2^52 and goes into the exponent by an integer add: conversions, roundings and ldexp of 64-bit numbers
+// run at a quarter of the rate of the adds and products.
 __device__ __forceinline__ double exp2_64(double y) {
     y = fmax(y, -1100.0);
-    const double n = rint(y), f = y - n;
-    double p = 4.4455382718708114976e-10;                  // ln2^k / k!, k = 11 .. 1
-    p = fma(p, f, 7.0549116208011233299e-09);
-    p = fma(p, f, 1.0178086009239699728e-07);
-    p = fma(p, f, 1.3215486790144309488e-06);
-    p = fma(p, f, 1.5252733804059840280e-05);
-    p = fma(p, f, 1.5403530393381609954e-04);
-    p = fma(p, f, 1.3333558146428443423e-03);
-    p = fma(p, f, 9.6181291076284771619e-03);
-    p = fma(p, f, 5.5504108664821579953e-02);
-    p = fma(p, f, 2.4022650695910071233e-01);
-    p = fma(p, f, 6.9314718055994530942e-01);
+    const double s = y + 6755399441055744.0, f = y - (s - 6755399441055744.0);
+    const int n = (int)__double_as_longlong(s);
+    double p = 1.0203121063391729e-07;
+    p = fma(p, f, 1.3255224878668817e-06);
+    p = fma(p, f, 1.525268684626772e-05);
+    p = fma(p, f, 0.00015403455852453838);
+    p = fma(p, f, 0.0013333558179043112);
+    p = fma(p, f, 0.009618129159402558);
+    p = fma(p, f, 0.055504108664760424);
+    p = fma(p, f, 0.2402265069581299);
+    p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+    if (__ballot(n < -1020)) return ldexp(p, n);           // next to or below the normal range (-inf among them)
+    const long long b = __double_as_longlong(p);
+    return __longlong_as_double((long long)((uint32_t)(b >> 32) + ((uint32_t)n << 20)) << 32 | (uint32_t)b);
 }
 
 // ---- reductions of a workgroup of W waves: every thread gets the result; `red` is W entries of LDS -------------------
@@ -123,6 +125,23 @@ __device__ __forceinline__ double wave_sum(double v) {
     const long long b = __double_as_longlong(v);
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
     return __longlong_as_double((long long)hi << 32 | lo);
+}
+
+// The same for 64-bit integers.
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned long long dpp_add(unsigned long long v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+    return v + ((unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    v = dpp_add<0x143, 0xC>(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63);
+    return (unsigned long long)hi << 32 | lo;
 }
 
 template <int W, typename V, typename Op> __device__ __forceinline__ V block_reduce(V v, Op op, V* red) {
