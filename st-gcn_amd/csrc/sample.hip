@@ -45,6 +45,17 @@ struct Weight {
         if (inf) return x == INFINITY ? 1.0 : 0.0;
         return exp2_64(((double)x - xmax) * c);
     }
+    template <int N> __device__ __forceinline__ void many(const float* x, double* w) const {
+        if (inf) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = x[e] == INFINITY ? 1.0 : 0.0;
+            return;
+        }
+        double y[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = ((double)x[e] - xmax) * c;
+        exp2_64<N>(y, w);
+    }
 };
 
 // The kept set: x > xt, or x == xt and class <= ti.
@@ -55,9 +66,9 @@ struct Cut {
 
 template <int W, int CELLS> struct Shared {
     static constexpr int CAP = W * 256;            // four places a thread
-    static constexpr int COPIES = W * 4;           // of the bins: one for every fourth lane of a wave
-    union {
-        u64 bins[COPIES][BINS];
+    static constexpr int COPIES = 32;              // of the bins, one a lane of a half wave, each in banks of its own: a
+    union {                                        // wave's adds never meet, whatever the scores
+        u64 bins[BINS][COPIES];
         struct { u64 list[CAP]; double mass[CAP]; } l;
     };
     union { double sum[CELLS]; int count[CELLS]; } cell;
@@ -123,8 +134,9 @@ __device__ __forceinline__ int ties_needed(u64 over, u64 one, u64 target, int ti
 
 // Places in LDS, four a thread of a workgroup of W waves or, for lists of at most 256, of its first wave alone (V = 1: no
 // barriers).
-template <int V, typename S> struct List {
+template <typename T, int V, typename S> struct List {
     static constexpr int G = V * 64;
+    static constexpr int SHIFT = ET<T>::IS_BF16 ? 16 : 0;                  // bits of a key that carry nothing
     S& sh;
     int tid, lane, wave, n;                        // n: classes of the row
     u64 lp[4]; double lw[4];
@@ -163,11 +175,12 @@ template <int V, typename S> struct List {
     __device__ __forceinline__ void range(uint32_t& lo, uint32_t& hi) {
         uint32_t l = 0, h = 0;                     // ~ of the smallest key, the largest
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lp[i]) { l = max(l, ~(uint32_t)(lp[i] >> 32)); h = max(h, (uint32_t)(lp[i] >> 32)); }
+        for (int i = 0; i < 4; ++i) if (lp[i]) { l = max(l, ~key(lp[i])); h = max(h, key(lp[i])); }
         lo = ~block_reduce<V>(l, OpMax(), sh.red2[0]);
         hi = block_reduce<V>(h, OpMax(), sh.red2[1]);
     }
-    static __device__ __forceinline__ uint32_t key(u64 e) { return (uint32_t)(e >> 32); }
+    static __device__ __forceinline__ uint32_t key(u64 e) { return (uint32_t)(e >> (32 + SHIFT)); }
+    static __device__ __forceinline__ float score(uint32_t s) { return key_score(ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s); }
     // the m-th by class of the entries with key v
     __device__ __forceinline__ int tie(uint32_t v, int m) {
         return (int)~last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return count([&](u64 e) { return key(e) == v && (uint32_t)e >= mid; }) >= m; });
@@ -178,7 +191,7 @@ template <int V, typename S> struct List {
         range(lo, hi);
         const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return count([&](u64 e) { return key(e) >= mid; }) >= k; });
         const int above = count([&](u64 e) { return key(e) > v; }), ties = count([&](u64 e) { return key(e) == v; });
-        return {key_score(v), above + ties > k ? tie(v, k - above) : n};
+        return {score(v), above + ties > k ? tie(v, k - above) : n};
     }
     // the shortest prefix that, after `above`, reaches the target; `was`: what cut the entries so far
     __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Weight& weight, const Cut& was) {
@@ -187,7 +200,7 @@ template <int V, typename S> struct List {
         const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass(weight, [&](u64 e) { return key(e) >= mid; }) >= target; });
         const u64 over = above + mass(weight, [&](u64 e) { return key(e) > v; });
         const int ties = count([&](u64 e) { return key(e) == v; });
-        const float x = key_score(v);
+        const float x = score(v);
         const int m = ties_needed(over, weight.fixed(weight(x)), target, ties);
         return {x, m < ties ? tie(v, m) : x == was.xt ? was.ti : n};
     }
@@ -279,6 +292,19 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     if (k == 0 || k > n) k = n;
 
     Cut cut = {-INFINITY, n};
+    // Scores of a vector that are not kept become -inf, which weighs nothing.  False: none of the wave's is kept.
+    auto only_kept = [&](int i, const float* s, float* x, float lowest) {
+        const float lo = fmaxf(cut.xt, lowest);
+        bool some = false;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { x[e] = s[e] >= lo ? s[e] : -INFINITY; some |= s[e] >= lo; }
+        if (!__ballot(some)) return false;
+        if (cut.ti < n) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (s[e] == cut.xt && row.cls(i, e) > cut.ti) x[e] = -INFINITY;
+        }
+        return true;
+    };
     auto mass_target = [&](u64 all) { return (u64)ceil((double)p * (double)all); };
     auto count_waves = [&](int m) {                // sum over the waves of a number that is the same in a wave's lanes
         __syncthreads();
@@ -305,8 +331,15 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         u64 m = 0;
         row.each([&](int i, const float* s) {
             const bool ok = row.valid(i);
+            float x[VEC];
+            bool some = false;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) if (ok && pred(s[e], row.cls(i, e))) m += weight.fixed(weight(s[e]));
+            for (int e = 0; e < VEC; ++e) { const bool in = ok && pred(s[e], row.cls(i, e)); x[e] = in ? s[e] : -INFINITY; some |= in; }
+            if (!__ballot(some)) return;
+            double w[VEC];
+            weight.template many<VEC>(x, w);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m += weight.fixed(w[e]);
         });
         if (tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))) m += weight.fixed(weight(row.xe));
         return block_reduce<W>(m, OpSum(), sh.redu);
@@ -418,6 +451,7 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     // The kept scores (`cut`) by bins: one each, or their weights.
     float scale = 0.f;                             // quarter octaves of the weight, or finer where the row is narrower
     auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
+    auto in_bin = [&](float x, int b) { const float f = (xmax - x) * scale; return b < BINS - 1 ? f >= (float)b && f < (float)(b + 1) : !(f < (float)b); };
     auto fill_bins = [&](bool weigh) {
         const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
         scale = (float)fmin(4.0 * weight.c, 1e30);
@@ -425,21 +459,26 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         __syncthreads();
         for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
         __syncthreads();
-        u64* mybins = sh.bins[wave * 4 + (lane & 3)];
-        auto drop = [&](float x) {
-            const u64 v = weigh ? weight.fixed(weight(x)) : 1;
-            if (v) atomicAdd(&mybins[bin(x)], v);
-        };
+        auto drop = [&](float x, u64 v) { atomicAdd(&sh.bins[bin(x)][lane & 31], v); };
         row.each([&](int i, const float* s) {
-            const bool ok = row.valid(i);
+            float x[VEC];
+            if (!only_kept(i, s, x, -INFINITY)) return;
+            if (weigh) {
+                double w[VEC];
+                weight.template many<VEC>(x, w);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) if (ok && cut(s[e], row.cls(i, e))) drop(s[e]);
+                for (int e = 0; e < VEC; ++e) drop(s[e], weight.fixed(w[e]));
+            } else {
+                const u64 one = row.valid(i) ? 1 : 0;  // top_k comes first: every score counts
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) drop(s[e], one);
+            }
         });
-        if (tid < row.sp.edge && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe);
+        if (tid < row.sp.edge && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, weigh ? weight.fixed(weight(row.xe)) : 1);
         __syncthreads();
         for (int b = tid; b < BINS; b += G) {
             u64 s = 0;
-            for (int i = 0; i < S::COPIES; ++i) s += sh.bins[i][b];
+            for (int i = 0; i < S::COPIES; ++i) s += sh.bins[b][(i + tid) & (S::COPIES - 1)];
             sh.total[b] = s;
         }
         __syncthreads();
@@ -461,10 +500,10 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     // list(c): work on a list of c places by the first wave alone if they are few; its cut to all
     auto with_list = [&](int c, auto work) {
         if (c <= 256) {
-            if (wave == 0) { List<1, S> list(sh, c, n, weight); const Cut to = work(list); if (lane == 0) sh.cut = to; }
+            if (wave == 0) { List<T, 1, S> list(sh, c, n, weight); const Cut to = work(list); if (lane == 0) sh.cut = to; }
             __syncthreads();
             cut = sh.cut;
-        } else { List<W, S> list(sh, c, n, weight); cut = work(list); }
+        } else { List<T, W, S> list(sh, c, n, weight); cut = work(list); }
     };
     // What equal scores x leave of it: all, or the first `need` by class.
     auto cut_ties = [&](float x, int need, int ties) { cut = {x, need < ties ? nth(x, need) : x == cut.xt ? cut.ti : n}; };
@@ -484,16 +523,15 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
                     if (p < 1.f) { cut = list.cut_mass(0, mass_target(list.all(weight)), weight, cut); list.keep(cut); }
                     list.draw(u, least, answer);
                 };
-                if (c <= 256) { if (wave == 0) rest(List<1, S>(sh, c, n, weight)); }
-                else rest(List<W, S>(sh, c, n, weight));
+                if (c <= 256) { if (wave == 0) rest(List<T, 1, S>(sh, c, n, weight)); }
+                else rest(List<T, W, S>(sh, c, n, weight));
                 return;
             }
         }
         fill_bins(false);
         u64 above;
         const int b = bin_reach((u64)k, above);
-        auto inside = [&](float x, int) { return bin(x) == b; };
-        const int c = collect(inside), need = k - (int)above;
+        const int c = collect([&](float x, int) { return in_bin(x, b); }), need = k - (int)above;
         if (c <= CAP) with_list(c, [&](auto& list) { return list.cut_count(need); });
         else {                                     // many equal or nearly equal scores: bisection over the row
             const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) {
@@ -516,8 +554,7 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
             const u64 target = mass_target(bin_sum());
             u64 above;
             const int b = bin_reach(target, above);
-            auto inside = [&](float x, int j) { return bin(x) == b && cut(x, j); };
-            const int c = collect(inside);
+            const int c = collect([&](float x, int j) { return in_bin(x, b) && cut(x, j); });
             if (c <= CAP) with_list(c, [&](auto& list) { return list.cut_mass(above, target, weight, cut); });
             else {
                 const float x = key_score(wide_key(last_enough(0, top >> SHIFT, [&](uint32_t mid) {
@@ -537,11 +574,19 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     };
     __syncthreads();
     row.each([&](int i, const float* s) {
-        const bool ok = row.valid(i);
         double m = 0;
+        float x[VEC];
+        if (only_kept(i, s, x, xlow)) {
+            double w[VEC];
+            weight.template many<VEC>(x, w);
+            if (least > 0) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) if (ok) m += share(s[e], row.cls(i, e));
-        m = __ballot(m != 0) ? wave_sum(m) : 0.0;
+                for (int e = 0; e < VEC; ++e) w[e] = w[e] >= least ? w[e] : 0.0;
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m += w[e];
+            m = wave_sum(m);
+        }
         if (lane == 0) sh.cell.sum[row.cell(i)] = m;
     });
     const int cells = row.cells();

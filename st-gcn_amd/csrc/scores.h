@@ -80,23 +80,42 @@ __device__ __forceinline__ float exp2_32(float y) { return __builtin_amdgcn_exp2
 // (2^f - 1) / f at the nine Chebyshev points of [-1/2, 1/2] (3.7e-14 of the value at most, exactly 1 at y = 0).  n comes
 // from adding 1.5 * 2^52 and goes into the exponent by an integer add: conversions, roundings and ldexp of 64-bit numbers
 // run at a quarter of the rate of the adds and products.
+// N of them at once: the chains of N values side by side hide the latency of the 64-bit operations.
+template <int N> __device__ __forceinline__ void exp2_64(const double* y, double* out) {
+    double f[N], p[N];
+    int n[N];
+    bool tiny = false;                                     // next to or below the normal range, but not at -1100 (-inf among them)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const double v = fmax(y[e], -1100.0), s = v + 6755399441055744.0;
+        f[e] = v - (s - 6755399441055744.0);
+        n[e] = (int)__double_as_longlong(s);
+        tiny |= (uint32_t)(n[e] + 1099) < 79u;             // -1099 .. -1021
+        p[e] = 1.0203121063391729e-07;
+    }
+    constexpr double Q[9] = {1.3255224878668817e-06, 1.525268684626772e-05, 0.00015403455852453838, 0.0013333558179043112, 0.009618129159402558,
+                             0.055504108664760424, 0.2402265069581299, 0.6931471805599453, 1.0};
+#pragma unroll
+    for (int q = 0; q < 9; ++q) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[e] = fma(p[e], f[e], Q[q]);
+    }
+    if (__ballot(tiny)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = ldexp(p[e], n[e]);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const long long b = __double_as_longlong(p[e]);
+        const double w = __longlong_as_double((long long)((uint32_t)(b >> 32) + ((uint32_t)n[e] << 20)) << 32 | (uint32_t)b);
+        out[e] = n[e] < -1020 ? 0.0 : w;
+    }
+}
 __device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -1100.0);
-    const double s = y + 6755399441055744.0, f = y - (s - 6755399441055744.0);
-    const int n = (int)__double_as_longlong(s);
-    double p = 1.0203121063391729e-07;
-    p = fma(p, f, 1.3255224878668817e-06);
-    p = fma(p, f, 1.525268684626772e-05);
-    p = fma(p, f, 0.00015403455852453838);
-    p = fma(p, f, 0.0013333558179043112);
-    p = fma(p, f, 0.009618129159402558);
-    p = fma(p, f, 0.055504108664760424);
-    p = fma(p, f, 0.2402265069581299);
-    p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.0);
-    if (__ballot(n < -1020)) return ldexp(p, n);           // next to or below the normal range (-inf among them)
-    const long long b = __double_as_longlong(p);
-    return __longlong_as_double((long long)((uint32_t)(b >> 32) + ((uint32_t)n << 20)) << 32 | (uint32_t)b);
+    double w;
+    exp2_64<1>(&y, &w);
+    return w;
 }
 
 // ---- reductions of a workgroup of W waves: every thread gets the result; `red` is W entries of LDS -------------------
