@@ -189,7 +189,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(Dist
     i32x4 v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>();
-    float xe = tid < sp.edge ? load_elem(x, sp.edge_at(tid)) : -INFINITY;
+    float xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY;
     for (int i = tid; i < WORDS; i += G) bits[i] = 0;
     group_sync<W>();
 
@@ -208,8 +208,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(Dist
         if (__ballot(dup)) teacher_merge(a, lane, q, li_[sub], pk_[sub]);
         if (a.w > 0.0 && y >= n) q.bad = true;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_elem(x, q.my[e]) : -INFINITY;
-        if (hard) xy = load_elem(x, (size_t)y);
+        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_score(x, q.my[e]) : -INFINITY;
+        if (hard) xy = load_score(x, (size_t)y);
         if (W > 1 && lane == 0) { t_pr = q.pr; t_flags = (q.any ? 1 : 0) | (q.bad ? 2 : 0); }
     }
     group_sync<W>();
@@ -372,8 +372,8 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
         if (a.w > 0.0 && y >= n) q.bad = true;
         teacher_merge(a, lane, q, li, pk);
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_elem(x, q.my[e]) : -INFINITY;
-        if (hard) xy = load_elem(x, (size_t)y);
+        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_score(x, q.my[e]) : -INFINITY;
+        if (hard) xy = load_score(x, (size_t)y);
     }
     for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NV) {
         // classes of this segment: [c0, c1), the row's edges with the first one
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
             const int j = sp.edge_at(tid);
             bool is_listed = false;
             for (int o = 0; o < a.k; ++o) is_listed |= li[o] == j;
-            if (!is_listed) { const float f = load_elem(x, j); raise(f); add(f); }
+            if (!is_listed) { const float f = load_score(x, j); raise(f); add(f); }
         }
         i32x4 v[NV];
 #pragma unroll
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
             }
         }
     }
-    if (v0 == 0 && tid < sp.edge) { const int j = sp.edge_at(tid); store_elem(dx, j, empty ? 0.f : g(load_elem(x, j), gr)); }
+    if (v0 == 0 && tid < sp.edge) { const int j = sp.edge_at(tid); store_elem(dx, j, empty ? 0.f : g(load_score(x, j), gr)); }
     if (empty) return;
     group_sync<W>();
     // the classes of this piece; the row's edges belong to piece 0
@@ -506,13 +506,13 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
         if (p < 0.f) continue;
         const long long j = a.idx[r * a.k + e];
         if (j < 0 || j >= n || !here(j)) continue;
-        float d = g(load_elem(x, (size_t)j), gl) - a.fp * p * up;
+        float d = g(load_score(x, (size_t)j), gl) - a.fp * p * up;
         if (hard && j == y) { d -= a.w * up; mine = true; }
         store_elem(dx, (size_t)j, d);
     }
     if (!hard || !here(y)) return;
     if constexpr (W == 1) mine = __ballot(mine) != 0; else mine = __syncthreads_or(mine);
-    if (tid == 0 && !mine) store_elem(dx, (size_t)y, g(load_elem(x, (size_t)y), gr) - a.w * up);
+    if (tid == 0 && !mine) store_elem(dx, (size_t)y, g(load_score(x, (size_t)y), gr) - a.w * up);
 }
 
 // Sum of the rows' losses, added in row order within a thread and by fixed butterflies: the same bits every run.

@@ -12,18 +12,19 @@
 // registers was tried: fully unrolled passes with 64-bit weights spill).  What the cuts need of it:
 //   top_k up to a few hundred: k of the threads' maxima reach a bound that about k to 2k scores reach; those go to a list
 //     in LDS, where everything else happens, and no weight of any other class is computed;
-//   larger top_k, and top_p: the scores (or their weights) counted by 128 bins of the score; the bin in which the count
-//     (the sum) crosses gives a short list, in which the border is bisected.  Bins and list hold weights as 64-bit integers
+//   larger top_k, and top_p: the scores (or their weights) counted by bins of the score; the bin in which the count
+//     (the sum) crosses is split into bins of its own until it gives a short list, in which the border is bisected by one
+//     wave (a whole workgroup spent 12 us a list on barriers).  Bins and list hold weights as 64-bit integers
 //     in units of 2^-s (s = 42 to 50 by the class count): their sums are the same in any order.  A border that falls within
 //     such a unit of a class moves that class alone, by a share of 2^-s of the first class's weight;
 //   the answer: sums of the kept weights by cells (64 consecutive vectors: one wave's step), the cell in which u falls,
 //     then the lane, then the class.
 #include "scores.h"
+#include <type_traits>
 
 namespace {
 
 constexpr double LOG2E = 1.4426950408889634074;
-constexpr int BINS = 128;
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -40,6 +41,7 @@ __device__ __forceinline__ float place_score(u64 p) { return key_score((uint32_t
 // Weights relative to the row's maximum.  With a maximum of +inf its classes weigh 1, all others nothing.
 struct Weight {
     double xmax, c, unit; bool inf;                // unit: 2^(52 - s); the low 52 bits of w + unit are w in units of 2^-s
+    __device__ __forceinline__ double step() const { return unit * 2.2204460492503131e-16; }       // 2^-s
     __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double_as_longlong(w + unit) & ((1ull << 52) - 1); }
     __device__ __forceinline__ double operator()(float x) const {
         if (inf) return x == INFINITY ? 1.0 : 0.0;
@@ -58,43 +60,50 @@ struct Weight {
     }
 };
 
-// The kept set: x > xt, or x == xt and class <= ti.
+// The kept set: x > xt, or x == xt and class <= ti.  Tests that run for every score are written without && and ||, which
+// become branches: eight nests of them a vector took four times as long as the comparisons.
 struct Cut {
     float xt; int ti;
-    __device__ __forceinline__ bool operator()(float x, int j) const { return x > xt || (x == xt && j <= ti); }
+    __device__ __forceinline__ bool operator()(float x, int j) const { return (x > xt) | ((x == xt) & (j <= ti)); }
 };
 
+constexpr int CAP = 512;                           // places of a list: eight a lane of one wave
+
 template <int W, int CELLS> struct Shared {
-    static constexpr int CAP = W * 256;            // four places a thread
-    static constexpr int COPIES = 32;              // of the bins, one a lane of a half wave, each in banks of its own: a
-    union {                                        // wave's adds never meet, whatever the scores
+    // Bins, and copies of them: a lane adds to copy lane % COPIES, which has banks of its own, so few or none of a wave's
+    // adds meet, whatever the scores.  More bins, shorter lists (1 x 131072 at top-p 0.9: 1600 places with 128, 390 with 512).
+    static constexpr int BINS = W == 1 ? 64 : W >= 8 ? 512 : 128, COPIES = W == 1 ? 1 : W >= 8 ? 16 : 32;
+    union {
         u64 bins[BINS][COPIES];
-        struct { u64 list[CAP]; double mass[CAP]; } l;
+        u64 list[CAP];
     };
     union { double sum[CELLS]; int count[CELLS]; } cell;
-    u64 total[BINS];
-    double all; u64 redu[W]; int redi[W]; uint32_t red2[2][W];
+    alignas(16) u64 total[BINS];
+    double all; int redi[W]; uint32_t red2[2][W];
     int pick; double before; Cut cut;
 };
 
-// One row as its workgroup of W waves sees it: steps of one vector a thread.
-// Cells in the order of the classes: the row's front end, then vector cells (step i, wave w), then its back end.
+// One row as its workgroup of W waves sees it: every wave has a contiguous share of the whole vectors, `steps` of them a
+// lane.  Cells in the order of the classes: the row's front end, then the waves' runs of CELL steps, then its back end.
 template <typename T, int W> struct Row {
-    static constexpr int VEC = ET<T>::VEC, G = W * 64;
+    static constexpr int VEC = ET<T>::VEC, G = W * 64, CELL = 4;
     const T* x;
     RowSpan<T> sp;
-    int n, tid, lane, wave, steps;
+    int n, tid, lane, wave, steps, first;          // first: this lane's vector of step 0
     float xe;                                      // of the threads below sp.edge
 
     __device__ __forceinline__ Row(const T* x_, int n_) : x(x_), sp(x_, n_), n(n_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6) {
         steps = (sp.nvec + G - 1) / G;
-        xe = tid < sp.edge ? load_elem(x, sp.edge_at(tid)) : -INFINITY;
+        first = wave * steps * 64 + lane;
+        xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY;
     }
-    __device__ __forceinline__ i32x4 load(int i) const { return i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>(); }
-    __device__ __forceinline__ bool valid(int i) const { return i * G + tid < sp.nvec; }
-    __device__ __forceinline__ int cls(int i, int e) const { return sp.vec_at(i * G + tid) + e; }
-    __device__ __forceinline__ int cells() const { return steps * W + 2; }
-    __device__ __forceinline__ int cell(int i) const { return 1 + i * W + wave; }
+    __device__ __forceinline__ bool valid(int i) const { return i < steps && first + i * 64 < sp.nvec; }
+    __device__ __forceinline__ i32x4 load(int i) const { return valid(i) ? load_vec(x, sp.vec_at(first + i * 64)) : neg_inf_vec<T>(); }
+    __device__ __forceinline__ int cls(int i, int e) const { return sp.vec_at(first + i * 64) + e; }
+    __device__ __forceinline__ int wave_cells() const { return (steps + CELL - 1) / CELL; }
+    __device__ __forceinline__ int cells() const { return W * wave_cells() + 2; }
+    __device__ __forceinline__ int cell(int i) const { return 1 + wave * wave_cells() + i / CELL; }
+    __device__ __forceinline__ bool ends_cell(int i) const { return i % CELL == CELL - 1 || i == steps - 1; }
     // f(i, scores of vector i); scores beyond the row are -inf.  Three steps' loads are under way at a time.
     template <typename F> __device__ __forceinline__ void each(F f) const {
         i32x4 v0 = load(0), v1 = load(1), v2 = load(2);
@@ -106,13 +115,16 @@ template <typename T, int W> struct Row {
             f(i, s);
         }
     }
-    // f(scores of vector i), by the wave that has that cell
-    template <typename F> __device__ __forceinline__ void at_cell(int c, F f) const {
-        const int i = (c - 1) / W;
-        if (c < 1 || c > steps * W || (c - 1) % W != wave) return;
-        float s[VEC];
-        unpack16<T>(load(i), s);
-        f(i, s);
+    // f(i, scores of vector i) for the steps of cell c, by the wave that has it, until f says stop
+    template <typename F> __device__ __forceinline__ void in_cell(int c, F f) const {
+        const int wc = wave_cells();
+        if (c < 1 || c > W * wc || (c - 1) / wc != wave) return;
+        const int i0 = (c - 1) % wc * CELL;
+        for (int i = i0; i < i0 + CELL && i < steps; ++i) {
+            float s[VEC];
+            unpack16<T>(load(i), s);
+            if (f(i, s)) return;
+        }
     }
 };
 
@@ -132,61 +144,51 @@ __device__ __forceinline__ int ties_needed(u64 over, u64 one, u64 target, int ti
     return m < (u64)ties ? (int)m : ties;
 }
 
-// Places in LDS, four a thread of a workgroup of W waves or, for lists of at most 256, of its first wave alone (V = 1: no
-// barriers).
-template <typename T, int V, typename S> struct List {
-    static constexpr int G = V * 64;
-    static constexpr int SHIFT = ET<T>::IS_BF16 ? 16 : 0;                  // bits of a key that carry nothing
-    S& sh;
-    int tid, lane, wave, n;                        // n: classes of the row
-    u64 lp[4]; double lw[4];
-    __device__ __forceinline__ List(S& s, int c, int n_, const Weight& weight) : sh(s), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), n(n_) {
+// At most CAP places, held by one wave: steps of 64 that hold nothing are skipped.
+template <typename T> struct List {
+    static constexpr int R = CAP / 64, SHIFT = ET<T>::IS_BF16 ? 16 : 0;    // bits of a key that carry nothing
+    const Weight& weight;
+    int c, n;                                      // places; classes of the row
+    u64 lp[R], lw[R];                              // place (0: none) and weight in integer units
+    __device__ __forceinline__ List(const u64* list, int c_, int n_, const Weight& w) : weight(w), c(c_), n(n_) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { lp[i] = tid + G * i < c ? sh.l.list[tid + G * i] : 0; lw[i] = lp[i] ? weight(place_score(lp[i])) : 0.0; }
+        for (int i = 0; i < R; ++i) {
+            lp[i] = lw[i] = 0;
+            if (64 * i < c) {
+                if (lane + 64 * i < c) lp[i] = list[lane + 64 * i];
+                if (lp[i]) lw[i] = weight.fixed(weight(place_score(lp[i])));
+            }
+        }
     }
-    template <typename P> __device__ __forceinline__ int count(P pred) {
+    template <typename P> __device__ __forceinline__ int count(P pred) const {
         int m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m += __popcll(__ballot(lp[i] && pred(lp[i])));
-        if constexpr (V == 1) return m;
-        __syncthreads();
-        if (lane == 0) sh.redi[wave] = m;
-        __syncthreads();
-        m = 0;
-#pragma unroll
-        for (int w = 0; w < V; ++w) m += sh.redi[w];
+        for (int i = 0; i < R; ++i) if (64 * i < c) m += __popcll(__ballot((lp[i] != 0) & pred(lp[i])));
         return m;
     }
-    // weights of the entries that pass, in integer units
-    template <typename P> __device__ __forceinline__ u64 mass(const Weight& weight, P pred) {
+    template <typename P> __device__ __forceinline__ u64 mass(P pred) const {
         u64 m = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lp[i] && pred(lp[i])) m += weight.fixed(lw[i]);
-        m = wave_sum(m);
-        if constexpr (V == 1) return m;
-        __syncthreads();
-        if (lane == 0) sh.redu[wave] = m;
-        __syncthreads();
-        m = 0;
-#pragma unroll
-        for (int w = 0; w < V; ++w) m += sh.redu[w];
-        return m;
+        for (int i = 0; i < R; ++i) if (64 * i < c) m += pred(lp[i]) ? lw[i] : 0;
+        return wave_sum(m);
     }
-    __device__ __forceinline__ void range(uint32_t& lo, uint32_t& hi) {
-        uint32_t l = 0, h = 0;                     // ~ of the smallest key, the largest
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (lp[i]) { l = max(l, ~key(lp[i])); h = max(h, key(lp[i])); }
-        lo = ~block_reduce<V>(l, OpMax(), sh.red2[0]);
-        hi = block_reduce<V>(h, OpMax(), sh.red2[1]);
-    }
+    __device__ __forceinline__ u64 all() const { return mass([](u64) { return true; }); }
     static __device__ __forceinline__ uint32_t key(u64 e) { return (uint32_t)(e >> (32 + SHIFT)); }
     static __device__ __forceinline__ float score(uint32_t s) { return key_score(ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s); }
+    __device__ __forceinline__ void range(uint32_t& lo, uint32_t& hi) const {
+        uint32_t l = 0, h = 0;                     // ~ of the smallest key, the largest
+#pragma unroll
+        for (int i = 0; i < R; ++i) if (64 * i < c && lp[i]) { l = max(l, ~key(lp[i])); h = max(h, key(lp[i])); }
+        lo = ~wave_reduce(l, OpMax());
+        hi = wave_reduce(h, OpMax());
+    }
     // the m-th by class of the entries with key v
-    __device__ __forceinline__ int tie(uint32_t v, int m) {
-        return (int)~last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return count([&](u64 e) { return key(e) == v && (uint32_t)e >= mid; }) >= m; });
+    __device__ __forceinline__ int tie(uint32_t v, int m) const {
+        return (int)~last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return count([&](u64 e) { return (key(e) == v) & ((uint32_t)e >= mid); }) >= m; });
     }
     // the first k entries
-    __device__ __forceinline__ Cut cut_count(int k) {
+    __device__ __forceinline__ Cut cut_count(int k) const {
         uint32_t lo, hi;
         range(lo, hi);
         const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return count([&](u64 e) { return key(e) >= mid; }) >= k; });
@@ -194,58 +196,31 @@ template <typename T, int V, typename S> struct List {
         return {score(v), above + ties > k ? tie(v, k - above) : n};
     }
     // the shortest prefix that, after `above`, reaches the target; `was`: what cut the entries so far
-    __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Weight& weight, const Cut& was) {
+    __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Cut& was) const {
         uint32_t lo, hi;
         range(lo, hi);
-        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass(weight, [&](u64 e) { return key(e) >= mid; }) >= target; });
-        const u64 over = above + mass(weight, [&](u64 e) { return key(e) > v; });
+        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass([&](u64 e) { return key(e) >= mid; }) >= target; });
+        const u64 over = above + mass([&](u64 e) { return key(e) > v; });
         const int ties = count([&](u64 e) { return key(e) == v; });
         const float x = score(v);
         const int m = ties_needed(over, weight.fixed(weight(x)), target, ties);
         return {x, m < ties ? tie(v, m) : x == was.xt ? was.ti : n};
     }
-    __device__ __forceinline__ u64 all(const Weight& weight) { return mass(weight, [](u64) { return true; }); }
-    __device__ __forceinline__ void keep(const Cut& cut) {
+    template <typename K> __device__ __forceinline__ void keep(K kept) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lp[i] && !cut(place_score(lp[i]), place_class(lp[i]))) { lp[i] = 0; lw[i] = 0; }
+        for (int i = 0; i < R; ++i) if (64 * i < c && !(lp[i] && kept(place_score(lp[i]), place_class(lp[i])))) lp[i] = lw[i] = 0;
     }
-    // The answer, from entries that are all there is: (class, log of its share) by one thread.
-    template <typename A> __device__ __forceinline__ void draw(float u, double least, A answer) {
+    // The answer, from entries that are all there is, in integer units: the first class, in the order of the classes, at
+    // which the running mass exceeds u times all of it.
+    template <typename A> __device__ __forceinline__ void draw(float u, A answer) const {
+        const u64 sum = all(), most = (u64)floor((double)u * (double)sum);             // a running mass > most
+        // lower classes are larger ~class: the largest one down from which more than `most` has gathered
+        const uint32_t who = last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return mass([&](u64 e) { return (uint32_t)e >= mid; }) > most; });
+        const float lane_x = [&] { float x = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (lw[i] == 0 || lw[i] < least) lp[i] = 0;
-        int c = 0;                                 // packed: places and weights
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const u64 b = __ballot(lp[i] != 0);
-            int at = c;
-            if constexpr (V == 1) c += __popcll(b);
-            else {
-                __syncthreads();
-                if (lane == 0) sh.redi[wave] = __popcll(b);
-                __syncthreads();
-                for (int w = 0; w < V; ++w) { if (w < wave) at += sh.redi[w]; c += sh.redi[w]; }
-            }
-            if (lp[i]) { sh.l.list[at + lanes_below(b)] = lp[i]; sh.l.mass[at + lanes_below(b)] = lw[i]; }
-        }
-        if constexpr (V == 1) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); } else __syncthreads();
-        double all = 0, front[4] = {0, 0, 0, 0};   // the mass of lower classes
-        for (int o = 0; o < c; ++o) {
-            const u64 e = sh.l.list[o];
-            const double w = sh.l.mass[o];
-            all += w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if ((uint32_t)e > (uint32_t)lp[i]) front[i] += w;
-        }
-        const double target = (double)u * all;
-        // the first class whose sum exceeds the target; the last one if rounding leaves none.  Lower class = larger ~class.
-        u64 best = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lp[i]) best = max(best, front[i] + lw[i] > target ? (1ull << 32) | (uint32_t)lp[i] : (u64)(uint32_t)~(uint32_t)lp[i] + 1);
-        best = block_reduce<V>(best, OpMax(), sh.redu);
-        const uint32_t who = best >> 32 ? (uint32_t)best : ~(uint32_t)(best - 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (lp[i] && (uint32_t)lp[i] == who) answer(place_class(lp[i]), (float)log(lw[i] / all));
+            for (int i = 0; i < R; ++i) if (64 * i < c && lw[i] && (uint32_t)lp[i] == who) x = place_score(lp[i]);
+            return x; }();
+        if (lane_x > -INFINITY) answer((int)~who, (float)log(weight(lane_x) / ((double)sum * weight.step())));
     }
 };
 
@@ -253,7 +228,7 @@ template <typename T, int W, int CELLS>
 __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     typedef Row<T, W> R;
     typedef Shared<W, CELLS> S;
-    constexpr int VEC = R::VEC, G = R::G, CAP = S::CAP;
+    constexpr int VEC = R::VEC, G = R::G, BINS = S::BINS;
     __shared__ S sh;
     const size_t r = blockIdx.x;
     const R row((const T*)((const char*)a.x + r * a.stride * ET<T>::ES), a.n);
@@ -301,7 +276,7 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         if (!__ballot(some)) return false;
         if (cut.ti < n) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) if (s[e] == cut.xt && row.cls(i, e) > cut.ti) x[e] = -INFINITY;
+            for (int e = 0; e < VEC; ++e) x[e] = ((s[e] == cut.xt) & (row.cls(i, e) > cut.ti)) ? -INFINITY : x[e];
         }
         return true;
     };
@@ -315,45 +290,16 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         for (int w = 0; w < W; ++w) s += sh.redi[w];
         return s;
     };
-    // scores that pass, counted
-    auto count = [&](auto pred) {
-        int m = 0;
-        row.each([&](int i, const float* s) {
-            const bool ok = row.valid(i);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) m += __popcll(__ballot(ok && pred(s[e], row.cls(i, e))));
-        });
-        if (wave == 0) m += __popcll(__ballot(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))));
-        return count_waves(m);
-    };
-    // weights of the scores that pass, in integer units
-    auto mass = [&](auto pred) {
-        u64 m = 0;
-        row.each([&](int i, const float* s) {
-            const bool ok = row.valid(i);
-            float x[VEC];
-            bool some = false;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) { const bool in = ok && pred(s[e], row.cls(i, e)); x[e] = in ? s[e] : -INFINITY; some |= in; }
-            if (!__ballot(some)) return;
-            double w[VEC];
-            weight.template many<VEC>(x, w);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) m += weight.fixed(w[e]);
-        });
-        if (tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))) m += weight.fixed(weight(row.xe));
-        return block_reduce<W>(m, OpSum(), sh.redu);
-    };
     // counts by cells of the scores that pass, as prefix sums: cell.count[c] = how many lie in front of cell c.  Returns all.
     auto count_cells = [&](auto pred) {
         __syncthreads();
         const int cells = row.cells();
+        int m = 0;
         row.each([&](int i, const float* s) {
             const bool ok = row.valid(i);
-            int m = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) m += __popcll(__ballot(ok && pred(s[e], row.cls(i, e))));
-            if (lane == 0) sh.cell.count[row.cell(i)] = m;
+            for (int e = 0; e < VEC; ++e) m += __popcll(__ballot(ok & pred(s[e], row.cls(i, e))));
+            if (row.ends_cell(i)) { if (lane == 0) sh.cell.count[row.cell(i)] = m; m = 0; }
         });
         if (wave == 0) {
             const u64 b = __ballot(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid))), front = (1ull << row.sp.head) - 1;
@@ -381,21 +327,35 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         __syncthreads();
         if (tid == 0) sh.pick = 0;
         __syncthreads();
-        auto append = [&](bool in, float x, int j) {
-            const u64 b = __ballot(in);
-            if (b) {
-                int at = 0;
-                if (lane == 0) at = atomicAdd(&sh.pick, __popcll(b));
-                at = __builtin_amdgcn_readfirstlane(at) + lanes_below(b);
-                if (in && at < CAP) sh.l.list[at] = place(score_key(x), j);
-            }
-        };
         row.each([&](int i, const float* s) {
             const bool ok = row.valid(i);
+            uint32_t in = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) append(ok && pred(s[e], row.cls(i, e)), s[e], row.cls(i, e));
+            for (int e = 0; e < VEC; ++e) in |= (ok & pred(s[e], row.cls(i, e))) ? 1u << e : 0u;
+            if (!__ballot(in != 0)) return;
+            const int m = __popc(in);              // 8 at most
+            int below = 0, all = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const u64 q = __ballot(m >> b & 1);
+                below += lanes_below(q) << b;
+                all += __popcll(q) << b;
+            }
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&sh.pick, all);
+            at = __builtin_amdgcn_readfirstlane(at) + below;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (in >> e & 1) { if (at < CAP) sh.list[at] = place(score_key(s[e]), row.cls(i, e)); ++at; }
         });
-        if (wave == 0) append(tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid)), row.xe, row.sp.edge_at(tid));
+        if (wave == 0) {
+            const bool in = tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid));
+            const u64 b = __ballot(in);
+            int at = 0;
+            if (lane == 0 && b) at = atomicAdd(&sh.pick, __popcll(b));
+            at = __builtin_amdgcn_readfirstlane(at) + lanes_below(b);
+            if (in && at < CAP) sh.list[at] = place(score_key(row.xe), row.sp.edge_at(tid));
+        }
         __syncthreads();
         const int c = sh.pick;
         __syncthreads();
@@ -415,8 +375,8 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         }
         __syncthreads();
         const int c = sh.pick, cells = row.cells();
-        const int left = m - sh.cell.count[c];     // the left-th one of that cell
-        row.at_cell(c, [&](int i, const float* s) {
+        int left = m - sh.cell.count[c];           // the left-th one of that cell
+        row.in_cell(c, [&](int i, const float* s) {
             int own = 0;
             const bool ok = row.valid(i);
 #pragma unroll
@@ -424,11 +384,14 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
             int s0 = own;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(s0, d); if (lane >= d) s0 += o; }
+            const int here = __shfl(s0, 63);
+            if (here < left) { left -= here; return false; }
             if (s0 - own < left && left <= s0) {
                 int rank = s0 - own;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) if (s[e] == x && ++rank == left) sh.redi[0] = row.cls(i, e);
             }
+            return true;
         });
         if (wave == 0 && (c == 0 || c == cells - 1)) {
             const u64 b = __ballot(tid < row.sp.edge && row.xe == x), front = (1ull << row.sp.head) - 1, here = c == 0 ? b & front : b & ~front;
@@ -448,33 +411,31 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     const float xlow = xq - fabsf(xq) * 1e-6f;
 
     // ---- borders ----------------------------------------------------------------------------------------------------
-    // The kept scores (`cut`) by bins: one each, or their weights.
-    float scale = 0.f;                             // quarter octaves of the weight, or finer where the row is narrower
-    auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
-    auto in_bin = [&](float x, int b) { const float f = (xmax - x) * scale; return b < BINS - 1 ? f >= (float)b && f < (float)(b + 1) : !(f < (float)b); };
-    auto fill_bins = [&](bool weigh) {
-        const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
-        scale = (float)fmin(4.0 * weight.c, 1e30);
-        if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
+    // The kept scores with keys in [klo, khi] by bins of their distance to the first, index(x), and what each counts.
+    uint32_t klo = 0, khi = top;
+    auto fill_bins = [&](auto weigh, auto index) {
         __syncthreads();
         for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
         __syncthreads();
-        auto drop = [&](float x, u64 v) { atomicAdd(&sh.bins[bin(x)][lane & 31], v); };
+        const float xlo = klo ? key_score(klo) : -INFINITY, xhi = key_score(khi);
+        auto drop = [&](float x, u64 v) { if (x <= xhi) atomicAdd(&sh.bins[index(x)][lane & (S::COPIES - 1)], v); };
         row.each([&](int i, const float* s) {
             float x[VEC];
-            if (!only_kept(i, s, x, -INFINITY)) return;
-            if (weigh) {
+            if (!only_kept(i, s, x, xlo)) return;
+            u64 v[VEC];
+            if constexpr (decltype(weigh)::value) {
                 double w[VEC];
                 weight.template many<VEC>(x, w);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) drop(s[e], weight.fixed(w[e]));
+                for (int e = 0; e < VEC; ++e) v[e] = weight.fixed(w[e]);
             } else {
-                const u64 one = row.valid(i) ? 1 : 0;  // top_k comes first: every score counts
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) drop(s[e], one);
+                for (int e = 0; e < VEC; ++e) v[e] = (row.valid(i) & (s[e] >= xlo)) ? 1 : 0;
             }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) if (s[e] >= xlo) drop(s[e], v[e]);
         });
-        if (tid < row.sp.edge && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, weigh ? weight.fixed(weight(row.xe)) : 1);
+        if (tid < row.sp.edge && row.xe >= xlo && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, decltype(weigh)::value ? weight.fixed(weight(row.xe)) : 1);
         __syncthreads();
         for (int b = tid; b < BINS; b += G) {
             u64 s = 0;
@@ -483,111 +444,139 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         }
         __syncthreads();
     };
-    // Sum of the bins; the first bin at which the running sum reaches target (by every wave: two bins a lane).
-    auto bin_sum = [&]() { return wave_sum(sh.total[2 * lane] + sh.total[2 * lane + 1]); };
+    // Sum of the bins; the first bin at which the running sum, from `above` on, reaches target (every wave, BINS / 64 bins a lane).
+    constexpr int BL = BINS / 64;
+    auto bin_sum = [&]() {
+        u64 s = 0;
+#pragma unroll
+        for (int i = 0; i < BL; ++i) s += sh.total[BL * lane + i];
+        return wave_sum(s);
+    };
     auto bin_reach = [&](u64 target, u64& above) {
-        const u64 a0 = sh.total[2 * lane], a1 = sh.total[2 * lane + 1];
-        u64 s = a0 + a1;
+        u64 own = 0;
+#pragma unroll
+        for (int i = 0; i < BL; ++i) own += sh.total[BL * lane + i];
+        u64 s = own;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { const u64 o = __shfl_up(s, d); if (lane >= d) s += o; }
-        const u64 hit = __ballot(s >= target);
+        const u64 hit = __ballot(above + s >= target);
         const int l = hit ? __ffsll(hit) - 1 : 63;
-        const u64 f = __shfl(s, l) - __shfl(a0 + a1, l), m0 = __shfl(a0, l);   // in front of the pair, its first
-        const bool second = f + m0 < target;
-        above = second ? f + m0 : f;
-        return 2 * l + (second ? 1 : 0);
+        above += __shfl(s, l) - __shfl(own, l);
+        int b = BL * l;
+#pragma unroll
+        for (int i = 0; i < BL - 1; ++i)
+            if (b == BL * l + i && above + sh.total[b] < target) { above += sh.total[b]; ++b; }
+        return b;
     };
-    // list(c): work on a list of c places by the first wave alone if they are few; its cut to all
-    auto with_list = [&](int c, auto work) {
-        if (c <= 256) {
-            if (wave == 0) { List<T, 1, S> list(sh, c, n, weight); const Cut to = work(list); if (lane == 0) sh.cut = to; }
+    // The border of top_k (weigh false: target scores, `above` of them so far) or top_p (target of mass): bins, then the bin
+    // that the border is in split by keys until it holds a list or one key.
+    auto find_border = [&](auto weigh, u64 target, auto get_target) {
+        u64 above = 0;
+        klo = 0; khi = top;
+        // BINS over 32 octaves of the weight, or finer where the row is narrower
+        const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
+        float scale = (float)fmin(BINS / 32 * weight.c, 1e30);
+        if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
+        auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
+        fill_bins(weigh, bin);
+        target = get_target(target);
+        int b = bin_reach(target, above);
+        auto in_bin = [&](float x, int j) {
+            const float f = (xmax - x) * scale;
+            return !(f < (float)b) & ((b == BINS - 1) | (f < (float)(b + 1))) & cut(x, j);
+        };
+        int c = collect(in_bin);
+        if (c > CAP) {
+            // its keys
+            uint32_t l = 0, h = 0;
+            auto reach = [&](float x, bool in) { const uint32_t key = score_key(x); l = max(l, in ? ~key : 0u); h = max(h, in ? key : 0u); };
+            row.each([&](int i, const float* s) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) reach(s[e], row.valid(i) & in_bin(s[e], row.cls(i, e)));
+            });
+            if (tid < row.sp.edge) reach(row.xe, in_bin(row.xe, row.sp.edge_at(tid)));
+            klo = ~block_reduce<W>(l, OpMax(), sh.red2[0]);
+            khi = block_reduce<W>(h, OpMax(), sh.red2[1]);
+            while (c > CAP && klo < khi) {         // every round leaves 2 / BINS of the keys
+                int sh_bits = 0;
+                while ((khi - klo) >> sh_bits >= (uint32_t)BINS) ++sh_bits;
+                fill_bins(weigh, [&](float x) { return (int)((khi - score_key(x)) >> sh_bits); });
+                b = bin_reach(target, above);
+                const uint32_t to = khi - ((uint32_t)b << sh_bits), from = to - min(to - klo, (1u << sh_bits) - 1);
+                khi = to; klo = from;
+                const float xlo = key_score(klo), xhi = key_score(khi);
+                c = collect([&](float x, int j) { return (x >= xlo) & (x <= xhi) & cut(x, j); });
+            }
+        }
+        if (c <= CAP) {
+            if (wave == 0) {
+                const List<T> list(sh.list, c, n, weight);
+                const Cut to = decltype(weigh)::value ? list.cut_mass(above, target, cut) : list.cut_count((int)(target - above));
+                if (lane == 0) sh.cut = to;
+            }
             __syncthreads();
             cut = sh.cut;
-        } else { List<T, W, S> list(sh, c, n, weight); cut = work(list); }
+        } else {                                   // c equal scores
+            const float x = key_score(khi);
+            const int need = decltype(weigh)::value ? ties_needed(above, weight.fixed(weight(x)), target, c) : (int)(target - above);
+            if (x > -INFINITY) cut = {x, need < c ? nth(x, need) : x == cut.xt ? cut.ti : n};       // -inf weighs nothing: no cut
+        }
     };
-    // What equal scores x leave of it: all, or the first `need` by class.
-    auto cut_ties = [&](float x, int need, int ties) { cut = {x, need < ties ? nth(x, need) : x == cut.xt ? cut.ti : n}; };
+    auto kept_share = [&](float x, int j) { return cut(x, j) && !(least > 0 && weight(x) < least); };
 
-    // ---- top_k ------------------------------------------------------------------------------------------------------
-    if (k < n) {
-        if (k <= G / 2) {                          // k of the threads' maxima reach a bound
-            const uint32_t key = score_key(mine) >> SHIFT;
-            const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) { return count_waves(__popcll(__ballot(key >= mid))) >= k; });
-            const float bound = wide_key(v) > KEY_NEG_INF ? key_score(wide_key(v)) : NAN;
-            const int c = collect([&](float s, int) { return s >= bound; });
-            if (c >= k && c <= CAP) {
-                // the list holds everything: top_k, top_p and the answer from it
-                auto rest = [&](auto list) {
-                    cut = list.cut_count(k);
-                    list.keep(cut);
-                    if (p < 1.f) { cut = list.cut_mass(0, mass_target(list.all(weight)), weight, cut); list.keep(cut); }
-                    list.draw(u, least, answer);
-                };
-                if (c <= 256) { if (wave == 0) rest(List<T, 1, S>(sh, c, n, weight)); }
-                else rest(List<T, W, S>(sh, c, n, weight));
-                return;
-            }
-        }
-        fill_bins(false);
-        u64 above;
-        const int b = bin_reach((u64)k, above);
-        const int c = collect([&](float x, int) { return in_bin(x, b); }), need = k - (int)above;
-        if (c <= CAP) with_list(c, [&](auto& list) { return list.cut_count(need); });
-        else {                                     // many equal or nearly equal scores: bisection over the row
-            const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) {
-                const float s = key_score(wide_key(mid));
-                return wide_key(mid) <= KEY_NEG_INF || count([&](float x, int) { return x >= s; }) >= k; });
-            if (wide_key(v) > KEY_NEG_INF) {       // else only scores of -inf, which weigh nothing, are cut
-                const float x = key_score(wide_key(v));
-                const int over = count([&](float s, int) { return s > x; }), ties = count([&](float s, int) { return s == x; });
-                cut_ties(x, k - over, ties);
-            }
-        }
+    // ---- rows that fit in a list, and top_k of which the threads' maxima give one ---------------------------------------
+    int c = CAP + 1;
+    if (W == 1 || n <= CAP) c = collect([&](float x, int) { return x > -INFINITY; });
+    else if (k <= G / 2) {                         // k of the threads' maxima reach a bound
+        const uint32_t key = score_key(mine) >> SHIFT;
+        const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) { return count_waves(__popcll(__ballot(key >= mid))) >= k; });
+        const float bound = wide_key(v) > KEY_NEG_INF ? key_score(wide_key(v)) : NAN;
+        c = collect([&](float x, int) { return x >= bound; });
+        if (c < k) c = CAP + 1;
     }
-    // ---- top_p ------------------------------------------------------------------------------------------------------
-    if (p < 1.f) {
-        if (n <= CAP) {                            // a row that fits in the list
-            const int c = collect(cut);
-            with_list(c, [&](auto& list) { return list.cut_mass(0, mass_target(list.all(weight)), weight, cut); });
-        } else {
-            fill_bins(true);
-            const u64 target = mass_target(bin_sum());
-            u64 above;
-            const int b = bin_reach(target, above);
-            const int c = collect([&](float x, int j) { return in_bin(x, b) && cut(x, j); });
-            if (c <= CAP) with_list(c, [&](auto& list) { return list.cut_mass(above, target, weight, cut); });
-            else {
-                const float x = key_score(wide_key(last_enough(0, top >> SHIFT, [&](uint32_t mid) {
-                    const float s = key_score(wide_key(mid));
-                    return wide_key(mid) <= KEY_NEG_INF || mass([&](float x, int j) { return x >= s && cut(x, j); }) >= target; })));
-                const u64 over = mass([&](float s, int j) { return s > x && cut(s, j); });
-                const int ties = count([&](float s, int j) { return s == x && cut(s, j); });
-                cut_ties(x, ties_needed(over, weight.fixed(weight(x)), target, ties), ties);
-            }
-        }
+    if (c <= CAP) {
+        if (wave != 0) return;
+        List<T> list(sh.list, c, n, weight);
+        if (k < c) { cut = list.cut_count(k); list.keep(cut); }
+        if (p < 1.f) { cut = list.cut_mass(0, mass_target(list.all()), cut); list.keep(cut); }
+        if (least > 0) list.keep(kept_share);
+        list.draw(u, answer);
+        return;
+    }
+    if constexpr (W > 1) {                         // one wave: rows that fit in a list
+        if (k < n) find_border(std::false_type(), (u64)k, [](u64 t) { return t; });
+        if (p < 1.f) find_border(std::true_type(), 0, [&](u64) { return mass_target(bin_sum()); });
     }
     // ---- the answer -------------------------------------------------------------------------------------------------
     auto share = [&](float x, int j) {             // the weight of a class that is kept, else 0
         double w = 0;
-        if (x >= xlow && cut(x, j)) { w = weight(x); if (w < least) w = 0; }
+        if ((x >= xlow) & cut(x, j)) { w = weight(x); if (w < least) w = 0; }
         return w;
     };
-    __syncthreads();
-    row.each([&](int i, const float* s) {
-        double m = 0;
+    // weights of a vector's kept scores; false: there are none in the wave
+    auto shares = [&](int i, const float* s, double* w) {
         float x[VEC];
-        if (only_kept(i, s, x, xlow)) {
-            double w[VEC];
-            weight.template many<VEC>(x, w);
-            if (least > 0) {
+        if (!only_kept(i, s, x, xlow)) return false;
+        weight.template many<VEC>(x, w);
+        if (least > 0) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) w[e] = w[e] >= least ? w[e] : 0.0;
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) m += w[e];
-            m = wave_sum(m);
+            for (int e = 0; e < VEC; ++e) w[e] = w[e] >= least ? w[e] : 0.0;
         }
-        if (lane == 0) sh.cell.sum[row.cell(i)] = m;
+        return true;
+    };
+    __syncthreads();
+    double cell_sum = 0;
+    row.each([&](int i, const float* s) {
+        double w[VEC];
+        if (shares(i, s, w)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) cell_sum += w[e];
+        }
+        if (row.ends_cell(i)) {
+            cell_sum = wave_sum(cell_sum);
+            if (lane == 0) sh.cell.sum[row.cell(i)] = cell_sum;
+            cell_sum = 0;
+        }
     });
     const int cells = row.cells();
     if (wave == 0) {
@@ -616,47 +605,64 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         if (lane == 0) { sh.pick = found >= 0 ? found : last; sh.before = found >= 0 ? found_before : last_before; sh.all = all; }
     }
     __syncthreads();
-    const int c = sh.pick;
+    const int at = sh.pick;
     const double before = sh.before;
     all = sh.all;
     const double target = (double)u * all;
-    auto finish = [&](const double* w, const int* cl, int m) {             // one wave: m weights a lane, classes ascending over lanes
+    // the class within the cell: the lane in which the running sum exceeds the target, then its element; the last one that
+    // weighs anything if rounding leaves none
+    double run = before;
+    int last = -1; double last_w = 0;
+    row.in_cell(at, [&](int i, const float* s) {
+        double w[VEC];
+        if (!shares(i, s, w)) return false;
         double own = 0;
-        for (int e = 0; e < m; ++e) own += w[e];
-        double s = own;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(s, d); if (lane >= d) s += o; }
-        const double front = before + (s - own);
-        int hit = -1; double hw = 0, run = front;
-        int lastc = -1; double lastw = 0;
-        for (int e = 0; e < m; ++e) {
-            run += w[e];
-            if (w[e] > 0) { lastc = cl[e]; lastw = w[e]; if (hit < 0 && run > target) { hit = cl[e]; hw = w[e]; } }
+        for (int e = 0; e < VEC; ++e) own += w[e];
+        double p = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(p, d); if (lane >= d) p += o; }
+        const u64 hit = __ballot(own > 0 && run + p > target);
+        double front = run + (p - own);
+        int mine = -1, lastc = -1; double mw = 0, lastw = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            front += w[e];
+            if (w[e] > 0) {
+                lastc = row.cls(i, e); lastw = w[e];
+                if (mine < 0 && front > target) { mine = lastc; mw = lastw; }
+            }
         }
-        const u64 b = __ballot(hit >= 0), l = __ballot(lastc >= 0);
-        const int who = b ? __ffsll(b) - 1 : 63 - __clzll(l);
-        if (lane == who) answer(b ? hit : lastc, (float)log((b ? hw : lastw) / all));
-    };
-    row.at_cell(c, [&](int i, const float* s) {
-        double w[VEC]; int cl[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { cl[e] = row.cls(i, e); w[e] = row.valid(i) ? share(s[e], cl[e]) : 0.0; }
-        finish(w, cl, VEC);
+        if (mine < 0) { mine = lastc; mw = lastw; }
+        if (hit) {
+            if (lane == __ffsll(hit) - 1) answer(mine, (float)log(mw / all));
+            last = -1;
+            return true;
+        }
+        const u64 some = __ballot(own > 0);
+        if (some) { const int l = 63 - __clzll(some); last = __shfl(lastc, l); last_w = __shfl(lastw, l); }
+        run += __shfl(p, 63);
+        return false;
     });
-    if (wave == 0 && (c == 0 || c == cells - 1)) {
-        const bool here = tid < row.sp.edge && (tid < row.sp.head) == (c == 0);
+    if (lane == 0 && last >= 0) answer(last, (float)log(last_w / all));
+    if (wave == 0 && (at == 0 || at == cells - 1)) {
+        const bool here = tid < row.sp.edge && (tid < row.sp.head) == (at == 0);
         const int j = here ? row.sp.edge_at(tid) : 0;
         const double w = here ? share(row.xe, j) : 0.0;
-        finish(&w, &j, 1);
+        double p = w;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(p, d); if (lane >= d) p += o; }
+        const u64 hit = __ballot(w > 0 && before + p > target), some = __ballot(w > 0);
+        if (lane == (hit ? __ffsll(hit) - 1 : 63 - __clzll(some))) answer(j, (float)log(w / all));
     }
 }
 
 template <typename T> void launch(const SampleArgs& a, int rows, hipStream_t s) {
     constexpr int VEC = ET<T>::VEC;
     const int nv = a.n / VEC;
-    if (a.n <= 256) sample_kernel<T, 1, 4><<<rows, 64, 0, s>>>(a);
-    else if (nv <= 2048) sample_kernel<T, 4, 34><<<rows, 256, 0, s>>>(a);
-    else sample_kernel<T, 16, (1 << 20) / VEC / 64 + 18><<<rows, 1024, 0, s>>>(a);
+    if (a.n <= CAP) sample_kernel<T, 1, 2 + (CAP / VEC / 64 + 3) / 4><<<rows, 64, 0, s>>>(a);
+    else if (nv <= 2048) sample_kernel<T, 4, 10><<<rows, 256, 0, s>>>(a);
+    else sample_kernel<T, 16, (1 << 20) / VEC / 256 + 18><<<rows, 1024, 0, s>>>(a);
 }
 
 }  // namespace

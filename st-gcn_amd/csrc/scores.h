@@ -20,11 +20,18 @@ template <typename T> struct RowSpan {
     __device__ __forceinline__ int edge_at(int e) const { return e < head ? e : e + nvec * VEC; }   // class of edge element e
 };
 
+// Named as global memory: a pointer that went through a struct is a flat one to the compiler, and flat loads are waited
+// for with the LDS.
+#define STGCN_GLOBAL __attribute__((address_space(1)))
 template <typename T> __device__ __forceinline__ i32x4 load_vec(const T* row, int at) {
-    return *reinterpret_cast<const i32x4*>((const char*)row + (size_t)at * ET<T>::ES);
+    return *(const STGCN_GLOBAL i32x4*)((uintptr_t)row + (size_t)at * ET<T>::ES);
 }
 template <typename T> __device__ __forceinline__ void store_vec(T* row, int at, const i32x4& raw) {
-    *reinterpret_cast<i32x4*>((char*)row + (size_t)at * ET<T>::ES) = raw;
+    *(STGCN_GLOBAL i32x4*)((uintptr_t)row + (size_t)at * ET<T>::ES) = raw;
+}
+template <typename T> __device__ __forceinline__ float load_score(const T* row, size_t at) {
+    if constexpr (ET<T>::IS_BF16) return bf16_bits_to_f32(*(const STGCN_GLOBAL uint16_t*)((uintptr_t)row + at * 2));
+    else return *(const STGCN_GLOBAL float*)((uintptr_t)row + at * 4);
 }
 
 __device__ __forceinline__ int lanes_below(unsigned long long mask) {
@@ -77,20 +84,17 @@ __device__ __forceinline__ float key_score(uint32_t k) {
 __device__ __forceinline__ float exp2_32(float y) { return __builtin_amdgcn_exp2f(y); }
 
 // 2^y in 64 bits for y <= 1000: y = n + f, |f| <= 1/2, and 2^f = 1 + f q(f), q the polynomial of degree 8 that agrees with
-// (2^f - 1) / f at the nine Chebyshev points of [-1/2, 1/2] (3.7e-14 of the value at most, exactly 1 at y = 0).  n comes
-// from adding 1.5 * 2^52 and goes into the exponent by an integer add: conversions, roundings and ldexp of 64-bit numbers
-// run at a quarter of the rate of the adds and products.
-// N of them at once: the chains of N values side by side hide the latency of the 64-bit operations.
+// (2^f - 1) / f at the nine Chebyshev points of [-1/2, 1/2] (3.7e-14 of the value at most, exactly 1 at y = 0).  Every
+// 64-bit operation here, roundings and ldexp among them, issues at the rate of an add (4.8 cycles a wave and SIMD
+// measured, v_exp_f32 10.8).  N values at once: their chains side by side hide the latency.
 template <int N> __device__ __forceinline__ void exp2_64(const double* y, double* out) {
     double f[N], p[N];
     int n[N];
-    bool tiny = false;                                     // next to or below the normal range, but not at -1100 (-inf among them)
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        const double v = fmax(y[e], -1100.0), s = v + 6755399441055744.0;
-        f[e] = v - (s - 6755399441055744.0);
-        n[e] = (int)__double_as_longlong(s);
-        tiny |= (uint32_t)(n[e] + 1099) < 79u;             // -1099 .. -1021
+        const double v = fmax(y[e], -1100.0), r = rint(v);
+        f[e] = v - r;
+        n[e] = (int)r;
         p[e] = 1.0203121063391729e-07;
     }
     constexpr double Q[9] = {1.3255224878668817e-06, 1.525268684626772e-05, 0.00015403455852453838, 0.0013333558179043112, 0.009618129159402558,
@@ -100,17 +104,8 @@ template <int N> __device__ __forceinline__ void exp2_64(const double* y, double
 #pragma unroll
         for (int e = 0; e < N; ++e) p[e] = fma(p[e], f[e], Q[q]);
     }
-    if (__ballot(tiny)) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) out[e] = ldexp(p[e], n[e]);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const long long b = __double_as_longlong(p[e]);
-        const double w = __longlong_as_double((long long)((uint32_t)(b >> 32) + ((uint32_t)n[e] << 20)) << 32 | (uint32_t)b);
-        out[e] = n[e] < -1020 ? 0.0 : w;
-    }
+    for (int e = 0; e < N; ++e) out[e] = ldexp(p[e], n[e]);
 }
 __device__ __forceinline__ double exp2_64(double y) {
     double w;

@@ -214,7 +214,7 @@ __device__ void slow_row(const T* x, int lo, int hi, int tid, int k, Shared<W>& 
     for (int q = 0; q < k; ++q) {
         u64 best = 0;
         for (int j = lo + tid; j < hi; j += G) {
-            const u64 p = place(score_key(load_elem(x, j)), j);
+            const u64 p = place(score_key(load_score(x, j)), j);
             if (p > best && (q == 0 || p < last)) best = p;
         }
         best = wave_reduce(best, OpMax());
@@ -229,7 +229,7 @@ __device__ void slow_row(const T* x, int lo, int hi, int tid, int k, Shared<W>& 
     }
     rest = RestSum();
     for (int j = lo + tid; j < hi; j += G) {
-        const float v = load_elem(x, j);
+        const float v = load_score(x, j);
         if (place(score_key(v), j) < last) { if (v != v) rest.s = NAN; else rest.take(v, c); }
     }
     group_sync<W>();
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
             for (int e = 0; e < PER; ++e) pending |= (uint32_t)(mask[e] >> lane & 1) << e;
             auto cls = [&](int e) { return sp.vec_at(b * G * NB + (e / VEC) * G + tid) + e % VEC; };
             have = before;
-            const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, pending, [&](int e) { return load_elem(x, cls(e)); }, cls, rest, c);
+            const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, pending, [&](int e) { return load_score(x, cls(e)); }, cls, rest, c);
             top = -INFINITY;
 #pragma unroll
             for (int e = 0; e < PER; ++e) { if (kept >> e & 1) f[e] = -INFINITY; top = fmaxf(top, f[e]); }
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
     for (int end = 0; end < 2; ++end) {
         const int some = end ? sp.edge - sp.head : sp.head, j = end ? n - some + tid : tid;
         if (!(end ? with_tail : with_head) || some == 0) continue;
-        const float xe = tid < some ? load_elem(x, j) : 0.f;
+        const float xe = tid < some ? load_score(x, j) : 0.f;
         const u64 tau = sh.tau;
         const bool maybe = tid < some && (tau ? place(score_key(xe), j) > tau : !(xe <= sh.lim));
         const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, maybe ? 1u : 0u, [&](int) { return xe; }, [&](int) { return j; }, rest, c);
