@@ -20,6 +20,7 @@
 //   the answer: sums of the kept weights by cells (64 consecutive vectors: one wave's step), the cell in which u falls,
 //     then the lane, then the class.
 #include "scores.h"
+#include <cfloat>
 #include <type_traits>
 
 namespace {
@@ -104,14 +105,20 @@ template <typename T, int W> struct Row {
     __device__ __forceinline__ int cells() const { return W * wave_cells() + 2; }
     __device__ __forceinline__ int cell(int i) const { return 1 + wave * wave_cells() + i / CELL; }
     __device__ __forceinline__ bool ends_cell(int i) const { return i % CELL == CELL - 1 || i == steps - 1; }
-    // f(i, scores of vector i); scores beyond the row are -inf.  Three steps' loads are under way at a time.
+    // f(i, scores of vector i); scores beyond the row are -inf.  Three steps' loads are under way at a time (eight were slower:
+    // they are moved along every step).
     template <typename F> __device__ __forceinline__ void each(F f) const {
-        i32x4 v0 = load(0), v1 = load(1), v2 = load(2);
+        constexpr int D = 3;
+        i32x4 v[D];
+#pragma unroll
+        for (int d = 0; d < D; ++d) v[d] = load(d);
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             float s[VEC];
-            unpack16<T>(v0, s);
-            v0 = v1; v1 = v2; v2 = load(i + 3);
+            unpack16<T>(v[0], s);
+#pragma unroll
+            for (int d = 0; d + 1 < D; ++d) v[d] = v[d + 1];
+            v[D - 1] = load(i + D);
             f(i, s);
         }
     }
@@ -225,7 +232,7 @@ template <typename T> struct List {
 };
 
 template <typename T, int W, int CELLS>
-__global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
+__global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleArgs a) {
     typedef Row<T, W> R;
     typedef Shared<W, CELLS> S;
     constexpr int VEC = R::VEC, G = R::G, BINS = S::BINS;
@@ -321,41 +328,34 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         __syncthreads();
         return sh.pick;
     };
-    // The scores that pass, as places in the list (in no particular order: everything that is made of it is a set, or a sum
-    // of integers).  Returns how many there are; more than CAP are not all in it.
-    auto collect = [&](auto pred) {
+    // The kept scores in [xa, xb], xa > -inf, as places in the list (in no particular order: everything that is made of it is
+    // a set, or a sum of integers).  Returns how many there are; more than CAP are not all in it.  Few scores pass, so what
+    // counts is the test, two instructions a score, and that a lane with a hit handles it alone.
+    auto collect = [&](float xa, float xb) {
         __syncthreads();
         if (tid == 0) sh.pick = 0;
         __syncthreads();
+        xa = fmaxf(xa, cut.xt);
+        if (xa > xb) return 0;
+        auto append = [&](float x, int j) {
+            if (cut.ti < n && x == cut.xt && j > cut.ti) return;
+            const int at = atomicAdd(&sh.pick, 1);
+            if (at < CAP) sh.list[at] = place(score_key(x), j);
+        };
         row.each([&](int i, const float* s) {
-            const bool ok = row.valid(i);
             uint32_t in = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) in |= (ok & pred(s[e], row.cls(i, e))) ? 1u << e : 0u;
-            if (!__ballot(in != 0)) return;
-            const int m = __popc(in);              // 8 at most
-            int below = 0, all = 0;
+            for (int e = 0; e < VEC; ++e) in |= __builtin_amdgcn_fmed3f(s[e], xa, xb) == s[e] ? 1u << e : 0u;
+            while (in) {
+                const int e = __ffs(in) - 1;
+                in &= in - 1;
+                float x = s[0];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const u64 q = __ballot(m >> b & 1);
-                below += lanes_below(q) << b;
-                all += __popcll(q) << b;
+                for (int o = 1; o < VEC; ++o) x = e == o ? s[o] : x;
+                append(x, row.cls(i, e));
             }
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&sh.pick, all);
-            at = __builtin_amdgcn_readfirstlane(at) + below;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (in >> e & 1) { if (at < CAP) sh.list[at] = place(score_key(s[e]), row.cls(i, e)); ++at; }
         });
-        if (wave == 0) {
-            const bool in = tid < row.sp.edge && pred(row.xe, row.sp.edge_at(tid));
-            const u64 b = __ballot(in);
-            int at = 0;
-            if (lane == 0 && b) at = atomicAdd(&sh.pick, __popcll(b));
-            at = __builtin_amdgcn_readfirstlane(at) + lanes_below(b);
-            if (in && at < CAP) sh.list[at] = place(score_key(row.xe), row.sp.edge_at(tid));
-        }
+        if (tid < row.sp.edge && row.xe >= xa && row.xe <= xb) append(row.xe, row.sp.edge_at(tid));
         __syncthreads();
         const int c = sh.pick;
         __syncthreads();
@@ -413,11 +413,12 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
     // ---- borders ----------------------------------------------------------------------------------------------------
     // The kept scores with keys in [klo, khi] by bins of their distance to the first, index(x), and what each counts.
     uint32_t klo = 0, khi = top;
+    auto upper_score = [](uint32_t k) { return key_score(k == 0x7FFFFFFFu ? k - 1 : k); };  // no score has the key of -0, and as a number it is 0
     auto fill_bins = [&](auto weigh, auto index) {
         __syncthreads();
         for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
         __syncthreads();
-        const float xlo = klo ? key_score(klo) : -INFINITY, xhi = key_score(khi);
+        const float xlo = klo ? key_score(klo) : -INFINITY, xhi = upper_score(khi);
         auto drop = [&](float x, u64 v) { if (x <= xhi) atomicAdd(&sh.bins[index(x)][lane & (S::COPIES - 1)], v); };
         row.each([&](int i, const float* s) {
             float x[VEC];
@@ -481,32 +482,32 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
         fill_bins(weigh, bin);
         target = get_target(target);
         int b = bin_reach(target, above);
-        auto in_bin = [&](float x, int j) {
-            const float f = (xmax - x) * scale;
-            return !(f < (float)b) & ((b == BINS - 1) | (f < (float)(b + 1))) & cut(x, j);
-        };
-        int c = collect(in_bin);
-        if (c > CAP) {
-            // its keys
-            uint32_t l = 0, h = 0;
-            auto reach = [&](float x, bool in) { const uint32_t key = score_key(x); l = max(l, in ? ~key : 0u); h = max(h, in ? key : 0u); };
-            row.each([&](int i, const float* s) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) reach(s[e], row.valid(i) & in_bin(s[e], row.cls(i, e)));
-            });
-            if (tid < row.sp.edge) reach(row.xe, in_bin(row.xe, row.sp.edge_at(tid)));
-            klo = ~block_reduce<W>(l, OpMax(), sh.red2[0]);
-            khi = block_reduce<W>(h, OpMax(), sh.red2[1]);
-            while (c > CAP && klo < khi) {         // every round leaves 2 / BINS of the keys
-                int sh_bits = 0;
-                while ((khi - klo) >> sh_bits >= (uint32_t)BINS) ++sh_bits;
-                fill_bins(weigh, [&](float x) { return (int)((khi - score_key(x)) >> sh_bits); });
-                b = bin_reach(target, above);
-                const uint32_t to = khi - ((uint32_t)b << sh_bits), from = to - min(to - klo, (1u << sh_bits) - 1);
-                khi = to; klo = from;
-                const float xlo = key_score(klo), xhi = key_score(khi);
-                c = collect([&](float x, int j) { return (x >= xlo) & (x <= xhi) & cut(x, j); });
+        // the bin's scores: from the first key that is not beyond it to the last that has reached it, 64 keys tried at a time
+        auto last_key = [&](auto holds) {          // the last key up to top with holds(score), which holds for -inf and below
+            uint32_t lo = KEY_NEG_INF, hi = top;
+            while (lo < hi) {
+                const uint32_t step = (hi - lo) / 64 + 1, key = lo + lane * step;
+                const int m = __popcll(__ballot((lane == 0) | ((key > lo) & (key <= hi) & holds(key_score(min(max(key, lo), hi))))));
+                const uint32_t from = lo + (m - 1) * step;
+                hi = min(hi, from + (step - 1));
+                lo = from;
             }
+            return lo;
+        };
+        const uint32_t kb = last_key([&](float x) { return !((xmax - x) * scale < (float)b); });
+        const uint32_t ka = b == BINS - 1 ? KEY_NEG_INF : last_key([&](float x) { return !((xmax - x) * scale < (float)(b + 1)); }) + 1;
+        klo = max(ka, KEY_NEG_INF + 1);            // -inf weighs nothing: never in the list
+        khi = kb;
+        int c = collect(key_score(klo), upper_score(khi));
+        if (!decltype(weigh)::value && target > above + c) return;         // top_k reaches into scores of -inf: all others are kept
+        while (c > CAP && klo < khi) {             // every round leaves 2 / BINS of the keys
+            int sh_bits = 0;
+            while ((khi - klo) >> sh_bits >= (uint32_t)BINS) ++sh_bits;
+            fill_bins(weigh, [&](float x) { return (int)((khi - score_key(x)) >> sh_bits); });
+            b = bin_reach(target, above);
+            const uint32_t to = khi - ((uint32_t)b << sh_bits), from = to - min(to - klo, (1u << sh_bits) - 1);
+            khi = to; klo = from;
+            c = collect(key_score(klo), upper_score(khi));
         }
         if (c <= CAP) {
             if (wave == 0) {
@@ -526,13 +527,11 @@ __global__ __launch_bounds__(W * 64) void sample_kernel(SampleArgs a) {
 
     // ---- rows that fit in a list, and top_k of which the threads' maxima give one ---------------------------------------
     int c = CAP + 1;
-    if (W == 1 || n <= CAP) c = collect([&](float x, int) { return x > -INFINITY; });
+    if (W == 1 || n <= CAP) c = collect(-FLT_MAX, INFINITY);
     else if (k <= G / 2) {                         // k of the threads' maxima reach a bound
         const uint32_t key = score_key(mine) >> SHIFT;
         const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) { return count_waves(__popcll(__ballot(key >= mid))) >= k; });
-        const float bound = wide_key(v) > KEY_NEG_INF ? key_score(wide_key(v)) : NAN;
-        c = collect([&](float x, int) { return x >= bound; });
-        if (c < k) c = CAP + 1;
+        if (wide_key(v) > KEY_NEG_INF) c = collect(key_score(wide_key(v)), INFINITY);
     }
     if (c <= CAP) {
         if (wave != 0) return;
@@ -662,6 +661,7 @@ template <typename T> void launch(const SampleArgs& a, int rows, hipStream_t s) 
     const int nv = a.n / VEC;
     if (a.n <= CAP) sample_kernel<T, 1, 2 + (CAP / VEC / 64 + 3) / 4><<<rows, 64, 0, s>>>(a);
     else if (nv <= 2048) sample_kernel<T, 4, 10><<<rows, 256, 0, s>>>(a);
+    else if (rows > 256) sample_kernel<T, 8, (1 << 20) / VEC / 256 + 10><<<rows, 512, 0, s>>>(a);
     else sample_kernel<T, 16, (1 << 20) / VEC / 256 + 18><<<rows, 1024, 0, s>>>(a);
 }
 
