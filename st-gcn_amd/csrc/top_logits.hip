@@ -47,10 +47,10 @@ template <int W> struct Shared {
     static constexpr int EQ = W == 1 ? 128 : 1024;
     uint32_t maxima[EQ];                           // of the first batch; later the classes of equal scores
     u64 tau; float lim;                            // the bound; scores x with !(x <= lim) may be earlier in the order
-    int add[3][W], nkept;
+    int add[3][W];
     float rm[4]; double rs[4];
 };
-__device__ __forceinline__ int buffer_limit(int k) { return 2 * k + 64; }       // beyond it the bound is raised
+__host__ __device__ __forceinline__ int buffer_limit(int k) { return 2 * k + 64; }       // beyond it the bound is raised
 
 // The largest score before key `k` (> -inf) in the order of the scores.
 __device__ __forceinline__ float score_before(uint32_t k) { return key_score(k == 0x80000000u ? 0x7FFFFFFEu : k - 1); }   // -0 is 0
@@ -144,6 +144,22 @@ template <typename T, int W> __device__ __forceinline__ void compact(Shared<W>& 
     group_sync<W>();
 }
 
+// A key, to 16 bits, that k of the first 64 `some` (<= 64 MOST) maxima reach; by one wave.  0: not that many are there.
+template <int MOST> __device__ __forceinline__ uint32_t bound_of_maxima(const uint32_t* maxima, int some, int k) {
+    const int lane = threadIdx.x & 63;
+    uint32_t m[MOST], t = 0;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) m[i] = i < some ? maxima[lane + 64 * i] : 0;
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t to = t | 1u << bit;
+        int cnt = 0;
+#pragma unroll
+        for (int i = 0; i < MOST; ++i) if (i < some) cnt += __popcll(__ballot(m[i] >= to));
+        if (cnt >= k) t = to;
+    }
+    return t;
+}
+
 // What the waves append in a batch: `mine` entries of this wave; returns this wave's first slot, n becomes the new count
 // (which may be beyond CAP).
 template <int W> __device__ __forceinline__ int deal_slots(Shared<W>& sh, int tid, int& n, int& turn, int mine) {
@@ -170,10 +186,10 @@ __device__ __forceinline__ uint32_t offer(Shared<W>& sh, int tid, int& n, int& t
     constexpr int CAP = Shared<W>::CAP;
     uint32_t kept = 0;
     for (;;) {
-        const int m = __popc(pending);             // 17 at most
+        const int m = __popc(pending);
         int below = 0, all = 0;
 #pragma unroll
-        for (int b = 0; b < 5; ++b) {
+        for (int b = 0; b < 6; ++b) {
             const u64 q = __ballot(m >> b & 1);
             below += lanes_below(q) << b;
             all += __popcll(q) << b;
@@ -197,12 +213,12 @@ __device__ __forceinline__ uint32_t offer(Shared<W>& sh, int tid, int& n, int& t
     }
 }
 
-// Piece `piece` (of `pieces`) of row r.  With one piece the answer is written; else its k places, its rest's maximum and sum.
+// Piece `piece` (of `pieces`) of row r.  With one piece the answer is written; else what its buffer holds, its rest's maximum and sum.
 struct TopArgs {
     const void* x; size_t stride; int rows, n, k, pieces;
     float c; double T;
     float* values; long long* indices; float* rest;
-    u64* part; float2* part_rest;                  // [rows][pieces][k], [rows][pieces]
+    u64* part; float2* part_rest;                  // [rows][pieces][buffer_limit(k)], [rows][pieces]
 };
 
 template <typename T, int W>
@@ -327,18 +343,7 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
             } else sh.maxima[tid] = score_key(top);
             group_sync<W>();
             if (tid < 64) {
-                constexpr int MOST = W == 1 ? 1 : W * NB;
-                const int some = fine ? MOST : W;
-                uint32_t m[MOST], t = 0;
-#pragma unroll
-                for (int i = 0; i < MOST; ++i) m[i] = i < some ? sh.maxima[lane + 64 * i] : 0;
-                for (int bit = 31; bit >= 16; --bit) {
-                    const uint32_t to = t | 1u << bit;
-                    int cnt = 0;
-#pragma unroll
-                    for (int i = 0; i < MOST; ++i) if (i < some) cnt += __popcll(__ballot(m[i] >= to));
-                    if (cnt >= k) t = to;
-                }
+                const uint32_t t = bound_of_maxima<W == 1 ? 1 : W * NB>(sh.maxima, fine ? W * NB : W, k);
                 // a bound at or below -inf: everything
                 if (lane == 0) sh.lim = t <= KEY_NEG_INF ? NAN : score_before(t);
             }
@@ -399,7 +404,7 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
         const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, maybe ? 1u : 0u, [&](int) { return xe; }, [&](int) { return j; }, rest, c);
         if (tid < some && !kept) { if (xe != xe) rest.s = NAN; else rest.take(xe, c); }
     }
-    if (have > G || a.pieces > 1) compact<T, W>(sh, tid, have, k, rest, c);
+    if (have > G && a.pieces == 1) compact<T, W>(sh, tid, have, k, rest, c);
     else group_sync<W>();
     bool nan = rest.s != rest.s;
     if constexpr (W == 1) nan = __ballot(nan) != 0; else nan = __syncthreads_or(nan);
@@ -414,70 +419,59 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
     if (a.pieces == 1) {
         if (tid == 0) a.rest[r] = s != s ? NAN : m == -INFINITY ? -INFINITY : (float)((double)m / a.T + log(s));
     } else {
-        for (int i = tid; i < k; i += G) a.part[job * k + i] = i < have ? sh.cand[i] : 0;
+        const int limit = buffer_limit(k);
+        for (int i = tid; i < limit; i += G) a.part[job * limit + i] = i < have ? sh.cand[i] : 0;
         if (tid == 0) a.part_rest[job] = make_float2(m, (float)s);
     }
 }
 
-// A row's pieces joined: the k first of their places; the others go to the rest.  At most MAX_MERGE places.
+// A row's pieces joined, as a first batch of at most MAX_MERGE places: a bound from the threads' maxima, the places that
+// reach it into the buffer, the others into the rest.
 constexpr int MAX_MERGE = 8192;
 template <typename T>
 __global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a) {
     constexpr int R = MAX_MERGE / 256;
     __shared__ Shared<4> sh;
-    __shared__ int cnt[2][4];
-    const int tid = threadIdx.x, wave = tid >> 6, k = a.k, c = a.pieces * k;
+    const int tid = threadIdx.x, k = a.k, c = a.pieces * buffer_limit(k);
     const size_t r = blockIdx.x;
     const u64* part = a.part + r * c;
-    uint32_t key[R];
+    uint32_t key[R], top[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < R; ++i) key[i] = i * 256 < c && tid + 256 * i < c ? short_key<T>(part[tid + 256 * i]) : 0;
+    for (int i = 0; i < R; ++i) {
+        key[i] = 0;
+        if (256 * i < c && tid + 256 * i < c) key[i] = (uint32_t)(part[tid + 256 * i] >> 32);
+        top[i & 3] = max(top[i & 3], key[i]);
+    }
     RestSum rest;
     for (int i = tid; i < a.pieces; i += 256) {
         const float2 p = a.part_rest[r * a.pieces + i];
-        if (p.x > rest.m) { rest.raise(p.x, a.c); }
+        rest.raise(p.x, a.c);
         rest.s += p.x == rest.m ? p.y : p.y * exp2_32((p.x - (rest.m == -INFINITY ? 0.f : rest.m)) * a.c);
     }
-    // the k-th key, bit by bit; every thread counts its own, the waves' counts meet in LDS (two sets take turns)
-    uint32_t v = 0;
-    int turn = 0;
-    auto total = [&](int mine) {
-        if ((tid & 63) == 0) cnt[turn & 1][wave] = mine;
-        lds_barrier();
-        const int t = cnt[turn & 1][0] + cnt[turn & 1][1] + cnt[turn & 1][2] + cnt[turn & 1][3];
-        ++turn;
-        return t;
-    };
-    for (int b = 31 - KEY_SHIFT<T>; b >= 0; --b) {
-        int n = 0;
+    const bool fine = k > 64;
+    if (fine) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) if (256 * i < c) n += __popcll(__ballot(key[i] >= (v | 1u << b)));
-        if (total(n) >= k) v |= 1u << b;
-    }
-    int n = 0, e = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) if (256 * i < c) { n += __popcll(__ballot(key[i] > v)); e += __popcll(__ballot(key[i] == v)); }
-    const int above = total(n), equal = total(e);
-    uint32_t l = 0;
-    if (above + equal > k) {
-        for (int b = 31; b >= 0; --b) {
-            int m = 0;
-            for (int i = tid; i - tid < c; i += 256) m += __popcll(__ballot(i < c && short_key<T>(part[i < c ? i : 0]) == v && (uint32_t)part[i < c ? i : 0] >= (l | 1u << b)));
-            if (above + total(m) >= k) l |= 1u << b;
-        }
-    }
-    const u64 t = (u64)long_key<T>(v) << 32 | l;
-    if (tid == 0) sh.nkept = 0;
+        for (int i = 0; i < 4; ++i) sh.maxima[256 * i + tid] = top[i];
+    } else sh.maxima[tid] = max(max(top[0], top[1]), max(top[2], top[3]));
     __syncthreads();
+    if (tid < 64) {
+        const uint32_t t = bound_of_maxima<16>(sh.maxima, fine ? 16 : 4, k);
+        if (tid == 0) sh.tau = (u64)t << 32;
+    }
+    __syncthreads();
+    const uint32_t least = (uint32_t)(sh.tau >> 32);
+    uint32_t pending = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) if (key[i] && key[i] >= least) pending |= 1u << i;
+    int have = 0, turn = 0;
+    const uint32_t kept = offer<T, 4>(sh, tid, have, turn, k, pending, [&](int e) { return key_score((uint32_t)(part[tid + 256 * e] >> 32)); },
+                                      [&](int e) { return place_class(part[tid + 256 * e]); }, rest, a.c);
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (256 * i < c && tid + 256 * i < c) {
-            const u64 p = part[tid + 256 * i];
-            if (p >= t && p) { const int at = atomicAdd(&sh.nkept, 1); if (at < k) sh.cand[at] = p; }
-            else if (p) { const float x = key_score((uint32_t)(p >> 32)); if (x != x) rest.s = NAN; else rest.take(x, a.c); }
-        }
-    __syncthreads();
-    write_row<4>(a, r, sh, tid, k, rest);
+        if (key[i] && !(kept >> i & 1)) { const float x = key_score(key[i]); if (x != x) rest.s = NAN; else rest.take(x, a.c); }
+    if (have > 256) compact<T, 4>(sh, tid, have, k, rest, a.c);
+    else __syncthreads();
+    write_row<4>(a, r, sh, tid, have, rest);
     float m; double s;
     join_rest<4>(sh, tid, rest, a.c, m, s);
     if (tid == 0) a.rest[r] = s != s ? NAN : m == -INFINITY ? -INFINITY : (float)((double)m / a.T + log(s));
@@ -492,10 +486,10 @@ static int top_pieces(int rows, int ncls, int k) {
     const int batches = (ncls + 4095) / 4096;
     int p = (1024 + rows - 1) / rows;
     if (p > batches) p = batches;
-    if (p * k > MAX_MERGE) p = MAX_MERGE / k;
+    if (p * buffer_limit(k) > MAX_MERGE) p = MAX_MERGE / buffer_limit(k);
     return p;
 }
-static size_t top_workspace(int rows, int pieces, int k) { return pieces == 1 ? 0 : (size_t)rows * pieces * ((size_t)k * 8 + 8); }
+static size_t top_workspace(int rows, int pieces, int k) { return pieces == 1 ? 0 : (size_t)rows * pieces * ((size_t)buffer_limit(k) * 8 + 8); }
 
 extern "C" int stgcn_top_logits_workspace(int rows, int ncls, int k, size_t* bytes) {
     if (!bytes || rows < 1 || ncls < 1 || ncls > (1 << 20) || k < 1 || k > MAX_K || k > ncls) return STGCN_ERR_ARG;
@@ -510,7 +504,7 @@ extern "C" int stgcn_top_logits(int dtype, const void* logits, size_t row_stride
     const int pieces = top_pieces(rows, ncls, k);
     if (pieces > 1 && (!workspace || workspace_bytes < top_workspace(rows, pieces, k))) return STGCN_ERR_WORKSPACE;
     TopArgs a = {logits, row_stride, rows, ncls, k, pieces, (float)(LOG2E / temperature), temperature, values, (long long*)indices, rest,
-                 (u64*)workspace, (float2*)((char*)workspace + (pieces > 1 ? (size_t)rows * pieces * k * 8 : 0))};
+                 (u64*)workspace, (float2*)((char*)workspace + (pieces > 1 ? (size_t)rows * pieces * buffer_limit(k) * 8 : 0))};
     const hipStream_t s = (hipStream_t)stream;
     const unsigned grid = ncls <= 512 ? (unsigned)((rows + 3) / 4) : (unsigned)rows * pieces;
     if (dtype == STGCN_BF16) {
