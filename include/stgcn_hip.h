@@ -272,7 +272,7 @@ int stgcn_distill_bwd(int dtype, const void* logits, size_t row_stride, const in
                       const float* stats, const float* probs, const float* grad, int grad_per_row, double scale, int rows,
                       int ncls, int k, double temperature, double label_weight, void* dlogits, void* stream);
 
-/* Both in one: loss [1] (reduction 1 or 2) and its gradient.  A row of up to 131072 bf16 or 65536 float32 scores stays in
+/* Both in one: the loss and its gradient (reduction 0: of the sum of the rows' losses).  A row of up to 131072 bf16 or 65536 float32 scores stays in
  * registers between the two: one read and one write of the scores. */
 int stgcn_distill_step(int dtype, const void* logits, size_t row_stride, const float* values, const int64_t* indices,
                        const float* rest, const int64_t* labels, int rows, int ncls, int k, double temperature, double label_weight,

@@ -606,9 +606,9 @@ extern "C" int stgcn_distill_step(int dtype, const void* logits, size_t row_stri
                                   const float* rest, const int64_t* labels, int rows, int ncls, int k, double temperature,
                                   double label_weight, int reduction, float* loss, double* loss_rows, float* stats, float* probs, void* dlogits, void* stream) {
     if (bad_common(dtype, logits, row_stride, indices, rows, ncls, k, temperature, label_weight) || !values || !loss || !loss_rows || !stats
-        || !probs || !dlogits || (label_weight > 0 && !labels) || (reduction != 1 && reduction != 2)) return STGCN_ERR_ARG;
+        || !probs || !dlogits || (label_weight > 0 && !labels) || reduction < 0 || reduction > 2) return STGCN_ERR_ARG;
     DistillArgs a = fwd_args(logits, row_stride, values, indices, rest, labels, rows, ncls, k, temperature, label_weight);
-    a.loss_rows = loss_rows; a.dx = dlogits; a.scale = reduction == 1 ? (float)(1.0 / rows) : 1.f;
+    a.loss_rows = reduction ? loss_rows : nullptr; a.loss = loss; a.dx = dlogits; a.scale = reduction == 1 ? (float)(1.0 / rows) : 1.f;
     a.stats = (RowStats*)stats; a.probs = probs;
     const bool two = label_weight > 0 && temperature != 1.0;
     const hipStream_t s = (hipStream_t)stream;

@@ -609,13 +609,13 @@ class DistillCall:
         return loss
 
     def step(self):
-        """(loss, d loss / d logits) of one call."""
+        """(loss, d loss / d logits) of one call; reduction "none": the rows' losses, the gradient of their sum."""
         x = self.x
-        loss = torch.empty((), dtype=torch.float32, device=x.device)
+        loss = torch.empty((self.rows,) if self.reduction == "none" else (), dtype=torch.float32, device=x.device)
         dx = torch.empty((self.rows, self.ncls), dtype=x.dtype, device=x.device)
         if self.rows:
             self._forward("stgcn_distill_step", loss, dx.data_ptr())
-        else:
+        elif self.reduction != "none":
             loss.zero_()
         return loss, dx
 
