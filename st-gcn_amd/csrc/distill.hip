@@ -14,7 +14,7 @@
 
 namespace {
 
-constexpr int MAX_K = 256, EPL = MAX_K / 64;  // a row's entries: one wave's, EPL a lane
+constexpr int MAX_K = 256;
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.6931471805599453094;
 
 // What a row's forward leaves for its gradient: e^{z_j} = 2^{(x_j - xmax) c}, and the factors of the three sums.  xmax is
@@ -37,74 +37,103 @@ template <int W> __device__ __forceinline__ void group_sync() {
     else __syncthreads();
 }
 
-// ---- the teacher's side of a row, held by one wave -------------------------------------------------------------------
-struct Teacher {
-    int my[EPL]; float tv[EPL], xl[EPL];       // class (-1: none, or a class that an earlier entry has), score, student's score
-    double p[EPL];                             // the class's share; with duplicates their sum
-    double A, pr, own;                         // own: sum of p log p
-    bool any, bad;
+// ---- the teacher's side of a row, one wave's work ---------------------------------------------------------------------
+// Entries in LDS: class (-1: none, or a class that an earlier entry has), the student's score there, and the share p (with
+// duplicates their sum; before it is normalised, e^{t/T - max}).  Next to them what the others need: none of it waits for
+// the student's maximum or sums.
+struct Listed {
+    int cls[MAX_K]; float x[MAX_K]; double p[MAX_K];
+    double own, cross, pr;                     // sum of p log p (p_r among them), sum of p (z - the largest listed z), p_r
+    double sl, sl1; float xmax;                // sums of 2^{(x - xmax) c} over the listed classes, xmax their maximum
+    int flags;                                 // 1: there is a teacher, 2: an entry or the label is out of range
+    unsigned char later[MAX_K];
 };
+__device__ __forceinline__ void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
 
-// Entries into registers (nothing waits for them yet).
-__device__ __forceinline__ void teacher_load(const DistillArgs& a, size_t r, int lane, long long* i, float* t) {
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        i[e] = -1; t[e] = 0.f;
-        if (lane + 64 * e < a.k) { i[e] = a.idx[r * a.k + lane + 64 * e]; t[e] = a.val[r * a.k + lane + 64 * e]; }
-    }
-}
-
-// p, p_r and the sum of p log p, by one wave.  `rho` is only looked at where there is an entry.
-__device__ __forceinline__ void teacher_shares(const DistillArgs& a, const long long* i, const float* t, float rho32, Teacher& q) {
-    double z[EPL], m = -INFINITY;
+// Classes and student scores of the entries (loads only: issued before the row's own).
+template <typename T> __device__ __forceinline__ void listed_load(const DistillArgs& a, size_t r, const T* x, int lane, Listed& l) {
     bool bad = false, has = false;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        q.my[e] = i[e] >= 0 && i[e] < a.n ? (int)i[e] : -1;
-        q.p[e] = 0; z[e] = -INFINITY;
-        if (i[e] >= a.n) bad = true;
-        if (q.my[e] >= 0) {
-            if (!(t[e] < INFINITY)) bad = true;
-            else if (t[e] > -INFINITY) { z[e] = (double)t[e] / a.T; has = true; }
-        }
-        m = fmax(m, z[e]);
+    for (int e = lane; e < a.k; e += 64) {
+        const long long i = a.idx[r * a.k + e];
+        const float t = a.val[r * a.k + e];
+        const bool in = i >= 0 && i < a.n;
+        l.cls[e] = in ? (int)i : -1;
+        l.x[e] = in ? load_score(x, (size_t)i) : -INFINITY;
+        bad |= i >= a.n || (in && !(t < INFINITY));
+        const float u = in && t < INFINITY ? t : -INFINITY;
+        l.p[e] = (double)u;
+        has |= u > -INFINITY;
     }
-    q.any = __ballot(has) != 0 && a.w < 1.0;
-    q.bad = __ballot(bad) != 0;
-    q.A = 0; q.pr = 0; q.own = 0;
-    if (!q.any) return;
-    const double rho = (double)rho32;
-    if (!(rho < INFINITY)) { q.bad = true; return; }
-    m = fmax(wave_reduce(m, OpMax()), rho);
-    double s = 0;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) if (64 * e < a.k) { z[e] = z[e] > -INFINITY ? z[e] - m : -INFINITY; q.p[e] = exp(z[e]); s += q.p[e]; }
-    const double er = exp(rho - m);
-    s = wave_reduce(s, OpSum()) + er;
-    const double ls = log(s), inv = 1.0 / s;
-    q.A = m + ls; q.pr = er * inv;
-    double own = 0;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) if (q.p[e] > 0) { q.p[e] *= inv; own += q.p[e] * (z[e] - ls); }
-    q.own = own;                               // this lane's
-    if (q.pr > 0) q.own += (threadIdx.x & 63) == 0 ? q.pr * (rho - m - ls) : 0.0;
+    const int flags = (__ballot(has) != 0 && a.w < 1.0 ? 1 : 0) | (__ballot(bad) != 0 ? 2 : 0);
+    if (lane == 0) l.flags = flags;
+    wave_sync();
 }
 
-// Entries of one class: the first keeps the sum of their p, the others leave the list.  Rare; `li` is MAX_K ints and `pk`
-// MAX_K doubles of LDS that only this wave uses.
-__device__ void teacher_merge(const DistillArgs& a, int lane, Teacher& q, int* li, double* pk) {
-    for (int e = 0; e < EPL; ++e) { li[lane + 64 * e] = q.my[e]; pk[lane + 64 * e] = q.p[e]; }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    for (int e = 0; e < EPL; ++e) {
-        if (q.my[e] < 0) continue;
-        const int at = lane + 64 * e;
-        double s = 0;
-        bool first = true;
-        for (int o = 0; o < a.k; ++o)
-            if (li[o] == q.my[e]) { if (o < at) first = false; s += pk[o]; }
-        if (first) q.p[e] = s; else { q.my[e] = -1; q.p[e] = 0; }
+// Shares and sums.  `rho` is only looked at where there is an entry.
+template <bool TWO> __device__ __forceinline__ void listed_sums(const DistillArgs& a, int lane, float rho32, Listed& l) {
+    float tmax = -INFINITY, xmax = -INFINITY;
+    for (int e = lane; e < a.k; e += 64) { tmax = fmaxf(tmax, (float)l.p[e]); xmax = fmaxf(xmax, l.x[e]); }
+    tmax = wave_max(tmax); xmax = wave_max(xmax);
+    int flags = l.flags;
+    const bool any = flags & 1;
+    if (any && !(rho32 < INFINITY)) flags |= 2;
+    const double invT = 1.0 / a.T, rho = (double)rho32, m = any ? fmax((double)tmax * invT, rho) : 0.0;
+    double s = 0, sz = 0, sx = 0;
+    float sl = 0.f, sl1 = 0.f;
+    for (int e = lane; e < a.k; e += 64) {
+        const double t = l.p[e];
+        const float x = l.x[e];
+        double p = 0;
+        if (any && t > -INFINITY) {
+            const double z = t * invT - m;
+            p = exp2_64(z * LOG2E);
+            s += p; sz += p * z;
+            if (p > 0) sx += p * ((double)x - (xmax > -INFINITY ? (double)xmax : 0.0));
+        }
+        l.p[e] = p;
+        if (l.cls[e] >= 0 && xmax > -INFINITY) {
+            sl += exp2_32((x - xmax) * a.c);
+            if constexpr (TWO) sl1 += exp2_32((x - xmax) * a.c1);
+        }
     }
+    s = wave_sum(s); sz = wave_sum(sz); sx = wave_sum(sx);
+    const double er = any ? exp2_64((rho - m) * LOG2E) : 0.0;
+    s += er;
+    const double inv = any ? 1.0 / s : 0.0, ls = any ? ln_64(s) : 0.0;
+    for (int e = lane; e < a.k; e += 64) l.p[e] *= inv;
+    const double pr = er * inv, sl64 = wave_sum((double)sl), sl164 = TWO ? wave_sum((double)sl1) : 0.0;
+    if (lane == 0) {
+        l.own = (sz + (er > 0 ? er * (rho - m) : 0.0)) * inv - ls;         // sum of p log p = sum of p (z - ln s), all p being 1
+        l.cross = sx * inv * (double)a.c * LN2;
+        l.pr = pr; l.sl = sl64; l.sl1 = sl164; l.xmax = xmax; l.flags = flags;
+    }
+    wave_sync();
+}
+
+// Entries of one class: the first keeps the sum of their p, the others leave the list; sums are made anew.  Rare.
+template <bool TWO> __device__ __forceinline__ void listed_merge(const DistillArgs& a, int lane, Listed& l) {
+    for (int e = lane; e < a.k; e += 64) {
+        bool later = false;
+        for (int o = 0; o < e; ++o) later |= l.cls[o] == l.cls[e];
+        l.later[e] = later;
+    }
+    wave_sync();
+    float sl = 0.f, sl1 = 0.f;
+    for (int e = lane; e < a.k; e += 64) {
+        if (l.later[e] || l.cls[e] < 0) continue;
+        double p = 0;
+        for (int o = e; o < a.k; ++o) if (l.cls[o] == l.cls[e]) p += l.p[o];           // later ones are nobody else's to change
+        l.p[e] = p;
+        if (l.xmax > -INFINITY) {
+            sl += exp2_32((l.x[e] - l.xmax) * a.c);
+            if constexpr (TWO) sl1 += exp2_32((l.x[e] - l.xmax) * a.c1);
+        }
+    }
+    const double s = wave_sum((double)sl), s1 = TWO ? wave_sum((double)sl1) : 0.0;
+    wave_sync();
+    for (int e = lane; e < a.k; e += 64) if (l.later[e]) l.cls[e] = -1;
+    if (lane == 0) { l.sl = s; l.sl1 = s1; }
+    wave_sync();
 }
 
 // ---- bit map of the listed classes -----------------------------------------------------------------------------------
@@ -116,33 +145,53 @@ template <typename T> __device__ __forceinline__ uint32_t vec_bits(const uint32_
     return ET<T>::IS_BF16 ? byte : (byte >> (b & 7)) & 15u;
 }
 // ---- loss and factors of a row from its sums -------------------------------------------------------------------------
-// In every thread; the loss (a few logarithms in 64 bits) in one.
-struct RowSums { double sr, sl, s1; };
-__device__ __forceinline__ RowStats row_factors(const DistillArgs& a, const RowSums& s, float xmax, bool any, bool hard, bool bad, double pr) {
+// sr, s1: sums over the classes that are not listed, relative to their maximum m; joined with the listed ones'.
+struct RowSums { float xmax; double sl, sr, s1; };
+template <bool TWO> __device__ __forceinline__ RowSums join_sums(const DistillArgs& a, const Listed& l, float m, double sr, double s1) {
+    RowSums s;
+    const float both = fmaxf(m, l.xmax);
+    s.xmax = both == -INFINITY ? 0.f : both;
+    // a maximum of -inf: its sum is 0 (or NaN) and is taken as it is
+    s.sr = sr * (m == -INFINITY ? 1.0 : (double)exp2_32((m - s.xmax) * a.c));
+    s.sl = l.xmax == -INFINITY ? l.sl : l.sl * (double)exp2_32((l.xmax - s.xmax) * a.c);
+    if constexpr (TWO) s.s1 = s1 * (m == -INFINITY ? 1.0 : (double)exp2_32((m - s.xmax) * a.c1)) + (l.xmax == -INFINITY ? l.sl1 : l.sl1 * (double)exp2_32((l.xmax - s.xmax) * a.c1));
+    else s.s1 = s.sl + s.sr;
+    return s;
+}
+// In every thread; the loss (three logarithms in 64 bits, a lane each) by one wave.
+__device__ __forceinline__ RowStats row_factors(const DistillArgs& a, const RowSums& s, bool hard, int flags, double pr) {
     const double S = s.sl + s.sr;
-    RowStats st = {xmax, 0.f, 0.f, 0.f};
+    const bool any = flags & 1, bad = flags & 2;
+    RowStats st = {s.xmax, 0.f, 0.f, 0.f};
     if (any) {
-        const double f = (1.0 - a.w) * a.T;
-        st.gl = (float)(f / S);
-        st.gr = (float)(f * (1.0 / S - (pr > 0 && s.sr > 0 ? pr / s.sr : 0.0)));
+        const double f = (1.0 - a.w) * a.T, inv = 1.0 / S;
+        st.gl = (float)(f * inv);
+        st.gr = (float)(f * (inv - (pr > 0 && s.sr > 0 ? pr / s.sr : 0.0)));
     }
     if (hard) st.g1 = (float)(a.w / s.s1);
     if (bad || S != S || s.s1 != s.s1) st.gl = st.gr = st.g1 = NAN;
     if (!bad && ((!any && !hard) || S == 0)) st.xmax = NAN;   // nothing to learn from, or no class to learn: zeros
     return st;
 }
-// `terms` = sum of p (log p - z_k) over the entries, z relative to xmax, plus p_r log p_r
-__device__ __forceinline__ double row_loss(const DistillArgs& a, const RowSums& s, const RowStats& st, bool any, bool hard, double pr, double terms, float xy, float xmax) {
+__device__ __forceinline__ double row_loss(const DistillArgs& a, const RowSums& s, const RowStats& st, bool hard, const Listed& l, int lane, float xy) {
+    const double ln = ln_64(lane == 0 ? s.sl + s.sr : lane == 1 ? s.sr : s.s1);
+    const long long b = __double_as_longlong(ln);
+    auto of = [&](int who) {
+        return __longlong_as_double((long long)__builtin_amdgcn_readlane((int)(b >> 32), who) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)b, who));
+    };
+    const double lnS = of(0), lnr = of(1), ln1 = of(2);
     if (st.xmax != st.xmax) return 0.0;
     if (st.gl != st.gl) return NAN;
     double loss = 0;
-    if (any) {
-        // sum of p is 1 - p_r for the listed classes, so log S enters with weight 1 in all
-        double kl = terms + log(s.sl + s.sr);
-        if (pr > 0) kl -= pr * log(s.sr);
+    if (l.flags & 1) {
+        // z = x / T; the sums are relative to xmax, `cross` to the listed classes' largest score, whose shares add up to 1 - p_r.
+        // (Relative throughout: next to scores of 1e38 a log would vanish.)
+        double kl = l.own - l.cross + lnS;
+        if (l.xmax > -INFINITY) kl += (1.0 - l.pr) * (((double)s.xmax - (double)l.xmax) * (double)a.c * LN2);
+        if (l.pr > 0) kl -= l.pr * lnr;
         loss = (1.0 - a.w) * a.T * a.T * kl;
     }
-    if (hard) loss += a.w * (log(s.s1) - ((double)xy - (double)xmax) * (double)a.c1 * LN2);
+    if (hard) loss += a.w * (ln1 - ((double)xy - (double)s.xmax) * (double)a.c1 * LN2);
     return loss;
 }
 
@@ -163,58 +212,52 @@ template <typename T, bool TWO> __device__ __forceinline__ i32x4 grad_vec(const 
 
 // One row by W waves, its scores held in registers (NV vectors a thread): read once, and with GRAD the gradient is
 // written from there, so loss and gradient cost one read and one write of the scores.
-// What the listed classes need (their student scores, p, the gradient at their places) is wave 0's.  The gradient is first
-// written as if no class were listed; behind a barrier the listed ones and the label are written over.
+// What the listed classes need is wave 0's.  The gradient is first written as if no class were listed; behind a barrier the
+// listed ones and the label are written over.
 template <typename T, int W, int NV, bool TWO, bool GRAD>
-__global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(DistillArgs a) {
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 : 7) void distill_row_kernel(DistillArgs a) {
     constexpr int VEC = ET<T>::VEC, G = W * 64, ROWS = W == 1 ? 4 : 1, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
     __shared__ uint32_t bits_[ROWS][WORDS];
-    __shared__ int li_[ROWS][MAX_K];
-    __shared__ double pk_[ROWS][MAX_K];
-    __shared__ double rsum[4][W];
+    __shared__ Listed l_[ROWS];
+    __shared__ double rsum[2][W];
     __shared__ float rmax[W];
-    __shared__ double t_pr; __shared__ int t_flags;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x, sub = W == 1 ? wave : 0;
     const size_t r = (size_t)blockIdx.x * ROWS + sub;
     if (W == 1 && r >= (size_t)a.rows) return;
     const bool lead = W == 1 || wave == 0;
     uint32_t* bits = bits_[sub];
+    Listed& l = l_[sub];
     const int n = a.n;
     const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
     const RowSpan<T> sp(x, n);
 
-    long long ei[EPL]; float et[EPL]; float rho = -INFINITY;
-    if (lead) { teacher_load(a, r, lane, ei, et); if (a.rest) rho = a.rest[r]; }
     const long long y = a.labels ? a.labels[r] : -1;
+    const bool hard = a.w > 0.0 && y >= 0 && y < n;
     i32x4 v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>();
-    float xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY;
+    float xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY, xy = 0.f;
+    if (lead) {
+        listed_load(a, r, x, lane, l);
+        if (hard) xy = load_score(x, (size_t)y);
+    }
     for (int i = tid; i < WORDS; i += G) bits[i] = 0;
     group_sync<W>();
-
-    Teacher q;
-    const bool hard = a.w > 0.0 && y >= 0 && y < n;
-    float xy = 0.f;
     if (lead) {
-        teacher_shares(a, ei, et, rho, q);
         bool dup = false;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-            if (q.my[e] >= 0) {
-                const int b = BIT0 + q.my[e] - sp.head;
+        for (int e = lane; e < a.k; e += 64)
+            if (l.cls[e] >= 0) {
+                const int b = BIT0 + l.cls[e] - sp.head;
                 dup |= (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1;
             }
-        if (__ballot(dup)) teacher_merge(a, lane, q, li_[sub], pk_[sub]);
-        if (a.w > 0.0 && y >= n) q.bad = true;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_score(x, q.my[e]) : -INFINITY;
-        if (hard) xy = load_score(x, (size_t)y);
-        if (W > 1 && lane == 0) { t_pr = q.pr; t_flags = (q.any ? 1 : 0) | (q.bad ? 2 : 0); }
+        if (lane == 0 && a.w > 0.0 && y >= n) l.flags |= 2;
+        wave_sync();
+        listed_sums<TWO>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
+        if (__ballot(dup)) listed_merge<TWO>(a, lane, l);
     }
     group_sync<W>();
 
-    // the maximum; listed classes leave the registers
+    // the maximum of the classes that are not listed; listed ones leave the registers
     float m = -INFINITY;
     if (xe > -INFINITY || xe != xe) {
         const int b = BIT0 + sp.edge_at(tid) - sp.head;
@@ -229,21 +272,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(Dist
             m = fmaxf(m, vec_max<T>(v[i]));
         }
     }
-    if (lead) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) m = fmaxf(m, q.xl[e]);
-    }
-    m = wave_reduce(m, OpFMax());
+    m = wave_max(m);
     if constexpr (W > 1) {
         if (lane == 0) rmax[wave] = m;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) m = fmaxf(m, rmax[w]);
     }
-    const float xmax = m == -INFINITY ? 0.f : m;
 
-    // the sums
-    float s = exp2_32((xe - xmax) * a.c), s1 = TWO ? exp2_32((xe - xmax) * a.c1) : 0.f;
+    // their sums
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = exp2_32((xe - ref) * a.c), s1 = TWO ? exp2_32((xe - ref) * a.c1) : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (i * G < sp.nvec) {
@@ -251,51 +290,32 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(Dist
             unpack16<T>(v[i], f);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float t = f[j] - xmax;
+                const float t = f[j] - ref;
                 s += exp2_32(t * a.c);
                 if constexpr (TWO) s1 += exp2_32(t * a.c1);
             }
         }
     }
-    RowSums sum = {wave_reduce((double)s, OpSum()), 0, TWO ? wave_reduce((double)s1, OpSum()) : 0.0};
-    double terms = 0;
-    if (lead) {
-        double sl = 0, sl1 = 0, t = q.any ? q.own : 0.0;
-#pragma unroll
-        for (int e = 0; e < EPL; ++e)
-            if (64 * e < a.k && q.my[e] >= 0) {
-                const float d = q.xl[e] - xmax;
-                sl += (double)exp2_32(d * a.c);
-                if constexpr (TWO) sl1 += (double)exp2_32(d * a.c1);
-                if (q.p[e] > 0) t -= q.p[e] * ((double)q.xl[e] - (double)xmax) * (double)a.c * LN2;
-            }
-        sum.sl = wave_reduce(sl, OpSum());
-        if constexpr (TWO) sum.s1 += wave_reduce(sl1, OpSum());
-        terms = wave_reduce(t, OpSum());
-    }
-    bool any = q.any, bad = q.bad;
-    double pr = q.pr;
+    double sr = wave_sum((double)s), sr1 = TWO ? wave_sum((double)s1) : 0.0;
     if constexpr (W > 1) {
-        if (lane == 0) { rsum[0][wave] = sum.sr; rsum[1][wave] = sum.s1; if (wave == 0) rsum[2][0] = sum.sl; }
+        if (lane == 0) { rsum[0][wave] = sr; if constexpr (TWO) rsum[1][wave] = sr1; }
         __syncthreads();
-        sum = {0, rsum[2][0], 0};
+        sr = sr1 = 0;
 #pragma unroll
-        for (int w = 0; w < W; ++w) { sum.sr += rsum[0][w]; if constexpr (TWO) sum.s1 += rsum[1][w]; }
-        any = t_flags & 1; bad = t_flags & 2; pr = t_pr;
+        for (int w = 0; w < W; ++w) { sr += rsum[0][w]; if constexpr (TWO) sr1 += rsum[1][w]; }
     }
-    if constexpr (!TWO) sum.s1 = sum.sl + sum.sr;
-    const RowStats st = row_factors(a, sum, xmax, any, hard, bad, pr);
+    const RowSums sum = join_sums<TWO>(a, l, m, sr, sr1);
+    const RowStats st = row_factors(a, sum, hard, l.flags, l.pr);
     const bool empty = st.xmax != st.xmax;
-    if (lead && lane == 0) {
-        const double loss = row_loss(a, sum, st, any, hard, pr, terms, xy, xmax);
-        if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
-        if constexpr (!GRAD) a.stats[r] = st;
+    if (lead) {
+        const double loss = row_loss(a, sum, st, hard, l, lane, xy);
+        if (lane == 0) {
+            if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
+            if constexpr (!GRAD) a.stats[r] = st;
+        }
     }
     if constexpr (!GRAD) {
-        if (lead) {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) if (lane + 64 * e < a.k) a.probs[r * a.k + lane + 64 * e] = q.my[e] >= 0 ? (float)q.p[e] : -1.f;
-        }
+        if (lead) for (int e = lane; e < a.k; e += 64) a.probs[r * a.k + e] = l.cls[e] >= 0 ? (float)l.p[e] : -1.f;
     } else {
         T* dx = (T*)a.dx + r * (size_t)n;
         const Grad<T, TWO> g = {empty ? 0.f : st.xmax, a.c, a.c1, st.g1 * a.scale};
@@ -321,13 +341,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64) void distill_row_kernel(Dist
         if (lead && !empty) {
             const float fp = a.fp * a.scale, w = a.w1 * a.scale;
             bool mine = false;
-#pragma unroll
-            for (int e = 0; e < EPL; ++e)
-                if (q.my[e] >= 0) {
-                    float d = g(q.xl[e], gl) - fp * (float)q.p[e];
-                    if (hard && q.my[e] == (int)y) { d -= w; mine = true; }
-                    store_elem(dx, q.my[e], d);
-                }
+            for (int e = lane; e < a.k; e += 64) {
+                const int j = l.cls[e];
+                if (j < 0) continue;
+                float d = g(l.x[e], gl) - fp * (float)l.p[e];
+                if (hard && j == (int)y) { d -= w; mine = true; }
+                store_elem(dx, j, d);
+            }
             if (hard && !__ballot(mine) && lane == 0) store_elem(dx, (size_t)y, g(xy, gr) - w);
         }
     }
@@ -339,9 +359,8 @@ template <typename T, bool TWO>
 __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
     constexpr int VEC = ET<T>::VEC, W = 16, G = 1024, NV = 64 / VEC, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
     __shared__ uint32_t bits[WORDS];
-    __shared__ int li[MAX_K];
-    __shared__ double pk[MAX_K];
-    __shared__ double rsum[3][W];
+    __shared__ Listed l;
+    __shared__ double rsum[2][W];
     __shared__ float rmax[W];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = threadIdx.x, n = a.n;
     const size_t r = blockIdx.x;
@@ -350,12 +369,10 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
     const bool lead = wave == 0;
     const long long y = a.labels ? a.labels[r] : -1;
     const bool hard = a.w > 0.0 && y >= 0 && y < n;
-    Teacher q;
     float m = -INFINITY, s = 0.f, s1 = 0.f, xy = 0.f;
     auto raise = [&](float to) {
         if (to > m) {
-            const float up = m == -INFINITY ? 0.f : exp2_32((m - to) * a.c);
-            s *= up;
+            s *= m == -INFINITY ? 0.f : exp2_32((m - to) * a.c);
             if constexpr (TWO) s1 *= m == -INFINITY ? 0.f : exp2_32((m - to) * a.c1);
             m = to;
         }
@@ -366,33 +383,28 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
         if constexpr (TWO) s1 += exp2_32(t * a.c1);
     };
     if (lead) {
-        long long ei[EPL]; float et[EPL];
-        teacher_load(a, r, lane, ei, et);
-        teacher_shares(a, ei, et, a.rest ? a.rest[r] : -INFINITY, q);
-        if (a.w > 0.0 && y >= n) q.bad = true;
-        teacher_merge(a, lane, q, li, pk);
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) q.xl[e] = q.my[e] >= 0 ? load_score(x, q.my[e]) : -INFINITY;
+        listed_load(a, r, x, lane, l);
+        if (lane == 0 && a.w > 0.0 && y >= n) l.flags |= 2;
+        wave_sync();
+        listed_sums<TWO>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
+        listed_merge<TWO>(a, lane, l);
         if (hard) xy = load_score(x, (size_t)y);
     }
     for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NV) {
-        // classes of this segment: [c0, c1), the row's edges with the first one
-        const int base = sp.vec_at(v0);
+        const int base = sp.vec_at(v0);            // the segment's first class; the row's ends go with the first segment
         __syncthreads();
         for (int i = tid; i < WORDS; i += G) bits[i] = 0;
         __syncthreads();
-        if (lead) {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) {
-                const int b = BIT0 + q.my[e] - base;
-                if (q.my[e] >= base && q.my[e] < base + G * NV * VEC) atomicOr(&bits[b >> 5], 1u << (b & 31));
+        if (lead)
+            for (int e = lane; e < a.k; e += 64) {
+                const int j = l.cls[e], b = BIT0 + j - base;
+                if (j >= base && j < base + G * NV * VEC) atomicOr(&bits[b >> 5], 1u << (b & 31));
             }
-        }
         __syncthreads();
         if (v0 == 0 && tid < sp.edge) {
             const int j = sp.edge_at(tid);
             bool is_listed = false;
-            for (int o = 0; o < a.k; ++o) is_listed |= li[o] == j;
+            for (int e = 0; e < a.k; ++e) is_listed |= l.cls[e] == j;
             if (!is_listed) { const float f = load_score(x, j); raise(f); add(f); }
         }
         i32x4 v[NV];
@@ -414,38 +426,19 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
             for (int j = 0; j < VEC; ++j) add(f[j]);
         }
     }
-    float all = m;
-    if (lead) {
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) all = fmaxf(all, q.xl[e]);
-    }
-    all = block_reduce<W>(all, OpFMax(), rmax);
-    const float xmax = all == -INFINITY ? 0.f : all;
+    const float all = block_reduce<W>(m, OpFMax(), rmax);
     const bool none = m == -INFINITY;              // then s is 0, or NaN
-    RowSums sum;
-    sum.sr = block_reduce<W>((double)s * (none ? 1.0 : (double)exp2_32((m - xmax) * a.c)), OpSum(), rsum[0]);
-    sum.s1 = TWO ? block_reduce<W>((double)s1 * (none ? 1.0 : (double)exp2_32((m - xmax) * a.c1)), OpSum(), rsum[1]) : 0.0;
+    const double sr = block_reduce<W>((double)s * (none ? 1.0 : (double)exp2_32((m - all) * a.c)), OpSum(), rsum[0]);
+    const double sr1 = TWO ? block_reduce<W>((double)s1 * (none ? 1.0 : (double)exp2_32((m - all) * a.c1)), OpSum(), rsum[1]) : 0.0;
     if (!lead) return;
-    double sl = 0, sl1 = 0, terms = q.any ? q.own : 0.0;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e)
-        if (q.my[e] >= 0) {
-            const float d = q.xl[e] - xmax;
-            sl += (double)exp2_32(d * a.c);
-            if constexpr (TWO) sl1 += (double)exp2_32(d * a.c1);
-            if (q.p[e] > 0) terms -= q.p[e] * ((double)q.xl[e] - (double)xmax) * (double)a.c * LN2;
-        }
-    sum.sl = wave_reduce(sl, OpSum());
-    sum.s1 = TWO ? sum.s1 + wave_reduce(sl1, OpSum()) : sum.sl + sum.sr;
-    terms = wave_reduce(terms, OpSum());
-    const RowStats st = row_factors(a, sum, xmax, q.any, hard, q.bad, q.pr);
+    const RowSums sum = join_sums<TWO>(a, l, all, sr, sr1);
+    const RowStats st = row_factors(a, sum, hard, l.flags, l.pr);
+    const double loss = row_loss(a, sum, st, hard, l, lane, xy);
     if (lane == 0) {
-        const double loss = row_loss(a, sum, st, q.any, hard, q.pr, terms, xy, xmax);
         if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
         a.stats[r] = st;
     }
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) if (lane + 64 * e < a.k) a.probs[r * a.k + lane + 64 * e] = q.my[e] >= 0 ? (float)q.p[e] : -1.f;
+    for (int e = lane; e < a.k; e += 64) a.probs[r * a.k + e] = l.cls[e] >= 0 ? (float)l.p[e] : -1.f;
 }
 
 struct GradArgs {

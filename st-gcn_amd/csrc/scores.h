@@ -113,6 +113,16 @@ __device__ __forceinline__ double exp2_64(double y) {
     return w;
 }
 
+// ln x in 64 bits: x = m 2^e, y = v_log_f32(m), and one Newton step on 2^y = m: y + (m 2^-y - 1) log2(e), within 1e-14.
+// 0 and +inf answer -inf and +inf, less than 0 and NaN answer NaN.
+__device__ __forceinline__ double ln_64(double x) {
+    int e;
+    const double m = frexp(x, &e);
+    if (!(m > 0) || m == INFINITY) return m == 0 ? -INFINITY : m == INFINITY ? m : NAN;
+    const double y = (double)__builtin_amdgcn_logf((float)m);
+    return ((double)e + y + fma(m, exp2_64(-y), -1.0) * 1.4426950408889634074) * 0.6931471805599453094;
+}
+
 // ---- reductions of a workgroup of W waves: every thread gets the result; `red` is W entries of LDS -------------------
 struct OpMax { template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct OpFMax { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
@@ -139,6 +149,21 @@ __device__ __forceinline__ double wave_sum(double v) {
     const long long b = __double_as_longlong(v);
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)b, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63);
     return __longlong_as_double((long long)hi << 32 | lo);
+}
+
+// Maximum over the wave the same way (fmaxf: NaN is no number).
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_max(float v) {
+    const int o = __builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xF, false);    // itself where there is none
+    return fmaxf(v, __int_as_float(o));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    v = dpp_max<0x143, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // The same for 64-bit integers.
