@@ -28,32 +28,32 @@ struct DistillArgs {
     void* dx; float scale;                     // of the gradient, where it is written
     int rows, n, k;
     float c, c1, fp, w1;                       // log2(e) / T, log2(e), (1 - w) T, w
-    double T, w;
+    double T, invT, w;
 };
 
-// Waves that work on one row: W of them, and for W = 1 four rows share a workgroup and no barrier is needed.
+// Waves that work on one row: W of them, and for W = 1 several rows share a workgroup and no barrier is needed.
 template <int W> __device__ __forceinline__ void group_sync() {
     if constexpr (W == 1) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
     else __syncthreads();
 }
 
-// ---- the teacher's side of a row, one wave's work ---------------------------------------------------------------------
+// ---- the teacher's side of a row, the work of one group of L lanes (scores.h) ---------------------------------------------------------------------
 // Entries in LDS: class (-1: none, or a class that an earlier entry has), the student's score there, and the share p (with
 // duplicates their sum; before it is normalised, e^{t/T - max}).  Next to them what the others need: none of it waits for
 // the student's maximum or sums.
-struct Listed {
-    int cls[MAX_K]; float x[MAX_K]; double p[MAX_K];
+template <int K> struct Listed {                // K: entries at most
+    int cls[K]; float x[K]; double p[K];
     double own, cross, pr;                     // sum of p log p (p_r among them), sum of p (z - the largest listed z), p_r
     double sl, sl1; float xmax;                // sums of 2^{(x - xmax) c} over the listed classes, xmax their maximum
     int flags;                                 // 1: there is a teacher, 2: an entry or the label is out of range
-    unsigned char later[MAX_K];
+    unsigned char later[K];
 };
 __device__ __forceinline__ void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
 
 // Classes and student scores of the entries (loads only: issued before the row's own).
-template <typename T> __device__ __forceinline__ void listed_load(const DistillArgs& a, size_t r, const T* x, int lane, Listed& l) {
+template <typename T, int L, int K> __device__ __forceinline__ void listed_load(const DistillArgs& a, size_t r, const T* x, int lane, Listed<K>& l) {
     bool bad = false, has = false;
-    for (int e = lane; e < a.k; e += 64) {
+    for (int e = lane; e < a.k; e += L) {
         const long long i = a.idx[r * a.k + e];
         const float t = a.val[r * a.k + e];
         const bool in = i >= 0 && i < a.n;
@@ -64,23 +64,23 @@ template <typename T> __device__ __forceinline__ void listed_load(const DistillA
         l.p[e] = (double)u;
         has |= u > -INFINITY;
     }
-    const int flags = (__ballot(has) != 0 && a.w < 1.0 ? 1 : 0) | (__ballot(bad) != 0 ? 2 : 0);
+    const int flags = (group_any<L>(has) && a.w < 1.0 ? 1 : 0) | (group_any<L>(bad) ? 2 : 0);
     if (lane == 0) l.flags = flags;
     wave_sync();
 }
 
 // Shares and sums.  `rho` is only looked at where there is an entry.
-template <bool TWO> __device__ __forceinline__ void listed_sums(const DistillArgs& a, int lane, float rho32, Listed& l) {
+template <bool TWO, int L, int K> __device__ __forceinline__ void listed_sums(const DistillArgs& a, int lane, float rho32, Listed<K>& l) {
     float tmax = -INFINITY, xmax = -INFINITY;
-    for (int e = lane; e < a.k; e += 64) { tmax = fmaxf(tmax, (float)l.p[e]); xmax = fmaxf(xmax, l.x[e]); }
-    tmax = wave_max(tmax); xmax = wave_max(xmax);
+    for (int e = lane; e < a.k; e += L) { tmax = fmaxf(tmax, (float)l.p[e]); xmax = fmaxf(xmax, l.x[e]); }
+    tmax = group_max<L>(tmax); xmax = group_max<L>(xmax);
     int flags = l.flags;
     const bool any = flags & 1;
     if (any && !(rho32 < INFINITY)) flags |= 2;
-    const double invT = 1.0 / a.T, rho = (double)rho32, m = any ? fmax((double)tmax * invT, rho) : 0.0;
+    const double invT = a.invT, rho = (double)rho32, m = any ? fmax((double)tmax * invT, rho) : 0.0;
     double s = 0, sz = 0, sx = 0;
     float sl = 0.f, sl1 = 0.f;
-    for (int e = lane; e < a.k; e += 64) {
+    for (int e = lane; e < a.k; e += L) {
         const double t = l.p[e];
         const float x = l.x[e];
         double p = 0;
@@ -96,12 +96,12 @@ template <bool TWO> __device__ __forceinline__ void listed_sums(const DistillArg
             if constexpr (TWO) sl1 += exp2_32((x - xmax) * a.c1);
         }
     }
-    s = wave_sum(s); sz = wave_sum(sz); sx = wave_sum(sx);
+    s = group_sum<L>(s); sz = group_sum<L>(sz); sx = group_sum<L>(sx);
     const double er = any ? exp2_64((rho - m) * LOG2E) : 0.0;
     s += er;
     const double inv = any ? 1.0 / s : 0.0, ls = any ? ln_64(s) : 0.0;
-    for (int e = lane; e < a.k; e += 64) l.p[e] *= inv;
-    const double pr = er * inv, sl64 = wave_sum((double)sl), sl164 = TWO ? wave_sum((double)sl1) : 0.0;
+    for (int e = lane; e < a.k; e += L) l.p[e] *= inv;
+    const double pr = er * inv, sl64 = group_sum<L>((double)sl), sl164 = TWO ? group_sum<L>((double)sl1) : 0.0;
     if (lane == 0) {
         l.own = (sz + (er > 0 ? er * (rho - m) : 0.0)) * inv - ls;         // sum of p log p = sum of p (z - ln s), all p being 1
         l.cross = sx * inv * (double)a.c * LN2;
@@ -111,15 +111,15 @@ template <bool TWO> __device__ __forceinline__ void listed_sums(const DistillArg
 }
 
 // Entries of one class: the first keeps the sum of their p, the others leave the list; sums are made anew.  Rare.
-template <bool TWO> __device__ __forceinline__ void listed_merge(const DistillArgs& a, int lane, Listed& l) {
-    for (int e = lane; e < a.k; e += 64) {
+template <bool TWO, int L, int K> __device__ __forceinline__ void listed_merge(const DistillArgs& a, int lane, Listed<K>& l) {
+    for (int e = lane; e < a.k; e += L) {
         bool later = false;
         for (int o = 0; o < e; ++o) later |= l.cls[o] == l.cls[e];
         l.later[e] = later;
     }
     wave_sync();
     float sl = 0.f, sl1 = 0.f;
-    for (int e = lane; e < a.k; e += 64) {
+    for (int e = lane; e < a.k; e += L) {
         if (l.later[e] || l.cls[e] < 0) continue;
         double p = 0;
         for (int o = e; o < a.k; ++o) if (l.cls[o] == l.cls[e]) p += l.p[o];           // later ones are nobody else's to change
@@ -129,9 +129,9 @@ template <bool TWO> __device__ __forceinline__ void listed_merge(const DistillAr
             if constexpr (TWO) sl1 += exp2_32((l.x[e] - l.xmax) * a.c1);
         }
     }
-    const double s = wave_sum((double)sl), s1 = TWO ? wave_sum((double)sl1) : 0.0;
+    const double s = group_sum<L>((double)sl), s1 = TWO ? group_sum<L>((double)sl1) : 0.0;
     wave_sync();
-    for (int e = lane; e < a.k; e += 64) if (l.later[e]) l.cls[e] = -1;
+    for (int e = lane; e < a.k; e += L) if (l.later[e]) l.cls[e] = -1;
     if (lane == 0) { l.sl = s; l.sl1 = s1; }
     wave_sync();
 }
@@ -147,7 +147,7 @@ template <typename T> __device__ __forceinline__ uint32_t vec_bits(const uint32_
 // ---- loss and factors of a row from its sums -------------------------------------------------------------------------
 // sr, s1: sums over the classes that are not listed, relative to their maximum m; joined with the listed ones'.
 struct RowSums { float xmax; double sl, sr, s1; };
-template <bool TWO> __device__ __forceinline__ RowSums join_sums(const DistillArgs& a, const Listed& l, float m, double sr, double s1) {
+template <bool TWO, int K> __device__ __forceinline__ RowSums join_sums(const DistillArgs& a, const Listed<K>& l, float m, double sr, double s1) {
     RowSums s;
     const float both = fmaxf(m, l.xmax);
     s.xmax = both == -INFINITY ? 0.f : both;
@@ -158,7 +158,7 @@ template <bool TWO> __device__ __forceinline__ RowSums join_sums(const DistillAr
     else s.s1 = s.sl + s.sr;
     return s;
 }
-// In every thread; the loss (three logarithms in 64 bits, a lane each) by one wave.
+// In every thread; the loss (three logarithms in 64 bits, a lane each) by one group.
 __device__ __forceinline__ RowStats row_factors(const DistillArgs& a, const RowSums& s, bool hard, int flags, double pr) {
     const double S = s.sl + s.sr;
     const bool any = flags & 1, bad = flags & 2;
@@ -173,13 +173,9 @@ __device__ __forceinline__ RowStats row_factors(const DistillArgs& a, const RowS
     if (!bad && ((!any && !hard) || S == 0)) st.xmax = NAN;   // nothing to learn from, or no class to learn: zeros
     return st;
 }
-__device__ __forceinline__ double row_loss(const DistillArgs& a, const RowSums& s, const RowStats& st, bool hard, const Listed& l, int lane, float xy) {
+template <int L, int K> __device__ __forceinline__ double row_loss(const DistillArgs& a, const RowSums& s, const RowStats& st, bool hard, const Listed<K>& l, int lane, float xy) {
     const double ln = ln_64(lane == 0 ? s.sl + s.sr : lane == 1 ? s.sr : s.s1);
-    const long long b = __double_as_longlong(ln);
-    auto of = [&](int who) {
-        return __longlong_as_double((long long)__builtin_amdgcn_readlane((int)(b >> 32), who) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)b, who));
-    };
-    const double lnS = of(0), lnr = of(1), ln1 = of(2);
+    const double lnS = lane_value<L, 0>(ln), lnr = lane_value<L, 1>(ln), ln1 = lane_value<L, 2>(ln);
     if (st.xmax != st.xmax) return 0.0;
     if (st.gl != st.gl) return NAN;
     double loss = 0;
@@ -214,19 +210,20 @@ template <typename T, bool TWO> __device__ __forceinline__ i32x4 grad_vec(const 
 // written from there, so loss and gradient cost one read and one write of the scores.
 // What the listed classes need is wave 0's.  The gradient is first written as if no class were listed; behind a barrier the
 // listed ones and the label are written over.
-template <typename T, int W, int NV, bool TWO, bool GRAD>
-__global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 : 7) void distill_row_kernel(DistillArgs a) {
-    constexpr int VEC = ET<T>::VEC, G = W * 64, ROWS = W == 1 ? 4 : 1, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
+// W = 1: a group of L lanes a row, L = 16 with at most 64 entries.
+template <typename T, int W, int L, int NV, bool TWO, bool GRAD>
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV == 8 ? 6 : W == 1 ? 6 : 7) void distill_row_kernel(DistillArgs a) {
+    constexpr int VEC = ET<T>::VEC, G = W * L, ROWS = W == 1 ? 256 / L : 1, K = L == 64 ? MAX_K : 64, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
     __shared__ uint32_t bits_[ROWS][WORDS];
-    __shared__ Listed l_[ROWS];
+    __shared__ Listed<K> l_[ROWS];
     __shared__ double rsum[2][W];
     __shared__ float rmax[W];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = W == 1 ? lane : threadIdx.x, sub = W == 1 ? wave : 0;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & (L - 1), tid = W == 1 ? lane : threadIdx.x, sub = W == 1 ? threadIdx.x / L : 0;
     const size_t r = (size_t)blockIdx.x * ROWS + sub;
     if (W == 1 && r >= (size_t)a.rows) return;
     const bool lead = W == 1 || wave == 0;
     uint32_t* bits = bits_[sub];
-    Listed& l = l_[sub];
+    Listed<K>& l = l_[sub];
     const int n = a.n;
     const T* x = (const T*)((const char*)a.x + r * a.stride * ET<T>::ES);
     const RowSpan<T> sp(x, n);
@@ -238,22 +235,22 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 :
     for (int i = 0; i < NV; ++i) v[i] = i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>();
     float xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY, xy = 0.f;
     if (lead) {
-        listed_load(a, r, x, lane, l);
+        listed_load<T, L>(a, r, x, lane, l);
         if (hard) xy = load_score(x, (size_t)y);
     }
     for (int i = tid; i < WORDS; i += G) bits[i] = 0;
     group_sync<W>();
     if (lead) {
         bool dup = false;
-        for (int e = lane; e < a.k; e += 64)
+        for (int e = lane; e < a.k; e += L)
             if (l.cls[e] >= 0) {
                 const int b = BIT0 + l.cls[e] - sp.head;
                 dup |= (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1;
             }
         if (lane == 0 && a.w > 0.0 && y >= n) l.flags |= 2;
         wave_sync();
-        listed_sums<TWO>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
-        if (__ballot(dup)) listed_merge<TWO>(a, lane, l);
+        listed_sums<TWO, L>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
+        if (group_any<L>(dup)) listed_merge<TWO, L>(a, lane, l);
     }
     group_sync<W>();
 
@@ -272,7 +269,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 :
             m = fmaxf(m, vec_max<T>(v[i]));
         }
     }
-    m = wave_max(m);
+    m = group_max<L>(m);
     if constexpr (W > 1) {
         if (lane == 0) rmax[wave] = m;
         __syncthreads();
@@ -296,7 +293,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 :
             }
         }
     }
-    double sr = wave_sum((double)s), sr1 = TWO ? wave_sum((double)s1) : 0.0;
+    double sr = group_sum<L>((double)s), sr1 = TWO ? group_sum<L>((double)s1) : 0.0;
     if constexpr (W > 1) {
         if (lane == 0) { rsum[0][wave] = sr; if constexpr (TWO) rsum[1][wave] = sr1; }
         __syncthreads();
@@ -308,14 +305,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 :
     const RowStats st = row_factors(a, sum, hard, l.flags, l.pr);
     const bool empty = st.xmax != st.xmax;
     if (lead) {
-        const double loss = row_loss(a, sum, st, hard, l, lane, xy);
+        const double loss = row_loss<L>(a, sum, st, hard, l, lane, xy);
         if (lane == 0) {
             if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
             if constexpr (!GRAD) a.stats[r] = st;
         }
     }
     if constexpr (!GRAD) {
-        if (lead) for (int e = lane; e < a.k; e += 64) a.probs[r * a.k + e] = l.cls[e] >= 0 ? (float)l.p[e] : -1.f;
+        if (lead) for (int e = lane; e < a.k; e += L) a.probs[r * a.k + e] = l.cls[e] >= 0 ? (float)l.p[e] : -1.f;
     } else {
         T* dx = (T*)a.dx + r * (size_t)n;
         const Grad<T, TWO> g = {empty ? 0.f : st.xmax, a.c, a.c1, st.g1 * a.scale};
@@ -341,14 +338,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 ? 4 : NV == 8 ? 6 :
         if (lead && !empty) {
             const float fp = a.fp * a.scale, w = a.w1 * a.scale;
             bool mine = false;
-            for (int e = lane; e < a.k; e += 64) {
+            for (int e = lane; e < a.k; e += L) {
                 const int j = l.cls[e];
                 if (j < 0) continue;
                 float d = g(l.x[e], gl) - fp * (float)l.p[e];
                 if (hard && j == (int)y) { d -= w; mine = true; }
                 store_elem(dx, j, d);
             }
-            if (hard && !__ballot(mine) && lane == 0) store_elem(dx, (size_t)y, g(xy, gr) - w);
+            if (hard && !group_any<L>(mine) && lane == 0) store_elem(dx, (size_t)y, g(xy, gr) - w);
         }
     }
 }
@@ -359,7 +356,7 @@ template <typename T, bool TWO>
 __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
     constexpr int VEC = ET<T>::VEC, W = 16, G = 1024, NV = 64 / VEC, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
     __shared__ uint32_t bits[WORDS];
-    __shared__ Listed l;
+    __shared__ Listed<MAX_K> l;
     __shared__ double rsum[2][W];
     __shared__ float rmax[W];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, tid = threadIdx.x, n = a.n;
@@ -383,11 +380,11 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
         if constexpr (TWO) s1 += exp2_32(t * a.c1);
     };
     if (lead) {
-        listed_load(a, r, x, lane, l);
+        listed_load<T, 64>(a, r, x, lane, l);
         if (lane == 0 && a.w > 0.0 && y >= n) l.flags |= 2;
         wave_sync();
-        listed_sums<TWO>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
-        listed_merge<TWO>(a, lane, l);
+        listed_sums<TWO, 64>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
+        listed_merge<TWO, 64>(a, lane, l);
         if (hard) xy = load_score(x, (size_t)y);
     }
     for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NV) {
@@ -433,7 +430,7 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
     if (!lead) return;
     const RowSums sum = join_sums<TWO>(a, l, all, sr, sr1);
     const RowStats st = row_factors(a, sum, hard, l.flags, l.pr);
-    const double loss = row_loss(a, sum, st, hard, l, lane, xy);
+    const double loss = row_loss<64>(a, sum, st, hard, l, lane, xy);
     if (lane == 0) {
         if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
         a.stats[r] = st;
@@ -528,15 +525,17 @@ template <typename T> constexpr int row_fits() { return 1024 * 16 * ET<T>::VEC; 
 template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a, hipStream_t s) {
     constexpr int VEC = ET<T>::VEC;
     const int nv = a.n / VEC;                      // at most, whatever the alignment
-    const unsigned rows = (unsigned)a.rows, quads = (unsigned)((a.rows + 3) / 4);
-    if (nv <= 64) distill_row_kernel<T, 1, 1, TWO, GRAD><<<quads, 256, 0, s>>>(a);
-    else if (nv <= 128) distill_row_kernel<T, 1, 2, TWO, GRAD><<<quads, 256, 0, s>>>(a);
-    else if (nv <= 256) distill_row_kernel<T, 1, 4, TWO, GRAD><<<quads, 256, 0, s>>>(a);
-    else if (nv <= 1024) distill_row_kernel<T, 4, 4, TWO, GRAD><<<rows, 256, 0, s>>>(a);
-    else if (nv <= 2048) distill_row_kernel<T, 4, 8, TWO, GRAD><<<rows, 256, 0, s>>>(a);
-    else if (nv <= 4096) distill_row_kernel<T, 8, 8, TWO, GRAD><<<rows, 512, 0, s>>>(a);
-    else if (nv <= 8192) distill_row_kernel<T, 8, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
-    else distill_row_kernel<T, 16, 16, TWO, GRAD><<<rows, 1024, 0, s>>>(a);
+    const unsigned rows = (unsigned)a.rows, quads = (unsigned)((a.rows + 3) / 4), sixteens = (unsigned)((a.rows + 15) / 16);
+    // A narrow row is mostly what every row costs, some 1300 instructions: four rows a wave share them.
+    if (nv <= 32 && a.k <= 64) distill_row_kernel<T, 1, 16, 2, TWO, GRAD><<<sixteens, 256, 0, s>>>(a);
+    else if (nv <= 128 && a.k <= 64) distill_row_kernel<T, 1, 16, 8, TWO, GRAD><<<sixteens, 256, 0, s>>>(a);
+    else if (nv <= 128) distill_row_kernel<T, 1, 64, 2, TWO, GRAD><<<quads, 256, 0, s>>>(a);
+    else if (nv <= 256) distill_row_kernel<T, 1, 64, 4, TWO, GRAD><<<quads, 256, 0, s>>>(a);
+    else if (nv <= 1024) distill_row_kernel<T, 4, 64, 4, TWO, GRAD><<<rows, 256, 0, s>>>(a);
+    else if (nv <= 2048) distill_row_kernel<T, 4, 64, 8, TWO, GRAD><<<rows, 256, 0, s>>>(a);
+    else if (nv <= 4096) distill_row_kernel<T, 8, 64, 8, TWO, GRAD><<<rows, 512, 0, s>>>(a);
+    else if (nv <= 8192) distill_row_kernel<T, 8, 64, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
+    else distill_row_kernel<T, 16, 64, 16, TWO, GRAD><<<rows, 1024, 0, s>>>(a);
 }
 template <typename T> void launch_fwd(const DistillArgs& a, bool two, hipStream_t s) {
     if (a.n <= row_fits<T>()) { if (two) launch_rows<T, true, false>(a, s); else launch_rows<T, false, false>(a, s); }
@@ -559,7 +558,7 @@ DistillArgs fwd_args(const void* logits, size_t row_stride, const float* values,
                      int rows, int ncls, int k, double temperature, double label_weight) {
     return {logits, row_stride, values, (const long long*)indices, rest, label_weight > 0 ? (const long long*)labels : nullptr,
             nullptr, nullptr, nullptr, nullptr, nullptr, 1.f, rows, ncls, k, (float)(LOG2E / temperature), (float)LOG2E,
-            (float)((1.0 - label_weight) * temperature), (float)label_weight, temperature, label_weight};
+            (float)((1.0 - label_weight) * temperature), (float)label_weight, temperature, 1.0 / temperature, label_weight};
 }
 int loss_sum(const double* loss_rows, int rows, int reduction, float* loss, hipStream_t s) {
     if (reduction) loss_sum_kernel<<<1, 1024, 0, s>>>(loss_rows, rows, reduction == 1 ? 1.0 / rows : 1.0, loss);

@@ -183,6 +183,39 @@ __device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {
     return (unsigned long long)hi << 32 | lo;
 }
 
+// Groups of L lanes: a whole wave (64), or a row of 16 (four groups side by side, for which one instruction serves all four).
+// Lane WHO's value for every lane of its group.
+template <int L, int WHO> __device__ __forceinline__ int lane_value(int v) {
+    if constexpr (L == 64) return __builtin_amdgcn_readlane(v, WHO);
+    else return __builtin_amdgcn_update_dpp(0, v, 0x150 + WHO, 0xF, 0xF, true);          // row_newbcast
+}
+template <int L, int WHO> __device__ __forceinline__ double lane_value(double v) {
+    const long long b = __double_as_longlong(v);
+    const uint32_t lo = (uint32_t)lane_value<L, WHO>((int)b), hi = (uint32_t)lane_value<L, WHO>((int)(b >> 32));
+    return __longlong_as_double((long long)hi << 32 | lo);
+}
+template <int L> __device__ __forceinline__ double group_sum(double v) {
+    if constexpr (L == 64) return wave_sum(v);
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    return lane_value<16, 15>(v);
+}
+template <int L> __device__ __forceinline__ float group_max(float v) {
+    if constexpr (L == 64) return wave_max(v);
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    return __int_as_float(lane_value<16, 15>(__float_as_int(v)));
+}
+template <int L> __device__ __forceinline__ bool group_any(bool b) {
+    const unsigned long long m = __ballot(b);
+    if constexpr (L == 64) return m != 0;
+    return (m >> (threadIdx.x & 48) & 0xFFFF) != 0;
+}
+
 template <int W, typename V, typename Op> __device__ __forceinline__ V block_reduce(V v, Op op, V* red) {
     v = wave_reduce(v, op);
     if constexpr (W == 1) return v;

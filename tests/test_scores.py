@@ -216,7 +216,7 @@ def check_distill(rt, x, val, idx, rest, labels, T, w, rows_grad=None):
         close(pair[1], G, (Q * e1 * f) + hs * torch.nan_to_num(G.abs()) + flush, red + " pair")
 
 
-DIST = [(1, 1, 1), (6, 256, 30), (5, 512, 40), (3, 1024, 9), (2, 16384, 33), (2, 32768, 20), (1, 65536, 64), (3, 2, 1), (5, 7, 7), (64, 60, 5), (7, 61, 20), (9, 400, 16), (3, 401, 256), (4, 1027, 100), (2, 4099, 64),
+DIST = [(1, 1, 1), (17, 100, 64), (35, 511, 33), (18, 1023, 65),  (6, 256, 30), (5, 512, 40), (3, 1024, 9), (2, 16384, 33), (2, 32768, 20), (1, 65536, 64), (3, 2, 1), (5, 7, 7), (64, 60, 5), (7, 61, 20), (9, 400, 16), (3, 401, 256), (4, 1027, 100), (2, 4099, 64),
         (2, 8191, 128), (3, 16390, 9), (2, 33000, 256), (1, 65537, 30), (2, 131075, 64), (1, 131072, 256), (1, 140001, 50)]
 
 
