@@ -350,11 +350,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
     }
 }
 
-// A row that does not fit in registers: segment after segment, every thread with a running maximum and sums relative to
-// it.  Forward only; the gradient then reads the scores a second time (distill_bwd_kernel).
-template <typename T, bool TWO>
-__global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
-    constexpr int VEC = ET<T>::VEC, W = 16, G = 1024, NV = 64 / VEC, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
+// The loss alone, which needs no score twice: a row goes by in batches of four vectors a thread, with the next batch on its
+// way, every thread with a running maximum and sums relative to it.  Bit map of SEG classes at a time.
+constexpr int SEG = 131072;
+template <typename T, int W, bool TWO>
+__global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void distill_stream_kernel(DistillArgs a) {
+    constexpr int VEC = ET<T>::VEC, G = W * 64, NB = 4, BATCHES = SEG / VEC / (G * NB), WORDS = (SEG + 2 * BIT0 + 31) / 32;
     __shared__ uint32_t bits[WORDS];
     __shared__ Listed<MAX_K> l;
     __shared__ double rsum[2][W];
@@ -374,53 +375,73 @@ __global__ __launch_bounds__(1024) void distill_stream_kernel(DistillArgs a) {
             m = to;
         }
     };
-    auto add = [&](float f) {
-        const float t = f - (m == -INFINITY ? 0.f : m);
-        s += exp2_32(t * a.c);
-        if constexpr (TWO) s1 += exp2_32(t * a.c1);
+    i32x4 nx[NB];
+    auto load = [&](int v0) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) nx[i] = v0 + i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(v0 + i * G + tid)) : neg_inf_vec<T>();
     };
+    load(0);
     if (lead) {
         listed_load<T, 64>(a, r, x, lane, l);
         if (lane == 0 && a.w > 0.0 && y >= n) l.flags |= 2;
         wave_sync();
         listed_sums<TWO, 64>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
-        listed_merge<TWO, 64>(a, lane, l);
         if (hard) xy = load_score(x, (size_t)y);
     }
-    for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NV) {
+    const int some = min(n, SEG) / 32 + 2;         // words of the bit map that are looked at
+    for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NB * BATCHES) {
         const int base = sp.vec_at(v0);            // the segment's first class; the row's ends go with the first segment
         __syncthreads();
-        for (int i = tid; i < WORDS; i += G) bits[i] = 0;
+        for (int i = tid; i < some; i += G) bits[i] = 0;
         __syncthreads();
-        if (lead)
+        if (lead) {
+            bool dup = false;
             for (int e = lane; e < a.k; e += 64) {
                 const int j = l.cls[e], b = BIT0 + j - base;
-                if (j >= base && j < base + G * NV * VEC) atomicOr(&bits[b >> 5], 1u << (b & 31));
+                if (j >= base && j - base < SEG) dup |= (atomicOr(&bits[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1;
+                dup |= j >= 0 && (j < base || j - base >= SEG);        // listed elsewhere: not seen by this bit map
             }
+            if (v0 == 0 && group_any<64>(dup)) listed_merge<TWO, 64>(a, lane, l);
+        }
         __syncthreads();
         if (v0 == 0 && tid < sp.edge) {
             const int j = sp.edge_at(tid);
             bool is_listed = false;
             for (int e = 0; e < a.k; ++e) is_listed |= l.cls[e] == j;
-            if (!is_listed) { const float f = load_score(x, j); raise(f); add(f); }
+            if (!is_listed) {
+                const float f = load_score(x, j);
+                raise(f);
+                const float t = f - (m == -INFINITY ? 0.f : m);
+                s += exp2_32(t * a.c);
+                if constexpr (TWO) s1 += exp2_32(t * a.c1);
+            }
         }
-        i32x4 v[NV];
+#pragma unroll 1
+        for (int b = 0; b < BATCHES && v0 + b * G * NB < sp.nvec; ++b) {
+            i32x4 v[NB];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = v0 + i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(v0 + i * G + tid)) : neg_inf_vec<T>();
-        float top = -INFINITY;
+            for (int i = 0; i < NB; ++i) v[i] = nx[i];
+            load(v0 + (b + 1) * G * NB);
+            float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t b = vec_bits<T>(bits, i * G + tid);
-            if (b) drop_listed<T>(v[i], b);
-            top = fmaxf(top, vec_max<T>(v[i]));
-        }
-        raise(top);
+            for (int i = 0; i < NB; ++i) {
+                const uint32_t q = vec_bits<T>(bits, b * G * NB + i * G + tid);
+                if (q) drop_listed<T>(v[i], q);
+                top = fmaxf(top, vec_max<T>(v[i]));
+            }
+            raise(top);
+            const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            float f[VEC];
-            unpack16<T>(v[i], f);
+            for (int i = 0; i < NB; ++i) {
+                float f[VEC];
+                unpack16<T>(v[i], f);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) add(f[j]);
+                for (int j = 0; j < VEC; ++j) {
+                    const float t = f[j] - ref;
+                    s += exp2_32(t * a.c);
+                    if constexpr (TWO) s1 += exp2_32(t * a.c1);
+                }
+            }
         }
     }
     const float all = block_reduce<W>(m, OpFMax(), rmax);
@@ -537,10 +558,12 @@ template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a
     else if (nv <= 8192) distill_row_kernel<T, 8, 64, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
     else distill_row_kernel<T, 16, 64, 16, TWO, GRAD><<<rows, 1024, 0, s>>>(a);
 }
-template <typename T> void launch_fwd(const DistillArgs& a, bool two, hipStream_t s) {
-    if (a.n <= row_fits<T>()) { if (two) launch_rows<T, true, false>(a, s); else launch_rows<T, false, false>(a, s); }
-    else if (two) distill_stream_kernel<T, true><<<a.rows, 1024, 0, s>>>(a);
-    else distill_stream_kernel<T, false><<<a.rows, 1024, 0, s>>>(a);
+// The loss alone.  Wide rows go by in batches: four waves a row where there are rows enough to fill the chip (1000 x 50001
+// float32: 68 us with the row in registers), sixteen for few rows that no registers hold.
+template <typename T, bool TWO> void launch_fwd(const DistillArgs& a, hipStream_t s) {
+    if (a.n / ET<T>::VEC > 2048 && a.rows >= 512) distill_stream_kernel<T, 4, TWO><<<a.rows, 256, 0, s>>>(a);
+    else if (a.n <= row_fits<T>()) launch_rows<T, TWO, false>(a, s);
+    else distill_stream_kernel<T, 16, TWO><<<a.rows, 1024, 0, s>>>(a);
 }
 template <typename T, bool TWO> void launch_bwd(const GradArgs& a, hipStream_t s) {
     constexpr int VEC = ET<T>::VEC;
@@ -575,7 +598,9 @@ extern "C" int stgcn_distill_fwd(int dtype, const void* logits, size_t row_strid
     DistillArgs a = fwd_args(logits, row_stride, values, indices, rest, labels, rows, ncls, k, temperature, label_weight);
     a.loss_rows = reduction ? loss_rows : nullptr; a.loss = loss; a.stats = (RowStats*)stats; a.probs = probs;
     const bool two = label_weight > 0 && temperature != 1.0;
-    if (dtype == STGCN_BF16) launch_fwd<bf16>(a, two, (hipStream_t)stream); else launch_fwd<float>(a, two, (hipStream_t)stream);
+    const hipStream_t s = (hipStream_t)stream;
+    if (dtype == STGCN_BF16) { if (two) launch_fwd<bf16, true>(a, s); else launch_fwd<bf16, false>(a, s); }
+    else { if (two) launch_fwd<float, true>(a, s); else launch_fwd<float, false>(a, s); }
     return loss_sum(loss_rows, rows, reduction, loss, (hipStream_t)stream);
 }
 
@@ -605,7 +630,8 @@ extern "C" int stgcn_distill_step(int dtype, const void* logits, size_t row_stri
     const bool two = label_weight > 0 && temperature != 1.0;
     const hipStream_t s = (hipStream_t)stream;
     if (ncls > (dtype == STGCN_BF16 ? row_fits<bf16>() : row_fits<float>())) {
-        if (dtype == STGCN_BF16) launch_fwd<bf16>(a, two, s); else launch_fwd<float>(a, two, s);
+        if (dtype == STGCN_BF16) { if (two) launch_fwd<bf16, true>(a, s); else launch_fwd<bf16, false>(a, s); }
+        else { if (two) launch_fwd<float, true>(a, s); else launch_fwd<float, false>(a, s); }
         const int rc = stgcn_distill_bwd(dtype, logits, row_stride, indices, labels, stats, probs, nullptr, 0, reduction == 1 ? 1.0 / rows : 1.0, rows, ncls, k,
                                          temperature, label_weight, dlogits, stream);
         if (rc != STGCN_OK) return rc;

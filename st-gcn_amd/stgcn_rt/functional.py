@@ -412,6 +412,7 @@ class DistillationFn(torch.autograd.Function):
             return loss
         loss = call.forward()
         ctx.save_for_backward(logits, call.indices, call.labels, call.kept)
+        ctx.rows_ok = call.x is logits                                                       # else a contiguous copy was read
         call.x = call.values = call.indices = call.rest = call.labels = call.kept = None     # the sizes stay
         ctx.call = call
         return loss
@@ -424,7 +425,9 @@ class DistillationFn(torch.autograd.Function):
             dx = dx * (g[:, None] if ctx.rowwise else g)
         else:
             logits, indices, labels, kept = ctx.saved_tensors
-            dx = ctx.call.backward(P._check_scores(logits), indices, labels, kept, g.contiguous())
+            if not ctx.rows_ok:
+                logits = P._check_scores(logits)
+            dx = ctx.call.backward(logits, indices, labels, kept, g.contiguous())
         return dx, None, None, None, None, None, None, None
 
 

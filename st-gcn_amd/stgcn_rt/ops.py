@@ -586,14 +586,14 @@ class DistillCall:
         check_device(x, "logits")
         self.reduction = reduction
 
-    def _key(self):
-        return () if TIMING is None else (str(self.x.dtype), self.rows, self.ncls, self.k)
+    def _key(self, x):
+        return () if TIMING is None else (str(x.dtype), self.rows, self.ncls, self.k)
 
     def _forward(self, name, loss, *more):
         x, rows = self.x, self.rows
         self.kept = torch.empty(rows * (6 + self.k), dtype=torch.float32, device=x.device)
         at = self.kept.data_ptr()                       # losses [rows] float64, factors [rows][4], shares [rows][k]
-        _launch(self._key(), name, L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), self.values.data_ptr(), self.indices.data_ptr(),
+        _launch(self._key(x), name, L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), self.values.data_ptr(), self.indices.data_ptr(),
                 L.ptr(self.rest), L.ptr(self.labels), rows, self.ncls, self.k, self.temperature, self.label_weight,
                 _REDUCTIONS[self.reduction], loss.data_ptr(), at, at + 8 * rows, at + 24 * rows, *more, L.stream_ptr())
 
@@ -622,13 +622,14 @@ class DistillCall:
     def backward(self, x, indices, labels, kept, grad):
         """d loss / d logits times grad (a float32 tensor on the device: one number, or one a row for "none") from what a
         forward kept."""
-        rows = self.rows
-        dx = torch.empty((rows, self.ncls), dtype=x.dtype, device=x.device)
+        rows, ncls = self.rows, self.ncls
+        dx = torch.empty((rows, ncls), dtype=x.dtype, device=x.device)
         if rows:
             at = kept.data_ptr()
-            _launch(self._key(), "stgcn_distill_bwd", L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), indices.data_ptr(), L.ptr(labels),
-                    at + 8 * rows, at + 24 * rows, grad.data_ptr(), 1 if self.reduction == "none" else 0,
-                    1.0 / rows if self.reduction == "mean" else 1.0, rows, self.ncls, self.k, self.temperature, self.label_weight, dx.data_ptr(),
+            none = self.reduction == "none"
+            _launch(self._key(x), "stgcn_distill_bwd", L.dtype_code(x.dtype), x.data_ptr(), max(x.stride(0), ncls), indices.data_ptr(),
+                    None if labels is None else labels.data_ptr(), at + 8 * rows, at + 24 * rows, grad.data_ptr(), none,
+                    1.0 / rows if self.reduction == "mean" else 1.0, rows, ncls, self.k, self.temperature, self.label_weight, dx.data_ptr(),
                     L.stream_ptr())
         return dx
 
