@@ -171,7 +171,7 @@ template <typename T> struct List {
     template <typename P> __device__ __forceinline__ int count(P pred) const {
         int m = 0;
 #pragma unroll
-        for (int i = 0; i < R; ++i) if (64 * i < c) m += __popcll(__ballot(lp[i] != 0 && pred(lp[i])));
+        for (int i = 0; i < R; ++i) if (64 * i < c) m += __popcll(__ballot((lp[i] != 0) & pred(lp[i])));
         return m;
     }
     template <typename P> __device__ __forceinline__ u64 mass(P pred) const {
