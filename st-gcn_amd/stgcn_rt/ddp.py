@@ -244,7 +244,13 @@ class Trainer:
     outside the graph (the learning rate may change freely, and no RCCL call is ever captured).  With more than one
     rank the step is captured as two graphs (SPLIT_BLOCK): the gradients of the first backward segment are all-reduced
     while the second is replayed.  If the capture fails the trainer says so on stderr and keeps stepping launch by
-    launch."""
+    launch.
+
+    teacher=model: the loss is functional.distillation against the teacher's teacher_k (or all, if fewer) top logits of
+    the same batch at `temperature`, and against the labels with label_weight (a label < 0: none).  The teacher is put
+    into eval mode, runs without gradients ahead of every step, outside the graph (its scores' top logits are copied into
+    the graph's static buffers), and shares no parameter with the model.  step(..., target=...) takes the top logits from
+    the caller instead (evaluate.teacher_targets collects them)."""
 
     GRAPH_WARMUP = 2
     # With more than one rank the captured step is TWO graphs: forward, loss and the backward of the head and of blocks
@@ -253,8 +259,18 @@ class Trainer:
     # collective is ever captured.
     SPLIT_BLOCK = 7
 
-    def __init__(self, model, lr=0.1, momentum=0.9, weight_decay=1e-4, nesterov=True, bucket_bytes=4 << 20, graph=False, split=None):
+    def __init__(self, model, lr=0.1, momentum=0.9, weight_decay=1e-4, nesterov=True, bucket_bytes=4 << 20, graph=False, split=None,
+                 teacher=None, teacher_k=16, temperature=2.0, label_weight=0.5):
+        if teacher is not None:
+            mine = {id(p) for p in model.parameters()}
+            if teacher is model or any(id(p) in mine for p in teacher.parameters()):
+                raise ValueError("the teacher shares parameters with the model")
+        if not 1 <= int(teacher_k) <= 256 or not 0.0 < float(temperature) < 1e30 or not 0.0 <= float(label_weight) <= 1.0:
+            raise ValueError("a teacher wants 1 to 256 top logits, a temperature above 0 and a label_weight from 0 to 1, got %r, %r, %r"
+                             % (teacher_k, temperature, label_weight))
         self.model = model
+        self.teacher, self.teacher_k = teacher, int(teacher_k)
+        self.temperature, self.label_weight = float(temperature), float(label_weight)
         self.flat = FlatParams(model, reverse_execution_order(model))
         self.bucketer = GradBucketer(self.flat, bucket_bytes)
         self.opt = SGD(self.flat, lr, momentum, weight_decay, nesterov)
@@ -262,8 +278,9 @@ class Trainer:
         self.loss_fn = F_.cross_entropy          # nn.CrossEntropyLoss() with its defaults, one launch each way
         self.use_graph = bool(graph)
         self.split = split                    # capture the step as two graphs: None = when there is more than one rank
-        self._graphs = {}                     # (data shape, label shape) -> (graph, static data, static label, static loss)
+        self._graphs = {}                     # (data shape, label shape, target's) -> (graph, static data, static label, static target, static loss)
         self._eager_steps = 0
+        self._taught_steps = 0                # of these with a target
         self._grads_bound = False             # whether every p.grad is the parameter's slice of the flat gradient
 
     def broadcast_from_rank0(self):
@@ -271,6 +288,12 @@ class Trainer:
             broadcast0(self.flat.flat)
             for b in self.model.buffers():
                 broadcast0(b)
+            if self.teacher is not None:      # every rank learns from the same teacher
+                for t in list(self.teacher.parameters()) + list(self.teacher.buffers()):
+                    broadcast0(t.data)
+                drop = getattr(self.teacher, "invalidate_plan", None)
+                if drop is not None:
+                    drop()
 
     def graph_ready(self):
         return bool(self._graphs)
@@ -280,10 +303,27 @@ class Trainer:
         graph, 0 without a graph."""
         return max((2 if isinstance(ent[0], tuple) else 1 for ent in self._graphs.values()), default=0)
 
-    def _forward_backward(self, data, label):
+    def target(self, data):
+        """The teacher's top logits of a batch (functional.TopLogits), None without a teacher."""
+        if self.teacher is None:
+            return None
+        from . import functional as F_
+        if self.teacher.training:
+            self.teacher.eval()
+        with torch.no_grad():
+            out = self.teacher(data)
+            return F_.top_logits(out, min(self.teacher_k, out.shape[-1]), self.temperature)
+
+    def _loss(self, out, label, target):
+        if target is None:
+            return self.loss_fn(out, label)
+        from . import functional as F_
+        return F_.distillation(out, *target, labels=label, temperature=self.temperature, label_weight=self.label_weight)
+
+    def _forward_backward(self, data, label, target):
         self.flat.zero_grad()
         out = self.model(data)
-        loss = self.loss_fn(out, label)
+        loss = self._loss(out, label, target)
         loss.backward()
         return loss.detach()                  # not the graph's root: a kept loss would keep every autograd node of the step alive
 
@@ -304,7 +344,7 @@ class Trainer:
             return None
         return n
 
-    def _capture_split(self, data, label, nlate):
+    def _capture_split(self, data, label, target, nlate):
         """Two graphs sharing one memory pool (always replayed in capture order): see SPLIT_BLOCK.  Gradients are taken
         with torch.autograd.grad and copied into the flat buffer inside the graphs; the roots of the second segment
         are the activation entering block SPLIT_BLOCK and the late blocks' A * importance tensors, whose gradients the
@@ -313,7 +353,7 @@ class Trainer:
         if P.TIMING is not None:
             return None
         m, flat = self.model, self.flat
-        sx, sl = data.clone(), label.clone()
+        sx, sl, st = data.clone(), label.clone(), self._static(target)
         g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
         late, early = flat.params[:nlate], flat.params[nlate:]
         self.bucketer.hooks_enabled = False
@@ -322,7 +362,7 @@ class Trainer:
             torch.cuda.synchronize()
             with torch.cuda.graph(g1, capture_error_mode="thread_local"):
                 flat.zero_grad()
-                loss = self.loss_fn(m(sx), sl)
+                loss = self._loss(m(sx), sl, st)
                 mid = m._mid
                 adj = [t for t in (m._a_eff[self.SPLIT_BLOCK:] if m._a_eff is not None else []) if isinstance(t, torch.Tensor) and t.requires_grad]
                 roots = [mid] + adj
@@ -358,9 +398,13 @@ class Trainer:
         self.bucketer.hooks_enabled = True
         m.split_block = None
         m._mid = m._a_eff = None
-        return ((g1, g2, flat.offsets[nlate]), sx, sl, loss)
+        return ((g1, g2, flat.offsets[nlate]), sx, sl, st, loss)
 
-    def _capture(self, data, label):
+    @staticmethod
+    def _static(target):
+        return None if target is None else tuple(None if t is None else t.clone() for t in target)
+
+    def _capture(self, data, label, target):
         from . import ops as P
         if P.TIMING is not None:
             return None
@@ -368,8 +412,8 @@ class Trainer:
         if want:
             nlate = self._split_point()
             if nlate is not None:
-                return self._capture_split(data, label, nlate)
-        sx, sl = data.clone(), label.clone()
+                return self._capture_split(data, label, target, nlate)
+        sx, sl, st = data.clone(), label.clone(), self._static(target)
         g = torch.cuda.CUDAGraph()
         self.bucketer.hooks_enabled = False
         try:
@@ -378,7 +422,7 @@ class Trainer:
             # events of earlier all-reduces with hipEventQuery; under the default (global) mode such a call from
             # another thread during the capture is an error that the watchdog turns into an abort of the process.
             with torch.cuda.graph(g, capture_error_mode="thread_local"):
-                loss = self._forward_backward(sx, sl)
+                loss = self._forward_backward(sx, sl, st)
                 self.flat.gather(range(len(self.flat.params)))
         except Exception as e:                # stay in this process: step launch by launch from now on
             import sys
@@ -388,36 +432,54 @@ class Trainer:
             torch.cuda.synchronize()
             return None
         self.bucketer.hooks_enabled = True
-        return (g, sx, sl, loss)
+        return (g, sx, sl, st, loss)
 
-    def _graph_for(self, data, label):
-        key = (tuple(data.shape), data.dtype, tuple(label.shape))
+    def _graph_wanted(self, target):
+        warm = self._eager_steps if target is None else self._taught_steps
+        return self.use_graph and self.model.training and warm >= self.GRAPH_WARMUP
+
+    def _graph_for(self, data, label, target):
+        key = (tuple(data.shape), data.dtype, tuple(label.shape),
+               None if target is None else (self.temperature, self.label_weight, tuple(None if t is None else tuple(t.shape) for t in target)))
         ent = self._graphs.get(key)
         if ent is None:
-            ent = self._capture(data, label)
+            ent = self._capture(data, label, target)
             if ent is not None:
                 self._graphs[key] = ent
         return ent
 
-    def prepare_graph(self, data, label):
+    def prepare_graph(self, data, label, target=None):
         """Captures the graph for this input shape now (no step is performed) instead of inside the first step() that
         would use it; needs the warm-up steps done.  Returns whether a graph is ready."""
-        if self.use_graph and self.model.training and self._eager_steps >= self.GRAPH_WARMUP:
-            return self._graph_for(data, label) is not None
+        target = self._target_of(data, target)
+        if self._graph_wanted(target):
+            return self._graph_for(data, label, target) is not None
         return False
 
-    def step(self, data, label, eager=False):
+    def _target_of(self, data, target):
+        if target is None:
+            return self.target(data)
+        if len(target) != 3:
+            raise ValueError("a target is (values, indices, rest or None), as top_logits returns it")
+        return tuple(target)
+
+    def step(self, data, label, eager=False, target=None):
         """One iteration; returns the loss (a device tensor; with a graph, the graph's own output buffer, overwritten
-        by the next replay).  eager=True forces the launch-by-launch path for this call."""
+        by the next replay).  eager=True forces the launch-by-launch path for this call.  target: the batch's top logits
+        (values, indices, rest or None) to learn from, taken instead of the teacher's."""
         from . import ops as P
-        if self.use_graph and not eager and P.TIMING is None and self.model.training and self._eager_steps >= self.GRAPH_WARMUP:
-            ent = self._graph_for(data, label)
+        target = self._target_of(data, target)
+        if not eager and P.TIMING is None and self._graph_wanted(target):
+            ent = self._graph_for(data, label, target)
             if ent is not None:
-                g, sx, sl, loss = ent
+                g, sx, sl, st, loss = ent
                 if data.data_ptr() != sx.data_ptr():
                     sx.copy_(data, non_blocking=True)
                 if label.data_ptr() != sl.data_ptr():
                     sl.copy_(label, non_blocking=True)
+                for s, t in zip(st or (), target or ()):
+                    if s is not None and s.data_ptr() != t.data_ptr():
+                        s.copy_(t, non_blocking=True)
                 if isinstance(g, tuple):
                     # two segments: the late parameters' gradients travel while the second segment runs
                     g1, g2, cut = g
@@ -443,8 +505,9 @@ class Trainer:
                 return loss
         self._grads_bound = False
         self.bucketer.reset()
-        loss = self._forward_backward(data, label)
+        loss = self._forward_backward(data, label, target)
         scale = self.bucketer.finish()
         self.opt.step(scale)
         self._eager_steps += 1
+        self._taught_steps += target is not None
         return loss

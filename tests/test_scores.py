@@ -241,6 +241,16 @@ def test_distillation(rt, rows, n, k, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,dt", [(520, 8211, torch.float32), (513, 20003, torch.bfloat16), (515, 401, torch.float32)])
+def test_distillation_many_rows(rt, rows, n, dt):
+    """Enough rows that each gets fewer waves."""
+    x = scores(rows, n, dt, n, offset=1, gap=2)
+    val, idx, rest = teacher_lists(x, 20, 2.0, n, pad=0.1)
+    lab = torch.randint(-1, n, (rows,), generator=torch.Generator().manual_seed(rows)).to(DEV)
+    check_distill(rt, x, val, idx, rest, lab, 2.0, 0.25)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [60, 1500, 40000])
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_distillation_rows_without_anything(rt, n, dt):
