@@ -39,10 +39,23 @@ __device__ __forceinline__ u64 place(uint32_t key, int j) { return ((u64)key << 
 __device__ __forceinline__ int place_class(u64 p) { return (int)~(uint32_t)p; }
 __device__ __forceinline__ float place_score(u64 p) { return key_score((uint32_t)(p >> 32)); }
 
+// A value that is the same in all lanes, as a scalar: what comes through LDS or a shuffle is none to the compiler, and every
+// loop and test on it would be one per lane.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+__device__ __forceinline__ u64 uniform(u64 v) { return (u64)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
+__device__ __forceinline__ double uniform(double v) { return __longlong_as_double((long long)uniform((u64)__double_as_longlong(v))); }
+// lane l's value, l the same in all lanes
+__device__ __forceinline__ int lane_at(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ u64 lane_at(u64 v, int l) { return (u64)(uint32_t)lane_at((int)(v >> 32), l) << 32 | (uint32_t)lane_at((int)v, l); }
+__device__ __forceinline__ double lane_at(double v, int l) { return __longlong_as_double((long long)lane_at((u64)__double_as_longlong(v), l)); }
+
 // Weights relative to the row's maximum.  With a maximum of +inf its classes weigh 1, all others nothing.
 struct Weight {
     double xmax, c, unit; bool inf;                // unit: 2^(52 - s); the low 52 bits of w + unit are w in units of 2^-s
     __device__ __forceinline__ double step() const { return unit * 2.2204460492503131e-16; }       // 2^-s
+    __device__ __forceinline__ u64 units(double w) const { return (u64)rint(w * (4503599627370496.0 / unit)); }      // of any w, 2^52 / unit = 2^s
     __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double_as_longlong(w + unit) & ((1ull << 52) - 1); }
     __device__ __forceinline__ double operator()(float x) const {
         if (inf) return x == INFINITY ? 1.0 : 0.0;
@@ -54,10 +67,14 @@ struct Weight {
             for (int e = 0; e < N; ++e) w[e] = x[e] == INFINITY ? 1.0 : 0.0;
             return;
         }
-        double y[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) y[e] = ((double)x[e] - xmax) * c;
-        exp2_64<N>(y, w);
+        for (int h = 0; h < N; h += 4) {           // four chains hide the latency; eight want twice the registers
+            double y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = ((double)x[h + e] - xmax) * c;
+            exp2_64<4>(y, w + h);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 };
 
@@ -78,10 +95,46 @@ template <int W, int CELLS> struct Shared {
         u64 bins[BINS][COPIES];
         u64 list[CAP];
     };
-    union { double sum[CELLS]; int count[CELLS]; } cell;
+    union { double sum[CELLS]; u64 units[CELLS]; int count[CELLS]; } cell;
     alignas(16) u64 total[BINS];
-    double all; int redi[W]; uint32_t red2[2][W];
+    double all; int redi; uint32_t red[W];
     int pick; double before; Cut cut;
+};
+
+// Largest and smallest finite score, and NaN, of raw vectors: as signed integers whose order is that of the scores (bits
+// other than the sign turned over where it is set), two a register with bf16.  A NaN is beyond +inf or -inf.
+template <typename T> struct Extremes {
+    static constexpr bool B = ET<T>::IS_BF16;
+    typedef typename std::conditional<B, short, int>::type I;
+    typedef typename std::conditional<B, unsigned short, uint32_t>::type UI;
+    typedef I IV __attribute__((ext_vector_type(B ? 2 : 1)));
+    typedef UI UV __attribute__((ext_vector_type(B ? 2 : 1)));
+    static constexpr I MAG = B ? 0x7FFF : 0x7FFFFFFF, INF = B ? 0x7F80 : 0x7F800000, NEG_INF = (I)(~(UI)INF);
+    IV hi, lo; UV fin;                             // fin: from the key behind -inf on, -inf itself being the largest
+    __device__ __forceinline__ Extremes() : hi((IV)NEG_INF), lo((IV)INF), fin((UV)(UI)~0u) {}
+    __device__ __forceinline__ void add(const i32x4& v) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int word = v[q];
+            const IV b = __builtin_bit_cast(IV, word), k = b ^ ((b >> (IV)(I)(sizeof(I) * 8 - 1)) & (IV)MAG);
+            hi = __builtin_elementwise_max(hi, k);
+            lo = __builtin_elementwise_min(lo, k);
+            fin = __builtin_elementwise_min(fin, __builtin_bit_cast(UV, k) + (UV)(UI)~(UI)NEG_INF);
+        }
+    }
+    static __device__ __forceinline__ float score(I k) {
+        const I b = k ^ ((k >> (sizeof(I) * 8 - 1)) & MAG);
+        return __uint_as_float((uint32_t)(UI)b << (B ? 16 : 0));
+    }
+    __device__ __forceinline__ void join(float& mine, float& low, bool& nan) const {
+#pragma unroll
+        for (int e = 0; e < (B ? 2 : 1); ++e) {
+            nan |= (hi[e] > INF) | (lo[e] < NEG_INF);
+            mine = fmaxf(mine, score(hi[e]));
+            const I f = (I)(UI)(fin[e] + (UI)(NEG_INF + 1));
+            low = fminf(low, ((f > NEG_INF) & (f < INF)) ? score(f) : INFINITY);
+        }
+    }
 };
 
 // One row as its workgroup of W waves sees it: every wave has a contiguous share of the whole vectors, `steps` of them a
@@ -93,43 +146,59 @@ template <typename T, int W> struct Row {
     int n, tid, lane, wave, steps, first;          // first: this lane's vector of step 0
     float xe;                                      // of the threads below sp.edge
 
-    __device__ __forceinline__ Row(const T* x_, int n_) : x(x_), sp(x_, n_), n(n_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6) {
+    __device__ __forceinline__ Row(const T* x_, int n_) : x(x_), sp(x_, n_), n(n_), tid(threadIdx.x), lane(threadIdx.x & 63), wave(uniform((int)threadIdx.x >> 6)) {
         steps = (sp.nvec + G - 1) / G;
         first = wave * steps * 64 + lane;
         xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY;
     }
     __device__ __forceinline__ bool valid(int i) const { return i < steps && first + i * 64 < sp.nvec; }
-    __device__ __forceinline__ i32x4 load(int i) const { return valid(i) ? load_vec(x, sp.vec_at(first + i * 64)) : neg_inf_vec<T>(); }
+    // Vector i, or the last one of the row in the place of one beyond it (use() takes care of it): a load that is not always
+    // made is waited for together with all that follow it.  nvec > 0.
+    __device__ __forceinline__ i32x4 load(int i) const { return load_vec(x, sp.vec_at(min(first + i * 64, sp.nvec - 1))); }
+    __device__ __forceinline__ i32x4 use(int i, const i32x4& v) const { return wave * steps * 64 + i * 64 + 64 > sp.nvec && !valid(i) ? neg_inf_vec<T>() : v; }
     __device__ __forceinline__ int cls(int i, int e) const { return sp.vec_at(first + i * 64) + e; }
     __device__ __forceinline__ int wave_cells() const { return (steps + CELL - 1) / CELL; }
     __device__ __forceinline__ int cells() const { return W * wave_cells() + 2; }
     __device__ __forceinline__ int cell(int i) const { return 1 + wave * wave_cells() + i / CELL; }
+    // the cell of class j; the wave by a product: (v + 0.5) / share is at least 0.5 / 32768 away from a whole number
+    __device__ __forceinline__ int cell_of(int j) const {
+        const int v = (j - sp.head) / VEC, share = steps * 64;
+        if (j < sp.head) return 0;
+        if (v >= sp.nvec) return cells() - 1;
+        const int w = (int)(((float)v + 0.5f) * __builtin_amdgcn_rcpf((float)share));
+        return 1 + w * wave_cells() + (v - w * share) / (64 * CELL);
+    }
     __device__ __forceinline__ bool ends_cell(int i) const { return i % CELL == CELL - 1 || i == steps - 1; }
-    // f(i, scores of vector i); scores beyond the row are -inf.  Three steps' loads are under way at a time (eight were slower:
-    // they are moved along every step).
-    template <typename F> __device__ __forceinline__ void each(F f) const {
-        constexpr int D = 3;
-        i32x4 v[D];
+    // f(i, vector i); scores beyond the row are -inf.  U loads are under way at a time, each into registers of its
+    // own: moving them along would wait for them.  U = 1 where f itself takes longer than a load.
+    template <int U, typename F> __device__ __forceinline__ void each_raw(F f) const {
+        if (steps == 0) return;
+        i32x4 v[U];
 #pragma unroll
-        for (int d = 0; d < D; ++d) v[d] = load(d);
+        for (int d = 0; d < U; ++d) v[d] = load(d);
 #pragma unroll 1
-        for (int i = 0; i < steps; ++i) {
-            float s[VEC];
-            unpack16<T>(v[0], s);
+        for (int i = 0; i < steps; i += U) {
 #pragma unroll
-            for (int d = 0; d + 1 < D; ++d) v[d] = v[d + 1];
-            v[D - 1] = load(i + D);
-            f(i, s);
+            for (int d = 0; d < U; ++d) {
+                const i32x4 w = use(i + d, v[d]);
+                v[d] = load(i + d + U);
+                if (i + d < steps) f(i + d, w);
+            }
         }
+    }
+    // f(i, scores of vector i)
+    template <int U, typename F> __device__ __forceinline__ void each(F f) const {
+        each_raw<U>([&](int i, const i32x4& v) { float s[VEC]; unpack16<T>(v, s); f(i, s); });
     }
     // f(i, scores of vector i) for the steps of cell c, by the wave that has it, until f says stop
     template <typename F> __device__ __forceinline__ void in_cell(int c, F f) const {
         const int wc = wave_cells();
         if (c < 1 || c > W * wc || (c - 1) / wc != wave) return;
         const int i0 = (c - 1) % wc * CELL;
+#pragma unroll 1
         for (int i = i0; i < i0 + CELL && i < steps; ++i) {
             float s[VEC];
-            unpack16<T>(load(i), s);
+            unpack16<T>(use(i, load(i)), s);
             if (f(i, s)) return;
         }
     }
@@ -137,6 +206,7 @@ template <typename T, int W> struct Row {
 
 // Largest v in [lo, hi] with enough(v), which holds at lo.
 template <typename F> __device__ __forceinline__ uint32_t last_enough(uint32_t lo, uint32_t hi, F enough) {
+#pragma unroll 1
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
         if (enough(mid)) lo = mid; else hi = mid - 1;
@@ -157,21 +227,29 @@ template <typename T> struct List {
     const Weight& weight;
     int c, n;                                      // places; classes of the row
     u64 lp[R], lw[R];                              // place (0: none) and weight in integer units
-    __device__ __forceinline__ List(const u64* list, int c_, int n_, const Weight& w) : weight(w), c(c_), n(n_) {
+    uint32_t lo, hi, under;                        // smallest and largest key; bit i: weight i is less than min_p
+    __device__ __forceinline__ List(const u64* list, int c_, int n_, const Weight& w_, double least) : weight(w_), c(c_), n(n_) {
         const int lane = threadIdx.x & 63;
+        float x[R];
+        double w[R];
+        uint32_t l = 0, h = 0;                     // ~ of the smallest key, the largest
+        under = 0;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            lp[i] = lw[i] = 0;
-            if (64 * i < c) {
-                if (lane + 64 * i < c) lp[i] = list[lane + 64 * i];
-                if (lp[i]) lw[i] = weight.fixed(weight(place_score(lp[i])));
-            }
+            lp[i] = lane + 64 * i < c ? list[lane + 64 * i] : 0;
+            x[i] = lp[i] ? place_score(lp[i]) : -INFINITY;
+            if (lp[i]) { l = max(l, ~key(lp[i])); h = max(h, key(lp[i])); }
         }
+        weight.template many<R>(x, w);
+#pragma unroll
+        for (int i = 0; i < R; ++i) { lw[i] = weight.fixed(w[i]); under |= w[i] < least ? 1u << i : 0u; }
+        lo = ~wave_max(l);
+        hi = wave_max(h);
     }
     template <typename P> __device__ __forceinline__ int count(P pred) const {
         int m = 0;
 #pragma unroll
-        for (int i = 0; i < R; ++i) if (64 * i < c) m += __popcll(__ballot((lp[i] != 0) & pred(lp[i])));
+        for (int i = 0; i < R; ++i) if (64 * i < c) m += __popcll(__ballot(pred(lp[i])));
         return m;
     }
     template <typename P> __device__ __forceinline__ u64 mass(P pred) const {
@@ -182,40 +260,34 @@ template <typename T> struct List {
     }
     __device__ __forceinline__ u64 all() const { return mass([](u64) { return true; }); }
     static __device__ __forceinline__ uint32_t key(u64 e) { return (uint32_t)(e >> (32 + SHIFT)); }
-    static __device__ __forceinline__ float score(uint32_t s) { return key_score(ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s); }
-    __device__ __forceinline__ void range(uint32_t& lo, uint32_t& hi) const {
-        uint32_t l = 0, h = 0;                     // ~ of the smallest key, the largest
-#pragma unroll
-        for (int i = 0; i < R; ++i) if (64 * i < c && lp[i]) { l = max(l, ~key(lp[i])); h = max(h, key(lp[i])); }
-        lo = ~wave_reduce(l, OpMax());
-        hi = wave_reduce(h, OpMax());
+    // The last place that the sum of the entries from the first one on, enough(place) says whether up to a place, needs.
+    template <typename F> __device__ __forceinline__ Cut border(const Cut& was, F enough) const {
+        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return enough((u64)mid << (32 + SHIFT)); });
+        const u64 first = (u64)(ET<T>::IS_BF16 ? v << 16 | ((v & 0x8000u) ? 0u : 0xFFFFu) : v) << 32;
+        Cut to = {place_score(first), n};
+        if (count([&](u64 e) { return (e ^ first) >> 32 == 0; }) > 1)
+            to.ti = (int)~last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return enough(first | mid); });
+        if (to.xt == was.xt) to.ti = min(to.ti, was.ti);
+        return to;
     }
-    // the m-th by class of the entries with key v
-    __device__ __forceinline__ int tie(uint32_t v, int m) const {
-        return (int)~last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return count([&](u64 e) { return (key(e) == v) & ((uint32_t)e >= mid); }) >= m; });
+    __device__ __forceinline__ Cut cut_count(int k, const Cut& was) const {
+        return border(was, [&](u64 from) { return count([&](u64 e) { return e >= from; }) >= k; });
     }
-    // the first k entries
-    __device__ __forceinline__ Cut cut_count(int k) const {
-        uint32_t lo, hi;
-        range(lo, hi);
-        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return count([&](u64 e) { return key(e) >= mid; }) >= k; });
-        const int above = count([&](u64 e) { return key(e) > v; }), ties = count([&](u64 e) { return key(e) == v; });
-        return {score(v), above + ties > k ? tie(v, k - above) : n};
-    }
-    // the shortest prefix that, after `above`, reaches the target; `was`: what cut the entries so far
     __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Cut& was) const {
-        uint32_t lo, hi;
-        range(lo, hi);
-        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return above + mass([&](u64 e) { return key(e) >= mid; }) >= target; });
-        const u64 over = above + mass([&](u64 e) { return key(e) > v; });
-        const int ties = count([&](u64 e) { return key(e) == v; });
-        const float x = score(v);
-        const int m = ties_needed(over, weight.fixed(weight(x)), target, ties);
-        return {x, m < ties ? tie(v, m) : x == was.xt ? was.ti : n};
+        return border(was, [&](u64 from) { return above + mass([&](u64 e) { return e >= from; }) >= target; });
     }
-    template <typename K> __device__ __forceinline__ void keep(K kept) {
+    __device__ __forceinline__ void keep(const Cut& cut) {
+        const u64 last = place(score_key(cut.xt), cut.ti);
 #pragma unroll
-        for (int i = 0; i < R; ++i) if (64 * i < c && !(lp[i] && kept(place_score(lp[i]), place_class(lp[i])))) lp[i] = lw[i] = 0;
+        for (int i = 0; i < R; ++i) if (lp[i] < last) lp[i] = lw[i] = 0;
+    }
+    __device__ __forceinline__ void drop_under() {
+#pragma unroll
+        for (int i = 0; i < R; ++i) if (under >> i & 1) lw[i] = 0;
+    }
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int i = 0; i < R; ++i) if (64 * i < c && lw[i]) f(place_class(lp[i]), lw[i]);
     }
     // The answer, from entries that are all there is, in integer units: the first class, in the order of the classes, at
     // which the running mass exceeds u times all of it.
@@ -223,16 +295,47 @@ template <typename T> struct List {
         const u64 sum = all(), most = (u64)floor((double)u * (double)sum);             // a running mass > most
         // lower classes are larger ~class: the largest one down from which more than `most` has gathered
         const uint32_t who = last_enough(~(uint32_t)(n - 1), ~0u, [&](uint32_t mid) { return mass([&](u64 e) { return (uint32_t)e >= mid; }) > most; });
-        const float lane_x = [&] { float x = -INFINITY;
+        float x = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < R; ++i) if (64 * i < c && lw[i] && (uint32_t)lp[i] == who) x = place_score(lp[i]);
-            return x; }();
-        if (lane_x > -INFINITY) answer((int)~who, (float)log(weight(lane_x) / ((double)sum * weight.step())));
+        for (int i = 0; i < R; ++i) if (64 * i < c && lw[i] && (uint32_t)lp[i] == who) x = place_score(lp[i]);
+        if (x > -INFINITY) answer((int)~who, weight(x), (double)sum * weight.step());
     }
 };
 
+// A list of at most 64 places, one a lane, compared with each other one by one.
+template <typename A> __device__ __forceinline__ void draw_short(const u64* list, int c, int k, float p, double least, float u, const Weight& weight, A answer) {
+    const int lane = threadIdx.x & 63;
+    const u64 e = lane < c ? list[lane] : 0;
+    const double w = lane < c ? weight(place_score(e)) : 0.0;
+    u64 f = weight.fixed(w);
+    if (k < c || p < 1.f) {
+        u64 above = 0;                             // mass and number of the entries in front of this one
+        int rank = 0;
+#pragma unroll 1
+        for (int i = 0; i < c; i += 4) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {          // lanes from c on hold 0
+                const bool front = lane_at(e, i + d) > e;
+                above += front ? lane_at(f, i + d) : 0;
+                rank += front;
+            }
+        }
+        if (rank >= k) f = 0;
+        if (p < 1.f && above >= (u64)ceil((double)p * (double)wave_sum(f))) f = 0;
+    }
+    if (w < least) f = 0;
+    const u64 sum = wave_sum(f), most = (u64)floor((double)u * (double)sum);
+    u64 before = 0;                                // mass of the kept entries of lower classes
+#pragma unroll 1
+    for (int i = 0; i < c; i += 4) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) before += (uint32_t)lane_at(e, i + d) > (uint32_t)e ? lane_at(f, i + d) : 0;
+    }
+    if (before <= most && most < before + f) answer(place_class(e), w, (double)sum * weight.step());
+}
+
 template <typename T, int W, int CELLS>
-__global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleArgs a) {
+__global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
     typedef Row<T, W> R;
     typedef Shared<W, CELLS> S;
     constexpr int VEC = R::VEC, G = R::G, BINS = S::BINS;
@@ -242,36 +345,51 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
     const int tid = row.tid, lane = row.lane, wave = row.wave, n = a.n;
     const float u = a.u[r], t = a.tp ? a.tp[r] : a.t, p = a.pp ? a.pp[r] : a.p, q = a.qp ? a.qp[r] : a.q;
     int k = a.kp ? a.kp[r] : a.k;
-    auto answer = [&](int label, float lp) { a.labels[r] = label; a.logp[r] = lp; };       // by one thread
+    auto fixed_answer = [&](int label, float lp) { a.labels[r] = label; a.logp[r] = lp; };                 // by one thread
+    auto answer = [&](int label, double w, double all) { fixed_answer(label, (float)ln_64(w / all)); };
 
+    auto block_max = [&](uint32_t v) {
+        v = wave_max(v);
+        if constexpr (W == 1) return v;
+        __syncthreads();
+        if (lane == 0) sh.red[wave] = v;
+        __syncthreads();
+        return wave_max(lane < W ? sh.red[lane] : 0u);
+    };
     // the row's maximum, its smallest finite score, and whether a NaN is there
     float mine = row.xe, low = row.xe > -INFINITY ? row.xe : INFINITY;
     bool nan = row.xe != row.xe;
-    row.each([&](int i, const float* s) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { mine = fmaxf(mine, s[e]); nan |= s[e] != s[e]; low = fminf(low, s[e] > -INFINITY ? s[e] : INFINITY); }
-    });
-    const uint32_t top = block_reduce<W>(nan ? KEY_NAN : score_key(mine), OpMax(), sh.red2[0]);
+    {
+        Extremes<T> x;
+        row.template each_raw<4>([&](int i, const i32x4& v) { x.add(v); });
+        if (row.steps) x.join(mine, low, nan);
+    }
+    const uint32_t top = block_max(nan ? KEY_NAN : score_key(mine));
     if (top == KEY_NAN || !(t >= 0.f) || !(t < INFINITY) || k < 0 || !(p > 0.f) || !(p <= 1.f) || !(q >= 0.f) || !(q <= 1.f) || !(u >= 0.f) || !(u < 1.f)) {
-        if (tid == 0) answer(-1, NAN);
+        if (tid == 0) fixed_answer(-1, NAN);
         return;
     }
-    if (top == KEY_NEG_INF) { if (tid == 0) answer(-1, -INFINITY); return; }
+    if (top == KEY_NEG_INF) { if (tid == 0) fixed_answer(-1, -INFINITY); return; }
     const float xmax = key_score(top);
     const int s = min(50, 30 + __clz(n));          // n sums of at most 2^s stay below 2^63
     const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, (double)(1ull << (52 - s)), xmax == INFINITY};
     if (t == 0.f || k == 1) {
         int at = n;
-        row.each([&](int i, const float* s) {
+        row.template each<4>([&](int i, const float* s) {
 #pragma unroll
             for (int e = VEC - 1; e >= 0; --e) if (s[e] == xmax) at = min(at, row.cls(i, e));
         });
         if (tid < row.sp.edge && row.xe == xmax) at = min(at, row.sp.edge_at(tid));
-        at = (int)~block_reduce<W>(~(uint32_t)at, OpMax(), sh.red2[1]);
-        if (tid == 0) answer(at, 0.f);
+        at = (int)~block_max(~(uint32_t)at);
+        if (tid == 0) fixed_answer(at, 0.f);
         return;
     }
     if (k == 0 || k > n) k = n;
+
+    // min_p: a weight is only computed where a 32-bit estimate of the border, with room, says that it may pass
+    const double least = q > 0.f ? (double)q : 0.0;
+    const float xq = q > 0.f && !weight.inf ? (float)((double)xmax + (double)(__builtin_amdgcn_logf(q) - 1e-3f) / weight.c) : -INFINITY;
+    const float xlow = xq - fabsf(xq) * 1e-6f;
 
     Cut cut = {-INFINITY, n};
     // Scores of a vector that are not kept become -inf, which weighs nothing.  False: none of the wave's is kept.
@@ -287,22 +405,12 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         }
         return true;
     };
-    auto mass_target = [&](u64 all) { return (u64)ceil((double)p * (double)all); };
-    auto count_waves = [&](int m) {                // sum over the waves of a number that is the same in a wave's lanes
-        __syncthreads();
-        if (lane == 0) sh.redi[wave] = m;
-        __syncthreads();
-        int s = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) s += sh.redi[w];
-        return s;
-    };
     // counts by cells of the scores that pass, as prefix sums: cell.count[c] = how many lie in front of cell c.  Returns all.
     auto count_cells = [&](auto pred) {
         __syncthreads();
         const int cells = row.cells();
         int m = 0;
-        row.each([&](int i, const float* s) {
+        row.template each<2>([&](int i, const float* s) {
             const bool ok = row.valid(i);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) m += __popcll(__ballot(ok & pred(s[e], row.cls(i, e))));
@@ -315,23 +423,23 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         __syncthreads();
         if (wave == 0) {
             int run = 0;
-            for (int c = 0; c < cells; c += 64) {
+#pragma unroll 1
+        for (int c = 0; c < cells; c += 64) {
                 const int m = c + lane < cells ? sh.cell.count[c + lane] : 0;
-                int s = m;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(s, d); if (lane >= d) s += o; }
+                const int s = wave_scan(m);
                 if (c + lane < cells) sh.cell.count[c + lane] = run + s - m;
-                run += __shfl(s, 63);
+                run += lane_at(s, 63);
             }
             if (lane == 0) sh.pick = run;
         }
         __syncthreads();
-        return sh.pick;
+        return uniform(sh.pick);
     };
     // The kept scores in [xa, xb], xa > -inf, as places in the list (in no particular order: everything that is made of it is
     // a set, or a sum of integers).  Returns how many there are; more than CAP are not all in it.  Few scores pass, so what
-    // counts is the test, two instructions a score, and that a lane with a hit handles it alone.
-    auto collect = [&](float xa, float xb) {
+    // counts is the test, two instructions a score, and that a lane with a hit handles it alone.  With sum, the weights of the
+    // scores beyond xb that min_p leaves are added up by cells, in integer units.
+    auto collect = [&](float xa, const float xb, bool sum) {
         __syncthreads();
         if (tid == 0) sh.pick = 0;
         __syncthreads();
@@ -342,22 +450,45 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
             const int at = atomicAdd(&sh.pick, 1);
             if (at < CAP) sh.list[at] = place(score_key(x), j);
         };
-        row.each([&](int i, const float* s) {
-            uint32_t in = 0;
+        double cell_sum = 0;
+        row.template each<2>([&](int i, const float* s) {
+            u64 some = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) in |= __builtin_amdgcn_fmed3f(s[e], xa, xb) == s[e] ? 1u << e : 0u;
-            while (in) {
-                const int e = __ffs(in) - 1;
-                in &= in - 1;
-                float x = s[0];
+            for (int e = 0; e < VEC; ++e) some |= __ballot(__builtin_amdgcn_fmed3f(s[e], xa, xb) == s[e]);
+            if (some) {
+                uint32_t in = 0;
 #pragma unroll
-                for (int o = 1; o < VEC; ++o) x = e == o ? s[o] : x;
-                append(x, row.cls(i, e));
+                for (int e = 0; e < VEC; ++e) in |= __builtin_amdgcn_fmed3f(s[e], xa, xb) == s[e] ? 1u << e : 0u;
+                while (in) {
+                    const int e = __ffs(in) - 1;
+                    in &= in - 1;
+                    float x = s[0];
+#pragma unroll
+                    for (int o = 1; o < VEC; ++o) x = e == o ? s[o] : x;
+                    append(x, row.cls(i, e));
+                }
+            }
+            if (sum) {
+                float x[VEC];
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) { const bool k = (s[e] > xb) & (s[e] >= xlow); x[e] = k ? s[e] : -INFINITY; any |= k; }
+                if (__ballot(any)) {
+                    double w[VEC];
+                    weight.template many<VEC>(x, w);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) cell_sum += w[e] >= least ? w[e] : 0.0;
+                }
+                if (row.ends_cell(i)) {
+                    cell_sum = wave_sum(cell_sum);
+                    if (lane == 0) sh.cell.units[row.cell(i)] = weight.units(cell_sum);
+                    cell_sum = 0;
+                }
             }
         });
         if (tid < row.sp.edge && row.xe >= xa && row.xe <= xb) append(row.xe, row.sp.edge_at(tid));
         __syncthreads();
-        const int c = sh.pick;
+        const int c = uniform(sh.pick);
         __syncthreads();
         return c;
     };
@@ -367,6 +498,7 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         count_cells(is);
         if (wave == 0) {                           // the last cell with fewer than m in front of it
             int c = 0;
+#pragma unroll 1
             for (int b = 0; b < row.cells(); b += 64) {
                 const bool in = b + lane < row.cells() && sh.cell.count[b + lane] < m;
                 c += __popcll(__ballot(in));
@@ -374,72 +506,92 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
             if (lane == 0) sh.pick = c - 1;
         }
         __syncthreads();
-        const int c = sh.pick, cells = row.cells();
-        int left = m - sh.cell.count[c];           // the left-th one of that cell
+        const int c = uniform(sh.pick), cells = row.cells();
+        int left = m - uniform(sh.cell.count[c]);           // the left-th one of that cell
         row.in_cell(c, [&](int i, const float* s) {
             int own = 0;
             const bool ok = row.valid(i);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) own += ok && s[e] == x ? 1 : 0;
-            int s0 = own;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) { const int o = __shfl_up(s0, d); if (lane >= d) s0 += o; }
-            const int here = __shfl(s0, 63);
+            const int s0 = wave_scan(own), here = lane_at(s0, 63);
             if (here < left) { left -= here; return false; }
             if (s0 - own < left && left <= s0) {
                 int rank = s0 - own;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) if (s[e] == x && ++rank == left) sh.redi[0] = row.cls(i, e);
+                for (int e = 0; e < VEC; ++e) if (s[e] == x && ++rank == left) sh.redi = row.cls(i, e);
             }
             return true;
         });
         if (wave == 0 && (c == 0 || c == cells - 1)) {
             const u64 b = __ballot(tid < row.sp.edge && row.xe == x), front = (1ull << row.sp.head) - 1, here = c == 0 ? b & front : b & ~front;
-            if ((here >> lane & 1) && lanes_below(here) == left - 1) sh.redi[0] = row.sp.edge_at(tid);
+            if ((here >> lane & 1) && lanes_below(here) == left - 1) sh.redi = row.sp.edge_at(tid);
         }
         __syncthreads();
-        const int j = sh.redi[0];
+        const int j = uniform(sh.redi);
         __syncthreads();
         return j;
     };
-    constexpr int SHIFT = ET<T>::IS_BF16 ? 16 : 0; // bits of a key that carry nothing
-    auto wide_key = [](uint32_t s) { return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s; };
-
-    // min_p: a weight is only computed where a 32-bit estimate of the border, with room, says that it may pass
-    const double least = q > 0.f ? (double)q : 0.0;
-    const float xq = q > 0.f && !weight.inf ? (float)((double)xmax + (log2((double)q) - 1e-3) / weight.c) : -INFINITY;
-    const float xlow = xq - fabsf(xq) * 1e-6f;
+    // A key that k of the threads' maxima reach, to 16 bits (bisected by one wave).
+    auto bound = [&] {
+        uint32_t* maxima = (uint32_t*)sh.bins;
+        maxima[tid] = score_key(mine) >> 16;
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t m[W];
+#pragma unroll
+            for (int w = 0; w < W; ++w) m[w] = maxima[w * 64 + lane];
+            const uint32_t v = last_enough(0, top >> 16, [&](uint32_t mid) {
+                int s = 0;
+#pragma unroll
+                for (int w = 0; w < W; ++w) s += __popcll(__ballot(m[w] >= mid));
+                return s >= k;
+            });
+            if (lane == 0) sh.pick = (int)(v << 16);
+        }
+        __syncthreads();
+        return uniform((uint32_t)sh.pick);
+    };
 
     // ---- borders ----------------------------------------------------------------------------------------------------
-    // The kept scores with keys in [klo, khi] by bins of their distance to the first, index(x), and what each counts.
+    // The kept scores with keys in [klo, khi] by bins, and what each weighs (mass) or counts: bins of the distance to the first
+    // score, or (shift >= 0) of the keys down from khi.
     uint32_t klo = 0, khi = top;
+    float scale = 0;
     auto upper_score = [](uint32_t k) { return key_score(k == 0x7FFFFFFFu ? k - 1 : k); };  // no score has the key of -0, and as a number it is 0
-    auto fill_bins = [&](auto weigh, auto index) {
+    auto fill_bins = [&](bool mass, int shift) {
         __syncthreads();
+#pragma unroll 1
         for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
         __syncthreads();
         const float xlo = klo ? key_score(klo) : -INFINITY, xhi = upper_score(khi);
-        auto drop = [&](float x, u64 v) { if (x <= xhi) atomicAdd(&sh.bins[index(x)][lane & (S::COPIES - 1)], v); };
-        row.each([&](int i, const float* s) {
+        auto drop = [&](float x, u64 v) {
+            if (x > xhi) return;
+            const int b = shift < 0 ? (int)fminf((xmax - x) * scale, (float)(BINS - 1)) : (int)((khi - score_key(x)) >> shift);
+            atomicAdd(&sh.bins[b][lane & (S::COPIES - 1)], v);
+        };
+        row.template each<1>([&](int i, const float* s) {
             float x[VEC];
             if (!only_kept(i, s, x, xlo)) return;
             u64 v[VEC];
-            if constexpr (decltype(weigh)::value) {
+            if (mass) {
                 double w[VEC];
                 weight.template many<VEC>(x, w);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[e] = weight.fixed(w[e]);
             } else {
+                const u64 one = row.valid(i);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = (row.valid(i) & (s[e] >= xlo)) ? 1 : 0;
+                for (int e = 0; e < VEC; ++e) v[e] = one;
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) if (s[e] >= xlo) drop(s[e], v[e]);
         });
-        if (tid < row.sp.edge && row.xe >= xlo && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, decltype(weigh)::value ? weight.fixed(weight(row.xe)) : 1);
+        if (tid < row.sp.edge && row.xe >= xlo && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, mass ? weight.fixed(weight(row.xe)) : 1);
         __syncthreads();
+#pragma unroll 1
         for (int b = tid; b < BINS; b += G) {
             u64 s = 0;
+#pragma unroll 8
             for (int i = 0; i < S::COPIES; ++i) s += sh.bins[b][(i + tid) & (S::COPIES - 1)];
             sh.total[b] = s;
         }
@@ -457,95 +609,107 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         u64 own = 0;
 #pragma unroll
         for (int i = 0; i < BL; ++i) own += sh.total[BL * lane + i];
-        u64 s = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const u64 o = __shfl_up(s, d); if (lane >= d) s += o; }
+        const u64 s = wave_scan(own);
         const u64 hit = __ballot(above + s >= target);
         const int l = hit ? __ffsll(hit) - 1 : 63;
-        above += __shfl(s, l) - __shfl(own, l);
+        above += lane_at(s - own, l);
         int b = BL * l;
-#pragma unroll
-        for (int i = 0; i < BL - 1; ++i)
-            if (b == BL * l + i && above + sh.total[b] < target) { above += sh.total[b]; ++b; }
+#pragma unroll 1
+        for (int i = 0; i < BL - 1; ++i) {
+            const u64 next = above + uniform(sh.total[b]);
+            if (next >= target) break;
+            above = next;
+            ++b;
+        }
         return b;
     };
-    // The border of top_k (weigh false: target scores, `above` of them so far) or top_p (target of mass): bins, then the bin
-    // that the border is in split by keys until it holds a list or one key.
-    auto find_border = [&](auto weigh, u64 target, auto get_target) {
-        u64 above = 0;
-        klo = 0; khi = top;
-        // BINS over 32 octaves of the weight, or finer where the row is narrower
-        const float smallest = key_score(~block_reduce<W>(~score_key(low), OpMax(), sh.red2[0]));
-        float scale = (float)fmin(BINS / 32 * weight.c, 1e30);
-        if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
-        auto bin = [&](float x) { return (int)fminf((xmax - x) * scale, (float)(BINS - 1)); };
-        fill_bins(weigh, bin);
-        target = get_target(target);
-        int b = bin_reach(target, above);
-        // the bin's scores: from the first key that is not beyond it to the last that has reached it, 64 keys tried at a time
-        auto last_key = [&](auto holds) {          // the last key up to top with holds(score), which holds for -inf and below
-            uint32_t lo = KEY_NEG_INF, hi = top;
-            while (lo < hi) {
-                const uint32_t step = (hi - lo) / 64 + 1, key = lo + lane * step;
-                const int m = __popcll(__ballot((lane == 0) | ((key > lo) & (key <= hi) & holds(key_score(min(max(key, lo), hi))))));
-                const uint32_t from = lo + (m - 1) * step;
-                hi = min(hi, from + (step - 1));
-                lo = from;
-            }
-            return lo;
-        };
-        const uint32_t kb = last_key([&](float x) { return !((xmax - x) * scale < (float)b); });
-        const uint32_t ka = b == BINS - 1 ? KEY_NEG_INF : last_key([&](float x) { return !((xmax - x) * scale < (float)(b + 1)); }) + 1;
-        klo = max(ka, KEY_NEG_INF + 1);            // -inf weighs nothing: never in the list
-        khi = kb;
-        int c = collect(key_score(klo), upper_score(khi));
-        if (!decltype(weigh)::value && target > above + c) return;         // top_k reaches into scores of -inf: all others are kept
-        while (c > CAP && klo < khi) {             // every round leaves 2 / BINS of the keys
-            int sh_bits = 0;
-            while ((khi - klo) >> sh_bits >= (uint32_t)BINS) ++sh_bits;
-            fill_bins(weigh, [&](float x) { return (int)((khi - score_key(x)) >> sh_bits); });
-            b = bin_reach(target, above);
-            const uint32_t to = khi - ((uint32_t)b << sh_bits), from = to - min(to - klo, (1u << sh_bits) - 1);
-            khi = to; klo = from;
-            c = collect(key_score(klo), upper_score(khi));
+    // the last key up to top with holds(score), which holds for -inf and below: 64 keys tried at a time
+    auto last_key = [&](auto holds) {
+        uint32_t lo = KEY_NEG_INF, hi = top;
+#pragma unroll 1
+        while (lo < hi) {
+            const uint32_t step = (hi - lo) / 64 + 1, key = lo + lane * step;
+            const int m = __popcll(__ballot((lane == 0) | ((key > lo) & (key <= hi) & holds(key_score(min(max(key, lo), hi))))));
+            const uint32_t from = lo + (m - 1) * step;
+            hi = min(hi, from + (step - 1));
+            lo = from;
         }
+        return lo;
+    };
+
+    // Pass 0: rows that fit in a list, and top_k of which the threads' maxima give one; the list is all there is.
+    // Pass 1: the border of top_k, pass 2: the border of top_p.  Bins; then the bin that the border is in, split by keys until
+    // it holds a list or one key.  The last of the two also adds up what is kept for certain.  One loop, so that there is one
+    // copy of everything (written out for each use the code was 87 KB, more than the instruction cache holds).
+    bool summed = false;                           // the cells hold what is kept, in integer units
+#pragma unroll 1
+    for (int pass = 0; pass < (W == 1 ? 1 : 3); ++pass) {
+        const bool mass = pass == 2, sum = mass || (pass == 1 && !(p < 1.f));
+        u64 above = 0, target = (u64)k;
+        int shift = -1, c;
+        if (pass == 0) {
+            klo = KEY_NEG_INF + 1;                 // -inf weighs nothing: never in the list
+            if (W > 1 && n > CAP) {
+                if (k > G / 2) continue;
+                klo = bound();
+                if (klo <= KEY_NEG_INF) continue;
+            }
+            khi = top;
+        } else {
+            if (mass ? !(p < 1.f) : k == n) continue;
+            klo = 0; khi = top;
+            // BINS over 32 octaves of the weight, or finer where the row is narrower
+            const float smallest = key_score(~block_max(~score_key(low)));
+            scale = (float)fmin(BINS / 32 * weight.c, 1e30);
+            if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
+        }
+#pragma unroll 1
+        for (;;) {
+            if (pass) {
+                fill_bins(mass, shift);
+                if (mass && shift < 0) target = (u64)ceil((double)p * (double)bin_sum());
+                const int b = bin_reach(target, above);
+                if (shift < 0) {                   // from the first key that is not beyond the bin to the last that has reached it
+                    khi = last_key([&](float x) { return !((xmax - x) * scale < (float)b); });
+                    klo = b == BINS - 1 ? KEY_NEG_INF + 1 : max(KEY_NEG_INF, last_key([&](float x) { return !((xmax - x) * scale < (float)(b + 1)); })) + 1;
+                } else {
+                    khi -= (uint32_t)b << shift;
+                    klo = khi - min(khi - klo, (1u << shift) - 1);
+                }
+            }
+            c = collect(key_score(klo), upper_score(khi), sum);
+            if (!pass || c <= CAP || klo >= khi) break;
+            shift = 0;                             // every round leaves 2 / BINS of the keys
+            while ((khi - klo) >> shift >= (uint32_t)BINS) ++shift;
+        }
+        if (pass == 0 && c > CAP) continue;
+        if (pass == 1 && target > above + c) continue;                     // top_k reaches into scores of -inf: all others are kept
         if (c <= CAP) {
             if (wave == 0) {
-                const List<T> list(sh.list, c, n, weight);
-                const Cut to = decltype(weigh)::value ? list.cut_mass(above, target, cut) : list.cut_count((int)(target - above));
-                if (lane == 0) sh.cut = to;
+                if (!pass && c <= 64) { draw_short(sh.list, c, k, p, least, u, weight, answer); return; }
+                List<T> list(sh.list, c, n, weight, least);
+                if (pass ? !mass : k < c) { cut = list.cut_count((int)(target - above), cut); list.keep(cut); }
+                if (pass ? mass : p < 1.f) {
+                    if (!pass) target = (u64)ceil((double)p * (double)list.all());
+                    cut = list.cut_mass(above, target, cut);
+                    list.keep(cut);
+                }
+                list.drop_under();
+                if (!pass) { list.draw(u, answer); return; }
+                if (sum) list.each([&](int j, u64 w) { const int at = row.cell_of(j); if (at > 0 && at < row.cells() - 1) atomicAdd(&sh.cell.units[at], w); });
+                if (lane == 0) sh.cut = cut;
             }
+            if (!pass) return;
             __syncthreads();
-            cut = sh.cut;
+            cut = {uniform(sh.cut.xt), uniform(sh.cut.ti)};
+            summed = sum;
         } else {                                   // c equal scores
             const float x = key_score(khi);
-            const int need = decltype(weigh)::value ? ties_needed(above, weight.fixed(weight(x)), target, c) : (int)(target - above);
-            if (x > -INFINITY) cut = {x, need < c ? nth(x, need) : x == cut.xt ? cut.ti : n};       // -inf weighs nothing: no cut
+            const int need = mass ? ties_needed(above, weight.fixed(weight(x)), target, c) : (int)(target - above);
+            if (x > -INFINITY) cut = {x, need < c ? nth(x, need) : x == cut.xt ? cut.ti : n};           // -inf weighs nothing: no cut
         }
-    };
-    auto kept_share = [&](float x, int j) { return cut(x, j) && !(least > 0 && weight(x) < least); };
-
-    // ---- rows that fit in a list, and top_k of which the threads' maxima give one ---------------------------------------
-    int c = CAP + 1;
-    if (W == 1 || n <= CAP) c = collect(-FLT_MAX, INFINITY);
-    else if (k <= G / 2) {                         // k of the threads' maxima reach a bound
-        const uint32_t key = score_key(mine) >> SHIFT;
-        const uint32_t v = last_enough(0, top >> SHIFT, [&](uint32_t mid) { return count_waves(__popcll(__ballot(key >= mid))) >= k; });
-        if (wide_key(v) > KEY_NEG_INF) c = collect(key_score(wide_key(v)), INFINITY);
     }
-    if (c <= CAP) {
-        if (wave != 0) return;
-        List<T> list(sh.list, c, n, weight);
-        if (k < c) { cut = list.cut_count(k); list.keep(cut); }
-        if (p < 1.f) { cut = list.cut_mass(0, mass_target(list.all()), cut); list.keep(cut); }
-        if (least > 0) list.keep(kept_share);
-        list.draw(u, answer);
-        return;
-    }
-    if constexpr (W > 1) {                         // one wave: rows that fit in a list
-        if (k < n) find_border(std::false_type(), (u64)k, [](u64 t) { return t; });
-        if (p < 1.f) find_border(std::true_type(), 0, [&](u64) { return mass_target(bin_sum()); });
-    }
+    if constexpr (W == 1) return;                  // one wave: rows that fit in a list
     // ---- the answer -------------------------------------------------------------------------------------------------
     auto share = [&](float x, int j) {             // the weight of a class that is kept, else 0
         double w = 0;
@@ -564,8 +728,10 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         return true;
     };
     __syncthreads();
+    auto set_cell = [&](int c, double s) { if (summed) sh.cell.units[c] = weight.units(s); else sh.cell.sum[c] = s; };
+    auto cell_at = [&](int c) { return summed ? (double)sh.cell.units[c] * weight.step() : sh.cell.sum[c]; };
     double cell_sum = 0;
-    row.each([&](int i, const float* s) {
+    if (!summed) row.template each<1>([&](int i, const float* s) {
         double w[VEC];
         if (shares(i, s, w)) {
 #pragma unroll
@@ -581,32 +747,32 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
     if (wave == 0) {
         const double w = tid < row.sp.edge ? share(row.xe, row.sp.edge_at(tid)) : 0.0;
         const double f = wave_sum(tid < row.sp.head ? w : 0.0), b = wave_sum(tid < row.sp.head ? 0.0 : w);
-        if (lane == 0) { sh.cell.sum[0] = f; sh.cell.sum[cells - 1] = b; }
+        if (lane == 0) { set_cell(0, f); set_cell(cells - 1, b); }
     }
     __syncthreads();
     double all = 0;
     if (wave == 0) {
-        for (int c = 0; c < cells; c += 64) all += wave_sum(c + lane < cells ? sh.cell.sum[c + lane] : 0.0);
+#pragma unroll 1
+        for (int c = 0; c < cells; c += 64) all += wave_sum(c + lane < cells ? cell_at(c + lane) : 0.0);
         const double target = (double)u * all;
         // the first cell whose running sum exceeds the target, or the last one that holds anything
         double run = 0, found_before = 0;
         int found = -1, last = 0; double last_before = 0;
+#pragma unroll 1
         for (int c = 0; c < cells; c += 64) {
-            const double m = c + lane < cells ? sh.cell.sum[c + lane] : 0.0;
-            double s = m;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(s, d); if (lane >= d) s += o; }
+            const double m = c + lane < cells ? cell_at(c + lane) : 0.0;
+            const double s = wave_scan(m);
             const u64 hit = __ballot(m > 0 && run + s > target), some = __ballot(m > 0);
-            if (some) { const int l = 63 - __clzll(some); last = c + l; last_before = run + __shfl(s - m, l); }
-            if (hit) { const int l = __ffsll(hit) - 1; found = c + l; found_before = run + __shfl(s - m, l); break; }
-            run += __shfl(s, 63);
+            if (some) { const int l = 63 - __clzll(some); last = c + l; last_before = run + lane_at(s - m, l); }
+            if (hit) { const int l = __ffsll(hit) - 1; found = c + l; found_before = run + lane_at(s - m, l); break; }
+            run += lane_at(s, 63);
         }
         if (lane == 0) { sh.pick = found >= 0 ? found : last; sh.before = found >= 0 ? found_before : last_before; sh.all = all; }
     }
     __syncthreads();
-    const int at = sh.pick;
-    const double before = sh.before;
-    all = sh.all;
+    const int at = uniform(sh.pick);
+    const double before = uniform(sh.before);
+    all = uniform(sh.all);
     const double target = (double)u * all;
     // the class within the cell: the lane in which the running sum exceeds the target, then its element; the last one that
     // weighs anything if rounding leaves none
@@ -618,9 +784,7 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         double own = 0;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) own += w[e];
-        double p = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(p, d); if (lane >= d) p += o; }
+        const double p = wave_scan(own);
         const u64 hit = __ballot(own > 0 && run + p > target);
         double front = run + (p - own);
         int mine = -1, lastc = -1; double mw = 0, lastw = 0;
@@ -634,25 +798,23 @@ __global__ __launch_bounds__(W * 64, W == 1 ? 5 : 4) void sample_kernel(SampleAr
         }
         if (mine < 0) { mine = lastc; mw = lastw; }
         if (hit) {
-            if (lane == __ffsll(hit) - 1) answer(mine, (float)log(mw / all));
+            if (lane == __ffsll(hit) - 1) answer(mine, mw, all);
             last = -1;
             return true;
         }
         const u64 some = __ballot(own > 0);
-        if (some) { const int l = 63 - __clzll(some); last = __shfl(lastc, l); last_w = __shfl(lastw, l); }
-        run += __shfl(p, 63);
+        if (some) { const int l = 63 - __clzll(some); last = lane_at(lastc, l); last_w = lane_at(lastw, l); }
+        run += lane_at(p, 63);
         return false;
     });
-    if (lane == 0 && last >= 0) answer(last, (float)log(last_w / all));
+    if (lane == 0 && last >= 0) answer(last, last_w, all);
     if (wave == 0 && (at == 0 || at == cells - 1)) {
         const bool here = tid < row.sp.edge && (tid < row.sp.head) == (at == 0);
         const int j = here ? row.sp.edge_at(tid) : 0;
         const double w = here ? share(row.xe, j) : 0.0;
-        double p = w;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(p, d); if (lane >= d) p += o; }
+        const double p = wave_scan(w);
         const u64 hit = __ballot(w > 0 && before + p > target), some = __ballot(w > 0);
-        if (lane == (hit ? __ffsll(hit) - 1 : 63 - __clzll(some))) answer(j, (float)log(w / all));
+        if (lane == (hit ? __ffsll(hit) - 1 : 63 - __clzll(some))) answer(j, w, all);
     }
 }
 

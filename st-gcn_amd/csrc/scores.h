@@ -101,8 +101,10 @@ template <int N> __device__ __forceinline__ void exp2_64(const double* y, double
                              0.055504108664760424, 0.2402265069581299, 0.6931471805599453, 1.0};
 #pragma unroll
     for (int q = 0; q < 9; ++q) {
+        double c = Q[q];
+        asm volatile("" : "+s"(c));               // in scalar registers, here: else all are carried along, in 20 vector registers
 #pragma unroll
-        for (int e = 0; e < N; ++e) p[e] = fma(p[e], f[e], Q[q]);
+        for (int e = 0; e < N; ++e) p[e] = fma(p[e], f[e], c);
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) out[e] = ldexp(p[e], n[e]);
@@ -181,6 +183,30 @@ __device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {
     v = dpp_add<0x143, 0xC>(v);
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63);
     return (unsigned long long)hi << 32 | lo;
+}
+
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true); }
+// The sum over this lane and those below it: the same steps, before the last lane's is handed to all.
+template <typename V> __device__ __forceinline__ V wave_scan(V v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xF, false);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    v = dpp_max<0x143, 0xC>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Groups of L lanes: a whole wave (64), or a row of 16 (four groups side by side, for which one instruction serves all four).
