@@ -316,20 +316,24 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int at = b * G * NB + i * G + tid;
-            to[i] = at < v1 ? load_vec(x, sp.vec_at(at)) : neg_inf_vec<T>();
+            to[i] = load_vec(x, sp.vec_at(min(at, v1 - 1)));           // always: the last vector in the place of one beyond it
         }
     };
-    load(b0, nx);
+    if (v1 > 0) load(b0, nx);
 
     for (int b = b0; b < b1 || b == b0; ++b) {
         float f[PER];
+        if ((b + 1) * G * NB > v1) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) if (b * G * NB + i * G + tid >= v1) nx[i] = neg_inf_vec<T>();
+        }
 #pragma unroll
         for (int i = 0; i < NB; ++i) unpack16<T>(nx[i], f + i * VEC);
         if (b + 1 < b1) load(b + 1, nx);
-        float top = f[0];
-#pragma unroll
-        for (int e = 1; e < PER; ++e) top = fmaxf(top, f[e]);
         if (b == b0) {
+            float top = f[0];
+#pragma unroll
+            for (int e = 1; e < PER; ++e) top = fmaxf(top, f[e]);
             // a bound that k scores of this batch reach, to 16 bits of the key: from 64 W maxima of threads, or 64 W NB of vectors
             const bool fine = W > 1 && k > 64;
             if (fine) {
@@ -353,17 +357,21 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
         // only scores beyond the bound's are earlier in the order.  lim is NaN while there is no bound.
         const float lim = sh.lim;
         u64 mask[PER];                             // lanes whose score e may be among the first, in scalar registers
+        u64 any = 0;
         int found = 0;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             mask[e] = __ballot(!(f[e] <= lim) && b * G * NB + (e / VEC) * G + tid < v1);
-            found += __popcll(mask[e]);
+            any |= mask[e];
+        }
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) found += __popcll(mask[e]);
         }
         const int before = have;
         int slot = deal_slots<W>(sh, tid, have, turn, found);
         if (have <= Shared<W>::CAP) {
             if (found) {
-                top = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
                     if (mask[e]) {
@@ -373,7 +381,6 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
                         }
                         slot += __popcll(mask[e]);
                     }
-                    top = fmaxf(top, f[e]);
                 }
             }
             if (have > buffer_limit(k)) compact<T, W>(sh, tid, have, k, rest, c);
@@ -384,11 +391,17 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
             auto cls = [&](int e) { return sp.vec_at(b * G * NB + (e / VEC) * G + tid) + e % VEC; };
             have = before;
             const uint32_t kept = offer<T, W>(sh, tid, have, turn, k, pending, [&](int e) { return load_score(x, cls(e)); }, cls, rest, c);
-            top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < PER; ++e) { if (kept >> e & 1) f[e] = -INFINITY; top = fmaxf(top, f[e]); }
+            for (int e = 0; e < PER; ++e) if (kept >> e & 1) f[e] = -INFINITY;
         }
-        rest.raise(top, c);
+        // What is left is not beyond lim: with lim less than 60 octaves above the running maximum nothing can overflow, and
+        // the batch's maximum need not be known.
+        if (!((lim - rest.m) * c < 60.f)) {
+            float top = f[0];
+#pragma unroll
+            for (int e = 1; e < PER; ++e) top = fmaxf(top, f[e]);
+            rest.raise(top, c);
+        }
         const float ref = rest.m == -INFINITY ? 0.f : rest.m;
 #pragma unroll
         for (int e = 0; e < PER; ++e) rest.s += exp2_32((f[e] - ref) * c);
