@@ -365,6 +365,34 @@ def test_sample_labels_special_rows(rt, n, dt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n", [600, 9001, 40003])
+def test_sample_labels_crowded_rows(rt, n, dt):
+    """Thousands of scores in a small part of the row's range, around one value, two, or all over a bin: the borders take
+    several rounds."""
+    g = torch.Generator().manual_seed(n)
+    noise = torch.randn(n, generator=g)
+    rows = [noise * 1e-3, noise * 1e-3 - 7, 2 + noise * 1e-6, torch.where(torch.arange(n) % 3 == 0, 4 + noise * 1e-4, -4 + noise * 1e-4),
+            torch.where(torch.arange(n) % 2 == 0, noise * 1e-3, -math.inf), noise.abs() * -1e-30]
+    x = torch.stack(rows)
+    x[0, 5], x[1, n - 1], x[3, 0] = 25.0, 1.0, 4.5
+    x = x.to(dt).to(DEV)
+    for j, (k, p, q) in enumerate([(0, 0.9, 0.0), (0, 0.3, 0.0), (n // 3, 1.0, 0.0), (n // 2, 0.5, 0.0), (0, 0.99, 0.2), (n - 7, 0.97, 1e-3), (n // 4, 1.0, 0.999)]):
+        check_sample(rt[0], x, uniforms(len(rows), 7 * n + j), k=k, p=p, q=q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,dt", [(270, 9001, torch.float32), (260, 16500, torch.bfloat16)])
+def test_sample_labels_many_rows(rt, rows, n, dt):
+    """Enough rows that each gets fewer waves, every row with cuts of its own."""
+    x = scores(rows, n, dt, n, sigma=2.5, masked=n // 9, offset=3, gap=5)
+    g = torch.Generator().manual_seed(rows)
+    pick = lambda *v: torch.tensor(v, dtype=torch.float32)[torch.randint(0, len(v), (rows,), generator=g)].to(DEV)         # noqa: E731
+    check_sample(rt[0], x, uniforms(rows, rows), T=pick(0.0, 0.5, 1.0, 1.7), k=pick(0, 1, 40, 300, 4000).int(), p=pick(0.2, 0.9, 0.999, 1.0),
+                 q=pick(0.0, 0.0, 0.01, 1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("n", [400, 9001])
 def test_sample_labels_parameters_per_row(rt, n, dt):
     """Every combination of cuts in one batch, and parameters out of range, each row by itself."""
