@@ -8,6 +8,11 @@
 // comes from the first batch: k of its threads' (or vectors') maxima reach it, so about k to 2k of the batch's scores
 // do.  When more than a few k have gathered, the k-th of them becomes the bound.  A score that is not kept, or is dropped
 // from the buffer, enters the sum of the rest at once, under a running maximum, so nothing is read twice.
+//
+// Many rows are bound by their instructions (a score costs a conversion, a comparison and a 2^y), then by what a row costs
+// by itself (the first bound, ranking the answer): 4096 x 65536 bf16, k 64, 204 us, 2.6 TB/s, of which k 1 leaves 160.  Few
+// rows are cut into pieces, or one compute unit would read each alone (4 x 131071 float32, k 128: 170 us in one piece, 29
+// in 25, half of it the join).
 #include "scores.h"
 
 namespace {
