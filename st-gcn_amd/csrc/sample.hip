@@ -837,7 +837,7 @@ template <typename T> void launch(const SampleArgs& a, int rows, hipStream_t s) 
 extern "C" int stgcn_sample_labels(int dtype, const void* logits, size_t row_stride, const float* u, const float* temperatures, float temperature,
                                    const int* top_ks, int top_k, const float* top_ps, float top_p, const float* min_ps, float min_p,
                                    int64_t* labels, float* logp, int rows, int ncls, void* stream) {
-    if (!logits || !u || !labels || !logp || rows < 1 || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls) return STGCN_ERR_ARG;
+    if (!logits || !u || !labels || !logp || rows < 1 || rows >= (1 << 24) || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls) return STGCN_ERR_ARG;
     SampleArgs a = {logits, row_stride, u, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p, (long long*)labels, logp, ncls};
     if (dtype == STGCN_BF16) launch<bf16>(a, rows, (hipStream_t)stream);
     else if (dtype == STGCN_F32) launch<float>(a, rows, (hipStream_t)stream);

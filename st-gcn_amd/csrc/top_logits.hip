@@ -510,14 +510,14 @@ static int top_pieces(int rows, int ncls, int k) {
 static size_t top_workspace(int rows, int pieces, int k) { return pieces == 1 ? 0 : (size_t)rows * pieces * ((size_t)buffer_limit(k) * 8 + 8); }
 
 extern "C" int stgcn_top_logits_workspace(int rows, int ncls, int k, size_t* bytes) {
-    if (!bytes || rows < 1 || ncls < 1 || ncls > (1 << 20) || k < 1 || k > MAX_K || k > ncls) return STGCN_ERR_ARG;
+    if (!bytes || rows < 1 || rows >= (1 << 24) || ncls < 1 || ncls > (1 << 20) || k < 1 || k > MAX_K || k > ncls) return STGCN_ERR_ARG;
     *bytes = top_workspace(rows, top_pieces(rows, ncls, k), k);
     return STGCN_OK;
 }
 
 extern "C" int stgcn_top_logits(int dtype, const void* logits, size_t row_stride, int rows, int ncls, int k, double temperature,
                                 float* values, int64_t* indices, float* rest, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!logits || !values || !indices || !rest || rows < 1 || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls || k < 1 || k > MAX_K
+    if (!logits || !values || !indices || !rest || rows < 1 || rows >= (1 << 24) || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls || k < 1 || k > MAX_K
         || k > ncls || !(temperature > 0.0) || !(temperature < 1e30) || (dtype != STGCN_F32 && dtype != STGCN_BF16)) return STGCN_ERR_ARG;
     const int pieces = top_pieces(rows, ncls, k);
     if (pieces > 1 && (!workspace || workspace_bytes < top_workspace(rows, pieces, k))) return STGCN_ERR_WORKSPACE;

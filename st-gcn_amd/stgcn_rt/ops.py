@@ -502,8 +502,8 @@ def _check_scores(x, name="logits"):
     L.dtype_code(x.dtype)
     if not 1 <= x.shape[1] <= MAX_CLASSES:
         raise ValueError("%s: 1 to %d classes, got %d" % (name, MAX_CLASSES, x.shape[1]))
-    if x.shape[0] >= 1 << 31:
-        raise ValueError("%s: fewer than 2^31 rows, got %d" % (name, x.shape[0]))
+    if x.shape[0] >= 1 << 24:                       # 2^32 threads are more than a launch holds
+        raise ValueError("%s: fewer than 2^24 rows, got %d" % (name, x.shape[0]))
     if x.is_contiguous():
         return x
     if (x.stride(1) == 1 or x.shape[1] == 1) and (x.shape[0] < 2 or x.stride(0) >= x.shape[1]):

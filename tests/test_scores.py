@@ -601,6 +601,8 @@ def test_refusals():
             (V, "got k = 257", lambda: F.top_logits(torch.zeros(1, 400), 257)),
             (V, "classes", lambda: F.top_logits(torch.zeros(1, 0), 1)),
             (V, "classes", lambda: F.top_logits(torch.zeros(1, (1 << 20) + 1), 1)),
+            (V, "2.24 rows", lambda: F.top_logits(x[:1].expand(1 << 24, 10), 3)),
+            (V, "2.24 rows", lambda: F.sample_labels(x[:1].expand(1 << 24, 10), u[:1].expand(1 << 24))),
             (V, "temperature", lambda: F.top_logits(x, 3, temperature=0.0)),
             (V, "temperature", lambda: F.top_logits(x, 3, temperature=math.nan)),
             (R, "no CPU fallback", lambda: F.top_logits(x, 3)),
@@ -644,6 +646,7 @@ def test_c_entry_points_refuse():
     top = lambda dt=0, x=p, st=10, r=4, n=10, k=3, T=1.0: l.stgcn_top_logits(dt, x, st, r, n, k, T, p, p, p, None, 0, None)   # noqa: E731
     for kw in (dict(dt=7), dict(x=None), dict(st=9), dict(r=0), dict(n=0), dict(n=1 << 21, st=1 << 21), dict(k=0), dict(k=11), dict(T=0.0), dict(T=math.nan)):
         assert top(**kw) == 1, kw
+    assert top(r=1 << 24) == 1 and top(r=1 << 30) == 1
     assert top(n=100000, st=100000) == 3                       # few rows want a workspace
     need = ctypes.c_size_t(7)
     assert l.stgcn_top_logits_workspace(4, 100000, 3, ctypes.addressof(need)) == 0 and need.value > 0
