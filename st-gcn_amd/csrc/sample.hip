@@ -265,9 +265,8 @@ template <typename T> struct List {
     }
     __device__ __forceinline__ u64 all() const { return mass([](u64) { return true; }); }
     static __device__ __forceinline__ uint32_t key(u64 e) { return (uint32_t)(e >> (32 + SHIFT)); }
-    // The last place that the sum of the entries from the first one on, enough(place) says whether up to a place, needs.
-    template <typename F> __device__ __forceinline__ Cut border(const Cut& was, F enough) const {
-        const uint32_t v = last_enough(lo, hi, [&](uint32_t mid) { return enough((u64)mid << (32 + SHIFT)); });
+    // The border among the entries of key v: enough(place) says whether the entries up to a place are.
+    template <typename F> __device__ __forceinline__ Cut border_at(uint32_t v, const Cut& was, F enough) const {
         const u64 first = (u64)(ET<T>::IS_BF16 ? v << 16 | ((v & 0x8000u) ? 0u : 0xFFFFu) : v) << 32;
         Cut to = {place_score(first), n};
         if (count([&](u64 e) { return (e ^ first) >> 32 == 0; }) > 1)
@@ -276,10 +275,56 @@ template <typename T> struct List {
         return to;
     }
     __device__ __forceinline__ Cut cut_count(int k, const Cut& was) const {
-        return border(was, [&](u64 from) { return count([&](u64 e) { return e >= from; }) >= k; });
+        auto enough = [&](u64 from) { return count([&](u64 e) { return e >= from; }) >= k; };
+        return border_at(last_enough(lo, hi, [&](uint32_t mid) { return enough((u64)mid << (32 + SHIFT)); }), was, enough);
     }
-    __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Cut& was) const {
-        return border(was, [&](u64 from) { return above + mass([&](u64 e) { return e >= from; }) >= target; });
+    // The place at which, after `above`, the target is reached.  Bisected only until at most 32 entries are left, which are
+    // then compared one by one (32 bits of a key to the end: 64 x 400 float32, top-p 0.9: 13.4 us instead of 15.2).  Overwrites list.
+    __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Cut& was, u64* list) const {
+        const int lane = threadIdx.x & 63;
+        const u64 need = target - above;
+        uint32_t l = lo, h = hi;
+        int left = c, beyond = 0;                  // entries with keys from l on, and beyond h; the mass of the latter
+        u64 m_beyond = 0;
+#pragma unroll 1
+        while (l < h && left - beyond > 32) {
+            const uint32_t mid = l + (h - l + 1) / 2;
+            u64 m = 0;
+            int k = 0;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (64 * i < c) {
+                    const bool in = key(lp[i]) >= mid;
+                    m += in ? lw[i] : 0;
+                    k += __popcll(__ballot(in));
+                }
+            m = wave_sum(m);
+            if (m >= need) { l = mid; left = k; } else { h = mid - 1; beyond = k; m_beyond = m; }
+        }
+        if (l == h) return border_at(l, was, [&](u64 from) { return mass([&](u64 e) { return e >= from; }) >= need; });
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (64 * i < c) {
+                const bool in = lp[i] && key(lp[i]) >= l && key(lp[i]) <= h;
+                const u64 b = __ballot(in);
+                if (in) { const int to = at + lanes_below(b); list[to] = lp[i]; list[CAP / 2 + to] = lw[i]; }
+                at += __popcll(b);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        const u64 e = lane < at ? list[lane] : 0, f = lane < at ? list[CAP / 2 + lane] : 0;
+        u64 front = m_beyond;
+#pragma unroll 1
+        for (int i = 0; i < at; i += 4) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) front += lane_at(e, i + d) > e ? lane_at(f, i + d) : 0;      // lanes from `at` on hold 0
+        }
+        const u64 hit = __ballot(e && front < need && front + f >= need);
+        const u64 last = lane_at(e, hit ? __ffsll(hit) - 1 : 0);
+        Cut to = {place_score(last), place_class(last)};
+        if (to.xt == was.xt) to.ti = min(to.ti, was.ti);
+        return to;
     }
     __device__ __forceinline__ void keep(const Cut& cut) {
         const u64 last = place(score_key(cut.xt), cut.ti);
@@ -696,7 +741,7 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
                 if (pass ? !mass : k < c) { cut = list.cut_count((int)(target - above), cut); list.keep(cut); }
                 if (pass ? mass : p < 1.f) {
                     if (!pass) target = (u64)ceil((double)p * (double)list.all());
-                    cut = list.cut_mass(above, target, cut);
+                    cut = list.cut_mass(above, target, cut, sh.list);
                     list.keep(cut);
                 }
                 list.drop_under();
