@@ -666,7 +666,7 @@ def test_c_entry_points_refuse():
 
 
 def test_plain_forms_agree_with_the_definitions():
-    """The checker itself: whole-list distillation is torch's KL divergence, its gradient torch's."""
+    """The oracle itself: whole-list distillation is torch's KL divergence, its gradient torch's."""
     g = torch.Generator().manual_seed(0)
     t, s = torch.randn(3, 20, generator=g, dtype=torch.float64), torch.randn(3, 20, generator=g, dtype=torch.float64)
     v, i, rest = O.top_logits(t, 20, 2.0)
