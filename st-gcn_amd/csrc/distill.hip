@@ -54,19 +54,40 @@ template <int K> struct Listed {                // K: entries at most
 };
 __device__ __forceinline__ void wave_sync() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
 
-// Classes and student scores of the entries (loads only: issued before the row's own).
-template <typename T, int L, int K> __device__ __forceinline__ void listed_load(const DistillArgs& a, size_t r, const T* x, int lane, Listed<K>& l) {
+// The entries as they come from the teacher: read ahead of the row, whose loads then need not be waited for (they return in
+// order), and always, the last entry in the place of one beyond it.
+template <int L, int K> struct Entries {
+    long long i[K / L]; float t[K / L];
+    __device__ __forceinline__ void load(const DistillArgs& a, size_t r, int lane) {
+#pragma unroll
+        for (int c = 0; c < K / L; ++c) {
+            const size_t at = r * a.k + min(lane + c * L, a.k - 1);
+            i[c] = a.idx[at];
+            t[c] = a.val[at];
+        }
+    }
+};
+
+// Classes and student scores of the entries.
+template <typename T, int L, int K> __device__ __forceinline__ void listed_load(const DistillArgs& a, const Entries<L, K>& from, const T* x, int lane, Listed<K>& l) {
     bool bad = false, has = false;
-    for (int e = lane; e < a.k; e += L) {
-        const long long i = a.idx[r * a.k + e];
-        const float t = a.val[r * a.k + e];
-        const bool in = i >= 0 && i < a.n;
-        l.cls[e] = in ? (int)i : -1;
-        l.x[e] = in ? load_score(x, (size_t)i) : -INFINITY;
-        bad |= i >= a.n || (in && !(t < INFINITY));
-        const float u = in && t < INFINITY ? t : -INFINITY;
-        l.p[e] = (double)u;
-        has |= u > -INFINITY;
+    float s[K / L];
+#pragma unroll
+    for (int c = 0; c < K / L; ++c) s[c] = load_score(x, (size_t)(from.i[c] >= 0 && from.i[c] < a.n ? from.i[c] : 0));
+#pragma unroll
+    for (int c = 0; c < K / L; ++c) {
+        const int e = lane + c * L;
+        if (e < a.k) {
+            const long long i = from.i[c];
+            const float t = from.t[c];
+            const bool in = i >= 0 && i < a.n;
+            l.cls[e] = in ? (int)i : -1;
+            l.x[e] = in ? s[c] : -INFINITY;
+            bad |= i >= a.n || (in && !(t < INFINITY));
+            const float u = in && t < INFINITY ? t : -INFINITY;
+            l.p[e] = (double)u;
+            has |= u > -INFINITY;
+        }
     }
     const int flags = (group_any<L>(has) && a.w < 1.0 ? 1 : 0) | (group_any<L>(bad) ? 2 : 0);
     if (lane == 0) l.flags = flags;
@@ -235,11 +256,15 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
     const long long y = a.labels ? a.labels[r] : -1;
     const bool hard = a.w > 0.0 && y >= 0 && y < n;
     i32x4 v[NV];
+    Entries<L, K> entries;
+    if (lead) entries.load(a, r, lane);
+    if (sp.nvec > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(i * G + tid)) : neg_inf_vec<T>();
+        for (int i = 0; i < NV; ++i) v[i] = load_vec(x, sp.vec_at(min(i * G + tid, sp.nvec - 1)));
+    }
     float xe = tid < sp.edge ? load_score(x, sp.edge_at(tid)) : -INFINITY, xy = 0.f;
     if (lead) {
-        listed_load<T, L>(a, r, x, lane, l);
+        listed_load<T>(a, entries, x, lane, l);
         if (hard) xy = load_score(x, (size_t)y);
     }
     for (int i = tid; i < WORDS; i += G) bits[i] = 0;
@@ -267,6 +292,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+        if (i * G + tid >= sp.nvec) v[i] = neg_inf_vec<T>();
         if (i * G < sp.nvec) {
             const uint32_t b = vec_bits<T>(bits, i * G + tid);
             if (b) drop_listed<T>(v[i], b);
@@ -384,9 +410,11 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void distill_stream_kernel
 #pragma unroll
         for (int i = 0; i < NB; ++i) nx[i] = v0 + i * G + tid < sp.nvec ? load_vec(x, sp.vec_at(v0 + i * G + tid)) : neg_inf_vec<T>();
     };
+    Entries<64, MAX_K> entries;
+    if (lead) entries.load(a, r, lane);
     load(0);
     if (lead) {
-        listed_load<T, 64>(a, r, x, lane, l);
+        listed_load<T>(a, entries, x, lane, l);
         if (lane == 0 && a.w > 0.0 && y >= n) l.flags |= 2;
         wave_sync();
         listed_sums<TWO, 64>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
