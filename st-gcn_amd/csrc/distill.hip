@@ -12,8 +12,8 @@
 // carries nearly all of the mass would leave nothing of the difference but rounding.
 //
 // Bound by memory where rows are wide: loss and gradient in one pass with the row in registers move what a copy moves, at a
-// copy's rate (8192 x 65536 bf16, 414 us, 5.2 TB/s).  Narrow rows are bound by what a row costs whatever its width, so four
-// share a wave (16384 x 400 float32: 19 us, of 6 to 10 for the bytes).
+// copy's rate (8192 x 65536 bf16, 405 us, 5.3 TB/s).  Narrow rows are bound by what a row costs whatever its width, so four
+// share a wave (16384 x 400 float32: 20 us, of 6 to 10 for the bytes).
 #include "scores.h"
 
 namespace {
