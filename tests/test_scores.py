@@ -381,7 +381,7 @@ def test_sample_labels_crowded_rows(rt, n, dt):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,n,dt", [(270, 9001, torch.float32), (260, 16500, torch.bfloat16)])
+@pytest.mark.parametrize("rows,n,dt", [(270, 9001, torch.float32), (260, 16500, torch.bfloat16), (300, 3001, torch.float32)])
 def test_sample_labels_many_rows(rt, rows, n, dt):
     """Enough rows that each gets fewer waves, every row with cuts of its own."""
     x = scores(rows, n, dt, n, sigma=2.5, masked=n // 9, offset=3, gap=5)
