@@ -15,6 +15,7 @@
 // copy's rate (8192 x 65536 bf16, 405 us, 5.3 TB/s).  Narrow rows are bound by what a row costs whatever its width, so four
 // share a wave (16384 x 400 float32: 20 us, of 6 to 10 for the bytes).
 #include "scores.h"
+#include "listed_map.h"
 
 namespace {
 
@@ -161,9 +162,7 @@ template <bool TWO, int L, int K> __device__ __forceinline__ void listed_merge(c
     wave_sync();
 }
 
-// ---- bit map of the listed classes -----------------------------------------------------------------------------------
-// Bit BIT0 + (class - base): a vector's bits lie within one byte (base = the first whole vector's class, or a vector's).
-constexpr int BIT0 = 16;
+// ---- bit map of the listed classes (listed_map.h) --------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ uint32_t vec_bits(const uint32_t* bits, int v) {
     const int b = BIT0 + v * ET<T>::VEC;
     const uint32_t byte = ((const uint8_t*)bits)[b >> 3];
@@ -382,11 +381,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
 
 // The loss alone, which needs no score twice: a row goes by in batches of four vectors a thread, with the next batch on its
 // way, every thread with a running maximum and sums relative to it.  Bit map of SEG classes at a time.
-constexpr int SEG = 131072;
 template <typename T, int W, bool TWO>
 __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void distill_stream_kernel(DistillArgs a) {
-    constexpr int VEC = ET<T>::VEC, G = W * 64, NB = 4, BATCHES = SEG / VEC / (G * NB), WORDS = (SEG + 2 * BIT0 + 31) / 32;
-    __shared__ uint32_t bits[WORDS];
+    constexpr int VEC = ET<T>::VEC, G = W * 64, NB = 4, BATCHES = SEG / VEC / (G * NB);
+    __shared__ uint32_t bits[SEG_WORDS];
     __shared__ Listed<MAX_K> l;
     __shared__ double rsum[2][W];
     __shared__ float rmax[W];
@@ -420,7 +418,7 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void distill_stream_kernel
         listed_sums<TWO, 64>(a, lane, a.rest ? a.rest[r] : -INFINITY, l);
         if (hard) xy = load_score(x, (size_t)y);
     }
-    const int some = min(n, SEG) / 32 + 2;         // words of the bit map that are looked at
+    const int some = segment_words(n);             // words of the bit map that are looked at
     for (int v0 = 0; v0 == 0 || v0 < sp.nvec; v0 += G * NB * BATCHES) {
         const int base = sp.vec_at(v0);            // the segment's first class; the row's ends go with the first segment
         __syncthreads();

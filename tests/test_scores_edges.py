@@ -1,0 +1,125 @@
+"""Operators over class scores where their formulas, maps and sums reach an end: wide gaps between scores, NaN in every
+place, rows longer than one segment of the bit map, long sums, infinite incoming gradients.  Tolerances as in
+tests/test_scores.py, derived at each check."""
+import os
+import subprocess
+
+import pytest
+import torch
+
+from oracle import scores_oracle as O
+from tests.test_scores import DEV, U, eps_sum, half_step, rt, scores, teacher_lists  # noqa: F401  (rt: a fixture)
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "st-gcn_amd", "csrc")
+
+
+# ---- bit map of the listed classes (CPU) ---------------------------------------------------------------------------
+
+MAP = """
+#include "%s/listed_map.h"
+#include <cstdio>
+int main() {
+    long bad = 0;
+    for (int n = 1; n <= 1 << 20; ++n) {
+        const int some = segment_words(n), last = n < SEG ? n - 1 : SEG - 1;     // words cleared; last class of a segment from its base on
+        if (some > SEG_WORDS) ++bad;                                            // cleared beyond the map
+        if ((BIT0 + last) / 32 >= some) ++bad;                                  // looked at, not cleared
+    }
+    printf("%%ld %%d", bad, (int)(SEG_WORDS * 4 >= (BIT0 + SEG + 7) / 8));       // the bytes of every vector of a segment are the map's
+}
+"""
+
+
+def test_the_bit_map_of_a_segment_holds_what_is_cleared_and_read(tmp_path):
+    src, exe = tmp_path / "map.cpp", tmp_path / "map"
+    src.write_text(MAP % CSRC)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", str(src), "-o", str(exe)])
+    assert subprocess.check_output([str(exe)], text=True) == "0 1"
+
+
+# ---- distillation over selected rows -------------------------------------------------------------------------------
+
+def row_parts(x, val, idx, rho, label, T, w, es):
+    """(sizes of a gradient's parts [n], tolerance of the loss) of one live row x (float64).  The loss: log S and log S_r enter
+    with weight 1 and p_r (es each); the listed classes' z, and log S_r's own maximum, with the rounding of c (2^-24)."""
+    x = x - x.max()
+    q, size = torch.zeros_like(x), 0.0
+    tea = O.teacher(val, idx, rho, T) if w < 1 else None
+    if tea is not None:
+        z = x / T
+        S = O.lse(z)
+        other = torch.ones(x.numel(), dtype=torch.bool)
+        other[tea[2]] = False
+        So = O.lse(z[other])
+        qz = torch.exp(z - S)
+        q += (1 - w) * T * qz
+        if tea[1] > 0 and So > -float("inf"):
+            q[other] += (1 - w) * T * tea[1] * torch.exp(z[other] - So)
+            size += (1 - w) * T * T * tea[1] * (abs(float(z[other].max())) * U + es)
+        for i, p in tea[0]:
+            q[i] += (1 - w) * T * p
+            size += (1 - w) * T * T * p * abs(float(z[i])) * U
+        size += (1 - w) * T * T * es
+    if w > 0 and label is not None and label >= 0:
+        q += w * torch.exp(x - O.lse(x))
+        q[label] += w
+        size += w * (es + abs(float(x[label])) * U)
+    return q, size
+
+
+def close(got, want, tol, what):
+    got, want = got.detach().cpu().double(), want.double()
+    nan, inf = torch.isnan(want), torch.isinf(want)
+    assert torch.equal(torch.isnan(got), nan), (what, got, want)
+    assert torch.equal(got[inf], want[inf]), (what, got, want)
+    ok = ~(nan | inf)
+    bad = ((got - want).abs() > torch.broadcast_to(tol, want.shape)) & ok
+    assert not bool(bad.any()), (what, got[bad][:5], want[bad][:5], torch.broadcast_to(tol, want.shape)[bad][:5])
+
+
+def check_rows(rt, x, val, idx, rest, labels, T, w, sel=None):
+    """Losses and gradients of the rows `sel` (all): the loss with its backward, and the pair."""
+    F, P = rt
+    rows, n = x.shape
+    sel = list(range(rows)) if sel is None else sel
+    more = dict(rest=rest, labels=labels, temperature=T, label_weight=w)
+    leaf = x.detach().requires_grad_(True)
+    loss = F.distillation(leaf, val, idx, reduction="none", **more)
+    (dx,) = torch.autograd.grad(loss, leaf, torch.full((rows,), -1.25, device=DEV))
+    _, pair = P.distillation(x, val, idx, reduction="sum", **more)
+    got, dx, pair = loss[sel].detach().cpu(), dx[sel].cpu(), pair[sel].cpu()
+    xs, val, idx = x[sel].detach().float().cpu(), val[sel].cpu(), idx[sel].cpu()
+    rest, labels = (None if t is None else t[sel].cpu() for t in (rest, labels))
+    L, G = O.distill(xs, val, idx, rest, labels, T, w)
+    es = eps_sum(xs, T)
+    e1 = es + (8 + (es - 2.0 ** -23) / U) * U
+    hs, flush = half_step(x.dtype), 2.0 ** -125 * max(1.0, T)         # e, and its product with a factor below 2 T, may be flushed
+    for r in range(len(sel)):
+        q, size = torch.zeros(n, dtype=torch.float64), 0.0
+        if bool(torch.isfinite(L[r])) and float(xs[r].max()) > -float("inf"):
+            q, size = row_parts(xs[r].double(), val[r], idx[r], None if rest is None else float(rest[r]), None if labels is None else int(labels[r]), T, w, es)
+        what = (x.dtype, rows, n, T, w, "row", sel[r])
+        close(got[r], L[r], torch.tensor(size + U * (abs(float(L[r])) if bool(torch.isfinite(L[r])) else 0.0) + 1e-12), what + ("loss",))
+        for g, f in ((dx, -1.25), (pair, 1.0)):
+            close(g[r], G[r] * f, q * e1 * abs(f) + hs * torch.nan_to_num(G[r] * f).abs() + flush, what + ("gradient", f))
+
+
+DTS = pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("rows,n", [(513, 140001), (1, 270000), (3, 131072)])
+def test_distillation_over_several_segments(rt, rows, n, dt):
+    """Classes on both sides of every border of the bit map, with the same class in the list twice."""
+    x = scores(rows, n, dt, n, offset=3, gap=2)
+    val, idx, rest = teacher_lists(x[:3], 12, 2.0, 1)
+    most = torch.tensor([131060, 131071, n - 1, min(n - 1, 131072), min(n - 1, 131080), min(n - 2, 262143), 0, 5], device=DEV)
+    idx[:, 4:] = most
+    val, idx, rest = (torch.cat([t] * (rows // t.shape[0] + 1))[:rows].contiguous() for t in (val, idx, rest))
+    labels = torch.arange(rows, device=DEV) * 251 % n
+    labels[0] = 131071
+    sel = sorted({0, rows // 2, rows - 1})
+    for T, w in ((2.0, 0.3), (1.0, 0.0)):
+        print("segments", rows, n, dt, T, w, flush=True)
+        check_rows(rt, x, val, idx, rest, labels, T, w, sel)
