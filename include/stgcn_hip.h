@@ -262,7 +262,7 @@ int stgcn_top_logits_workspace(int rows, int ncls, int k, size_t* bytes);      /
  * A row without an entry has no first term, without a label no second; with neither, or with every logit -inf, it is 0
  * and so is its gradient.  Classes >= ncls and teacher scores that are NaN or +inf make the row's loss and gradient NaN.
  * reduction 0: loss [rows]; 1: loss [1] = mean over all rows; 2: loss [1] = sum (1 and 2 add up loss_rows, double [rows],
- * in a fixed order).  stats [rows][4] and probs [rows][k] are what the gradient needs. */
+ * in a fixed order).  stats [rows][6] and probs [rows][k] are what the gradient needs. */
 int stgcn_distill_fwd(int dtype, const void* logits, size_t row_stride, const float* values, const int64_t* indices,
                       const float* rest, const int64_t* labels, int rows, int ncls, int k, double temperature, double label_weight,
                       int reduction, float* loss, double* loss_rows, float* stats, float* probs, void* stream);

@@ -70,13 +70,12 @@ def distill_row(x, val, idx, rho, label, T, w):
         for i, p in entries:
             if p > 0:
                 kl += p * (math.log(p) - float(z[i]) + S) if float(z[i]) > -math.inf else math.inf
-        f = torch.ones(n, dtype=torch.float64)
         if pr > 0:
             So = lse(z[other])
             kl += pr * (math.log(pr) - So + S) if So > -math.inf else math.inf
             if So > -math.inf:
-                f[other] = 1 - pr * math.exp(S - So)
-        g += (1 - w) * T * q * f
+                q[other] -= pr * torch.exp(z[other] - So)
+        g += (1 - w) * T * q
         for i, p in entries:
             g[i] -= (1 - w) * T * p
         loss += (1 - w) * T * T * kl

@@ -9,7 +9,10 @@
 //   d loss / d x_j = (1 - w) T e^{z_j} (1/S - [j not listed] p_r/S_r) - (1 - w) T sum_{k: i_k = j} p_k
 //                    + w (e^{x_j} / sum e^x - [j = y])
 // S_r is summed without the listed classes (a bit map of the row in LDS) instead of as S - S_l: a teacher whose list
-// carries nearly all of the mass would leave nothing of the difference but rounding.
+// carries nearly all of the mass would leave nothing of the difference but rounding.  It stays relative to its own largest
+// score m, as do the gradients of its classes: with M the row's largest score and a = e^{(m - M)/T}, the gradient of a class
+// that is not listed is (1 - w) T e^{(x - m)/T} (a/S' - p_r/S_r'), S' relative to M, S_r' to m.  Relative to M, e^z of all of
+// them is 0 in 32 bits from a gap of 87 T on, and p_r with it.
 //
 // Bound by memory where rows are wide: loss and gradient in one pass with the row in registers move what a copy moves, at a
 // copy's rate (8192 x 65536 bf16, 405 us, 5.3 TB/s).  Narrow rows are bound by what a row costs whatever its width, so four
@@ -22,9 +25,10 @@ namespace {
 constexpr int MAX_K = 256;
 constexpr double LOG2E = 1.4426950408889634074, LN2 = 0.6931471805599453094;
 
-// What a row's forward leaves for its gradient: e^{z_j} = 2^{(x_j - xmax) c}, and the factors of the three sums.  xmax is
-// NaN for a row whose gradient is zero whatever it holds.
-struct RowStats { float xmax, gl, gr, g1; };   // gl = (1-w) T / S, gr = (1-w) T (1/S - p_r/S_r), g1 = w / sum e^x
+// What a row's forward leaves for its gradient: the largest score xl of the row, which listed classes are relative to, the
+// largest xr of those that are not listed, which these are relative to, and the factors g of e^{./T} and h of e^. on either
+// side.  xl is NaN for a row whose gradient is zero whatever it holds.
+struct RowStats { float xl, xr, gl, gr, hl, hr; };
 
 struct DistillArgs {
     const void* x; size_t stride;
@@ -169,64 +173,85 @@ template <typename T> __device__ __forceinline__ uint32_t vec_bits(const uint32_
     return ET<T>::IS_BF16 ? byte : (byte >> (b & 7)) & 15u;
 }
 // ---- loss and factors of a row from its sums -------------------------------------------------------------------------
-// sr, s1: sums over the classes that are not listed, relative to their maximum m; joined with the listed ones'.
-struct RowSums { float xmax; double sl, sr, s1; };
+// sr, s1: sums over the classes that are not listed, relative to their maximum m; S and the label's s1 over all of them,
+// relative to the row's maximum.
+struct RowSums { float xmax, m; double S, sr, a, s1, a1; };        // a, a1: 2^{(m - xmax) c}, 2^{(m - xmax) c1}
 template <bool TWO, int K> __device__ __forceinline__ RowSums join_sums(const DistillArgs& a, const Listed<K>& l, float m, double sr, double s1) {
     RowSums s;
     const float both = fmaxf(m, l.xmax);
     s.xmax = both == -INFINITY ? 0.f : both;
+    s.m = m == -INFINITY ? s.xmax : m;
     // a maximum of -inf: its sum is 0 (or NaN) and is taken as it is
-    s.sr = sr * (m == -INFINITY ? 1.0 : (double)exp2_32((m - s.xmax) * a.c));
-    s.sl = l.xmax == -INFINITY ? l.sl : l.sl * (double)exp2_32((l.xmax - s.xmax) * a.c);
-    if constexpr (TWO) s.s1 = s1 * (m == -INFINITY ? 1.0 : (double)exp2_32((m - s.xmax) * a.c1)) + (l.xmax == -INFINITY ? l.sl1 : l.sl1 * (double)exp2_32((l.xmax - s.xmax) * a.c1));
-    else s.s1 = s.sl + s.sr;
+    s.sr = sr;
+    s.a = (double)exp2_32((s.m - s.xmax) * a.c);
+    s.S = sr * s.a + (l.xmax == -INFINITY ? l.sl : l.sl * (double)exp2_32((l.xmax - s.xmax) * a.c));
+    if constexpr (TWO) {
+        s.a1 = (double)exp2_32((s.m - s.xmax) * a.c1);
+        s.s1 = s1 * s.a1 + (l.xmax == -INFINITY ? l.sl1 : l.sl1 * (double)exp2_32((l.xmax - s.xmax) * a.c1));
+    } else { s.a1 = s.a; s.s1 = s.S; }
     return s;
+}
+// A row of one wave or more: its numbers in scalar registers (next to 64 registers of scores others would be spilled).
+template <int L> __device__ __forceinline__ float row_value(float v) {
+    if constexpr (L == 64) return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); else return v;
+}
+template <int L> __device__ __forceinline__ double row_value(double v) { if constexpr (L == 64) return lane_value<64, 0>(v); else return v; }
+template <int L> __device__ __forceinline__ RowSums row_value(const RowSums& s) {
+    return {row_value<L>(s.xmax), row_value<L>(s.m), row_value<L>(s.S), row_value<L>(s.sr), row_value<L>(s.a), row_value<L>(s.s1), row_value<L>(s.a1)};
+}
+template <int L> __device__ __forceinline__ RowStats row_value(const RowStats& s) {
+    return {row_value<L>(s.xl), row_value<L>(s.xr), row_value<L>(s.gl), row_value<L>(s.gr), row_value<L>(s.hl), row_value<L>(s.hr)};
 }
 // In every thread; the loss (three logarithms in 64 bits, a lane each) by one group.
 __device__ __forceinline__ RowStats row_factors(const DistillArgs& a, const RowSums& s, bool hard, int flags, double pr) {
-    const double S = s.sl + s.sr;
     const bool any = flags & 1, bad = flags & 2;
-    RowStats st = {s.xmax, 0.f, 0.f, 0.f};
+    RowStats st = {s.xmax, s.m, 0.f, 0.f, 0.f, 0.f};
     if (any) {
-        const double f = (1.0 - a.w) * a.T, inv = 1.0 / S;
+        const double f = (1.0 - a.w) * a.T, inv = 1.0 / s.S;
         st.gl = (float)(f * inv);
-        st.gr = (float)(f * (inv - (pr > 0 && s.sr > 0 ? pr / s.sr : 0.0)));
+        st.gr = (float)(f * (s.a * inv - (pr > 0 && s.sr > 0 ? pr / s.sr : 0.0)));
     }
-    if (hard) st.g1 = (float)(a.w / s.s1);
-    if (bad || S != S || s.s1 != s.s1) st.gl = st.gr = st.g1 = NAN;
-    if (!bad && ((!any && !hard) || S == 0)) st.xmax = NAN;   // nothing to learn from, or no class to learn: zeros
+    if (hard) { const double h = a.w / s.s1; st.hl = (float)h; st.hr = (float)(h * s.a1); }
+    if (bad || s.S != s.S || s.s1 != s.s1) st.gl = st.gr = st.hl = st.hr = NAN;
+    if (!bad && ((!any && !hard) || s.S == 0)) st.xl = NAN;   // nothing to learn from, or no class to learn: zeros
     return st;
 }
 template <int L, int K> __device__ __forceinline__ double row_loss(const DistillArgs& a, const RowSums& s, const RowStats& st, bool hard, const Listed<K>& l, int lane, float xy) {
-    const double ln = ln_64(lane == 0 ? s.sl + s.sr : lane == 1 ? s.sr : s.s1);
+    double arg = s.s1;
+    const double S = s.S, sr = s.sr;               // read in any case: a choice of members keeps the struct in memory
+    if (lane == 0) arg = S;
+    if (lane == 1) arg = sr;
+    const double ln = ln_64(arg);
     const double lnS = lane_value<L, 0>(ln), lnr = lane_value<L, 1>(ln), ln1 = lane_value<L, 2>(ln);
-    if (st.xmax != st.xmax) return 0.0;
+    if (st.xl != st.xl) return 0.0;
     if (st.gl != st.gl) return NAN;
     double loss = 0;
     if (l.flags & 1) {
-        // z = x / T; the sums are relative to xmax, `cross` to the listed classes' largest score, whose shares add up to 1 - p_r.
-        // (Relative throughout: next to scores of 1e38 a log would vanish.)
+        // z = x / T; the sums are relative to xmax, that of the others to m, `cross` to the listed classes' largest score, whose
+        // shares add up to 1 - p_r.  (Relative throughout: next to scores of 1e38 a log would vanish.)
         double kl = l.own - l.cross + lnS;
         if (l.xmax > -INFINITY) kl += (1.0 - l.pr) * (((double)s.xmax - (double)l.xmax) * (double)a.c * LN2);
-        if (l.pr > 0) kl -= l.pr * lnr;
+        if (l.pr > 0) kl -= l.pr * (lnr + ((double)s.m - (double)s.xmax) * (double)a.c * LN2);
         loss = (1.0 - a.w) * a.T * a.T * kl;
     }
     if (hard) loss += a.w * (ln1 - ((double)xy - (double)s.xmax) * (double)a.c1 * LN2);
     return loss;
 }
 
+// The gradient of a score: of one side's classes, listed or not, relative to that side's reference.
 template <typename T, bool TWO> struct Grad {
-    float m, c, c1, g1;
-    __device__ __forceinline__ float operator()(float x, float gz) const {
+    float m, c, c1, g, h;
+    __device__ __forceinline__ Grad(float m_, float c_, float c1_, float g_, float h_, float up) : m(m_), c(c_), c1(c1_), g((TWO ? g_ : g_ + h_) * up), h(h_ * up) {}
+    __device__ __forceinline__ float operator()(float x) const {
         const float t = x - m, e = exp2_32(t * c);
-        if constexpr (TWO) return fmaf(gz, e, g1 * exp2_32(t * c1)); else return gz * e;   // one temperature: g1 is in gz
+        if constexpr (TWO) return fmaf(g, e, h * exp2_32(t * c1)); else return g * e;      // one temperature: h is in g
     }
 };
-template <typename T, bool TWO> __device__ __forceinline__ i32x4 grad_vec(const i32x4& v, const Grad<T, TWO>& g, float gz) {
+template <typename T, bool TWO> __device__ __forceinline__ i32x4 grad_vec(const i32x4& v, const Grad<T, TWO>& g) {
     float f[ET<T>::VEC];
     unpack16<T>(v, f);
 #pragma unroll
-    for (int j = 0; j < ET<T>::VEC; ++j) f[j] = g(f[j], gz);
+    for (int j = 0; j < ET<T>::VEC; ++j) f[j] = g(f[j]);
     return pack16<T>(f);
 }
 
@@ -330,9 +355,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
 #pragma unroll
         for (int w = 0; w < W; ++w) { sr += rsum[0][w]; if constexpr (TWO) sr1 += rsum[1][w]; }
     }
-    const RowSums sum = join_sums<TWO>(a, l, m, sr, sr1);
-    const RowStats st = row_factors(a, sum, hard, l.flags, l.pr);
-    const bool empty = st.xmax != st.xmax;
+    const RowSums sum = row_value<L>(join_sums<TWO>(a, l, m, sr, sr1));
+    const RowStats st = row_value<L>(row_factors(a, sum, hard, l.flags, l.pr));
+    const bool empty = st.xl != st.xl;
     if (lead) {
         const double loss = row_loss<L>(a, sum, st, hard, l, lane, xy);
         if (lane == 0) {
@@ -344,13 +369,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
         if (lead) for (int e = lane; e < a.k; e += L) a.probs[r * a.k + e] = l.cls[e] >= 0 ? (float)l.p[e] : -1.f;
     } else {
         T* dx = (T*)a.dx + r * (size_t)n;
-        const Grad<T, TWO> g = {empty ? 0.f : st.xmax, a.c, a.c1, st.g1 * a.scale};
-        const float gr = (TWO ? st.gr : st.gr + st.g1) * a.scale, gl = (TWO ? st.gl : st.gl + st.g1) * a.scale;
+        const Grad<T, TWO> g(st.xr, a.c, a.c1, st.gr, st.hr, a.scale);
         const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (i * G + tid < sp.nvec) {
-                i32x4 o = grad_vec<T, TWO>(v[i], g, gr);
+                i32x4 o = grad_vec<T, TWO>(v[i], g);
                 if (empty) o = zero16();
                 const int at = sp.vec_at(i * G + tid);
                 if (same) store_vec(dx, at, o);
@@ -362,19 +386,20 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
                 }
             }
         }
-        if (tid < sp.edge) store_elem(dx, sp.edge_at(tid), empty ? 0.f : g(xe, gr));
+        if (tid < sp.edge) store_elem(dx, sp.edge_at(tid), empty ? 0.f : g(xe));
         group_sync<W>();
         if (lead && !empty) {
+            const Grad<T, TWO> listed(st.xl, a.c, a.c1, st.gl, st.hl, a.scale);
             const float fp = a.fp * a.scale, w = a.w1 * a.scale;
             bool mine = false;
             for (int e = lane; e < a.k; e += L) {
                 const int j = l.cls[e];
                 if (j < 0) continue;
-                float d = g(l.x[e], gl) - fp * (float)l.p[e];
+                float d = listed(l.x[e]) - fp * (float)l.p[e];
                 if (hard && j == (int)y) { d -= w; mine = true; }
                 store_elem(dx, j, d);
             }
-            if (hard && !group_any<L>(mine) && lane == 0) store_elem(dx, (size_t)y, g(xy, gr) - w);
+            if (hard && !group_any<L>(mine) && lane == 0) store_elem(dx, (size_t)y, g(xy) - w);
         }
     }
 }
@@ -513,17 +538,16 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) if (v0 + i * G + tid < sp.nvec) v[i] = load_vec(x, sp.vec_at(v0 + i * G + tid));
     const RowStats st = a.stats[r];
-    const bool empty = st.xmax != st.xmax;
+    const bool empty = st.xl != st.xl;
     const float up = (a.g ? a.g[a.g_per_row ? r : 0] : 1.f) * a.scale;
     const long long y = a.labels ? a.labels[r] : -1;
     const bool hard = a.w > 0.f && y >= 0 && y < n;
-    const Grad<T, TWO> g = {empty ? 0.f : st.xmax, a.c, a.c1, st.g1 * up};
-    const float gr = (TWO ? st.gr : st.gr + st.g1) * up, gl = (TWO ? st.gl : st.gl + st.g1) * up;
+    const Grad<T, TWO> g(st.xr, a.c, a.c1, st.gr, st.hr, up), listed(st.xl, a.c, a.c1, st.gl, st.hl, up);
     const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (v0 + i * G + tid < sp.nvec) {
-            i32x4 o = grad_vec<T, TWO>(v[i], g, gr);
+            i32x4 o = grad_vec<T, TWO>(v[i], g);
             if (empty) o = zero16();
             const int at = sp.vec_at(v0 + i * G + tid);
             if (same) store_vec(dx, at, o);
@@ -535,7 +559,7 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
             }
         }
     }
-    if (v0 == 0 && tid < sp.edge) { const int j = sp.edge_at(tid); store_elem(dx, j, empty ? 0.f : g(load_score(x, j), gr)); }
+    if (v0 == 0 && tid < sp.edge) { const int j = sp.edge_at(tid); store_elem(dx, j, empty ? 0.f : g(load_score(x, j))); }
     if (empty) return;
     group_sync<W>();
     // the classes of this piece; the row's edges belong to piece 0
@@ -547,13 +571,13 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
         if (p < 0.f) continue;
         const long long j = a.idx[r * a.k + e];
         if (j < 0 || j >= n || !here(j)) continue;
-        float d = g(load_score(x, (size_t)j), gl) - a.fp * p * up;
+        float d = listed(load_score(x, (size_t)j)) - a.fp * p * up;
         if (hard && j == y) { d -= a.w * up; mine = true; }
         store_elem(dx, (size_t)j, d);
     }
     if (!hard || !here(y)) return;
     if constexpr (W == 1) mine = __ballot(mine) != 0; else mine = __syncthreads_or(mine);
-    if (tid == 0 && !mine) store_elem(dx, (size_t)y, g(load_score(x, (size_t)y), gr) - a.w * up);
+    if (tid == 0 && !mine) store_elem(dx, (size_t)y, g(load_score(x, (size_t)y)) - a.w * up);
 }
 
 // Sum of the rows' losses, added in row order within a thread and in a fixed order over them: the same bits every run.

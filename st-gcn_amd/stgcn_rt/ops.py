@@ -560,7 +560,7 @@ def top_logits(logits, k, temperature=1.0):
 
 class DistillCall:
     """The checked arguments of one distillation call.  forward() and step() leave `kept` (one buffer: the rows' losses in 64
-    bits, four factors and k shares a row), which the gradient is made from."""
+    bits, six factors and k shares a row), which the gradient is made from."""
 
     __slots__ = ("x", "rows", "ncls", "k", "values", "indices", "rest", "labels", "temperature", "label_weight", "reduction", "kept")
 
@@ -591,11 +591,11 @@ class DistillCall:
 
     def _forward(self, name, loss, *more):
         x, rows = self.x, self.rows
-        self.kept = torch.empty(rows * (6 + self.k), dtype=torch.float32, device=x.device)
-        at = self.kept.data_ptr()                       # losses [rows] float64, factors [rows][4], shares [rows][k]
+        self.kept = torch.empty(rows * (8 + self.k), dtype=torch.float32, device=x.device)
+        at = self.kept.data_ptr()                       # losses [rows] float64, factors [rows][6], shares [rows][k]
         _launch(self._key(x), name, L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), self.values.data_ptr(), self.indices.data_ptr(),
                 L.ptr(self.rest), L.ptr(self.labels), rows, self.ncls, self.k, self.temperature, self.label_weight,
-                _REDUCTIONS[self.reduction], loss.data_ptr(), at, at + 8 * rows, at + 24 * rows, *more, L.stream_ptr())
+                _REDUCTIONS[self.reduction], loss.data_ptr(), at, at + 8 * rows, at + 32 * rows, *more, L.stream_ptr())
 
     def forward(self):
         none = self.reduction == "none"
@@ -628,7 +628,7 @@ class DistillCall:
             at = kept.data_ptr()
             none = self.reduction == "none"
             _launch(self._key(x), "stgcn_distill_bwd", L.dtype_code(x.dtype), x.data_ptr(), max(x.stride(0), ncls), indices.data_ptr(),
-                    None if labels is None else labels.data_ptr(), at + 8 * rows, at + 24 * rows, grad.data_ptr(), none,
+                    None if labels is None else labels.data_ptr(), at + 8 * rows, at + 32 * rows, grad.data_ptr(), none,
                     1.0 / rows if self.reduction == "mean" else 1.0, rows, ncls, self.k, self.temperature, self.label_weight, dx.data_ptr(),
                     L.stream_ptr())
         return dx

@@ -123,3 +123,43 @@ def test_distillation_over_several_segments(rt, rows, n, dt):
     for T, w in ((2.0, 0.3), (1.0, 0.0)):
         print("segments", rows, n, dt, T, w, flush=True)
         check_rows(rt, x, val, idx, rest, labels, T, w, sel)
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("rows,n,k", [(3, 20, 2), (4, 400, 5), (2, 1500, 70), (2, 5000, 8), (1, 140001, 4), (514, 9001, 8)])
+def test_distillation_gap_between_listed_and_others(rt, rows, n, k, dt):
+    """A student far surer of the listed classes than of the others, and the other way: each side's sum is its own, however
+    far the other's maximum lies above it."""
+    for j, (gap, T, w) in enumerate([(90.0, 1.0, 0.0), (200.0, 0.7, 0.3), (1e4, 1.0, 0.0), (1e4, 4.0, 0.5), (95.0, 1.0, 0.4), (61.0, 0.7, 0.0), (350.0, 4.0, 0.0),
+                                     (-90.0, 1.0, 0.0), (-1e4, 2.0, 0.3)]):
+        print("gap", rows, n, k, dt, gap, T, w, flush=True)
+        x = scores(rows, n, dt, n + j, sigma=1.0, offset=1)
+        val, idx, _ = teacher_lists(x, k, T, j)
+        x.scatter_add_(1, idx, torch.full(idx.shape, gap, dtype=dt, device=DEV))
+        # the teacher's rest: 0.3 of its mass
+        rest = torch.logsumexp(val / T, 1) - 0.85
+        labels = torch.arange(rows, device=DEV) * 7 % n
+        labels[0] = idx[0, 0]
+        check_rows(rt, x, val, idx, rest, labels, T, w, sorted({0, 1 % rows, rows - 1}))
+
+
+@pytest.mark.gpu
+def test_distillation_gap_gradient_against_differences(rt):
+    """Central differences of the 64-bit loss where e^z of the others would vanish next to the listed ones'."""
+    x = scores(2, 40, torch.float32, 3, sigma=0.7)
+    val, idx, _ = teacher_lists(x, 3, 1.0, 1)
+    x.scatter_add_(1, idx, torch.full(idx.shape, 120.0, device=DEV))
+    rest = torch.logsumexp(val, 1) - 0.5
+    _, dx = rt[1].distillation(x, val, idx, rest=rest, reduction="sum")
+    h = 1e-4
+    for r in range(2):
+        for j in range(40):
+            f = []
+            for s in (h, -h):
+                xx = x[r].cpu().double()
+                xx[j] += s
+                f.append(O.distill_row(xx, val[r].cpu(), idx[r].cpu(), float(rest[r]), None, 1.0, 0.0)[0])
+            # the difference's own error: h^2 / 6 times a third derivative below 1, and 2^-52 |loss| / h (loss < 100); the gradient's: parts of 1
+            # at most, es = 2^-23 + (2.1 * 127 + 40) 2^-24 and its 8 roundings
+            assert abs(float(dx[r, j]) - (f[0] - f[1]) / (2 * h)) < h * h + 100 * 2.0 ** -52 / h + 2 * (2.1 * 127 + 50) * U, (r, j)
