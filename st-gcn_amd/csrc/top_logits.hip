@@ -60,11 +60,12 @@ __host__ __device__ __forceinline__ int buffer_limit(int k) { return 2 * k + 64;
 // The largest score before key `k` (> -inf) in the order of the scores.
 __device__ __forceinline__ float score_before(uint32_t k) { return key_score(k == 0x80000000u ? 0x7FFFFFFEu : k - 1); }   // -0 is 0
 
-// Bits of a key that carry something: a bf16 score has 16.
+// Bits of a key that carry something: a bf16 score has 16.  long_key gives back the lowest 16, which are the sign's, and those
+// of NaN, whose one key is all ones.
 template <typename T> constexpr int KEY_SHIFT = ET<T>::IS_BF16 ? 16 : 0;
 template <typename T> __device__ __forceinline__ uint32_t short_key(u64 p) { return (uint32_t)(p >> (32 + KEY_SHIFT<T>)); }
 template <typename T> __device__ __forceinline__ uint32_t long_key(uint32_t s) {
-    return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) ? 0u : 0xFFFFu) : s;
+    return ET<T>::IS_BF16 ? s << 16 | ((s & 0x8000u) && s != KEY_NAN >> 16 ? 0u : 0xFFFFu) : s;
 }
 
 

@@ -163,3 +163,31 @@ def test_distillation_gap_gradient_against_differences(rt):
             # the difference's own error: h^2 / 6 times a third derivative below 1, and 2^-52 |loss| / h (loss < 100); the gradient's: parts of 1
             # at most, es = 2^-23 + (2.1 * 127 + 40) 2^-24 and its 8 roundings
             assert abs(float(dx[r, j]) - (f[0] - f[1]) / (2 * h)) < h * h + 100 * 2.0 ** -52 / h + 2 * (2.1 * 127 + 50) * U, (r, j)
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("rows,n,k", [(5, 61, 1), (5, 400, 5), (5, 512, 200), (5, 5000, 16), (5, 20011, 100), (5, 70001, 256), (515, 5000, 33)])
+def test_top_logits_many_nan(rt, rows, n, k, dt):
+    """NaN come first, by class, however many there are; one that is not listed makes the rest NaN."""
+    x = scores(rows, n, dt, n + k)
+    g = torch.Generator().manual_seed(k)
+    x[0] = float("nan")
+    x[1, torch.randperm(n, generator=g)[:n // 2].to(DEV)] = float("nan")
+    x[2, torch.randperm(n, generator=g)[:k].to(DEV)] = float("nan")
+    x[3, n // 2:] = float("nan")
+    x[4, torch.randperm(n, generator=g)[:k + 1].to(DEV)] = float("nan")
+    x[rows - 1, ::3] = -x[rows - 1, ::3].abs() * float("nan")
+    got = rt[0].top_logits(x, k, 2.0)
+    sel = [0, 1, 2, 3, 4, rows - 1]
+    xc = x[sel].float().cpu()
+    v, i, rest = O.top_logits(xc, k, 2.0)                    # its rest passes NaN over
+    left = torch.ones_like(xc, dtype=torch.bool).scatter_(1, i, False)
+    rest[(torch.isnan(xc) & left).any(1)] = float("nan")
+    assert torch.equal(got.indices[sel].cpu(), i)
+    assert torch.equal(torch.nan_to_num(got.values[sel].cpu().double(), nan=5.0), torch.nan_to_num(v, nan=5.0))
+    g = got.rest[sel].cpu().double()
+    assert torch.equal(torch.isnan(g), torch.isnan(rest))
+    ok = torch.isfinite(rest)
+    # log of S (EPS_S), the maximum over T in 64 bits, one rounding to 32
+    assert bool(((g[ok] - rest[ok]).abs() <= eps_sum(x[2:3], 2.0) + 2.0 ** -23 + U * rest[ok].abs()).all()), (g, rest)
