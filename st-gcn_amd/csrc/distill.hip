@@ -121,7 +121,7 @@ template <bool TWO, int L, int K> __device__ __forceinline__ void listed_sums(co
             if (p > 0) sx += p * ((double)x - (xmax > -INFINITY ? (double)xmax : 0.0));
         }
         l.p[e] = p;
-        if (l.cls[e] >= 0 && xmax > -INFINITY) {
+        if (l.cls[e] >= 0 && (xmax > -INFINITY || x != x)) {           // a NaN is no maximum, and makes the sums NaN
             sl += exp2_32((x - xmax) * a.c);
             if constexpr (TWO) sl1 += exp2_32((x - xmax) * a.c1);
         }
@@ -154,7 +154,7 @@ template <bool TWO, int L, int K> __device__ __forceinline__ void listed_merge(c
         double p = 0;
         for (int o = e; o < a.k; ++o) if (l.cls[o] == l.cls[e]) p += l.p[o];           // later ones are nobody else's to change
         l.p[e] = p;
-        if (l.xmax > -INFINITY) {
+        if (l.xmax > -INFINITY || l.x[e] != l.x[e]) {
             sl += exp2_32((l.x[e] - l.xmax) * a.c);
             if constexpr (TWO) sl1 += exp2_32((l.x[e] - l.xmax) * a.c1);
         }

@@ -191,3 +191,27 @@ def test_top_logits_many_nan(rt, rows, n, k, dt):
     ok = torch.isfinite(rest)
     # log of S (EPS_S), the maximum over T in 64 bits, one rounding to 32
     assert bool(((g[ok] - rest[ok]).abs() <= eps_sum(x[2:3], 2.0) + 2.0 ** -23 + U * rest[ok].abs()).all()), (g, rest)
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("n", [60, 401, 5000, 140001])
+@pytest.mark.parametrize("k", [1, 4])
+def test_distillation_nan_on_every_listed_class(rt, n, k, dt):
+    """A NaN score makes its row NaN wherever it stands: on all listed classes, on some, twice in the list, next to -inf."""
+    for T, w in ((1.0, 0.0), (2.0, 0.5), (1.0, 1.0), (2.0, 1.0)):
+        for others in (0.0, -float("inf")):
+            print("nan", n, k, dt, T, w, others, flush=True)
+            x = scores(5, n, dt, n)
+            val, idx, rest = teacher_lists(x, k, T, 1)
+            if others:
+                x[:4].fill_(others)
+            x[0].scatter_(0, idx[0], float("nan"))
+            x[1, idx[1, k - 1]] = float("nan")
+            idx[2] = int(idx[2, 0])
+            x[2, idx[2, 0]] = float("nan")
+            x[3].scatter_(0, idx[3], -float("inf"))
+            x[3, idx[3, 0]] = float("nan")
+            labels = torch.arange(5, device=DEV)
+            labels[0] = idx[0, 0]
+            check_rows(rt, x, val, idx, rest, labels, T, w)
