@@ -277,6 +277,9 @@ int stgcn_distill_bwd(int dtype, const void* logits, size_t row_stride, const in
 int stgcn_distill_step(int dtype, const void* logits, size_t row_stride, const float* values, const int64_t* indices,
                        const float* rest, const int64_t* labels, int rows, int ncls, int k, double temperature, double label_weight,
                        int reduction, float* loss, double* loss_rows, float* stats, float* probs, void* dlogits, void* stream);
+/* out [rows][ncls] = a float32 gradient of stgcn_distill_step times grad (one float, or one a row), with its stats: rows that
+ * teach nothing stay 0 whatever grad is.  rows * ncls < 2^31. */
+int stgcn_distill_scale(const float* dlogits, const float* stats, const float* grad, int grad_per_row, int rows, int ncls, float* out, void* stream);
 
 /* A label per row drawn from softmax(logits / temperature) with the given random number u in [0, 1): of the classes in
  * order the first top_k (0: all); of these the shortest prefix that reaches top_p of their mass; of these those at least

@@ -362,7 +362,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV
         const double loss = row_loss<L>(a, sum, st, hard, l, lane, xy);
         if (lane == 0) {
             if (a.loss_rows) a.loss_rows[r] = loss; else a.loss[r] = (float)loss;
-            if constexpr (!GRAD) a.stats[r] = st;
+            a.stats[r] = st;
         }
     }
     if constexpr (!GRAD) {
@@ -580,6 +580,15 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(GradArgs a) {
     if (tid == 0 && !mine) store_elem(dx, (size_t)y, g(load_score(x, (size_t)y)) - a.w * up);
 }
 
+// A gradient times what comes in, except the rows whose gradient is zero whatever that is (0 * inf would be NaN).
+__global__ __launch_bounds__(256) void distill_scale_kernel(const float* dx, const RowStats* stats, const float* g, int g_per_row, unsigned n, unsigned total, float* out) {
+    const unsigned i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const unsigned r = i / n;
+    const float xl = stats[r].xl;
+    out[i] = xl != xl ? 0.f : dx[i] * g[g_per_row ? r : 0];
+}
+
 // Sum of the rows' losses, added in row order within a thread and in a fixed order over them: the same bits every run.
 // Eight loads are under way at a time (one after the other, 16384 rows took 5.5 us).
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const double* rows, int n, double scale, float* loss) {
@@ -684,6 +693,13 @@ extern "C" int stgcn_distill_bwd(int dtype, const void* logits, size_t row_strid
     const hipStream_t s = (hipStream_t)stream;
     if (dtype == STGCN_BF16) { if (two) launch_bwd<bf16, true>(a, s); else launch_bwd<bf16, false>(a, s); }
     else { if (two) launch_bwd<float, true>(a, s); else launch_bwd<float, false>(a, s); }
+    return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
+}
+
+extern "C" int stgcn_distill_scale(const float* dlogits, const float* stats, const float* grad, int grad_per_row, int rows, int ncls, float* out, void* stream) {
+    if (!dlogits || !stats || !grad || !out || rows < 1 || ncls < 1 || (size_t)rows * (size_t)ncls >= (1u << 31)) return STGCN_ERR_ARG;
+    const unsigned total = (unsigned)rows * (unsigned)ncls;
+    distill_scale_kernel<<<(total + 255) / 256, 256, 0, (hipStream_t)stream>>>(dlogits, (const RowStats*)stats, grad, grad_per_row, (unsigned)ncls, total, out);
     return hipGetLastError() == hipSuccess ? STGCN_OK : STGCN_ERR_LAUNCH;
 }
 

@@ -406,9 +406,9 @@ class DistillationFn(torch.autograd.Function):
         call = P.DistillCall(logits, values, indices, rest, labels, temperature, label_weight, reduction)
         ctx.fused = logits.dtype == torch.float32 and logits.numel() <= DistillationFn.FUSED and ctx.needs_input_grad[0]
         if ctx.fused:
-            ctx.rowwise = reduction == "none"
-            loss, dx = call.step()
-            ctx.save_for_backward(dx)
+            loss, kept = call.step_kept()
+            ctx.save_for_backward(kept)
+            ctx.sizes = logits.shape
             return loss
         loss = call.forward()
         ctx.save_for_backward(logits, call.indices, call.labels, call.kept)
@@ -418,17 +418,23 @@ class DistillationFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        # the wrapper that refuses a second differentiation takes 2 to 4 us: only where one may come
+        return DistillationFn._checked(ctx, g) if torch.is_grad_enabled() else DistillationFn._backward(ctx, g)
+
+    @staticmethod
+    def _backward(ctx, g):
         if ctx.fused:
-            (dx,) = ctx.saved_tensors
-            dx = dx * (g[:, None] if ctx.rowwise else g)
+            (kept,) = ctx.saved_tensors
+            dx = P.distill_scale(kept, *ctx.sizes, g.contiguous())
         else:
             logits, indices, labels, kept = ctx.saved_tensors
             if not ctx.rows_ok:
                 logits = P._check_scores(logits)
             dx = ctx.call.backward(logits, indices, labels, kept, g.contiguous())
         return dx, None, None, None, None, None, None, None
+
+    _checked = staticmethod(torch.autograd.function.once_differentiable(_backward.__func__))
 
 
 def distillation(logits, values, indices, rest=None, labels=None, temperature=1.0, label_weight=0.0, reduction="mean"):

@@ -56,6 +56,7 @@ _SIGS = {
     "stgcn_distill_fwd": [_i, _vp, _sz, _vp, _vp, _vp, _vp, _i, _i, _i, _d, _d, _i, _vp, _vp, _vp, _vp, _vp],
     "stgcn_distill_bwd": [_i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _i, _d, _i, _i, _i, _d, _d, _vp, _vp],
     "stgcn_distill_step": [_i, _vp, _sz, _vp, _vp, _vp, _vp, _i, _i, _i, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "stgcn_distill_scale": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
     "stgcn_sample_labels": [_i, _vp, _sz, _vp, _vp, _f, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _i, _i, _vp],
     "stgcn_pack_weights": [_i, _vp, _i, _sz, _vp],
     "stgcn_sgd_step": [_vp, _vp, _vp, _sz, _f, _f, _f, _i, _i, _f, _vp],

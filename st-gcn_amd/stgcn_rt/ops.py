@@ -584,14 +584,15 @@ class DistillCall:
         if reduction == "mean" and rows == 0:
             raise ValueError("distillation: the mean over no rows")
         check_device(x, "logits")
-        self.reduction = reduction
+        self.reduction, self.kept = reduction, None
 
     def _key(self, x):
         return () if TIMING is None else (str(x.dtype), self.rows, self.ncls, self.k)
 
     def _forward(self, name, loss, *more):
         x, rows = self.x, self.rows
-        self.kept = torch.empty(rows * (8 + self.k), dtype=torch.float32, device=x.device)
+        if self.kept is None:
+            self.kept = torch.empty(rows * (8 + self.k), dtype=torch.float32, device=x.device)
         at = self.kept.data_ptr()                       # losses [rows] float64, factors [rows][6], shares [rows][k]
         _launch(self._key(x), name, L.dtype_code(x.dtype), x.data_ptr(), _row_stride(x), self.values.data_ptr(), self.indices.data_ptr(),
                 L.ptr(self.rest), L.ptr(self.labels), rows, self.ncls, self.k, self.temperature, self.label_weight,
@@ -619,6 +620,18 @@ class DistillCall:
             loss.zero_()
         return loss, dx
 
+    def step_kept(self):
+        """(loss, kept) of one call on float32 scores, kept ending with the gradient, 16-byte aligned (distill_scale)."""
+        x, rows = self.x, self.rows
+        loss = torch.empty((rows,) if self.reduction == "none" else (), dtype=torch.float32, device=x.device)
+        at = (rows * (8 + self.k) + 3) & -4
+        self.kept = torch.empty(at + rows * self.ncls, dtype=torch.float32, device=x.device)
+        if rows:
+            self._forward("stgcn_distill_step", loss, self.kept.data_ptr() + 4 * at)
+        elif self.reduction != "none":
+            loss.zero_()
+        return loss, self.kept
+
     def backward(self, x, indices, labels, kept, grad):
         """d loss / d logits times grad (a float32 tensor on the device: one number, or one a row for "none") from what a
         forward kept."""
@@ -632,6 +645,17 @@ class DistillCall:
                     1.0 / rows if self.reduction == "mean" else 1.0, rows, ncls, self.k, self.temperature, self.label_weight, dx.data_ptr(),
                     L.stream_ptr())
         return dx
+
+
+def distill_scale(kept, rows, ncls, grad):
+    """The gradient of DistillCall.step_kept() times grad (float32, one number or one a row): rows that teach nothing stay 0
+    whatever grad is."""
+    dx = kept.new_empty((rows, ncls))
+    if rows:
+        at = kept.data_ptr()
+        _launch(() if TIMING is None else (rows, ncls), "stgcn_distill_scale", at + 4 * (kept.numel() - rows * ncls), at + 8 * rows, grad.data_ptr(), grad.dim(),
+                rows, ncls, dx.data_ptr(), L.stream_ptr())
+    return dx
 
 
 def distillation(logits, values, indices, rest=None, labels=None, temperature=1.0, label_weight=0.0, reduction="mean"):

@@ -215,3 +215,28 @@ def test_distillation_nan_on_every_listed_class(rt, n, k, dt):
             labels = torch.arange(5, device=DEV)
             labels[0] = idx[0, 0]
             check_rows(rt, x, val, idx, rest, labels, T, w)
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("rows,n", [(6, 60), (5, 401), (3, 400001)])
+def test_distillation_padding_takes_no_gradient(rt, rows, n, dt):
+    """Rows without entries and label keep a gradient of zero whatever comes in: infinite, NaN."""
+    F, _ = rt
+    x = scores(rows, n, dt, 1)
+    val, idx, rest = teacher_lists(x, 4, 2.0, 1)
+    labels = torch.arange(rows, device=DEV)
+    idx[1:] = -1
+    labels[2:] = -1
+    for red, up in [("none", float("inf")), ("none", float("nan")), ("mean", float("inf")), ("sum", float("nan")), ("mean", 3.0)]:
+        leaf = x.detach().requires_grad_(True)
+        loss = F.distillation(leaf, val, idx, rest=rest, labels=labels, temperature=2.0, label_weight=0.5, reduction=red)
+        (dx,) = torch.autograd.grad(loss, leaf, torch.full_like(loss, up))
+        assert dx.dtype == dt and bool((dx[2:] == 0).all()), (red, up)
+        # what has an entry or a label takes it
+        assert bool(torch.isfinite(dx[:2]).all()) == (up == 3.0) and bool((dx[:2] != 0).any(1).all())
+    # a second backward of one loss, with another gradient, leaves the first one's result as it is
+    leaf = x.detach().requires_grad_(True)
+    loss = F.distillation(leaf, val, idx, rest=rest, labels=labels, temperature=2.0, label_weight=0.5)
+    first, second = (torch.autograd.grad(loss * f, leaf, retain_graph=True)[0] for f in (2.0, 4.0))
+    assert first.data_ptr() != second.data_ptr() and torch.equal(first * 2, second)
