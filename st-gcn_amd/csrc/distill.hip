@@ -421,6 +421,20 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void distill_stream_kernel
     const long long y = a.labels ? a.labels[r] : -1;
     const bool hard = a.w > 0.0 && y >= 0 && y < n;
     float m = -INFINITY, s = 0.f, s1 = 0.f, xy = 0.f;
+    // The sums of the segments before, relative to mf: 512 terms a thread of a segment, then at most eight segments, not one
+    // chain of 4096.
+    float mf = -INFINITY, sf = 0.f, s1f = 0.f;
+    auto flush = [&] {
+        if (mf != m) {                             // relative to -inf they are 0, or NaN
+            if (mf > -INFINITY) {
+                sf *= exp2_32((mf - m) * a.c);
+                if constexpr (TWO) s1f *= exp2_32((mf - m) * a.c1);
+            }
+            mf = m;
+        }
+        sf += s; s = 0.f;
+        if constexpr (TWO) { s1f += s1; s1 = 0.f; }
+    };
     auto raise = [&](float to) {
         if (to > m) {
             s *= m == -INFINITY ? 0.f : exp2_32((m - to) * a.c);
@@ -498,11 +512,12 @@ __global__ __launch_bounds__(W * 64, W == 16 ? 4 : 6) void distill_stream_kernel
                 }
             }
         }
+        flush();
     }
     const float all = block_reduce<W>(m, OpFMax(), rmax);
     const bool none = m == -INFINITY;              // then s is 0, or NaN
-    const double sr = block_reduce<W>((double)s * (none ? 1.0 : (double)exp2_32((m - all) * a.c)), OpSum(), rsum[0]);
-    const double sr1 = TWO ? block_reduce<W>((double)s1 * (none ? 1.0 : (double)exp2_32((m - all) * a.c1)), OpSum(), rsum[1]) : 0.0;
+    const double sr = block_reduce<W>((double)sf * (none ? 1.0 : (double)exp2_32((m - all) * a.c)), OpSum(), rsum[0]);
+    const double sr1 = TWO ? block_reduce<W>((double)s1f * (none ? 1.0 : (double)exp2_32((m - all) * a.c1)), OpSum(), rsum[1]) : 0.0;
     if (!lead) return;
     const RowSums sum = join_sums<TWO>(a, l, all, sr, sr1);
     const RowStats st = row_factors(a, sum, hard, l.flags, l.pr);

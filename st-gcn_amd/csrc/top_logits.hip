@@ -54,7 +54,22 @@ template <int W> struct Shared {
     u64 tau; float lim;                            // the bound; scores x with !(x <= lim) may be earlier in the order
     int add[3][W];
     float rm[4]; double rs[4];
+    // A thread's sums of before, in 64 bits, relative to far_m: what a thread adds up in 32 bits is 512 terms at most, and
+    // what a compaction drops a lane (one wave's, 64 terms a batch where the scores ascend).  W = 1: rows of 512 classes.
+    double far_s[W == 1 ? 1 : W * 64]; float far_m[W == 1 ? 1 : W * 64];
 };
+constexpr int FLUSH = 32;                          // batches of 16 scores a thread
+
+// 2^{(from - to) c} for a sum relative to `from` (-inf: the sum is 0, or NaN)
+__device__ __forceinline__ double rebase(float from, float to, float c) { return from == to || from == -INFINITY ? 1.0 : (double)exp2_32((from - to) * c); }
+template <int W> __device__ __forceinline__ void far_clear(Shared<W>& sh, int tid) {
+    if constexpr (W > 1) { sh.far_s[tid] = 0; sh.far_m[tid] = -INFINITY; }
+}
+template <int W> __device__ __forceinline__ void far_add(Shared<W>& sh, int tid, const RestSum& r, float c) {
+    const float was = sh.far_m[tid], m = fmaxf(was, r.m);
+    sh.far_s[tid] = sh.far_s[tid] * rebase(was, m, c) + (double)r.s * rebase(r.m, m, c);
+    sh.far_m[tid] = m;
+}
 __host__ __device__ __forceinline__ int buffer_limit(int k) { return 2 * k + 64; }       // beyond it the bound is raised
 
 // The largest score before key `k` (> -inf) in the order of the scores.
@@ -137,13 +152,15 @@ template <typename T, int W> __device__ __forceinline__ void compact(Shared<W>& 
     if (tid < 64) {
         const u64 t = kth_place<T, Shared<W>::EQ>(sh.cand, sh.maxima, n, k);
         int at = 0;
+        RestSum dropped;
         for (int i = 0; i < n; i += 64) {          // entries only move towards the front
             const u64 p = i + tid < n ? sh.cand[i + tid] : 0;
             const u64 keep = __ballot(p >= t && p);
             if (p >= t && p) sh.cand[at + lanes_below(keep)] = p;
-            else if (p) rest.take(key_score((uint32_t)(p >> 32)), c);
+            else if (p) { if constexpr (W > 1) dropped.take(key_score((uint32_t)(p >> 32)), c); else rest.take(key_score((uint32_t)(p >> 32)), c); }
             at += __popcll(keep);
         }
+        if constexpr (W > 1) far_add<W>(sh, tid, dropped, c);
         if (tid == 0) { sh.tau = t; sh.lim = key_score((uint32_t)(t >> 32)); }
     }
     n = k;
@@ -259,13 +276,15 @@ __device__ void slow_row(const T* x, int lo, int hi, int tid, int k, Shared<W>& 
 
 // rest of the group: its threads' sums joined.  Every thread gets the pair.
 template <int W> __device__ __forceinline__ void join_rest(Shared<W>& sh, int tid, const RestSum& r, float c, float& m, double& s) {
-    m = wave_reduce(r.m, OpFMax());
+    const float own = W > 1 ? fmaxf(r.m, sh.far_m[tid]) : r.m;
+    m = wave_reduce(own, OpFMax());
     if constexpr (W > 1) {
         if ((tid & 63) == 0) sh.rm[tid >> 6] = m;
         __syncthreads();
         for (int w = 0; w < W; ++w) m = fmaxf(m, sh.rm[w]);
     }
-    s = (double)r.s * (r.m == m || r.m == -INFINITY ? 1.0 : (double)exp2_32((r.m - m) * c));
+    s = (double)r.s * rebase(r.m, m, c);
+    if constexpr (W > 1) s += sh.far_s[tid] * rebase(sh.far_m[tid], m, c);
     s = wave_reduce(s, OpSum());
     if constexpr (W > 1) {
         if ((tid & 63) == 0) sh.rs[tid >> 6] = s;
@@ -315,6 +334,7 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
     const int v1 = min(b1 * G * NB, sp.nvec);
 
     if (tid == 0) sh.tau = 0;
+    far_clear<W>(sh, tid);
     RestSum rest;
     int have = 0, turn = 0;                        // entries in the buffer
     i32x4 v[NB], nx[NB];
@@ -411,6 +431,7 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
         const float ref = rest.m == -INFINITY ? 0.f : rest.m;
 #pragma unroll
         for (int e = 0; e < PER; ++e) rest.s += exp2_32((f[e] - ref) * c);
+        if constexpr (W > 1) if (((b - b0) & (FLUSH - 1)) == FLUSH - 1) { far_add<W>(sh, tid, rest, c); rest.s = 0.f; }
     }
     // the row's ends, behind the last whole vector last in the order of classes; in front of the first they come first, so
     // those are held against the bound with their class
@@ -426,9 +447,10 @@ __global__ __launch_bounds__(256, (TOP_WAVES<T, W>)) void top_scan_kernel(TopArg
     if (have > G && a.pieces == 1) compact<T, W>(sh, tid, have, k, rest, c);
     else group_sync<W>();
     bool nan = rest.s != rest.s;
-    if constexpr (W == 1) nan = __ballot(nan) != 0; else nan = __syncthreads_or(nan);
+    if constexpr (W == 1) nan = __ballot(nan) != 0; else nan = __syncthreads_or(nan || sh.far_s[tid] != sh.far_s[tid]);
     if (nan) {
         const int lo = with_head ? 0 : sp.vec_at(b0 * G * NB), hi = with_tail ? n : sp.vec_at(v1);
+        far_clear<W>(sh, tid);
         slow_row<T, W>(x, lo, hi, tid, k, sh, rest, c);
         have = min(k, hi - lo);
     }
@@ -461,6 +483,7 @@ __global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a) {
         if (256 * i < c && tid + 256 * i < c) key[i] = (uint32_t)(part[tid + 256 * i] >> 32);
         top[i & 3] = max(top[i & 3], key[i]);
     }
+    far_clear<4>(sh, tid);
     RestSum rest;
     for (int i = tid; i < a.pieces; i += 256) {
         const float2 p = a.part_rest[r * a.pieces + i];

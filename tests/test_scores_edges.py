@@ -240,3 +240,36 @@ def test_distillation_padding_takes_no_gradient(rt, rows, n, dt):
     loss = F.distillation(leaf, val, idx, rest=rest, labels=labels, temperature=2.0, label_weight=0.5)
     first, second = (torch.autograd.grad(loss * f, leaf, retain_graph=True)[0] for f in (2.0, 4.0))
     assert first.data_ptr() != second.data_ptr() and torch.equal(first * 2, second)
+
+
+@pytest.mark.gpu
+@DTS
+def test_long_rows_add_up(rt, dt):
+    """The most classes, in rows that few threads share: every thread sees one, then thousands of e^{(x - max) / T} that lie a
+    little above a half, which a sum of 32 bits between 1024 and 2048 would lose the little of at each step (2^-14 of 2^-13
+    steps: a thousand units of the sum's last place).  Bound: the chain of tests/test_scores.py."""
+    F, P = rt
+    import math
+    rows, n, k = 512, 1 << 20, 2
+    low = -0.69140625                                               # a bf16 number
+    T = low / math.log(0.5 + 0.98 * 2.0 ** -14)
+    row = torch.full((n,), low)
+    row[:1 << 14] = 0.0                                             # every thread's first vectors
+    row[torch.tensor([77777, 999999])] = 3.0
+    x = row.to(dt).to(DEV).expand(rows, n).contiguous()
+    some = row[None].double()
+    check = [0, rows - 1]
+    top = F.top_logits(x, k, T)
+    v, i, rest = O.top_logits(some, k, T)
+    assert torch.equal(top.indices[check].cpu(), i.expand(2, k))
+    es = eps_sum(some, T)
+    assert bool(((top.rest[check].cpu().double() - rest).abs() <= es + U * abs(float(rest))).all()), (top.rest[check], rest, es)
+    up = torch.linspace(-9, 9, n).to(dt)                            # every batch is earlier in the order than those before it
+    got = F.top_logits(up.to(DEV).expand(rows, n).contiguous(), 64, 2.0)
+    v, i, rest = O.top_logits(up[None].double(), 64, 2.0)
+    assert torch.equal(got.indices[check].cpu(), i.expand(2, 64)) and torch.equal(got.values[check].cpu().double(), v.expand(2, 64))
+    assert bool(((got.rest[check].cpu().double() - rest).abs() <= eps_sum(up[None], 2.0) + U * abs(float(rest))).all()), (got.rest[check], rest)
+    val = torch.tensor([[1.0, 0.5]], device=DEV).expand(rows, k).contiguous()
+    tr = torch.full((rows,), 0.7, device=DEV)
+    check_rows(rt, x, val, top.indices, tr, None, T, 0.0, check)
+    check_rows(rt, x, val, top.indices, tr, torch.full((rows,), 5, device=DEV), T, 0.5, [1])
