@@ -250,9 +250,12 @@ class Trainer:
     the same batch at `temperature`, and against the labels with label_weight (a label < 0: none).  The teacher is put
     into eval mode, runs without gradients ahead of every step, outside the graph (its scores' top logits are copied into
     the graph's static buffers), and shares no parameter with the model.  step(..., target=...) takes the top logits from
-    the caller instead (evaluate.teacher_targets collects them)."""
+    the caller instead (evaluate.teacher_targets collects them).  `temperature` and `label_weight` may be set between steps.
+    They are part of a captured graph, which holds a step's memory: the GRAPHS_KEPT used last are kept for batches and targets
+    of one shape, and the first step at a value runs launch by launch (one that changes at every step is never captured)."""
 
     GRAPH_WARMUP = 2
+    GRAPHS_KEPT = 4
     # With more than one rank the captured step is TWO graphs: forward, loss and the backward of the head and of blocks
     # SPLIT_BLOCK.. (three quarters of the parameters) in the first, the rest of the backward in the second.  The
     # all-reduce of the first segment's gradients is issued between the two replays and runs under the second; no
@@ -278,9 +281,10 @@ class Trainer:
         self.loss_fn = F_.cross_entropy          # nn.CrossEntropyLoss() with its defaults, one launch each way
         self.use_graph = bool(graph)
         self.split = split                    # capture the step as two graphs: None = when there is more than one rank
-        self._graphs = {}                     # (data shape, label shape, target's) -> (graph, static data, static label, static target, static loss)
+        self._graphs = {}                     # (shapes of data, label and target; temperature and label_weight) -> (graph, static data, static label, static target, static loss)
         self._eager_steps = 0
         self._taught_steps = 0                # of these with a target
+        self._met = {}                        # (temperature, label_weight) of the last steps with a target
         self._grads_bound = False             # whether every p.grad is the parameter's slice of the flat gradient
 
     def broadcast_from_rank0(self):
@@ -439,14 +443,31 @@ class Trainer:
         return self.use_graph and self.model.training and warm >= self.GRAPH_WARMUP
 
     def _graph_for(self, data, label, target):
-        key = (tuple(data.shape), data.dtype, tuple(label.shape),
-               None if target is None else (self.temperature, self.label_weight, tuple(None if t is None else tuple(t.shape) for t in target)))
-        ent = self._graphs.get(key)
+        shapes = (tuple(data.shape), data.dtype, tuple(label.shape), None if target is None else tuple(None if t is None else tuple(t.shape) for t in target))
+        key = (shapes, None if target is None else (self.temperature, self.label_weight))
+        ent = self._graphs.pop(key, None)
         if ent is None:
+            old = [k for k in self._graphs if k[0] == shapes]
+            if len(old) >= self.GRAPHS_KEPT:  # only with targets: else there is one graph of a shape
+                if data.is_cuda:
+                    torch.cuda.synchronize()  # a replay may be under way
+                for k in old[:len(old) - self.GRAPHS_KEPT + 1]:
+                    del self._graphs[k]
             ent = self._capture(data, label, target)
-            if ent is not None:
-                self._graphs[key] = ent
+        if ent is not None:
+            self._graphs[key] = ent           # the one used last stands last
         return ent
+
+    def _settled(self, target):
+        """Whether an earlier step had this temperature and label_weight; remembers them."""
+        if target is None:
+            return True
+        now = (self.temperature, self.label_weight)
+        known = self._met.pop(now, False)
+        self._met[now] = True
+        if len(self._met) > 2 * self.GRAPHS_KEPT:
+            del self._met[next(iter(self._met))]
+        return known
 
     def prepare_graph(self, data, label, target=None):
         """Captures the graph for this input shape now (no step is performed) instead of inside the first step() that
@@ -469,7 +490,8 @@ class Trainer:
         (values, indices, rest or None) to learn from, taken instead of the teacher's."""
         from . import ops as P
         target = self._target_of(data, target)
-        if not eager and P.TIMING is None and self._graph_wanted(target):
+        settled = self._settled(target)
+        if not eager and P.TIMING is None and settled and self._graph_wanted(target):
             ent = self._graph_for(data, label, target)
             if ent is not None:
                 g, sx, sl, st, loss = ent
