@@ -37,6 +37,17 @@ def test_the_bit_map_of_a_segment_holds_what_is_cleared_and_read(tmp_path):
     assert subprocess.check_output([str(exe)], text=True) == "0 1"
 
 
+# ---- build (CPU) ---------------------------------------------------------------------------------------------------
+
+def test_a_change_of_flags_builds_every_object_again():
+    """Old objects, made with packed float32 instructions, must not be linked into a library whose flags leave them out.  (A dry run.)"""
+    sources = sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
+    plan = subprocess.check_output(["make", "-C", CSRC, "-n", "-W", "Makefile"], text=True)
+    built = [line.split(" -c ")[1].split()[0] for line in plan.splitlines() if " -c " in line]
+    assert sorted(built) == sources
+    assert all("-packed-fp32-ops" in line for line in plan.splitlines() if " -c " in line)
+
+
 # ---- distillation over selected rows -------------------------------------------------------------------------------
 
 def row_parts(x, val, idx, rho, label, T, w, es):
