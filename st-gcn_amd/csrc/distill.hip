@@ -107,7 +107,11 @@ template <bool TWO, int L, int K> __device__ __forceinline__ void listed_sums(co
     int flags = l.flags;
     const bool any = flags & 1;
     if (any && !(rho32 < INFINITY)) flags |= 2;
-    const double invT = a.invT, rho = (double)rho32, m = any ? fmax((double)tmax * invT, rho) : 0.0;
+    // Relative to the larger of t_max / T and rho; the scores' differences are taken before they are divided (a product less its
+    // own rounded value is no zero when it becomes one fused operation, and next to T = 1e-16 more than the whole).
+    const double invT = a.invT, rho = (double)rho32, over = rho - (double)tmax * invT;
+    const bool by_rho = over > 0;
+    const double ref = by_rho ? 0.0 : (double)tmax, z0 = by_rho ? -rho : 0.0, zr = by_rho ? 0.0 : over;
     double s = 0, sz = 0, sx = 0;
     float sl = 0.f, sl1 = 0.f;
     for (int e = lane; e < a.k; e += L) {
@@ -115,7 +119,7 @@ template <bool TWO, int L, int K> __device__ __forceinline__ void listed_sums(co
         const float x = l.x[e];
         double p = 0;
         if (any && t > -INFINITY) {
-            const double z = t * invT - m;
+            const double z = (t - ref) * invT + z0;
             p = exp2_64(z * LOG2E);
             s += p; sz += p * z;
             if (p > 0) sx += p * ((double)x - (xmax > -INFINITY ? (double)xmax : 0.0));
@@ -127,13 +131,13 @@ template <bool TWO, int L, int K> __device__ __forceinline__ void listed_sums(co
         }
     }
     s = group_sum<L>(s); sz = group_sum<L>(sz); sx = group_sum<L>(sx);
-    const double er = any ? exp2_64((rho - m) * LOG2E) : 0.0;
+    const double er = any ? exp2_64(zr * LOG2E) : 0.0;
     s += er;
     const double inv = any ? 1.0 / s : 0.0, ls = any ? ln_64(s) : 0.0;
     for (int e = lane; e < a.k; e += L) l.p[e] *= inv;
     const double pr = er * inv, sl64 = group_sum<L>((double)sl), sl164 = TWO ? group_sum<L>((double)sl1) : 0.0;
     if (lane == 0) {
-        l.own = (sz + (er > 0 ? er * (rho - m) : 0.0)) * inv - ls;         // sum of p log p = sum of p (z - ln s), all p being 1
+        l.own = (sz + (er > 0 ? er * zr : 0.0)) * inv - ls;         // sum of p log p = sum of p (z - ln s), all p being 1
         l.cross = sx * inv * (double)a.c * LN2;
         l.pr = pr; l.sl = sl64; l.sl1 = sl164; l.xmax = xmax; l.flags = flags;
     }

@@ -284,3 +284,19 @@ def test_long_rows_add_up(rt, dt):
     tr = torch.full((rows,), 0.7, device=DEV)
     check_rows(rt, x, val, top.indices, tr, None, T, 0.0, check)
     check_rows(rt, x, val, top.indices, tr, torch.full((rows,), 5, device=DEV), T, 0.5, [1])
+
+
+@pytest.mark.gpu
+@DTS
+def test_distillation_small_temperatures(rt, dt):
+    """The teacher's t / T are thousands to 1e20 then; differences of scores are what counts of them."""
+    F, P = rt
+    x = scores(6, 700, dt, 5)
+    for T, w in ((1e-3, 0.3), (1e-6, 0.0)):                     # small ones, where 64 bits still tell
+        print("small", dt, T, flush=True)
+        val, idx, rest = teacher_lists(x, 5, T, 3)
+        for more in (None, rest, torch.logsumexp(val / T, 1) + 0.5):
+            check_rows(rt, x, val, idx, more, torch.arange(6, device=DEV), T, w)
+    top = F.top_logits(x, 3, 1e-20)
+    loss, dx = P.distillation(x, top.values, top.indices, temperature=1e-20)
+    assert not bool(torch.isnan(dx).any()) and not bool(torch.isnan(loss))
