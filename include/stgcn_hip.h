@@ -245,7 +245,7 @@ int stgcn_cross_entropy(const float* logits, const int64_t* labels, float* loss,
  * No counterpart in the reference, whose training step knows hard labels only (processor/recognition.py:44, 91) and
  * whose test step keeps the scores as they are (recognition.py:110-143).
  * `logits` here: rows of ncls scores, float32 or bf16, `row_stride` ELEMENTS apart (>= ncls), any alignment of an element;
- * 1 <= ncls <= 2^20, 1 <= rows < 2^24.  Classes are ordered by (score descending, class ascending), NaN first. */
+ * 1 <= ncls <= 2^20, 1 <= rows < 2^24; 1e-30 < temperature < 1e30 where it divides in 32 bits (the first two operators).  Classes are ordered by (score descending, class ascending), NaN first. */
 
 /* The k (1..256, <= ncls) first classes of every row in that order: values [rows][k], indices [rows][k], and rest [rows] =
  * log sum over the other classes of exp(logits / temperature) (-inf: nothing is left).  Few rows are split over workgroups

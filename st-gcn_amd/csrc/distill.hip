@@ -631,7 +631,7 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const double* rows, int 
 
 bool bad_common(int dtype, const void* x, size_t stride, const void* idx, int rows, int ncls, int k, double T, double w) {
     return (dtype != STGCN_F32 && dtype != STGCN_BF16) || !x || !idx || rows < 1 || rows >= (1 << 24) || ncls < 1 || ncls > (1 << 20) || stride < (size_t)ncls
-        || k < 1 || k > MAX_K || !(T > 0.0) || !(T < 1e30) || !(w >= 0.0) || !(w <= 1.0);
+        || k < 1 || k > MAX_K || !temperature_ok(T) || !(w >= 0.0) || !(w <= 1.0);
 }
 
 // The widest row that fits in registers: 16 waves of 16 vectors a lane (64 registers of scores).

@@ -6,6 +6,9 @@
 #pragma once
 #include "stgcn_common.h"
 
+// Temperatures T whose log2(e) / T is a float32 number, with room: below, 0 * inf would make NaN of a row's largest score.
+inline bool temperature_ok(double T) { return T > 1e-30 && T < 1e30; }
+
 template <typename T> struct RowSpan {
     static constexpr int VEC = ET<T>::VEC;
     int head, nvec, edge;                  // elements in front, vectors, elements in front and behind together

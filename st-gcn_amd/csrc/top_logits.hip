@@ -542,7 +542,7 @@ extern "C" int stgcn_top_logits_workspace(int rows, int ncls, int k, size_t* byt
 extern "C" int stgcn_top_logits(int dtype, const void* logits, size_t row_stride, int rows, int ncls, int k, double temperature,
                                 float* values, int64_t* indices, float* rest, void* workspace, size_t workspace_bytes, void* stream) {
     if (!logits || !values || !indices || !rest || rows < 1 || rows >= (1 << 24) || ncls < 1 || ncls > (1 << 20) || row_stride < (size_t)ncls || k < 1 || k > MAX_K
-        || k > ncls || !(temperature > 0.0) || !(temperature < 1e30) || (dtype != STGCN_F32 && dtype != STGCN_BF16)) return STGCN_ERR_ARG;
+        || k > ncls || !temperature_ok(temperature) || (dtype != STGCN_F32 && dtype != STGCN_BF16)) return STGCN_ERR_ARG;
     const int pieces = top_pieces(rows, ncls, k);
     if (pieces > 1 && (!workspace || workspace_bytes < top_workspace(rows, pieces, k))) return STGCN_ERR_WORKSPACE;
     TopArgs a = {logits, row_stride, rows, ncls, k, pieces, (float)(LOG2E / temperature), temperature, values, (long long*)indices, rest,

@@ -268,7 +268,7 @@ class Trainer:
             mine = {id(p) for p in model.parameters()}
             if teacher is model or any(id(p) in mine for p in teacher.parameters()):
                 raise ValueError("the teacher shares parameters with the model")
-        if not 1 <= int(teacher_k) <= 256 or not 0.0 < float(temperature) < 1e30 or not 0.0 <= float(label_weight) <= 1.0:
+        if not 1 <= int(teacher_k) <= 256 or not 1e-30 < float(temperature) < 1e30 or not 0.0 <= float(label_weight) <= 1.0:
             raise ValueError("a teacher wants 1 to 256 top logits, a temperature above 0 and a label_weight from 0 to 1, got %r, %r, %r"
                              % (teacher_k, temperature, label_weight))
         self.model = model

@@ -524,9 +524,10 @@ def _check_like(t, name, shape, dtype, like):
 
 
 def _check_temperature(t):
+    """Scores are multiplied by log2(e) / t in 32 bits, which has to be a number."""
     t = float(t)
-    if not 0.0 < t < 1e30:
-        raise ValueError("temperature wants a positive number, got %r" % t)
+    if not 1e-30 < t < 1e30:
+        raise ValueError("temperature wants a positive number from 1e-30 to 1e30, got %r" % t)
     return t
 
 

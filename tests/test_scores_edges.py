@@ -48,6 +48,29 @@ def test_a_change_of_flags_builds_every_object_again():
     assert all("-packed-fp32-ops" in line for line in plan.splitlines() if " -c " in line)
 
 
+# ---- refusals (CPU) ------------------------------------------------------------------------------------------------
+
+def test_temperatures_without_a_32_bit_inverse_are_refused():
+    """log2(e) / T beyond float32 would make NaN of 0 * inf: both ends, through the operators and the C entries."""
+    from stgcn_rt import functional as F, lib as L
+    from stgcn_rt.ddp import Trainer
+    import net.st_gcn as m
+    x, v, i = torch.zeros(4, 10), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    l, p = L.load(), 4096                                      # p: never dereferenced by the host
+    net = [m.Model(3, 7, dict(layout="ntu-rgb+d", strategy="spatial"), True) for _ in range(2)]
+    for T in (1e-30, 1e-39, 1e-45, 5e-324, 1e30, 1e300):
+        for f in (lambda: F.top_logits(x, 3, temperature=T), lambda: F.distillation(x, v, i, temperature=T), lambda: Trainer(net[0], teacher=net[1], temperature=T)):
+            with pytest.raises(ValueError, match="temperature"):
+                f()
+        assert l.stgcn_top_logits(0, p, 10, 4, 10, 3, T, p, p, p, None, 0, None) == 1
+        assert l.stgcn_distill_fwd(0, p, 10, p, p, None, None, 4, 10, 3, T, 0.0, 1, p, p, p, p, None) == 1
+        assert l.stgcn_distill_step(0, p, 10, p, p, None, None, 4, 10, 3, T, 0.0, 1, p, p, p, p, p, None) == 1
+        assert l.stgcn_distill_bwd(0, p, 10, p, None, p, p, None, 0, 1.0, 4, 10, 3, T, 0.0, p, None) == 1
+    for T in (1.1e-30, 0.9e30):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            F.top_logits(x, 3, temperature=T)
+
+
 # ---- distillation over selected rows -------------------------------------------------------------------------------
 
 def row_parts(x, val, idx, rho, label, T, w, es):
@@ -284,6 +307,28 @@ def test_long_rows_add_up(rt, dt):
     tr = torch.full((rows,), 0.7, device=DEV)
     check_rows(rt, x, val, top.indices, tr, None, T, 0.0, check)
     check_rows(rt, x, val, top.indices, tr, torch.full((rows,), 5, device=DEV), T, 0.5, [1])
+
+
+@pytest.mark.gpu
+@DTS
+def test_the_ends_of_the_temperatures(rt, dt):
+    """As good as a maximum, and as good as equal shares: finite numbers, no NaN."""
+    F, P = rt
+    x = scores(6, 700, dt, 5)
+    for T in (1.1e-30, 1e-20, 0.9e30):
+        print("ends", dt, T, flush=True)
+        top = F.top_logits(x, 3, T)
+        v, i, rest = O.top_logits(x.float().cpu(), 3, T)
+        assert torch.equal(top.indices.cpu(), i)
+        # log of S: at most log 700, one rounding; beyond float32's range its infinity
+        want = rest.float().double()
+        assert bool((torch.isinf(want) == torch.isinf(top.rest.cpu())).all())
+        ok = torch.isfinite(want)
+        assert bool(((top.rest.cpu().double() - want).abs()[ok] <= 2 * U * want.abs()[ok] + eps_sum(x, 1.0)).all())
+        for more in (None, top.rest):
+            if more is None or bool(torch.isfinite(more).all()):
+                loss, dx = P.distillation(x, top.values, top.indices, rest=more, temperature=T)
+                assert not bool(torch.isnan(dx).any()) and not bool(torch.isnan(loss))
 
 
 @pytest.mark.gpu
