@@ -357,7 +357,7 @@ class Trainer:
         if P.TIMING is not None:
             return None
         m, flat = self.model, self.flat
-        sx, sl, st = data.clone(), label.clone(), self._static(target)
+        sx, sl, st = data.clone(), None if label is None else label.clone(), self._static(target)
         g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
         late, early = flat.params[:nlate], flat.params[nlate:]
         self.bucketer.hooks_enabled = False
@@ -417,7 +417,7 @@ class Trainer:
             nlate = self._split_point()
             if nlate is not None:
                 return self._capture_split(data, label, target, nlate)
-        sx, sl, st = data.clone(), label.clone(), self._static(target)
+        sx, sl, st = data.clone(), None if label is None else label.clone(), self._static(target)
         g = torch.cuda.CUDAGraph()
         self.bucketer.hooks_enabled = False
         try:
@@ -443,7 +443,7 @@ class Trainer:
         return self.use_graph and self.model.training and warm >= self.GRAPH_WARMUP
 
     def _graph_for(self, data, label, target):
-        shapes = (tuple(data.shape), data.dtype, tuple(label.shape), None if target is None else tuple(None if t is None else tuple(t.shape) for t in target))
+        shapes = (tuple(data.shape), data.dtype, None if label is None else tuple(label.shape), None if target is None else tuple(None if t is None else tuple(t.shape) for t in target))
         key = (shapes, None if target is None else (self.temperature, self.label_weight))
         ent = self._graphs.pop(key, None)
         if ent is None:
@@ -472,24 +472,40 @@ class Trainer:
     def prepare_graph(self, data, label, target=None):
         """Captures the graph for this input shape now (no step is performed) instead of inside the first step() that
         would use it; needs the warm-up steps done.  Returns whether a graph is ready."""
-        target = self._target_of(data, target)
+        target = self._target_of(data, label, target)
         if self._graph_wanted(target):
             return self._graph_for(data, label, target) is not None
         return False
 
-    def _target_of(self, data, target):
+    def _target_of(self, data, label, target):
+        """The target, checked as functional.distillation would: a captured step only copies it, and would cast and move."""
+        given = target is not None
+        if not given:
+            target = self.target(data)
         if target is None:
-            return self.target(data)
-        if len(target) != 3:
-            raise ValueError("a target is (values, indices, rest or None), as top_logits returns it")
-        return tuple(target)
+            return None
+        from . import ops as P
+        if given:
+            target = tuple(target)
+            if len(target) != 3 or not all(torch.is_tensor(t) for t in target[:2 if target[2] is None else 3]) or target[0].dim() != 2:
+                raise ValueError("a target is (values, indices, rest or None), as top_logits returns it")
+            n, (values, indices, rest) = data.shape[0], target
+            target = (P._check_like(values, "target values", (n, values.shape[1]), torch.float32, data),
+                      P._check_like(indices, "target indices", (n, values.shape[1]), torch.int64, data),
+                      None if rest is None else P._check_like(rest, "target rest", (n,), torch.float32, data))
+        if label is not None:
+            P._check_like(label, "labels", (data.shape[0],), torch.int64, data)
+        elif self.label_weight > 0:
+            raise ValueError("label_weight %g wants labels" % self.label_weight)
+        return target
 
     def step(self, data, label, eager=False, target=None):
         """One iteration; returns the loss (a device tensor; with a graph, the graph's own output buffer, overwritten
         by the next replay).  eager=True forces the launch-by-launch path for this call.  target: the batch's top logits
-        (values, indices, rest or None) to learn from, taken instead of the teacher's."""
+        (values, indices, rest or None) to learn from, taken instead of the teacher's; label may be None where that is all that
+        counts (label_weight 0)."""
         from . import ops as P
-        target = self._target_of(data, target)
+        target = self._target_of(data, label, target)
         settled = self._settled(target)
         if not eager and P.TIMING is None and settled and self._graph_wanted(target):
             ent = self._graph_for(data, label, target)
@@ -497,7 +513,7 @@ class Trainer:
                 g, sx, sl, st, loss = ent
                 if data.data_ptr() != sx.data_ptr():
                     sx.copy_(data, non_blocking=True)
-                if label.data_ptr() != sl.data_ptr():
+                if sl is not None and label.data_ptr() != sl.data_ptr():
                     sl.copy_(label, non_blocking=True)
                 for s, t in zip(st or (), target or ()):
                     if s is not None and s.data_ptr() != t.data_ptr():

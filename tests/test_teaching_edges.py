@@ -50,6 +50,29 @@ def test_a_value_is_captured_from_its_second_step_on():
     assert not tr._settled(top) and tr._settled(top)
 
 
+def test_targets_that_do_not_fit_are_refused():
+    """Before anything runs, with a graph and without: a replay would cast, broadcast or move what it copies."""
+    x, lab = torch.zeros(2, 3, 4, 25, 1), torch.zeros(2, dtype=torch.int64)
+    v, i, r = torch.zeros(2, 5), torch.zeros(2, 5, dtype=torch.int64), torch.zeros(2)
+    for graph in (False, True):
+        tr = cpu_trainer(graph=graph)
+        tr._eager_steps = tr._taught_steps = 5
+        tr._capture = lambda *a: pytest.fail("captured")
+        for target, match in [((v.double(), i, r), "values"), ((v[:1], i, r), "values"), ((v, i.int(), r), "indices"), ((v, i[:, :4], r), "indices"),
+                              ((v, i, r.double()), "rest"), ((v, i, r[:1]), "rest"), ((v, None, r), "a target"), ((None, i, r), "a target"), ((v[0], i, r), "a target"),
+                              ((v.tolist(), i, r), "a target"), ((v, i), "a target")]:
+            for f in (lambda: tr.step(x, lab, target=target), lambda: tr.prepare_graph(x, lab, target=target)):
+                with pytest.raises(ValueError, match=match):
+                    f()
+        for label in (lab.int(), lab.float(), lab[:1]):
+            with pytest.raises(ValueError, match="labels"):
+                tr.step(x, label, target=(v, i, r))
+        with pytest.raises(ValueError, match="wants labels"):
+            tr.step(x, None, target=(v, i, r))
+        with pytest.raises(RuntimeError, match="target values lives on"):
+            tr.step(x, lab, target=(v.to("meta"), i, r))
+
+
 @pytest.mark.gpu
 def test_annealed_temperature_keeps_its_memory(st):
     """Ten temperatures, four steps each: as launch by launch bit for bit, and the memory of the graphs that passed is free again."""
@@ -72,3 +95,16 @@ def test_annealed_temperature_keeps_its_memory(st):
     assert ends[0][0] == ends[1][0] and torch.equal(ends[0][1], ends[1][1])
     grows = held[1] - held[0]                                        # what one graph holds
     assert grows > 1 << 20 and held[9] <= held[4] + grows // 2, held
+
+
+@pytest.mark.gpu
+def test_steps_without_labels(st):
+    """label_weight 0 and no labels: launch by launch and captured, bit for bit as with labels that do not count."""
+    x, ends = clips(4, 81), []
+    for graph, lab in ((False, torch.tensor(LABELS, device=DEV)), (False, None), (True, None)):
+        tr = trainer(st, graph=graph, label_weight=0.0)
+        losses = [float(tr.step(x, lab).detach()) for _ in range(6)]
+        assert tr.graph_ready() == graph
+        ends.append((losses, tr.flat.flat.clone()))
+    for losses, params in ends[1:]:
+        assert losses == ends[0][0] and torch.equal(params, ends[0][1])
