@@ -15,8 +15,9 @@
 //   larger top_k, and top_p: the scores (or their weights) counted by bins of the score; the bin in which the count
 //     (the sum) crosses is split into bins of its own until it gives a short list, in which the border is bisected by one
 //     wave (a whole workgroup spent 12 us a list on barriers).  Bins and list hold weights as 64-bit integers
-//     in units of 2^-s (s = 42 to 50 by the class count): their sums are the same in any order.  A border that falls within
-//     such a unit of a class moves that class alone, by a share of 2^-s of the first class's weight;
+//     in units of 2^-s of the first class's (s = 50 up to 2^13 classes, one less for each doubling, 43 at 2^20): their sums are
+//     the same in any order.  Each is at most half a unit off, so the mass that a border of top-p is held against is off by
+//     n 2^-(s+1) at most (2^-24 at 2^20 classes, 2^-30 at 2^17): the border may lie that much mass away;
 //   the answer: sums of the kept weights by cells (four steps of 64 vectors), made by the pass that fills the last border's
 //     list where there is one, the cell in which u falls, then the lane, then the class.
 //
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
     }
     if (top == KEY_NEG_INF) { if (tid == 0) fixed_answer(-1, -INFINITY); return; }
     const float xmax = key_score(top);
-    const int s = min(50, 30 + __clz(n));          // n sums of at most 2^s stay below 2^63
+    const int s = min(50, 31 + __clz(n - 1));      // n sums of at most 2^s are at most 2^63
     const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, (double)(1ull << (52 - s)), xmax == INFINITY};
     if (t == 0.f || k == 1) {
         int at = n;

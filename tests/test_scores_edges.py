@@ -345,3 +345,31 @@ def test_distillation_small_temperatures(rt, dt):
     top = F.top_logits(x, 3, 1e-20)
     loss, dx = P.distillation(x, top.values, top.indices, temperature=1e-20)
     assert not bool(torch.isnan(dx).any()) and not bool(torch.isnan(loss))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dt", [(1 << 20, torch.float32), ((1 << 20) - 1, torch.bfloat16)])
+def test_the_most_classes(rt, n, dt):
+    """Few rows, which are split or have sixteen waves, and many, of which some are looked at."""
+    F, _ = rt
+    cuts = [(1.0, 0, 1.0, 0.0), (0.7, 0, 0.9, 0.0), (1.0, 300000, 1.0, 0.0), (1.0, 40, 0.8, 0.0), (2.0, 0, 0.5, 0.02), (1.5, n - 5, 0.999, 0.0)]
+    for j, (rows, sel) in enumerate(((2, [1]), (260, [131]))):
+        x = scores(2, n, dt, n + rows, sigma=2.5, offset=1)
+        if rows > 2:
+            x = torch.cat([x, x[:1].expand(rows - 3, n), -x[:1]])
+        got = F.top_logits(x, 200, 2.0)
+        xc = x[sel].float().cpu()
+        v, i, rest = O.top_logits(xc, 200, 2.0)
+        assert torch.equal(got.indices[sel].cpu(), i) and torch.equal(got.values[sel].cpu().double(), v)
+        assert bool(((got.rest[sel].cpu().double() - rest).abs() <= eps_sum(xc, 2.0) + U * rest.abs()).all())
+        val, idx, tr = teacher_lists(x[sel], 20, 2.0, 1)
+        val, idx, tr = (torch.zeros((rows,) + t.shape[1:], dtype=t.dtype, device=DEV).index_copy(0, torch.tensor(sel, device=DEV), t) for t in (val, idx, tr))
+        check_rows(rt, x, val, idx, tr, torch.full((rows,), n - 1, device=DEV), 2.0, 0.3, sel)
+        u = torch.full((rows,), 0.61, device=DEV)
+        for T, k, p, q in cuts[j::2]:
+            print("most", n, dt, rows, T, k, p, q, flush=True)
+            lab, lp = F.sample_labels(x, u, T, k, p, q)
+            want, wp = O.sample(xc, u[sel].cpu(), T, k, p, q)
+            assert torch.equal(lab[sel].cpu(), want)
+            # weights in units of 2^-43 of the first's at worst, half a unit off each and 64-bit sums: n 2^-44 of the kept mass, which is the first's weight at least
+            assert bool(((lp[sel].cpu().double() - wp).abs() <= U * wp.abs() + n * 2.0 ** -44 + 1e-10).all())
