@@ -264,8 +264,10 @@ template <typename T, bool TWO> __device__ __forceinline__ i32x4 grad_vec(const 
 // What the listed classes need is wave 0's.  The gradient is first written as if no class were listed; behind a barrier the
 // listed ones and the label are written over.
 // W = 1: a group of L lanes a row, L = 16 with at most 64 entries.
+// The registers are cut for 4 waves a SIMD: 6 or 7 where they would do gave the same times, 8 spills (8192 x 65536 bf16: 454 us
+// instead of 398).
 template <typename T, int W, int L, int NV, bool TWO, bool GRAD>
-__global__ __launch_bounds__(W == 1 ? 256 : W * 64, NV == 16 || L == 16 ? 4 : NV == 8 ? 6 : W == 1 ? 6 : 7) void distill_row_kernel(DistillArgs a) {
+__global__ __launch_bounds__(W == 1 ? 256 : W * 64, 4) void distill_row_kernel(DistillArgs a) {
     constexpr int VEC = ET<T>::VEC, G = W * L, ROWS = W == 1 ? 256 / L : 1, K = L == 64 ? MAX_K : 64, WORDS = (G * NV * VEC + 2 * BIT0 + 31) / 32;
     __shared__ uint32_t bits_[ROWS][WORDS];
     __shared__ Listed<K> l_[ROWS];
@@ -641,10 +643,15 @@ template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a
     constexpr int VEC = ET<T>::VEC;
     const int nv = a.n / VEC;                      // at most, whatever the alignment
     const unsigned rows = (unsigned)a.rows, quads = (unsigned)((a.rows + 3) / 4), sixteens = (unsigned)((a.rows + 15) / 16);
-    // A narrow row is mostly what every row costs, some 1300 instructions: four rows a wave share them.
+    // As few waves a row as hold it in registers: what every row costs, some 1300 instructions of its first wave, then runs for
+    // more rows at a time, and up to 64 entries four rows share a wave and its instructions.  Loss and gradient, us, by the
+    // lanes (or waves) a row and vectors a lane, many rows of 256 MB (64 rows: all within 1 us of each other up to 8192 vectors):
+    // 200000 x 128 float32 16 lanes x 2 81, x 8 86, a wave 260; 131072 x 512 16 lanes x 8 118, a wave x 4 196, four waves 491;
+    // 65536 x 1024 a wave x 4 144, four x 4 264, x 8 280; 16384 x 4096 four x 4 115, x 8 110, eight 173; 8192 x 8192 four x 8
+    // 105, eight x 8 117, x 16 154; 4096 x 16384 eight x 8 109, x 16 113, sixteen 209; 2048 x 32768 eight x 16 111, sixteen 155;
+    // bf16 alike.  100 entries: 100000 x 240 float32 a wave x 2 158, x 4 152; 100000 x 500 a wave x 4 176, four waves 409.
     if (nv <= 32 && a.k <= 64) distill_row_kernel<T, 1, 16, 2, TWO, GRAD><<<sixteens, 256, 0, s>>>(a);
     else if (nv <= 128 && a.k <= 64) distill_row_kernel<T, 1, 16, 8, TWO, GRAD><<<sixteens, 256, 0, s>>>(a);
-    else if (nv <= 128) distill_row_kernel<T, 1, 64, 2, TWO, GRAD><<<quads, 256, 0, s>>>(a);
     else if (nv <= 256) distill_row_kernel<T, 1, 64, 4, TWO, GRAD><<<quads, 256, 0, s>>>(a);
     else if (nv <= 1024) distill_row_kernel<T, 4, 64, 4, TWO, GRAD><<<rows, 256, 0, s>>>(a);
     else if (nv <= 2048) distill_row_kernel<T, 4, 64, 8, TWO, GRAD><<<rows, 256, 0, s>>>(a);
@@ -652,8 +659,11 @@ template <typename T, bool TWO, bool GRAD> void launch_rows(const DistillArgs& a
     else if (nv <= 8192) distill_row_kernel<T, 8, 64, 16, TWO, GRAD><<<rows, 512, 0, s>>>(a);
     else distill_row_kernel<T, 16, 64, 16, TWO, GRAD><<<rows, 1024, 0, s>>>(a);
 }
-// The loss alone.  Wide rows go by in batches: four waves a row where there are rows enough to fill the chip (1000 x 50001
-// float32: 68 us with the row in registers), sixteen for few rows that no registers hold.
+// The loss alone.  Wide rows go by in batches, by four waves a row, where there are two rows a compute unit or more; sixteen
+// waves take few rows that no registers hold.  Row in registers / four waves / sixteen, us: 512 x 16384 float32 10.4 / 11.3 / 17,
+// 1024 x 16384 21 / 17.5 / 36, 256 x 32768 10.7 / 12.9 / 11.3, 512 x 32768 20.8 / 16.8 / 23.9, 4096 x 65536 276 / 187 / 231,
+// 512 x 32768 bf16 13.8 / 14.5 / 19.7, 1024 x 32768 27.7 / 22.1 / 41, 128 x 65536 13.3 / 15.4 / 13.9; with 8192 scores both
+// first ones the same.
 template <typename T, bool TWO> void launch_fwd(const DistillArgs& a, hipStream_t s) {
     if (a.n / ET<T>::VEC > 2048 && a.rows >= 512) distill_stream_kernel<T, 4, TWO><<<a.rows, 256, 0, s>>>(a);
     else if (a.n <= row_fits<T>()) launch_rows<T, TWO, false>(a, s);

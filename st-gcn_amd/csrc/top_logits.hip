@@ -9,10 +9,10 @@
 // do.  When more than a few k have gathered, the k-th of them becomes the bound.  A score that is not kept, or is dropped
 // from the buffer, enters the sum of the rest at once, under a running maximum, so nothing is read twice.
 //
-// Many rows are bound by their instructions (a score costs a conversion, a comparison and a 2^y), then by what a row costs
-// by itself (the first bound, ranking the answer): 4096 x 65536 bf16, k 64, 204 us, 2.6 TB/s, of which k 1 leaves 160.  Few
-// rows are cut into pieces, or one compute unit would read each alone (4 x 131071 float32, k 128: 170 us in one piece, 29
-// in 25, half of it the join).
+// Many rows are bound by their instructions: 13 vector instructions a score with k 1 and 20 with k 64, whose issue takes 85 and
+// 76 of 100 cycles of every SIMD (4096 x 65536 bf16: 135 and 206 us, 2.6 TB/s with k 64); the rest is what a row costs by
+// itself, the first bound and the ranking of the answer.  Few rows are cut into pieces, or one compute unit would read each
+// alone (4 x 131071 float32, k 128: 170 us in one piece, 29 in 25, half of it the join).
 #include "scores.h"
 
 namespace {
@@ -522,7 +522,10 @@ __global__ __launch_bounds__(256) void top_merge_kernel(TopArgs a) {
 }  // namespace
 
 // Pieces a row is split into.  512 rows fill the chip (two workgroups of four waves a compute unit) and are not split;
-// fewer rows are cut into pieces of at least one batch (4096 scores) until 1024 workgroups run.
+// fewer rows are cut into pieces of at least one batch (4096 scores) until 1024 workgroups run.  float32, k 64, us in 1 / 2 / 4 /
+// 8 / 16 pieces: 32 x 65536 47 / 41 / 31 / 21 / 20, 128 x 65536 46 / 42 / 33 / 29 / 32, 256 x 65536 47 / 45 / 39 / 45 / 49,
+// 512 x 65536 51 / 54 / 62 / 64 / 82, 2048 x 65536 123 / 164 / 201 / 205 / 297; 64 x 9000 18.0 / 19.6 / 18.5 in three, with k 5
+// 11.3 / 17.6 / 16.8.
 static int top_pieces(int rows, int ncls, int k) {
     if (rows >= 512 || ncls <= 512) return 1;
     const int batches = (ncls + 4095) / 4096;
