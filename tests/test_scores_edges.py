@@ -373,3 +373,26 @@ def test_the_most_classes(rt, n, dt):
             assert torch.equal(lab[sel].cpu(), want)
             # weights in units of 2^-43 of the first's at worst, half a unit off each and 64-bit sums: n 2^-44 of the kept mass, which is the first's weight at least
             assert bool(((lp[sel].cpu().double() - wp).abs() <= U * wp.abs() + n * 2.0 ** -44 + 1e-10).all())
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("rows,n,k", [(4, 61, 3), (4, 400, 60), (4, 9001, 16), (4, 70001, 200), (515, 5000, 20)])
+def test_top_logits_many_infinities(rt, rows, n, k, dt):
+    """More +inf than are listed, and with NaN and -inf among them: listed by class, the rest +inf, or NaN."""
+    x = scores(rows, n, dt, n + k)
+    inf = float("inf")
+    x[0], x[1, ::2], x[1, 1::2] = inf, inf, -inf
+    x[2, n // 3:] = inf
+    x[3, ::3] = inf
+    x[3, 1], x[3, n - 1] = float("nan"), float("nan")
+    got = rt[0].top_logits(x, k)
+    xc = x[:4].float().cpu()
+    v, i, _ = O.top_logits(xc, k, 1.0)
+    left = torch.ones_like(xc, dtype=torch.bool).scatter_(1, i, False)
+    assert torch.equal(got.indices[:4].cpu(), i)
+    assert torch.equal(torch.nan_to_num(got.values[:4].cpu().double(), nan=5.0, posinf=6.0), torch.nan_to_num(v, nan=5.0, posinf=6.0))
+    want = [float("nan") if bool((torch.isnan(a) & b).any()) else inf if bool(((a == inf) & b).any()) else None for a, b in zip(xc, left)]
+    assert want[:3] == [inf] * 3
+    for g, w in zip(got.rest[:4].tolist(), want):
+        assert g == w or (w != w and g != g) or w is None, (g, w)
