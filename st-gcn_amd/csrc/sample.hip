@@ -16,8 +16,9 @@
 //     (the sum) crosses is split into bins of its own until it gives a short list, in which the border is bisected by one
 //     wave (a whole workgroup spent 12 us a list on barriers).  Bins and list hold weights as 64-bit integers
 //     in units of 2^-s of the first class's (s = 50 up to 2^13 classes, one less for each doubling, 43 at 2^20): their sums are
-//     the same in any order.  Each is at most half a unit off, so the mass that a border of top-p is held against is off by
-//     n 2^-(s+1) at most (2^-24 at 2^20 classes, 2^-30 at 2^17): the border may lie that much mass away;
+//     the same in any order.  Each is at most half a unit off (a list's lightest a whole one), so the mass that a border of
+//     top-p is held against is off by n 2^-(s+1) at most (2^-24 at 2^20 classes, 2^-30 at 2^17): the border may lie that
+//     much mass away;
 //   the answer: sums of the kept weights by cells (four steps of 64 vectors), made by the pass that fills the last border's
 //     list where there is one, the cell in which u falls, then the lane, then the class.
 //
@@ -63,6 +64,8 @@ struct Weight {
     __device__ __forceinline__ double step() const { return unit * 2.2204460492503131e-16; }       // 2^-s
     __device__ __forceinline__ u64 units(double w) const { return (u64)rint(w * (4503599627370496.0 / unit)); }      // of any w, 2^52 / unit = 2^s
     __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double_as_longlong(w + unit) & ((1ull << 52) - 1); }
+    // In a list, at least one unit for what weighs anything: u = 0 answers the first kept class, however light it is.
+    __device__ __forceinline__ u64 listed(double w) const { const u64 f = fixed(w); return f ? f : w > 0 ? 1 : 0; }
     __device__ __forceinline__ double operator()(float x) const {
         if (inf) return x == INFINITY ? 1.0 : 0.0;
         return exp2_64(((double)x - xmax) * c);
@@ -248,7 +251,7 @@ template <typename T> struct List {
         }
         weight.template many<R>(x, w);
 #pragma unroll
-        for (int i = 0; i < R; ++i) { lw[i] = weight.fixed(w[i]); under |= w[i] < least ? 1u << i : 0u; }
+        for (int i = 0; i < R; ++i) { lw[i] = weight.listed(w[i]); under |= w[i] < least ? 1u << i : 0u; }
         lo = ~wave_max(l);
         hi = wave_max(h);
     }
@@ -358,7 +361,7 @@ template <typename A> __device__ __forceinline__ void draw_short(const u64* list
     const int lane = threadIdx.x & 63;
     const u64 e = lane < c ? list[lane] : 0;
     const double w = lane < c ? weight(place_score(e)) : 0.0;
-    u64 f = weight.fixed(w);
+    u64 f = weight.listed(w);
     if (k < c || p < 1.f) {
         u64 above = 0;                             // mass and number of the entries in front of this one
         int rank = 0;
@@ -695,7 +698,7 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
     bool summed = false;                           // the cells hold what is kept, in integer units
 #pragma unroll 1
     for (int pass = 0; pass < (W == 1 ? 1 : 3); ++pass) {
-        const bool mass = pass == 2, sum = mass || (pass == 1 && !(p < 1.f));
+        const bool mass = pass == 2, sum = (mass || (pass == 1 && !(p < 1.f))) && u > 0.f;       // at u = 0 less than a unit counts
         u64 above = 0, target = (u64)k;
         int shift = -1, c;
         if (pass == 0) {

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import scores_oracle as O
-from tests.test_scores import DEV, U, eps_sum, half_step, rt, scores, teacher_lists  # noqa: F401  (rt: a fixture)
+from tests.test_scores import DEV, U, check_sample, eps_sum, half_step, rt, scores, teacher_lists  # noqa: F401  (rt: a fixture)
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "st-gcn_amd", "csrc")
 
@@ -396,3 +396,15 @@ def test_top_logits_many_infinities(rt, rows, n, k, dt):
     assert want[:3] == [inf] * 3
     for g, w in zip(got.rest[:4].tolist(), want):
         assert g == w or (w != w and g != g) or w is None, (g, w)
+
+
+@pytest.mark.gpu
+@DTS
+@pytest.mark.parametrize("rows,n", [(7, 25), (5, 400), (4, 600), (4, 9001), (270, 9001), (3, 70001)])
+def test_sample_labels_at_zero(rt, rows, n, dt):
+    """u = 0: the first kept class, by class number, however little it weighs next to the row's largest."""
+    for j, (T, k, p, q) in enumerate([(1.0, 0, 1.0, 0.0), (1.0, n // 2 + 1, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (1.0, 20, 0.999, 0.0), (2.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 1e-12),
+                                      (1.0, n - 3, 1.0, 1e-30)][::3 if rows > 200 else 1]):
+        print("zero", rows, n, dt, T, k, p, q, flush=True)
+        x = scores(rows, n, dt, n + j, sigma=15.0, offset=j)
+        check_sample(rt[0], x, torch.zeros(rows, device=DEV), T, k, p, q)
