@@ -268,9 +268,7 @@ class Trainer:
             mine = {id(p) for p in model.parameters()}
             if teacher is model or any(id(p) in mine for p in teacher.parameters()):
                 raise ValueError("the teacher shares parameters with the model")
-        if not 1 <= int(teacher_k) <= 256 or not 1e-30 < float(temperature) < 1e30 or not 0.0 <= float(label_weight) <= 1.0:
-            raise ValueError("a teacher wants 1 to 256 top logits, a temperature above 0 and a label_weight from 0 to 1, got %r, %r, %r"
-                             % (teacher_k, temperature, label_weight))
+        self._check_teaching(teacher_k, temperature, label_weight)
         self.model = model
         self.teacher, self.teacher_k = teacher, int(teacher_k)
         self.temperature, self.label_weight = float(temperature), float(label_weight)
@@ -286,6 +284,12 @@ class Trainer:
         self._taught_steps = 0                # of these with a target
         self._met = {}                        # (temperature, label_weight) of the last steps with a target
         self._grads_bound = False             # whether every p.grad is the parameter's slice of the flat gradient
+
+    @staticmethod
+    def _check_teaching(k, temperature, label_weight):
+        if not 1 <= int(k) <= 256 or not 1e-30 < float(temperature) < 1e30 or not 0.0 <= float(label_weight) <= 1.0:
+            raise ValueError("a teacher wants 1 to 256 top logits, a temperature above 0 and a label_weight from 0 to 1, got %r, %r, %r"
+                             % (k, temperature, label_weight))
 
     def broadcast_from_rank0(self):
         if self.bucketer.distributed:
@@ -480,6 +484,8 @@ class Trainer:
     def _target_of(self, data, label, target):
         """The target, checked as functional.distillation would: a captured step only copies it, and would cast and move."""
         given = target is not None
+        if given or self.teacher is not None:
+            self._check_teaching(self.teacher_k, self.temperature, self.label_weight)
         if not given:
             target = self.target(data)
         if target is None:

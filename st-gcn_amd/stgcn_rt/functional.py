@@ -391,7 +391,7 @@ TopLogits = collections.namedtuple("TopLogits", "values indices rest")
 
 def top_logits(logits, k, temperature=1.0):
     """What of a teacher's scores [rows, classes] is kept for distillation: TopLogits(values, indices, rest), see
-    ops.top_logits.  Carries no gradient."""
+    ops.top_logits.  Temperatures from 1e-30 to 1e30.  Carries no gradient."""
     return TopLogits(*P.top_logits(logits, k, temperature))
 
 
@@ -450,8 +450,8 @@ def distillation(logits, values, indices, rest=None, labels=None, temperature=1.
 
     A row without entries has no first term, one whose label is < 0 no second; a row with neither (padding) or with
     every score -inf gives 0 and a zero gradient, whatever it holds.  A class listed twice counts with both entries.  A
-    class or label >= classes, or a teacher score that is NaN or +inf, makes the row's loss and gradient NaN.  The mean is
-    over all rows.  Differentiable in logits, once."""
+    class or label >= classes, a teacher score that is NaN or +inf, or a student score that is, makes the row's loss and
+    gradient NaN.  The mean is over all rows.  1e-30 < T < 1e30.  Differentiable in logits, once."""
     return DistillationFn.apply(logits, values, indices, rest, labels, temperature, label_weight, reduction)
 
 

@@ -73,6 +73,20 @@ def test_targets_that_do_not_fit_are_refused():
             tr.step(x, lab, target=(v.to("meta"), i, r))
 
 
+def test_values_set_between_steps_are_checked():
+    """As in the constructor, before a step runs or is captured (a capture that fails would switch graphs off)."""
+    x, lab = torch.zeros(2, 3, 4, 25, 1), torch.zeros(2, dtype=torch.int64)
+    top = (torch.zeros(2, 5), torch.zeros(2, 5, dtype=torch.int64), torch.zeros(2))
+    for name, value in (("temperature", 0.0), ("temperature", float("nan")), ("temperature", -1.0), ("label_weight", 1.5), ("label_weight", float("nan"))):
+        tr = cpu_trainer(graph=True)
+        tr._eager_steps = tr._taught_steps = 5
+        tr._capture = lambda *a: pytest.fail("captured")
+        setattr(tr, name, value)
+        for f in (lambda: tr.step(x, lab, target=top), lambda: tr.prepare_graph(x, lab, target=top)):
+            with pytest.raises(ValueError, match="a teacher wants"):
+                f()
+
+
 @pytest.mark.gpu
 def test_annealed_temperature_keeps_its_memory(st):
     """Ten temperatures, four steps each: as launch by launch bit for bit, and the memory of the graphs that passed is free again."""
