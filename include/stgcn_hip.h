@@ -285,8 +285,8 @@ int stgcn_distill_scale(const float* dlogits, const float* stats, const float* g
  * order the first top_k (0: all); of these the shortest prefix that reaches top_p of their mass; of these those at least
  * min_p times as likely as the first; the label is the first of them, by class number, at which their running mass exceeds
  * u times their mass; logp is the log of its share of that mass.  temperature 0: the first class, logp 0.  Each parameter
- * is one number or, where its array is given, one a row.  Weights and sums are held in 64 bits, in units of 2^-43 (2^20 classes)
- * to 2^-50 (8192 and fewer) of the first class's weight where top_p's border is looked for.
+ * is one number or, where its array is given, one a row.  Weights and sums are held in 64 bits (a weight that decides top_p's
+ * border to 2^-43 of the largest near it at 2^20 classes, 2^-50 from 8192 down).
  * A row of -inf only answers label -1 and logp -inf; a row with a NaN, or with a parameter out of range (temperature >= 0,
  * top_k >= 0, 0 < top_p <= 1, 0 <= min_p <= 1, 0 <= u < 1), answers label -1 and logp NaN. */
 int stgcn_sample_labels(int dtype, const void* logits, size_t row_stride, const float* u, const float* temperatures, float temperature,

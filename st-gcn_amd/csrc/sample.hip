@@ -14,18 +14,18 @@
 //     in LDS, where everything else happens, and no weight of any other class is computed;
 //   larger top_k, and top_p: the scores (or their weights) counted by bins of the score; the bin in which the count
 //     (the sum) crosses is split into bins of its own until it gives a short list, in which the border is bisected by one
-//     wave (a whole workgroup spent 12 us a list on barriers).  Bins and list hold weights as 64-bit integers
-//     in units of 2^-s of the first class's (s = 50 up to 2^13 classes, one less for each doubling, 43 at 2^20): their sums are
-//     the same in any order.  Each is at most half a unit off (a list's lightest a whole one), so the mass that a border of
-//     top-p is held against is off by n 2^-(s+1) at most (2^-24 at 2^20 classes, 2^-30 at 2^17): the border may lie that
-//     much mass away;
+//     wave (a whole workgroup spent 12 us a list on barriers).  Bins hold weights as 64-bit integers, whose sums are the
+//     same in any order, in units of 2^-(s + E): s = 50 up to 2^13 classes, one less for each doubling, 43 at 2^20; E the
+//     octaves that a bin's weights lie below the first class's.  (Units of the first class's weight alone lose what decides in
+//     a tail of a million classes of e^-26 each.)  From bin to bin sums are 64-bit floating point; lists have units of
+//     2^-(50 + E), cells 2^-50;
 //   the answer: sums of the kept weights by cells (four steps of 64 vectors), made by the pass that fills the last border's
 //     list where there is one, the cell in which u falls, then the lane, then the class.
 //
 // Two looks at a row, for its maximum and its class, take 9.4 us at 256 x 65536 bf16 (temperature 0); those that weigh are bound by
-// their 64-bit instructions, some 17 a score at 4.8 cycles a wave each, 12 us a pass there.  A row costs 6 to 7 us of one wave's work on the list.
-// 512 x 65536 bf16, rows greedy, uncut, top-k, top-p, min-p and all at once by turns: 77 us; one row of 131072, top-k 50:
-// 24 us.
+// their 64-bit instructions, some 17 a score at 4.8 cycles a wave each, 12 us a pass there.  A row costs 6 to 7 us of one wave's
+// work on the list.  512 x 65536 bf16, rows greedy, uncut, top-k, top-p, min-p and all at once by turns: 77 us; one row of
+// 131072, top-k 50: 24 us.
 #include "scores.h"
 #include <cfloat>
 #include <type_traits>
@@ -60,12 +60,7 @@ __device__ __forceinline__ double lane_at(double v, int l) { return __longlong_a
 
 // Weights relative to the row's maximum.  With a maximum of +inf its classes weigh 1, all others nothing.
 struct Weight {
-    double xmax, c, unit; bool inf;                // unit: 2^(52 - s); the low 52 bits of w + unit are w in units of 2^-s
-    __device__ __forceinline__ double step() const { return unit * 2.2204460492503131e-16; }       // 2^-s
-    __device__ __forceinline__ u64 units(double w) const { return (u64)rint(w * (4503599627370496.0 / unit)); }      // of any w, 2^52 / unit = 2^s
-    __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double_as_longlong(w + unit) & ((1ull << 52) - 1); }
-    // In a list, at least one unit for what weighs anything: u = 0 answers the first kept class, however light it is.
-    __device__ __forceinline__ u64 listed(double w) const { const u64 f = fixed(w); return f ? f : w > 0 ? 1 : 0; }
+    double xmax, c; bool inf;
     __device__ __forceinline__ double operator()(float x) const {
         if (inf) return x == INFINITY ? 1.0 : 0.0;
         return exp2_64(((double)x - xmax) * c);
@@ -87,6 +82,13 @@ struct Weight {
     }
 };
 
+// w <= 1 as an integer in units of 2^-s: the low 52 bits of w + 2^(52 - s).  Lists of at most CAP places and cells of at most 2048
+// classes have units of 2^-50: their sums stay below 2^62.
+__device__ __forceinline__ u64 fixed(double w, double unit) { return (u64)__double_as_longlong(w + unit) & ((1ull << 52) - 1); }
+constexpr int FINE = 50;
+constexpr double FINE_UNIT = 4.0, FINE_STEP = 1.0 / (1ull << FINE);
+__device__ __forceinline__ u64 fine_units(double w) { return (u64)rint(w * (double)(1ull << FINE)); }       // of any w
+
 // The kept set: x > xt, or x == xt and class <= ti.  Tests that run for every score are written without && and ||, which
 // become branches: eight nests of them a vector took four times as long as the comparisons.
 struct Cut {
@@ -105,7 +107,7 @@ template <int W, int CELLS> struct Shared {
         u64 list[CAP];
     };
     union { double sum[CELLS]; u64 units[CELLS]; int count[CELLS]; } cell;
-    alignas(16) u64 total[BINS];
+    alignas(16) double total[BINS];
     double all; int redi; uint32_t red[W];
     int pick; double before; Cut cut;
 };
@@ -224,10 +226,10 @@ template <typename F> __device__ __forceinline__ uint32_t last_enough(uint32_t l
 }
 
 // How many of `ties` equal weights `one` the sum needs to get from `over` to target: at least one, at most all.
-__device__ __forceinline__ int ties_needed(u64 over, u64 one, u64 target, int ties) {
+__device__ __forceinline__ int ties_needed(double over, double one, double target, int ties) {
     if (one == 0 || over + one >= target) return one == 0 ? ties : 1;
-    const u64 m = (target - over + one - 1) / one;
-    return m < (u64)ties ? (int)m : ties;
+    const double m = ceil((target - over) / one);
+    return m < (double)ties ? (int)m : ties;
 }
 
 // At most CAP places, held by one wave: steps of 64 that hold nothing are skipped.
@@ -235,9 +237,10 @@ template <typename T> struct List {
     static constexpr int R = CAP / 64, SHIFT = ET<T>::IS_BF16 ? 16 : 0;    // bits of a key that carry nothing
     const Weight& weight;
     int c, n;                                      // places; classes of the row
-    u64 lp[R], lw[R];                              // place (0: none) and weight in integer units
+    u64 lp[R], lw[R];                              // place (0: none) and weight in units of 2^-(FINE + E)
+    int E;
     uint32_t lo, hi, under;                        // smallest and largest key; bit i: weight i is less than min_p
-    __device__ __forceinline__ List(const u64* list, int c_, int n_, const Weight& w_, double least) : weight(w_), c(c_), n(n_) {
+    __device__ __forceinline__ List(const u64* list, int c_, int n_, const Weight& w_, double least, int E_) : weight(w_), c(c_), n(n_), E(E_) {
         const int lane = threadIdx.x & 63;
         float x[R];
         double w[R];
@@ -251,10 +254,18 @@ template <typename T> struct List {
         }
         weight.template many<R>(x, w);
 #pragma unroll
-        for (int i = 0; i < R; ++i) { lw[i] = weight.listed(w[i]); under |= w[i] < least ? 1u << i : 0u; }
+        for (int i = 0; i < R; ++i) under |= w[i] < least ? 1u << i : 0u;
+        if (E) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) w[i] = ldexp(w[i], E);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) lw[i] = listed(w[i]);
         lo = ~wave_max(l);
         hi = wave_max(h);
     }
+    // At least one unit for what weighs anything: u = 0 answers the first kept class, however light it is.
+    static __device__ __forceinline__ u64 listed(double w) { const u64 f = fixed(w, FINE_UNIT); return f ? f : w > 0 ? 1 : 0; }
     template <typename P> __device__ __forceinline__ int count(P pred) const {
         int m = 0;
 #pragma unroll
@@ -282,11 +293,10 @@ template <typename T> struct List {
         auto enough = [&](u64 from) { return count([&](u64 e) { return e >= from; }) >= k; };
         return border_at(last_enough(lo, hi, [&](uint32_t mid) { return enough((u64)mid << (32 + SHIFT)); }), was, enough);
     }
-    // The place at which, after `above`, the target is reached.  Bisected only until at most 32 entries are left, which are
+    // The place at which the mass `need` is reached.  Bisected only until at most 32 entries are left, which are
     // then compared one by one (32 bits of a key to the end: 64 x 400 float32, top-p 0.9: 13.4 us instead of 15.2).  Overwrites list.
-    __device__ __forceinline__ Cut cut_mass(u64 above, u64 target, const Cut& was, u64* list) const {
+    __device__ __forceinline__ Cut cut_mass(u64 need, const Cut& was, u64* list) const {
         const int lane = threadIdx.x & 63;
-        const u64 need = target - above;
         uint32_t l = lo, h = hi;
         int left = c, beyond = 0;                  // entries with keys from l on, and beyond h; the mass of the latter
         u64 m_beyond = 0;
@@ -341,9 +351,9 @@ template <typename T> struct List {
     }
     template <typename F> __device__ __forceinline__ void each(F f) const {
 #pragma unroll
-        for (int i = 0; i < R; ++i) if (64 * i < c && lw[i]) f(place_class(lp[i]), lw[i]);
+        for (int i = 0; i < R; ++i) if (64 * i < c && lw[i]) f(place_class(lp[i]), (lw[i] + ((1ull << E) >> 1)) >> E);       // in cells' units
     }
-    // The answer, from entries that are all there is, in integer units: the first class, in the order of the classes, at
+    // The answer, from entries that are all there is (E = 0): the first class, in the order of the classes, at
     // which the running mass exceeds u times all of it.
     template <typename A> __device__ __forceinline__ void draw(float u, A answer) const {
         const u64 sum = all(), most = (u64)floor((double)u * (double)sum);             // a running mass > most
@@ -352,16 +362,16 @@ template <typename T> struct List {
         float x = -INFINITY;
 #pragma unroll
         for (int i = 0; i < R; ++i) if (64 * i < c && lw[i] && (uint32_t)lp[i] == who) x = place_score(lp[i]);
-        if (x > -INFINITY) answer((int)~who, weight(x), (double)sum * weight.step());
+        if (x > -INFINITY) answer((int)~who, weight(x), (double)sum * FINE_STEP);
     }
 };
 
 // A list of at most 64 places, one a lane, compared with each other one by one.
-template <typename A> __device__ __forceinline__ void draw_short(const u64* list, int c, int k, float p, double least, float u, const Weight& weight, A answer) {
+template <typename T, typename A> __device__ __forceinline__ void draw_short(const u64* list, int c, int k, float p, double least, float u, const Weight& weight, A answer) {
     const int lane = threadIdx.x & 63;
     const u64 e = lane < c ? list[lane] : 0;
     const double w = lane < c ? weight(place_score(e)) : 0.0;
-    u64 f = weight.listed(w);
+    u64 f = List<T>::listed(w);
     if (k < c || p < 1.f) {
         u64 above = 0;                             // mass and number of the entries in front of this one
         int rank = 0;
@@ -385,7 +395,7 @@ template <typename A> __device__ __forceinline__ void draw_short(const u64* list
 #pragma unroll
         for (int d = 0; d < 4; ++d) before += (uint32_t)lane_at(e, i + d) > (uint32_t)e ? lane_at(f, i + d) : 0;
     }
-    if (before <= most && most < before + f) answer(place_class(e), w, (double)sum * weight.step());
+    if (before <= most && most < before + f) answer(place_class(e), w, (double)sum * FINE_STEP);
 }
 
 template <typename T, int W, int CELLS>
@@ -425,8 +435,9 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
     }
     if (top == KEY_NEG_INF) { if (tid == 0) fixed_answer(-1, -INFINITY); return; }
     const float xmax = key_score(top);
-    const int s = min(50, 31 + __clz(n - 1));      // n sums of at most 2^s are at most 2^63
-    const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, (double)(1ull << (52 - s)), xmax == INFINITY};
+    const Weight weight = {(double)xmax, t > 0.f ? LOG2E / (double)t : 0.0, xmax == INFINITY};
+    // Bins have units of 2^-(s + E), E the octaves that all weights of a bin lie below the first one: n of at most 2^s are at most 2^63.
+    const double bin_unit = (double)(1ull << (52 - min(50, 31 + __clz(n - 1))));
     if (t == 0.f || k == 1) {
         int at = n;
         row.template each<4>([&](int i, const float* s) {
@@ -535,7 +546,7 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
                 }
                 if (row.ends_cell(i)) {
                     cell_sum = wave_sum(cell_sum);
-                    if (lane == 0) sh.cell.units[row.cell(i)] = weight.units(cell_sum);
+                    if (lane == 0) sh.cell.units[row.cell(i)] = fine_units(cell_sum);
                     cell_sum = 0;
                 }
             }
@@ -611,6 +622,8 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
     // score, or (shift >= 0) of the keys down from khi.
     uint32_t klo = 0, khi = top;
     float scale = 0;
+    int per_octave = 31;                           // 2^per_octave bins of the distance lie within an octave of the weight, or more
+    int octaves = 0;                               // that the weights from khi down lie below the first one
     auto upper_score = [](uint32_t k) { return key_score(k == 0x7FFFFFFFu ? k - 1 : k); };  // no score has the key of -0, and as a number it is 0
     auto fill_bins = [&](bool mass, int shift) {
         __syncthreads();
@@ -618,62 +631,61 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
         for (int i = tid; i < S::COPIES * BINS; i += G) (&sh.bins[0][0])[i] = 0;
         __syncthreads();
         const float xlo = klo ? key_score(klo) : -INFINITY, xhi = upper_score(khi);
-        auto drop = [&](float x, u64 v) {
+        // a count is a sum of weights of 1 in units of 1
+        const int eb = mass && shift < 0 ? per_octave : 31, unit0 = __double2hiint(mass ? bin_unit : 4503599627370496.0) - (octaves << 20);
+        auto unit = [&](int b) { return __hiloint2double(__mul24(b >> eb, -(1 << 20)) + unit0, 0); };       // 2^-(b >> eb)
+        auto drop = [&](float x, double w) {
             if (x > xhi) return;
             const int b = shift < 0 ? (int)fminf((xmax - x) * scale, (float)(BINS - 1)) : (int)((khi - score_key(x)) >> shift);
-            atomicAdd(&sh.bins[b][lane & (S::COPIES - 1)], v);
+            atomicAdd(&sh.bins[b][lane & (S::COPIES - 1)], fixed(w, unit(b)));
         };
         row.template each<1>([&](int i, const float* s) {
             float x[VEC];
             if (!only_kept(i, s, x, xlo)) return;
-            u64 v[VEC];
-            if (mass) {
-                double w[VEC];
-                weight.template many<VEC>(x, w);
+            double w[VEC];
+            if (mass) weight.template many<VEC>(x, w);
+            else {
+                const double one = row.valid(i) ? 1.0 : 0.0;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = weight.fixed(w[e]);
-            } else {
-                const u64 one = row.valid(i);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] = one;
+                for (int e = 0; e < VEC; ++e) w[e] = one;
             }
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) if (s[e] >= xlo) drop(s[e], v[e]);
+            for (int e = 0; e < VEC; ++e) if (s[e] >= xlo) drop(s[e], w[e]);
         });
-        if (tid < row.sp.edge && row.xe >= xlo && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, mass ? weight.fixed(weight(row.xe)) : 1);
+        if (tid < row.sp.edge && row.xe >= xlo && cut(row.xe, row.sp.edge_at(tid))) drop(row.xe, mass ? weight(row.xe) : 1.0);
         __syncthreads();
 #pragma unroll 1
         for (int b = tid; b < BINS; b += G) {
             u64 s = 0;
 #pragma unroll 8
             for (int i = 0; i < S::COPIES; ++i) s += sh.bins[b][(i + tid) & (S::COPIES - 1)];
-            sh.total[b] = s;
+            sh.total[b] = (double)s * (unit(b) * 2.2204460492503131e-16);           // 2^-52
         }
         __syncthreads();
     };
-    // Sum of the bins; the first bin at which the running sum, from `above` on, reaches target (every wave, BINS / 64 bins a lane).
+    // Sum of the bins; the first bin at which the running sum, from `above` on, reaches target, or the last one that holds anything
+    // if rounding leaves none (every wave, BINS / 64 bins a lane, the same sums in the same order).
     constexpr int BL = BINS / 64;
     auto bin_sum = [&]() {
-        u64 s = 0;
+        double s = 0;
 #pragma unroll
         for (int i = 0; i < BL; ++i) s += sh.total[BL * lane + i];
         return wave_sum(s);
     };
-    auto bin_reach = [&](u64 target, u64& above) {
-        u64 own = 0;
+    auto bin_reach = [&](double target, double& above) {
+        double own = 0;
 #pragma unroll
         for (int i = 0; i < BL; ++i) own += sh.total[BL * lane + i];
-        const u64 s = wave_scan(own);
-        const u64 hit = __ballot(above + s >= target);
-        const int l = hit ? __ffsll(hit) - 1 : 63;
-        above += lane_at(s - own, l);
+        const double s = wave_scan(own);
+        const u64 some = __ballot(own > 0), hit = __ballot(own > 0 && above + s >= target);
+        const int l = hit ? __ffsll(hit) - 1 : some ? 63 - __clzll(some) : 0;
+        double run = above + lane_at(s - own, l);
         int b = BL * l;
 #pragma unroll 1
-        for (int i = 0; i < BL - 1; ++i) {
-            const u64 next = above + uniform(sh.total[b]);
-            if (next >= target) break;
-            above = next;
-            ++b;
+        for (int i = 0; i < BL; ++i) {
+            const double v = uniform(sh.total[BL * l + i]);
+            if (v > 0) { b = BL * l + i; above = run; if (run + v >= target) break; }
+            run += v;
         }
         return b;
     };
@@ -699,7 +711,7 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
 #pragma unroll 1
     for (int pass = 0; pass < (W == 1 ? 1 : 3); ++pass) {
         const bool mass = pass == 2, sum = (mass || (pass == 1 && !(p < 1.f))) && u > 0.f;       // at u = 0 less than a unit counts
-        u64 above = 0, target = (u64)k;
+        double above = 0, target = (double)k;
         int shift = -1, c;
         if (pass == 0) {
             klo = KEY_NEG_INF + 1;                 // -inf weighs nothing: never in the list
@@ -711,18 +723,21 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
             khi = top;
         } else {
             if (mass ? !(p < 1.f) : k == n) continue;
-            klo = 0; khi = top;
+            klo = 0; khi = top; octaves = 0;
             // BINS over 32 octaves of the weight, or finer where the row is narrower
             const float smallest = key_score(~block_max(~score_key(low)));
             scale = (float)fmin(BINS / 32 * weight.c, 1e30);
             if ((xmax - smallest) * scale < (float)(BINS - 1) && xmax > smallest) scale = (float)(BINS - 1) / (xmax - smallest);
+            const float bins = (float)((double)scale / weight.c);
+            per_octave = weight.inf || !(bins < 1e9f) ? 31 : bins > 1.001f ? ilogbf(0.999f * bins) + 1 : 0;
         }
 #pragma unroll 1
         for (;;) {
             if (pass) {
                 fill_bins(mass, shift);
-                if (mass && shift < 0) target = (u64)ceil((double)p * (double)bin_sum());
+                if (mass && shift < 0) target = (double)p * bin_sum();
                 const int b = bin_reach(target, above);
+                if (mass && shift < 0) octaves = min(50, b >> per_octave);
                 if (shift < 0) {                   // from the first key that is not beyond the bin to the last that has reached it
                     khi = last_key([&](float x) { return !((xmax - x) * scale < (float)b); });
                     klo = b == BINS - 1 ? KEY_NEG_INF + 1 : max(KEY_NEG_INF, last_key([&](float x) { return !((xmax - x) * scale < (float)(b + 1)); })) + 1;
@@ -737,15 +752,17 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
             while ((khi - klo) >> shift >= (uint32_t)BINS) ++shift;
         }
         if (pass == 0 && c > CAP) continue;
-        if (pass == 1 && target > above + c) continue;                     // top_k reaches into scores of -inf: all others are kept
+        if (pass == 1 && target > above + (double)c) continue;                     // top_k reaches into scores of -inf: all others are kept
         if (c <= CAP) {
             if (wave == 0) {
-                if (!pass && c <= 64) { draw_short(sh.list, c, k, p, least, u, weight, answer); return; }
-                List<T> list(sh.list, c, n, weight, least);
+                if (!pass && c <= 64) { draw_short<T>(sh.list, c, k, p, least, u, weight, answer); return; }
+                List<T> list(sh.list, c, n, weight, least, octaves);
                 if (pass ? !mass : k < c) { cut = list.cut_count((int)(target - above), cut); list.keep(cut); }
                 if (pass ? mass : p < 1.f) {
-                    if (!pass) target = (u64)ceil((double)p * (double)list.all());
-                    cut = list.cut_mass(above, target, cut, sh.list);
+                    // what the bins' rounding says more than the list holds is all of it
+                    const u64 all = list.all();
+                    const double need = pass ? ldexp(target - above, FINE + list.E) : (double)p * (double)all;
+                    cut = list.cut_mass(need < (double)all ? max((u64)1, (u64)ceil(need)) : all, cut, sh.list);
                     list.keep(cut);
                 }
                 list.drop_under();
@@ -759,7 +776,7 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
             summed = sum;
         } else {                                   // c equal scores
             const float x = key_score(khi);
-            const int need = mass ? ties_needed(above, weight.fixed(weight(x)), target, c) : (int)(target - above);
+            const int need = mass ? ties_needed(above, weight(x), target, c) : (int)(target - above);
             if (x > -INFINITY) cut = {x, need < c ? nth(x, need) : x == cut.xt ? cut.ti : n};           // -inf weighs nothing: no cut
         }
     }
@@ -782,8 +799,8 @@ __global__ __launch_bounds__(W * 64, 4) void sample_kernel(SampleArgs a) {
         return true;
     };
     __syncthreads();
-    auto set_cell = [&](int c, double s) { if (summed) sh.cell.units[c] = weight.units(s); else sh.cell.sum[c] = s; };
-    auto cell_at = [&](int c) { return summed ? (double)sh.cell.units[c] * weight.step() : sh.cell.sum[c]; };
+    auto set_cell = [&](int c, double s) { if (summed) sh.cell.units[c] = fine_units(s); else sh.cell.sum[c] = s; };
+    auto cell_at = [&](int c) { return summed ? (double)sh.cell.units[c] * FINE_STEP : sh.cell.sum[c]; };
     double cell_sum = 0;
     if (!summed) row.template each<1>([&](int i, const float* s) {
         double w[VEC];
