@@ -24,7 +24,7 @@
 //
 // Two looks at a row, for its maximum and its class, take 9.4 us at 256 x 65536 bf16 (temperature 0); those that weigh are bound by
 // their 64-bit instructions, some 17 a score at 4.8 cycles a wave each, 12 us a pass there.  A row costs 6 to 7 us of one wave's
-// work on the list.  512 x 65536 bf16, rows greedy, uncut, top-k, top-p, min-p and all at once by turns: 77 us; one row of
+// work on the list.  512 x 65536 bf16, rows greedy, uncut, top-k, top-p, min-p and all at once by turns: 78 us; one row of
 // 131072, top-k 50: 24 us.
 #include "scores.h"
 #include <cfloat>
