@@ -1,4 +1,4 @@
-"""Checker of the operators over class scores, in 64 bits on the CPU, row by row from their definitions."""
+"""Oracle of the operators over class scores, in 64 bits on the CPU, row by row from their definitions."""
 import math
 
 import torch
